@@ -47,6 +47,7 @@ UNITS = {
     "mixers_chunks.o": ("mixers_chunks.cu", ("mixers.cuh", "common.cuh")),
     "mixers_window.o": ("mixers_window.cu", ("mixers.cuh", "common.cuh")),
     "mixers_streams.o": ("mixers_streams.cu", ("mixers.cuh", "common.cuh")),
+    "packed_cache.o": ("packed_cache.cu", ("packed_cache.cuh", "common.cuh")),
 }
 
 

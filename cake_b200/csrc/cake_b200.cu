@@ -33,6 +33,7 @@
 #include "gemm_skinny.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
+#include "packed_cache.cuh"
 #include "prefill.cuh"
 #include "sample.cuh"
 
@@ -294,6 +295,7 @@ struct cake_b200_cache {
   std::vector<uint32_t> last_tok;
   int embed_len = 0;
   unsigned wait_failures = 0;  // the context's count when the cache was created or cleared: another one, and its rows may be no results
+  int bits = 0;  // 4: k holds K and V rows in four bits (packed_cache.cuh), v nothing; 0: rows in D
 };
 
 template <typename U> struct TypeTag { typedef U type; };
@@ -897,11 +899,12 @@ extern "C" int cake_b200_block_set_variant(cake_b200_block *b, const cake_b200_b
 }
 
 // ------------------------------------------------------------------------------------------ cache
-extern "C" int cake_b200_cache_create(cake_b200_ctx *c, int batch, int max_seq, cake_b200_cache **out) {
+static int cache_create(cake_b200_ctx *c, int batch, int max_seq, int bits, cake_b200_cache **out) {
   if (!c || !out || batch < 1 || max_seq < 1) return fail(CAKE_B200_EINVAL, "bad cache arguments");
   if (max_seq > c->cfg.max_seq) return fail(CAKE_B200_EINVAL, "cache max_seq %d exceeds config max_seq %d (RoPE table rows)", max_seq, c->cfg.max_seq);
   CU(cudaSetDevice(c->device));
   auto *k = new cake_b200_cache{c, batch, max_seq, c->device};
+  k->bits = bits;
   k->gen = g_cache_gen.fetch_add(1);
   const int slots = c->cfg.layer_list ? 2 * c->cfg.n_layers : c->cfg.n_layers;  // a side mixer's entries follow the main ones
   k->k.assign(slots, nullptr);
@@ -932,9 +935,23 @@ extern "C" int cake_b200_cache_create(cake_b200_ctx *c, int batch, int max_seq, 
   *out = k;
   return CAKE_B200_OK;
 }
+extern "C" int cake_b200_cache_create(cake_b200_ctx *c, int batch, int max_seq, cake_b200_cache **out) { return cache_create(c, batch, max_seq, 0, out); }
+extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int max_seq, int bits, cake_b200_cache **out) {
+  if (!c || !out) return fail(CAKE_B200_EINVAL, "null argument");
+  if (bits != 4) return fail(CAKE_B200_EINVAL, "a packed cache holds 4 bits an entry, not %d", bits);
+  if (c->cfg.layer_list) return fail(CAKE_B200_EINVAL, "packed caches are for the Llama-family blocks");
+  if (!pc::head_dim_ok(c->cfg.head_dim)) return fail(CAKE_B200_EINVAL, "packed caches hold heads of 64, 128 or 256 entries, not %d", c->cfg.head_dim);
+  if (c->rot % 16) return fail(CAKE_B200_EINVAL, "packed caches rotate multiples of 16 entries of a head, not %d", c->rot);
+  return cache_create(c, batch, max_seq, bits, out);
+}
 static int cache_ensure(cake_b200_cache *k, int layer) {
   if (layer < 0 || layer >= (int)k->k.size()) return fail(CAKE_B200_EINVAL, "block_idx %d out of range", layer);
   if (k->k[layer]) return CAKE_B200_OK;
+  if (k->bits) {
+    const int hd = k->ctx->cfg.head_dim;
+    CU(cudaMalloc(&k->k[layer], (size_t)k->batch * k->ctx->cfg.n_kv_heads * pc::cap_blocks(k->cap) * pc::block_bytes(hd)));
+    return CAKE_B200_OK;
+  }
   const size_t bytes = (size_t)k->batch * k->ctx->cfg.n_kv_heads * k->cap * k->ctx->cfg.head_dim * k->ctx->es;
   CU(cudaMalloc(&k->k[layer], bytes + 16));
   CU(cudaMalloc(&k->v[layer], bytes + 16));
@@ -1000,15 +1017,122 @@ extern "C" int cake_b200_cache_read(cake_b200_cache *k, int block_idx, int which
   if (block_idx < 0 || block_idx >= (int)k->len.size() || !k->k[block_idx]) return fail(CAKE_B200_EINVAL, "layer %d has no cache", block_idx);
   const int len = k->len[block_idx];
   const int hd = k->kv_hd[block_idx] ? k->kv_hd[block_idx] : c->cfg.head_dim, nkv = k->kv_heads[block_idx] ? k->kv_heads[block_idx] : c->cfg.n_kv_heads;
-  if (which && !k->v[block_idx]) return fail(CAKE_B200_EINVAL, "layer %d keeps no V cache (its values are its keys)", block_idx);
+  if (which && !k->bits && !k->v[block_idx]) return fail(CAKE_B200_EINVAL, "layer %d keeps no V cache (its values are its keys)", block_idx);
   const size_t need = (size_t)k->batch * nkv * len * hd * c->es;
   if (bytes < need) return fail(CAKE_B200_EINVAL, "cache_read needs %zu bytes", need);
   RC(sync_results(c));
   RC(check_cache(k));
+  if (k->bits) {
+    if (!len) return CAKE_B200_OK;
+    void *rows = nullptr;
+    CU(cudaMalloc(&rows, need));
+    int rc = cake_b200_cache_unpack(k, block_idx, which, 0, len, rows);
+    if (rc == CAKE_B200_OK) rc = sync_results(c);
+    if (rc == CAKE_B200_OK) {
+      const cudaError_t e = cudaMemcpy(out_host, rows, need, cudaMemcpyDeviceToHost);
+      if (e != cudaSuccess) rc = fail(CAKE_B200_ECUDA, "cache_read: %s", cudaGetErrorString(e));
+    }
+    cudaFree(rows);
+    return rc;
+  }
   const char *src = (const char *)(which ? k->v[block_idx] : k->k[block_idx]);
   CU(cudaMemcpy2D(out_host, (size_t)len * hd * c->es, src, (size_t)k->cap * hd * c->es, (size_t)len * hd * c->es,
                   (size_t)k->batch * nkv, cudaMemcpyDeviceToHost));
   return CAKE_B200_OK;
+}
+// ---- caches in four bits (packed_cache.cuh)
+static uint64_t *launch_counter(cake_b200_ctx *c) { return c->capturing ? &c->g_kernels : &c->launches; }
+static int packed_call(const cake_b200_cache *k, int block_idx, const char *what) {
+  if (!k) return fail(CAKE_B200_EINVAL, "null argument");
+  if (!k->bits) return fail(CAKE_B200_EINVAL, "%s is for caches of cake_b200_cache_create_packed", what);
+  if (block_idx < 0 || block_idx >= (int)k->len.size()) return fail(CAKE_B200_EINVAL, "block_idx %d out of range", block_idx);
+  CU(cudaSetDevice(k->device));
+  RC(check_waits(k->ctx));
+  return check_cache(k);
+}
+static bool unaligned(const void *p, size_t s0 = 0, size_t s1 = 0) { return ((uintptr_t)p & 15) || s0 % 8 || s1 % 8; }
+extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const void *k_dev, size_t k_tok, size_t k_batch, const void *v_dev,
+                                     size_t v_tok, size_t v_batch, int seq, int index_pos) {
+  RC(packed_call(k, block_idx, "cache_write"));
+  if (!k_dev || !v_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
+  if (unaligned(k_dev, k_tok, k_batch) || unaligned(v_dev, v_tok, v_batch))
+    return fail(CAKE_B200_EINVAL, "cache_write takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
+  if (index_pos < 0 || index_pos > k->len[block_idx])
+    return fail(CAKE_B200_ESTATE, "block %d: index_pos %d is not within the cache's %d positions", block_idx, index_pos, k->len[block_idx]);
+  if ((long long)index_pos + seq > k->cap) return fail(CAKE_B200_ESTATE, "index_pos %d + seq %d exceeds cache capacity %d", index_pos, seq, k->cap);
+  RC(cache_ensure(k, block_idx));
+  const cake_b200_config &f = k->ctx->cfg;
+  pc::Write a{k->k[block_idx], k_dev, v_dev, (long long)k_tok, (long long)k_batch, (long long)v_tok, (long long)v_batch};
+  a.B = k->batch; a.S = seq; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(k->cap); a.pos0 = index_pos;
+  CU((cudaError_t)pc::write(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
+  k->len[block_idx] = index_pos + seq;
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int which, int first, int n, void *out_dev) {
+  RC(packed_call(k, block_idx, "cache_unpack"));
+  if (which != 0 && which != 1) return fail(CAKE_B200_EINVAL, "which is 0 (K) or 1 (V), not %d", which);
+  if (first < 0 || n < 1 || (long long)first + n > k->len[block_idx])
+    return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, first, n, k->len[block_idx]);
+  if (!out_dev || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "cache_unpack writes to a 16-byte boundary");
+  const cake_b200_config &f = k->ctx->cfg;
+  pc::Read a{k->k[block_idx], out_dev, k->batch, f.n_kv_heads, f.head_dim, pc::cap_blocks(k->cap), which, first, n, n};
+  CU((cudaError_t)pc::read(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
+  return CAKE_B200_OK;
+}
+// attention of S rows a batch row over a packed cache; the rows' own positions are in it
+static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, const void *q, size_t q_tok, size_t q_batch, void *out, int S, int pos0,
+                         int first, float scale, const int *d_pos = nullptr, int window = 0) {
+  const cake_b200_config &f = c->cfg;
+  pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, kc->batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
+  a.scale = scale; a.d_pos = d_pos; a.window = window;
+  CU((cudaError_t)pc::attend(c->stream, f.dtype, a, launch_counter(c)));
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq,
+                                      int index_pos, int first, float scale) {
+  RC(packed_call(k, block_idx, "cache_attend"));
+  if (!q_dev || !out_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
+  if (unaligned(q_dev, q_tok, q_batch) || unaligned(out_dev))
+    return fail(CAKE_B200_EINVAL, "cache_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
+  if (index_pos < 0 || (long long)index_pos + seq > k->len[block_idx])
+    return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, index_pos, seq, k->len[block_idx]);
+  if (first < 0 || !(scale >= 0.f && scale <= 3.402823466e38f)) return fail(CAKE_B200_EINVAL, "first %d or scale %g out of range", first, (double)scale);
+  return attend_packed(k->ctx, k, block_idx, q_dev, q_tok, q_batch, out_dev, seq, index_pos, first,
+                       scale > 0.f ? scale : (float)(1.0 / sqrt((double)k->ctx->cfg.head_dim)));
+}
+// a step's rows of a fused projection [tokens, heads + 2 kv heads, hd]: norms and rotation, q in place, k and v into the cache
+static int write_packed(cake_b200_ctx *c, const cake_b200_block *b, const cake_b200_cache *kc, int l, void *qkv, const void *qn, const void *kn, int S, int pos0,
+                        const int *d_pos = nullptr) {
+  const cake_b200_config &f = c->cfg;
+  char *p = (char *)qkv;
+  pc::Write a{kc->k[l], p + (size_t)f.n_heads * f.head_dim * c->es, p + (size_t)(f.n_heads + f.n_kv_heads) * f.head_dim * c->es, c->nqkv, (long long)S * c->nqkv,
+              c->nqkv, (long long)S * c->nqkv};
+  a.q = qkv; a.q_norm = qn; a.k_norm = kn; a.n_q = f.n_heads; a.rot = c->rot; a.eps = f.rms_eps; a.d_pos = d_pos;
+  if (b->use_rope && c->rot > 0) { a.cos_t = c->cos_t; a.sin_t = c->sin_t; }
+  a.B = kc->batch; a.S = S; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(kc->cap); a.pos0 = pos0;
+  CU((cudaError_t)pc::write(c->stream, f.dtype, a, launch_counter(c)));
+  return CAKE_B200_OK;
+}
+static int fill_packed(cake_b200_cache *k, int l, int len, uint32_t seed) {
+  cake_b200_ctx *c = k->ctx;
+  const cake_b200_config &f = c->cfg;
+  const long long row = (long long)f.n_kv_heads * f.head_dim;
+  const size_t n = (size_t)k->batch * len * row;
+  uint16_t *rows = nullptr;
+  CU(cudaMalloc(&rows, 2 * n * sizeof(uint16_t)));
+  int rc = DISPATCH_T(f.dtype, T_LAMBDA {
+    typedef typename decltype(tag_)::type T;
+    fill_synth_kernel<T><<<1024, 256, 0, c->stream>>>((T *)rows, n, seed + 2 * l, 1.0f);
+    fill_synth_kernel<T><<<1024, 256, 0, c->stream>>>((T *)rows + n, n, seed + 2 * l + 1, 1.0f);
+    return CAKE_B200_OK;
+  });
+  pc::Write a{k->k[l], rows, rows + n, row, len * row, row, len * row};
+  a.B = k->batch; a.S = len; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(k->cap); a.pos0 = 0;
+  cudaError_t e = (cudaError_t)pc::write(c->stream, f.dtype, a, launch_counter(c));
+  if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  cudaFree(rows);
+  if (e != cudaSuccess) rc = fail(CAKE_B200_ECUDA, "cache_fill_synthetic: %s", cudaGetErrorString(e));
+  return rc;
 }
 extern "C" int cake_b200_cache_fill_synthetic(cake_b200_cache *k, const int *block_idx, int n_blocks, int len,
                                               uint32_t seed) {
@@ -1020,6 +1144,11 @@ extern "C" int cake_b200_cache_fill_synthetic(cake_b200_cache *k, const int *blo
   for (int i = 0; i < n_blocks; i++) {
     const int l = block_idx[i];
     RC(cache_ensure(k, l));
+    if (k->bits) {
+      if (len) RC(fill_packed(k, l, len, seed));
+      k->len[l] = len;
+      continue;
+    }
     const size_t n = (size_t)k->batch * c->cfg.n_kv_heads * k->cap * c->cfg.head_dim;
     RC(DISPATCH_T(c->cfg.dtype, T_LAMBDA {
       typedef typename decltype(tag_)::type T;
@@ -1045,6 +1174,10 @@ static int enqueue_qkv(cake_b200_ctx *c, const cake_b200_block *b, const void *x
 static int enqueue_attn(cake_b200_ctx *c, const cake_b200_block *b, cake_b200_cache *kc, int l) {
   // qk-norm, RoPE, KV append, GQA attention                        attention.rs:202-346, cache.rs:184-210
   const cake_b200_config &f = c->cfg;
+  if (kc->bits) {
+    RC(write_packed(c, b, kc, l, c->qkv, b->qn, b->kn, 1, 0, kc->d_pos));
+    return attend_packed(c, kc, l, c->qkv, c->nqkv, c->nqkv, c->y, 1, 0, 0, (float)(1.0 / sqrt((double)f.head_dim)), kc->d_pos, f.sliding_window);
+  }
   AttnDecodeArgs a{};
   a.qkv = c->qkv; a.kcache = kc->k[l]; a.vcache = kc->v[l]; a.cos_t = c->cos_t; a.sin_t = c->sin_t;
   a.q_norm = b->qn; a.k_norm = b->kn; a.y = c->y; a.ws_ml = c->ws_ml; a.ws_acc = c->ws_acc;
@@ -1128,7 +1261,7 @@ struct MkPlan {
 // intermediate size above 71000).  Without layers only the head's sizes count.  The ranks of a sharded model have to agree: see decode_build.
 static bool plan_mega(const cake_b200_ctx *c, const cake_b200_cache *kc, int n_layers, bool with_head, MkPlan *p) {
   const cake_b200_config &f = c->cfg;
-  if (!c->use_mega || f.layer_list) return false;
+  if (!c->use_mega || f.layer_list || (kc && kc->bits)) return false;
   const int G = f.n_heads / f.n_kv_heads;
   if (!mk_kernel(f.dtype, f.head_dim, G)) return false;
   MkArgs &a = p->a;
@@ -1575,6 +1708,10 @@ static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *bloc
         qn = kn = nullptr;
       }
       const int rope_on = b->use_rope ? 1 : 0;
+      if (kc->bits) {
+        RC(write_packed(c, b, kc, l, c->pf_qkv, qn, kn, S, pos0));
+        RC(attend_packed(c, kc, l, c->pf_qkv, c->nqkv, (size_t)S * c->nqkv, c->pf_y, S, pos0, ws, (float)(1.0 / sqrt((double)hd))));
+      } else {
       {
         const long items = (long)M * (f.n_heads + 2 * f.n_kv_heads);
         if (hd == 128 && c->rot == 128 && ((uintptr_t)c->cos_t & 3) == 0) {  // full rotary on 128-wide heads: token-per-warp vector kernel
@@ -1626,6 +1763,7 @@ static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *bloc
         RC(launch_pdl(c, attn_prefill_v0_kernel<T>, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, (const T *)c->pf_qkv,
                       (const T *)kc->k[l] + wsoff, (const T *)kc->v[l] + wsoff, (T *)c->pf_y, B, S, f.n_heads, f.n_kv_heads, hd, kc->cap,
                       apos0, (float)(1.0 / sqrt((double)hd))));
+      }
       }
       if (b->pan) {  // olmo2/block.rs:77-79, gemma3/block.rs:120-122: x1 = x + rms_norm(o_proj(y))  (pf_h is free again here)
         if (use_tc && tc_gemm_ok(M, H, sq)) RC((gemm_tc_T<T, TCE_PLAIN>(c, c->pf_y, b->wo, nullptr, nullptr, c->pf_h, M, H, sq)));

@@ -1,0 +1,79 @@
+// packed_cache.cuh — a session's K and V rows in four bits (cake_b200_cache_create_packed): the format, and the launch interface of the
+// kernels in packed_cache.cu that write rows, read them back and attend over them.
+//
+// Format.  A row of hd entries (K: after norm and rotation) is cut into hd / 32 groups of neighbours.  With lo = min x (a D number) and step the
+// smallest D number that is not below (max x - lo) / 15 (D = bf16: and not below 2^-126 where the span is not 0), entry x is held as
+// n = floor((x - lo) / step + 1/2), 0 <= n <= 15, and stands for lo + step n.  A pair (step, lo) in D and 32 codes are 20 bytes for 32 entries.
+// step is rounded up so that 15 steps reach the maximum; lo and step are D numbers, so that n step and the codes' distances to their borders are
+// exact in fp32.  A group whose span is not finite (an infinity, a NaN) has the pair (NaN, NaN): all of it reads as NaN.
+//
+// Place.  16 positions of one (batch row, key head) are one block of 20 hd bytes: K's codes, K's pairs, V's codes, V's pairs; the blocks of a
+// (batch row, key head) follow one another, so that keys and values of a range of positions are one piece of memory.  Inside a block the
+// codes lie as the m16n8k16 products of the attention take them, a lane's codes side by side (lane = 4 g + t holds rows g and g + 8 and
+// columns 2t, 2t + 1, 2t + 8, 2t + 9 of an operand); 8 codes are a 32-bit word:
+//   K, position r:  word t hd/32 + j of the row holds entries 32 j + 8 t .. + 7; nibble i entry 2 i, nibble 4 + i entry 2 i + 1
+//   V, position r:  lane 4 g + (r & 7) / 2, slot (r & 1) + 2 (r >> 3): word w of the slot holds entries 64 w + 4 g .. + 3 (nibbles 0 .. 3) and
+//                   64 w + 32 + 4 g .. + 3 (nibbles 4 .. 7); a lane's words slot by slot, in pieces of 16 bytes, the pieces of all lanes side by side
+//   pairs:          word r hd/32 + j: step in the low half, lo in the high half
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace cake {
+namespace pc {
+
+constexpr int GROUP = 32, BLOCK = 16;   // entries of a pair; positions of a block
+__host__ __device__ constexpr int block_bytes(int hd) { return 20 * hd; }
+__host__ __device__ constexpr int k_pairs(int hd) { return 8 * hd; }        // byte offsets inside a block
+__host__ __device__ constexpr int v_codes(int hd) { return 10 * hd; }
+__host__ __device__ constexpr int v_pairs(int hd) { return 18 * hd; }
+// word (of the block's K or V codes) that holds entries 8u .. 8u + 7 of K's position r
+__host__ __device__ constexpr int k_word(int hd, int r, int u) { return r * (hd / 8) + (u & 3) * (hd / 32) + (u >> 2); }
+// and the one that holds entries 64 w + 4 g .. and 64 w + 32 + 4 g .. of V's position r
+__host__ __device__ constexpr int v_word(int hd, int r, int g, int w) {
+  const int lane = 4 * g + ((r & 7) >> 1), idx = ((r & 1) + 2 * (r >> 3)) * (hd / 64) + w;
+  return ((idx >> 2) * 32 + lane) * 4 + (idx & 3);
+}
+inline int cap_blocks(int cap) { return (cap + 63) / 64 * 4; }   // whole tiles of 64 positions
+inline bool head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
+
+// dtype codes are those of include/cake_b200.h (0 bf16, 1 f16).  Every function returns a cudaError_t cast to int and adds its launches to *launches.
+
+// Rows of a step join the cache.  In a block: of a fused projection [tokens, n_q + 2 n_kv heads, hd], q and k heads are normed (q_norm, k_norm)
+// and rotated (cos_t), q in place; by itself (n_q == 0): k and v as they are.
+struct Write {
+  void *cache;
+  const void *k, *v;             // rows of head 0, 16-byte aligned
+  long long k_tok, k_batch, v_tok, v_batch;   // strides in elements, multiples of 8; heads lie side by side
+  void *q = nullptr;             // [n_q heads] of a token, strides as k's
+  const void *cos_t = nullptr, *sin_t = nullptr, *q_norm = nullptr, *k_norm = nullptr;
+  int B, S, n_q = 0, n_kv, hd, rot = 0, blocks, pos0;   // blocks: of a (batch row, head)
+  const int *d_pos = nullptr;    // the position on the device instead of pos0
+  float eps = 0.f;
+};
+int write(cudaStream_t, int dtype, const Write &, uint64_t *launches);
+
+// positions [first, first + n) of K (which 0) or V (1) -> out [B, n_kv, n, hd] in D, a (batch row, head) every out_rows rows
+struct Read {
+  const void *cache;
+  void *out;
+  int B, n_kv, hd, blocks, which, first, n;
+  long long out_rows;
+};
+int read(cudaStream_t, int dtype, const Read &, uint64_t *launches);
+
+// Row t of S (position pos0 + t) of q attends to the positions first <= j <= pos0 + t; a row without any is zero.
+struct Attend {
+  const void *cache, *q;         // q: heads side by side, 16-byte aligned
+  long long q_tok, q_batch;      // strides in elements, multiples of 8
+  void *out;                     // [B, S, n_heads, hd] D
+  int B, S, n_heads, n_kv, hd, blocks, pos0, first;
+  const int *d_pos = nullptr;    // S == 1: the position on the device instead of pos0; first = max(0, position + 1 - window) with window > 0
+  int window = 0;
+  float scale;
+};
+int attend(cudaStream_t, int dtype, const Attend &, uint64_t *launches);
+
+}  // namespace pc
+}  // namespace cake
