@@ -148,6 +148,9 @@ struct cake_b200_ctx {
   void *pf_h = nullptr, *pf_qkv = nullptr, *pf_y = nullptr, *pf_x1 = nullptr, *pf_gu = nullptr, *pf_mm = nullptr;
   void *io_x = nullptr;
   size_t io_x_cap = 0;
+  // attention over caches in four bits: sums of keys cut over several CTAs, CTAs that have come
+  float *pc_ws = nullptr;
+  unsigned *pc_tickets = nullptr;
   // head of a batch: its logits where the caller keeps none, its tokens
   void *hd_logits = nullptr;
   size_t hd_logits_rows = 0;
@@ -655,7 +658,8 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
                   c->ws_acc, c->part_val, c->part_idx, c->d_step, c->attn_counters, c->argmax_counter, c->d_token,
                   c->token_ring, c->d_ids, c->d_pen, c->pf_h, c->pf_qkv, c->pf_y, c->pf_x1, c->pf_gu, c->pf_mm, c->io_x,
                   c->gbar, c->mk_pk, c->mk_part, c->mk_tab_dev, c->g_tab_dev, c->tickets, c->ring_seq, c->inbox, c->step_trace, c->trace,
-                  c->samp_p, c->samp_noise, c->hd_logits, c->hd_tokens, c->x0, c->sp_h, c->sp_hs, c->sp_in, c->sp_a, c->sp_hn, c->sp_logits, c->sp_rows_idx, c->mx_ws};
+                  c->samp_p, c->samp_noise, c->hd_logits, c->hd_tokens, c->x0, c->sp_h, c->sp_hs, c->sp_in, c->sp_a, c->sp_hn, c->sp_logits, c->sp_rows_idx, c->mx_ws,
+                  c->pc_ws, c->pc_tickets};
   for (void *b : bufs)
     if (b) cudaFree(b);
   if (c->bigram) cudaFree(c->bigram);
@@ -942,6 +946,18 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
   if (c->cfg.layer_list) return fail(CAKE_B200_EINVAL, "packed caches are for the Llama-family blocks");
   if (!pc::head_dim_ok(c->cfg.head_dim)) return fail(CAKE_B200_EINVAL, "packed caches hold heads of 64, 128 or 256 entries, not %d", c->cfg.head_dim);
   if (c->rot % 16) return fail(CAKE_B200_EINVAL, "packed caches rotate multiples of 16 entries of a head, not %d", c->rot);
+  if (batch < 1 || max_seq < 1) return fail(CAKE_B200_EINVAL, "bad cache arguments");
+  CU(cudaSetDevice(c->device));
+  if (!c->pc_tickets) {
+    CU((cudaError_t)pc::prepare(c->cfg.dtype, c->cfg.head_dim));
+    if (!c->pc_ws) CU(cudaMalloc(&c->pc_ws, pc::scratch_floats(c->sm_count) * sizeof(float)));
+    const size_t n = pc::scratch_tickets(c->sm_count) * sizeof(unsigned);
+    unsigned *tickets = nullptr;
+    CU(cudaMalloc(&tickets, n));
+    const cudaError_t e = cudaMemsetAsync(tickets, 0, n, c->stream);
+    if (e != cudaSuccess) { cudaFree(tickets); return fail(CAKE_B200_ECUDA, "cache_create: %s", cudaGetErrorString(e)); }
+    c->pc_tickets = tickets;
+  }
   return cache_create(c, batch, max_seq, bits, out);
 }
 static int cache_ensure(cake_b200_cache *k, int layer) {
@@ -1085,7 +1101,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
   const cake_b200_config &f = c->cfg;
   pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, kc->batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
   a.scale = scale; a.d_pos = d_pos; a.window = window;
-  CU((cudaError_t)pc::attend(c->stream, f.dtype, a, launch_counter(c)));
+  CU((cudaError_t)pc::attend(c->stream, f.dtype, a, pc::Scratch{c->pc_ws, c->pc_tickets, c->wait_err, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq,

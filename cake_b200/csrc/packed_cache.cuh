@@ -73,7 +73,17 @@ struct Attend {
   int window = 0;
   float scale;
 };
-int attend(cudaStream_t, int dtype, const Attend &, uint64_t *launches);
+// what the calls of one stream share: sums of keys cut over several CTAs, and how many of them have come (all zero between calls)
+struct Scratch {
+  float *ws;          // scratch_floats
+  unsigned *tickets;  // scratch_tickets
+  int *err;           // set by a kernel that gave up a bounded wait: its results are none
+  int sms;
+};
+size_t scratch_floats(int sms);
+size_t scratch_tickets(int sms);
+int prepare(int dtype, int hd);   // once per device and kind of cache, in front of the first call
+int attend(cudaStream_t, int dtype, const Attend &, const Scratch &, uint64_t *launches);
 
 }  // namespace pc
 }  // namespace cake

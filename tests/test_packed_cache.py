@@ -35,7 +35,8 @@ def stands_for(x):
 
 
 def attention(q, k, v, at, first, scale):
-    """q [b, s, heads, hd], k, v [b, n, kv, hd] in 64 bits -> (out, sum p |v|, largest sum |q||k| * scale of a row's seen keys)."""
+    """q [b, s, heads, hd], k, v [b, n, kv, hd] in 64 bits -> (out, sum p |v|, largest sum |q||k| * scale of a row's seen keys, largest |v| of an
+    entry's group that any row sees)."""
     b, s, heads, hd = q.shape
     n, G = k.shape[1], heads // k.shape[2]
     k, v = (t.repeat_interleave(G, 2).transpose(1, 2) for t in (k, v))
@@ -49,18 +50,23 @@ def attention(q, k, v, at, first, scale):
     p[:, :, some] = torch.softmax(sc[:, :, some], -1)
     mag = torch.where(seen, (q.abs() @ torch.nan_to_num(k, nan=0.0).abs().transpose(2, 3)) * scale, 0.0).amax(-1, keepdim=True)
     v = torch.nan_to_num(v, nan=0.0)
-    return (p @ v).transpose(1, 2), (p @ v.abs()).transpose(1, 2), mag.transpose(1, 2)
+    big = torch.where(((torch.arange(n) >= first) & (torch.arange(n) < at + s))[:, None], v.abs(), 0.0).amax(2, keepdim=True)
+    big = big.unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, -1, -1, 32).flatten(-2)
+    return (p @ v).transpose(1, 2), (p @ v.abs()).transpose(1, 2), mag.transpose(1, 2), big.transpose(1, 2)
 
 
 def check_attention(got, q, kx, vx, at, first, dtype, scale=None):
     """kx, vx: the rows written [b, n, kv, hd] in D.  Three things round: the held entries to D where a product takes them so (half a step each; of a
-    score that is at most h mag, which changes a weight by e^(2 h mag)), a weight to D's half step or finer, and the result; the sums are fp32."""
+    score that is at most h mag, which changes a weight by e^(2 h mag)), a weight to D's half step or finer, and the result.  The sums are fp32.  Where
+    a value is summed as p step (n - 8) and p (lo + 8 step), a sum that comes to nothing still has terms: with V the largest entry of the group, 8 step <= 1.08 V
+    (the span is at most 2 V) and |lo + 8 step| <= 1.07 V + step / 2, 2.3 V together, over at most 100 additions one behind the other of 2^-24 each (16 in a
+    product, one per block of a warp, the warps, the CTAs): 230 * 2^-24 V < 2^-16 V."""
     h = HALF[dtype]
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    ref, mass, mag = attention(q.double().cpu(), stands_for(kx).cpu(), stands_for(vx).cpu(), at, first, scale)
+    ref, mass, mag, big = attention(q.double().cpu(), stands_for(kx).cpu(), stands_for(vx).cpu(), at, first, scale)
     got = got.double().cpu()
     ds = mag * (h + 2.0 ** -16) + 1e-5
-    bound = 1.01 * h * ref.abs() + mass * (torch.expm1(2 * ds) + 2 * h + 1e-5) + 2.0 ** -24
+    bound = 1.01 * h * ref.abs() + mass * (torch.expm1(2 * ds) + 2 * h + 1e-5) + 2.0 ** -16 * big + 2.0 ** -24
     assert torch.isfinite(got).all()
     err = (got - ref).abs()
     assert (err <= bound).all(), float((err / bound).max())
@@ -294,6 +300,13 @@ def test_what_no_row_sees_may_be_anything(hd, s):
         got = cache.attend(0, q, at, first=first)
         check_attention(got[:, :-1], q[:, :-1], k, v, at, first, "bf16")
         assert got[:, -1].isnan().all()
+    # large finite rows there leave the seen ones their precision
+    x = torch.full((1, n, 2, hd), 2.0 ** 100, dtype=torch.bfloat16, device="cuda") * torch.randn((1, n, 2, hd), device="cuda").bfloat16()
+    k, v = rows(1, n, 2, hd, "bf16", 1), rows(1, n, 2, hd, "bf16", 2)
+    for t in (k, v):
+        t[:, :first], t[:, at + s:] = x[:, :first], x[:, at + s:]
+    cache.write(0, k, v, 0)
+    check_attention(cache.attend(0, q, at, first=first), q, k, v, at, first, "bf16")
     # seen NaN: the entries of V's group, or the whole row for K
     v[:, at - 1, 0, 3] = torch.nan
     cache.write(0, k[:, :at], v[:, :at], 0)
