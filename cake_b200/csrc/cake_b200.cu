@@ -1101,7 +1101,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
   const cake_b200_config &f = c->cfg;
   pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, kc->batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
   a.scale = scale; a.d_pos = d_pos; a.window = window;
-  CU((cudaError_t)pc::attend(c->stream, f.dtype, a, pc::Scratch{c->pc_ws, c->pc_tickets, c->wait_err, c->sm_count}, launch_counter(c)));
+  CU((cudaError_t)pc::attend(c->stream, f.dtype, a, pc::Scratch{c->pc_ws, c->pc_tickets, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq,

@@ -12,9 +12,9 @@
 // codes lie as the m16n8k16 products of the attention take them, a lane's codes side by side (lane = 4 g + t holds rows g and g + 8 and
 // columns 2t, 2t + 1, 2t + 8, 2t + 9 of an operand); 8 codes are a 32-bit word:
 //   K, position r:  word t hd/32 + j of the row holds entries 32 j + 8 t .. + 7; nibble i entry 2 i, nibble 4 + i entry 2 i + 1
-//   V, position r:  lane 4 g + (r & 7) / 2, slot (r & 1) + 2 (r >> 3): word w of the slot holds entries 64 w + 4 g .. + 3 (nibbles 0 .. 3) and
-//                   64 w + 32 + 4 g .. + 3 (nibbles 4 .. 7); a lane's words slot by slot, in pieces of 16 bytes, the pieces of all lanes side by side
-//   pairs:          word r hd/32 + j: step in the low half, lo in the high half
+//   V, positions r and r + 1 (r even): lane 4 g + (r & 7) / 2 has a word for every group j, r >> 3 and r's neighbour: entries 32 j + 4 g .. + 3 of r in
+//                   nibbles 0 .. 3 and of r + 1 in nibbles 4 .. 7; a lane's words lie in pieces of 16 bytes, the pieces of all lanes side by side
+//   pairs:          a row's even groups, then its odd ones: word r hd/32 + (j & 1) hd/64 + j / 2, step in the low half, lo in the high half
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -30,11 +30,12 @@ __host__ __device__ constexpr int v_codes(int hd) { return 10 * hd; }
 __host__ __device__ constexpr int v_pairs(int hd) { return 18 * hd; }
 // word (of the block's K or V codes) that holds entries 8u .. 8u + 7 of K's position r
 __host__ __device__ constexpr int k_word(int hd, int r, int u) { return r * (hd / 8) + (u & 3) * (hd / 32) + (u >> 2); }
-// and the one that holds entries 64 w + 4 g .. and 64 w + 32 + 4 g .. of V's position r
-__host__ __device__ constexpr int v_word(int hd, int r, int g, int w) {
-  const int lane = 4 * g + ((r & 7) >> 1), idx = ((r & 1) + 2 * (r >> 3)) * (hd / 64) + w;
-  return ((idx >> 2) * 32 + lane) * 4 + (idx & 3);
+// 16-bit half of V's codes that holds entries 32 j + 4 g .. + 3 of position r
+__host__ __device__ constexpr int v_half(int hd, int r, int g, int j) {
+  const int lane = 4 * g + ((r & 7) >> 1), idx = (r >> 3) * (hd / 32) + j;
+  return (((idx >> 2) * 32 + lane) * 4 + (idx & 3)) * 2 + (r & 1);
 }
+__host__ __device__ constexpr int pair_word(int hd, int r, int j) { return r * (hd / 32) + (j & 1) * (hd / 64) + (j >> 1); }   // group j of position r
 inline int cap_blocks(int cap) { return (cap + 63) / 64 * 4; }   // whole tiles of 64 positions
 inline bool head_dim_ok(int hd) { return hd == 64 || hd == 128 || hd == 256; }
 
@@ -77,7 +78,6 @@ struct Attend {
 struct Scratch {
   float *ws;          // scratch_floats
   unsigned *tickets;  // scratch_tickets
-  int *err;           // set by a kernel that gave up a bounded wait: its results are none
   int sms;
 };
 size_t scratch_floats(int sms);

@@ -117,15 +117,17 @@ def test_every_word_of_a_block_has_its_own_place(tmp_path):
 using namespace cake::pc;
 int main() {
   for (int hd : {64, 128, 256}) {
-    std::set<int> k, v;
+    std::set<int> k, v, p;
     for (int r = 0; r < BLOCK; r++) {
       for (int u = 0; u < hd / 8; u++) k.insert(k_word(hd, r, u));
       for (int g = 0; g < 8; g++)
-        for (int w = 0; w < hd / 64; w++) v.insert(v_word(hd, r, g, w));
+        for (int j = 0; j < hd / 32; j++) v.insert(v_half(hd, r, g, j));
+      for (int j = 0; j < hd / 32; j++) p.insert(pair_word(hd, r, j));
     }
     const int words = BLOCK * hd / 8;
     if ((int)k.size() != words || *k.begin() != 0 || *k.rbegin() != words - 1) return 1;
-    if ((int)v.size() != words || *v.begin() != 0 || *v.rbegin() != words - 1) return 2;
+    if ((int)v.size() != 2 * words || *v.begin() != 0 || *v.rbegin() != 2 * words - 1) return 2;
+    if ((int)p.size() != BLOCK * hd / 32 || *p.begin() != 0 || *p.rbegin() != BLOCK * hd / 32 - 1) return 6;
     const int codes = 4 * words, pairs = 4 * BLOCK * hd / GROUP;
     if (k_pairs(hd) != codes || v_codes(hd) != codes + pairs || v_pairs(hd) != 2 * codes + pairs || block_bytes(hd) != 2 * (codes + pairs)) return 3;
     if (block_bytes(hd) % 16) return 4;
