@@ -99,12 +99,38 @@ __device__ __forceinline__ void ft_drain(uint64_t *bars, int warp, int lane, int
 // all of them (a step of one token has G rows, not one) and a tile of a causal prompt spans 128 / G tokens: less of its last key
 // tiles is masked.  `splits` CTAs of a cluster cut the tile's keys between them where tiles alone don't fill the chip (few rows on a
 // long context); each finishes 128 / splits of the columns, with the partial sums and the running maxima exchanged over the cluster.
+//
+// Keys and values that come out of a packed cache as operands (packed_cache.cuh, Read::nan): a product with a weight of zero is NaN where the value is, so
+// such values are zero there and marked: word [slab][block of 16 positions], byte 0 the first position in the block whose key is NaN, byte 1 + j
+// that of the values' 32-entry group j, 255 none.  The blocks begin `off` positions in front of key 0.
+struct NanMarks {
+  const unsigned long long *words;  // nullptr: none
+  int blocks, off;
+};
+// bit j: group j of a row's result is NaN, the row's position (as the keys count) being pos.  Called by whole warps.
+template <int NG> __device__ __forceinline__ uint32_t nan_groups(const NanMarks &m, int slab, int pos, int lane) {
+  if (!m.words) return 0u;
+  const unsigned long long *w = m.words + (size_t)slab * m.blocks;
+  bool any = false;
+  for (int i = lane; i < m.blocks; i += 32) any = any || w[i] != ~0ull;
+  if (!__any_sync(0xffffffffu, any)) return 0u;
+  uint32_t bits = 0u;
+  for (int i = 0; i <= min((pos + m.off) >> 4, m.blocks - 1); i++) {
+    const unsigned long long v = w[i];
+    for (int c = 0; c <= NG; c++) {
+      const int at = (int)(v >> (8 * c) & 255u);
+      if (at != 255 && 16 * i + at <= pos + m.off) bits |= c ? 1u << (c - 1) : ~0u;
+    }
+  }
+  return bits;
+}
 struct FtParams {
   void *y;
   int S, n_heads, n_kv, pos0;
   int G, tpt, splits_log2;  // query heads per key head, tokens per tile
   float scale_log2, tau_log2;
   int *err;
+  NanMarks nan;  // keys and values expanded from a packed cache: what of them reads as NaN
 };
 
 // SPLIT: clusters that cut the keys; without it every CTA sees its rows' first key in its first tile.
@@ -327,13 +353,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   }
   // ---- epilogue: O / l, one rounding to D (attention.rs:346), store (b, s, h, hd) ---------------------------
   T *dst = reinterpret_cast<T *>(p.y) + ((size_t)(b * S + t0 + tok) * p.n_heads + kvh * G + row - tok * G) * FT_HD;
+  const uint32_t nan = warp < 4 ? nan_groups<FT_HD / 32>(p.nan, b * p.n_kv + kvh, pos0 + t0 + tok, lane) : 0u;  // of the row's 32-entry groups
   if (!SPLIT) {
     if (busy) {
-      const float inv = 1.0f / l_run;
+      const float inv_l = 1.0f / l_run;
 #pragma unroll 1
       for (int c0 = 0; c0 < FT_HD; c0 += 32) {
         uint32_t r[32];
         tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+        const float inv = nan >> (c0 / 32) & 1u ? __uint_as_float(0x7fffffffu) : inv_l;
         if (row < rows) {
           uint32_t o[16];
 #pragma unroll
@@ -392,7 +420,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       for (int c0 = 0; c0 < share; c0 += 8) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.f;
+        for (int i = 0; i < 8; i++) v[i] = nan >> ((rank * share + c0) / 32) & 1u ? __uint_as_float(0x7fffffffu) : 0.f;
         for (int q = 0; q < sp; q++)
 #pragma unroll
           for (int i = 0; i < 8; i++) v[i] += mine[(size_t)(q * share + c0 + i) * FT_BM];

@@ -61,6 +61,7 @@ static int fail(int code, const char *fmt, ...) {
   } while (0)
 
 struct cake_b200_ctx;
+static int round_up(int v, int m);
 static int wait_loads(cake_b200_ctx *c);
 static int check_waits(cake_b200_ctx *c);
 static int sync_results(cake_b200_ctx *c);
@@ -150,6 +151,8 @@ struct cake_b200_ctx {
   size_t io_x_cap = 0;
   // attention over caches in four bits: sums of keys cut over several CTAs, CTAs that have come
   float *pc_ws = nullptr;
+  void *pc_rows = nullptr;   // rows of such caches in D, for the kernels of prompts
+  size_t pc_rows_cap = 0;
   unsigned *pc_tickets = nullptr;
   // head of a batch: its logits where the caller keeps none, its tokens
   void *hd_logits = nullptr;
@@ -659,7 +662,7 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
                   c->token_ring, c->d_ids, c->d_pen, c->pf_h, c->pf_qkv, c->pf_y, c->pf_x1, c->pf_gu, c->pf_mm, c->io_x,
                   c->gbar, c->mk_pk, c->mk_part, c->mk_tab_dev, c->g_tab_dev, c->tickets, c->ring_seq, c->inbox, c->step_trace, c->trace,
                   c->samp_p, c->samp_noise, c->hd_logits, c->hd_tokens, c->x0, c->sp_h, c->sp_hs, c->sp_in, c->sp_a, c->sp_hn, c->sp_logits, c->sp_rows_idx, c->mx_ws,
-                  c->pc_ws, c->pc_tickets};
+                  c->pc_ws, c->pc_tickets, c->pc_rows};
   for (void *b : bufs)
     if (b) cudaFree(b);
   if (c->bigram) cudaFree(c->bigram);
@@ -1091,16 +1094,50 @@ extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int whi
     return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, first, n, k->len[block_idx]);
   if (!out_dev || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "cache_unpack writes to a 16-byte boundary");
   const cake_b200_config &f = k->ctx->cfg;
-  pc::Read a{k->k[block_idx], out_dev, k->batch, f.n_kv_heads, f.head_dim, pc::cap_blocks(k->cap), which, first, n, n};
+  pc::Read a{k->k[block_idx], which ? nullptr : out_dev, which ? out_dev : nullptr, k->batch, f.n_kv_heads, f.head_dim, pc::cap_blocks(k->cap), first, n, n};
   CU((cudaError_t)pc::read(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
   return CAKE_B200_OK;
 }
-// attention of S rows a batch row over a packed cache; the rows' own positions are in it
+template <typename T>
+static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_t q_batch, const void *k, const void *v, int cap, void *y, int B, int S, int pos0,
+                            float sc, const NanMarks &nan);
+// Attention of S rows a batch row over a packed cache; the rows' own positions are in it.  Many rows of heads of 128 entries take the kernel of
+// prompts, whose operands are rows in D: the keys and values that the call sees are expanded once (each entry rounded to D) into memory of the ctx, which
+// grows on first use; above PC_EXPAND_MOST a few batch rows at a time.  (Heads of 64: their prompt kernel, on mma.sync, does not cut the keys: 1024 rows of
+// 8 / 2 heads at 2000 positions 190 us, 58 on codes.)
+constexpr size_t PC_EXPAND_MOST = (size_t)1 << 30;
 static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, const void *q, size_t q_tok, size_t q_batch, void *out, int S, int pos0,
                          int first, float scale, const int *d_pos = nullptr, int window = 0) {
   const cake_b200_config &f = c->cfg;
   pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, kc->batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
   a.scale = scale; a.d_pos = d_pos; a.window = window;
+  const bool strides = q_tok > 0 && (q_batch > 0 || kc->batch == 1);   // (a tensor map has none of zero)
+  if (!d_pos && first <= pos0 && strides && pc::many_rows(a, c->sm_count)) {
+    const int hd = f.head_dim, n = pos0 + S - first, cap = round_up(n, 64), blocks = pc::read_blocks(first, n);
+    const size_t slab = (size_t)f.n_kv_heads * cap * hd * c->es, marks = (size_t)f.n_kv_heads * blocks * 8;   // of a batch row
+    const int group = (int)std::max<size_t>(1, std::min<size_t>(kc->batch, PC_EXPAND_MOST / (2 * slab)));
+    const size_t need = group * (2 * slab + marks);
+    if (need > c->pc_rows_cap) {
+      CU(cudaStreamSynchronize(c->stream));
+      if (c->pc_rows) { cudaFree(c->pc_rows); c->pc_rows = nullptr; c->pc_rows_cap = 0; }
+      CU(cudaMalloc(&c->pc_rows, need));
+      c->pc_rows_cap = need;
+    }
+    for (int b0 = 0; b0 < kc->batch; b0 += group) {
+      const int nb = std::min(group, kc->batch - b0);
+      char *kr = (char *)c->pc_rows, *vr = kr + group * slab;
+      unsigned long long *nan = (unsigned long long *)(vr + group * slab);
+      const char *from = (const char *)kc->k[l] + (size_t)b0 * f.n_kv_heads * a.blocks * pc::block_bytes(hd);
+      pc::Read r{from, kr, vr, nb, f.n_kv_heads, hd, a.blocks, first, n, cap, nan};
+      CU((cudaError_t)pc::read(c->stream, f.dtype, r, launch_counter(c)));
+      RC(DISPATCH_T(f.dtype, T_LAMBDA {
+        typedef typename decltype(tag_)::type T;
+        return prompt_attention<T>(c, (const T *)q + (size_t)b0 * q_batch, q_tok, kc->batch == 1 ? (size_t)S * q_tok : q_batch, kr, vr, cap,
+                                   (T *)out + (size_t)b0 * S * f.n_heads * hd, nb, S, pos0 - first, scale, NanMarks{nan, blocks, first & 15});
+      }));
+    }
+    return CAKE_B200_OK;
+  }
   CU((cudaError_t)pc::attend(c->stream, f.dtype, a, pc::Scratch{c->pc_ws, c->pc_tickets, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
@@ -1448,13 +1485,14 @@ static int make_tmap3(CUtensorMap *m, const void *ptr, uint64_t cols, uint64_t r
   return CAKE_B200_OK;
 }
 
-// the query heads of a fused projection [batch][seq][heads + 2 kv heads][hd] as a 4-D map with a (64 x G heads x tokens) box, 128-byte
-// swizzle: a tile's rows come out token by token, the G heads of one key head side by side; tokens past seq read as zeros
-static int make_tmap_q(CUtensorMap *m, const void *ptr, int hd, uint64_t heads, uint64_t seq, uint64_t batch, int dtype, uint32_t G, uint32_t tokens) {
+// query heads [batch][seq][heads][hd], side by side in a token whose rows lie tok (a batch row's batch_stride) elements apart, as those of a fused
+// projection do, as a 4-D map with a (64 x G heads x tokens) box, 128-byte swizzle: a tile's rows come out token by token, the G heads of one key
+// head side by side; tokens past seq read as zeros
+static int make_tmap_q(CUtensorMap *m, const void *ptr, int hd, uint64_t heads, uint64_t seq, uint64_t batch, uint64_t tok, uint64_t batch_stride, int dtype,
+                       uint32_t G, uint32_t tokens) {
   RC(tmap_init());
-  const uint64_t row = heads * (uint64_t)hd * 2;
   const cuuint64_t gdim[4] = {(cuuint64_t)hd, heads, seq, batch};
-  const cuuint64_t gstride[3] = {(cuuint64_t)hd * 2, row, row * seq};
+  const cuuint64_t gstride[3] = {(cuuint64_t)hd * 2, tok * 2, batch_stride * 2};
   const cuuint32_t box[4] = {64u, G, tokens, 1u};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = g_encode_tiled(m, dtype == CAKE_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
@@ -1680,6 +1718,31 @@ static int gemm_T(cake_b200_ctx *c, const void *A, const void *W, const void *bi
                     (T *)C, M, N, K);
 }
 
+// Attention of S rows a batch row on attn_prefill_tc_kernel (head_dim 128): q [B, S, heads, 128] (q_tok, q_batch: strides) over keys k, v [B, n_kv, cap, 128] in D;
+// row t, which key pos0 + t belongs to, sees the keys up to it.
+template <typename T>
+static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_t q_batch, const void *k, const void *v, int cap, void *y, int B, int S, int pos0,
+                            float sc, const NanMarks &nan) {
+  const cake_b200_config &f = c->cfg;
+  const int hd = f.head_dim;
+  static const float fa_tau = []() { const char *e = getenv("CAKE_B200_FA_TAU"); return e ? (float)atof(e) : 5.545f; }();
+  CUtensorMap mq, mk, mv;
+  const int G = f.n_heads / f.n_kv_heads, tpt = FT_BM / G;
+  RC(make_tmap_q(&mq, q, hd, (uint64_t)f.n_heads, (uint64_t)S, (uint64_t)B, q_tok, q_batch, f.dtype, (uint32_t)G, (uint32_t)tpt));
+  RC(make_tmap3(&mk, k, (uint64_t)hd, (uint64_t)hd, (uint64_t)(pos0 + S), (uint64_t)cap, (uint64_t)B * f.n_kv_heads, f.dtype, FT_BN));
+  RC(make_tmap3(&mv, v, (uint64_t)hd, (uint64_t)hd, (uint64_t)(pos0 + S), (uint64_t)cap, (uint64_t)B * f.n_kv_heads, f.dtype, FT_BN));
+  // keys cut between the CTAs of a cluster: as many as stay resident (two per SM), with at least three key tiles each
+  // (a prompt of 512 tokens: 14 us in one piece, 17 in two).  One-token steps of 16
+  // sequences at 1000 positions, 32 / 8 heads: 50 us as one row per tile, 32 x 16 CTAs; about 20 packed and cut in two
+  const int tiles = (S + tpt - 1) / tpt, key_tiles = (pos0 + S / 2 + FT_BN - 1) / FT_BN;  // (of an average tile)
+  int lg = 0;
+  while (lg < 3 && ((long)tiles * f.n_kv_heads * B << (lg + 1)) <= 2 * c->sm_count && key_tiles >= 6 << lg) lg++;
+  FtParams fp{y, S, f.n_heads, f.n_kv_heads, pos0, G, tpt, lg, sc * 1.4426950408889634f, fa_tau * 1.4426950408889634f, c->wait_err, nan};
+  const dim3 ga((unsigned)(tiles << lg), f.n_kv_heads, B), ta(FT_THREADS);
+  if (lg) return launch_cluster_pdl(c, attn_prefill_tc_kernel<T, true>, ga, ta, (size_t)FT_SMEM_BYTES, 1u << lg, mq, mk, mv, fp);
+  return launch_pdl(c, attn_prefill_tc_kernel<T, false>, ga, ta, (size_t)FT_SMEM_BYTES, mq, mk, mv, fp);
+}
+
 static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *blocks, const int *block_idx, int n,
                                   cake_b200_cache *kc, const void *x_in, void *x_out, int B, int S, int pos0) {
   const cake_b200_config &f = c->cfg;
@@ -1749,26 +1812,10 @@ static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *bloc
         const float sc = (float)(1.0 / sqrt((double)hd));
         // head_dim 128: tcgen05 flash attention (attn_prefill_tc.cuh); CAKE_B200_FA=mma keeps the mma.sync kernel (A/B aid)
         static const bool fa_mma = []() { const char *e = getenv("CAKE_B200_FA"); return e && !strcmp(e, "mma"); }();
-        static const float fa_tau = []() { const char *e = getenv("CAKE_B200_FA_TAU"); return e ? (float)atof(e) : 5.545f; }();
-        if (hd == 128 && !fa_mma) {
-          CUtensorMap mq, mk, mv;
-          const int G = f.n_heads / f.n_kv_heads, tpt = FT_BM / G;
-          RC(make_tmap_q(&mq, c->pf_qkv, hd, (uint64_t)(f.n_heads + 2 * f.n_kv_heads), (uint64_t)S, (uint64_t)B, f.dtype, (uint32_t)G, (uint32_t)tpt));
-          RC(make_tmap3(&mk, (const T *)kc->k[l] + wsoff, (uint64_t)hd, (uint64_t)hd, (uint64_t)(apos0 + S), (uint64_t)kc->cap,
-                        (uint64_t)B * f.n_kv_heads, f.dtype, FT_BN));
-          RC(make_tmap3(&mv, (const T *)kc->v[l] + wsoff, (uint64_t)hd, (uint64_t)hd, (uint64_t)(apos0 + S), (uint64_t)kc->cap,
-                        (uint64_t)B * f.n_kv_heads, f.dtype, FT_BN));
-          // keys cut between the CTAs of a cluster: as many as stay resident (two per SM), with at least three key tiles each
-          // (a prompt of 512 tokens: 14 us in one piece, 17 in two).  One-token steps of 16
-          // sequences at 1000 positions, 32 / 8 heads: 50 us as one row per tile, 32 x 16 CTAs; about 20 packed and cut in two
-          const int tiles = (S + tpt - 1) / tpt, key_tiles = (apos0 + S / 2 + FT_BN - 1) / FT_BN;  // (of an average tile)
-          int lg = 0;
-          while (lg < 3 && ((long)tiles * f.n_kv_heads * B << (lg + 1)) <= 2 * c->sm_count && key_tiles >= 6 << lg) lg++;
-          FtParams fp{c->pf_y, S, f.n_heads, f.n_kv_heads, apos0, G, tpt, lg, sc * 1.4426950408889634f, fa_tau * 1.4426950408889634f, c->wait_err};
-          const dim3 ga((unsigned)(tiles << lg), f.n_kv_heads, B), ta(FT_THREADS);
-          if (lg) RC(launch_cluster_pdl(c, attn_prefill_tc_kernel<T, true>, ga, ta, (size_t)FT_SMEM_BYTES, 1u << lg, mq, mk, mv, fp));
-          else RC(launch_pdl(c, attn_prefill_tc_kernel<T, false>, ga, ta, (size_t)FT_SMEM_BYTES, mq, mk, mv, fp));
-        } else if (hd == 128)
+        if (hd == 128 && !fa_mma)
+          RC(prompt_attention<T>(c, c->pf_qkv, c->nqkv, (size_t)S * c->nqkv, (const T *)kc->k[l] + wsoff, (const T *)kc->v[l] + wsoff, kc->cap, c->pf_y, B, S,
+                                 apos0, sc, NanMarks{}));
+        else if (hd == 128)
           RC(launch_pdl(c, attn_prefill_mma_kernel<T, 128>, grid, block, (size_t)4 * FA_BN * 128 * 2, (const T *)c->pf_qkv,
                         (const T *)kc->k[l] + wsoff, (const T *)kc->v[l] + wsoff, (T *)c->pf_y, S, f.n_heads, f.n_kv_heads, kc->cap, apos0, sc));
         else

@@ -32,145 +32,347 @@ template <typename T> __device__ __forceinline__ T round_up(float f);
 template <> __device__ __forceinline__ __nv_bfloat16 round_up<__nv_bfloat16>(float f) { return __float2bfloat16_ru(f); }
 template <> __device__ __forceinline__ __half round_up<__half>(float f) { return __float2half_ru(f); }
 template <typename T> __device__ __forceinline__ uint32_t bits(T v) { return *reinterpret_cast<const uint16_t *>(&v); }
+template <typename T> __device__ __forceinline__ float2 open_pair(uint32_t p) { return DT<T>::unpack2(p); }   // (step, lo)
 
-// 8 entries of a group of four neighbouring lanes -> this lane's codes, entry i in nibble i, and the group's pair
-// t inv + 1/2 is exact but for 2^-22 relative, and (x - lo) / step is k + 1/2 or at least the last place of x, lo or step away from it (in
-// steps): 2^-19 decides the former and leaves the latter, where x's last place is above step 2^-19.
-template <typename T> __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t *pair) {
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+template <int N> __device__ __forceinline__ void lds_words(const void *p, uint32_t (&w)[N]) {   // in pieces of up to 16 bytes
+  if (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
+  else if (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x; w[1 % N] = v.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad = bad || x[i] != x[i];
+    for (int i = 0; i < N / 4; i++) {
+      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+      w[(4 * i) % N] = v.x; w[(4 * i + 1) % N] = v.y; w[(4 * i + 2) % N] = v.z; w[(4 * i + 3) % N] = v.w;
+    }
   }
-  if (bad) hi = INFINITY;
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  const float span = hi - lo;   // NaN or infinite: the group has no code
-  const bool fine = span <= 3.402823466e38f;
-  T st = round_up<T>(fine ? span / 15.f : 0.f);
-  if (sizeof(T) == 2 && DT<T>::to_f(st) < 1.17549435e-38f && span > 0.f) st = DT<T>::from_f(1.17549435e-38f);
-  const float step = DT<T>::to_f(st), inv = step > 0.f ? 1.f / step : 0.f;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float n = fmaf(x[i] - lo, inv, 0.5f + 1.9073486328125e-6f);
-    w |= (fine ? min(15u, (uint32_t)n) : 0u) << (4 * i);
-  }
-  *pair = fine ? bits(st) | bits(DT<T>::from_f(lo)) << 16 : 0x7fff7fffu;
-  return w;
 }
 
-// a warp takes 256 / HD rows, a lane 8 neighbouring entries
+
+// pairs of D in a word
+template <typename T> struct Two;
+template <> struct Two<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+template <> struct Two<__half> { typedef __half2 type; };
+template <typename T> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {   // NaN where either is
+  typedef typename Two<T>::type U;
+  const U r = __hmin2_nan(*reinterpret_cast<const U *>(&a), *reinterpret_cast<const U *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  typedef typename Two<T>::type U;
+  const U r = __hmax2_nan(*reinterpret_cast<const U *>(&a), *reinterpret_cast<const U *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <typename T> __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {   // one rounding
+  typedef typename Two<T>::type U;
+  const U r = __hfma2(*reinterpret_cast<const U *>(&a), *reinterpret_cast<const U *>(&b), *reinterpret_cast<const U *>(&c));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t c) {   // (as two constants the compiler takes two operations)
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(m), "r"(c));
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------ rows into the cache
+// Bound by memory: 16 bits read and 5 written an entry.  A warp takes 8 positions of one head, a lane (r, t) of them entries 32 j + 8 t .. + 7 of
+// position r for all groups j: that is K's words of the lane as the cache has them, so that codes leave as one piece of 16 bytes a lane (hd 128);
+// V's words take a 16-bit half from the neighbouring position's lane.  Minimum and maximum of a group are taken in pairs (D's own comparisons, which
+// keep a NaN), minimum and negated maximum together over its four lanes; each lane then has the division of one group in four.  A code is
+// fma, add with rounding down (the integer in the lowest bits) and a multiply-add that moves it to its place: n = floor((x - lo) / step + 1/2) exactly,
+// since (x - lo) inv is exact but for 2^-22 relative and (x - lo) / step is k + 1/2 or at least the last place of x, lo or step away from
+// it: 2^-19 decides the former and leaves the latter, where x's last place is above step 2^-19.
+// 8 x 4096 rows of 8 heads of 128, written and read back: a row per 16 lanes, V in 16-bit stores 102 + 71 us on the device; so 41 + 30.
+template <typename T, bool ODDS_LAST> __device__ __forceinline__ uint32_t encode8(const uint32_t (&c)[4], float lo, float inv) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 x = DT<T>::unpack2(c[i]);
+    const uint32_t a = __float_as_uint(__fadd_rd(fmaf(x.x - lo, inv, 0.5f + 1.9073486328125e-6f), 8388608.f));
+    const uint32_t b = __float_as_uint(__fadd_rd(fmaf(x.y - lo, inv, 0.5f + 1.9073486328125e-6f), 8388608.f));
+    w += a * (1u << (4 * (ODDS_LAST ? i : 2 * i)));
+    w += b * (1u << (4 * (ODDS_LAST ? 4 + i : 2 * i + 1)));
+  }
+  return w - 0xfb000000u;   // the exponents: 0x4b000000 (1 + 16 + 16^2 ..) mod 2^32
+}
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) write_kernel(const Write a) {
   pdl_launch_dependents();
-  pdl_wait();
-  constexpr int LPR = HD / 8;
-  const int lane = threadIdx.x & 31, u = lane % LPR;
+  constexpr int NG = HD / 32;
+  const int lane = threadIdx.x & 31, t = lane & 3;
   const int heads = a.n_q + 2 * a.n_kv;
-  const long long rows = (long long)a.B * a.S * heads;
-  const long long row = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * (32 / LPR) + lane / LPR;
-  const bool in = row < rows;
-  const long long at = in ? row : rows - 1;
-  const int head = (int)(at % heads), t = (int)(at / heads % a.S), b = (int)(at / heads / a.S);
-  const int pos = (a.d_pos ? *a.d_pos : a.pos0) + t;
+  pdl_wait();
+  const int pos0 = a.d_pos ? *a.d_pos : a.pos0, eights = ((pos0 & 7) + a.S + 7) >> 3;   // runs of 8 positions that the step touches
+  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5);   // (the rows that fit a GPU's memory are fewer)
+  if (item >= (unsigned)a.B * eights * heads) return;
+  const int head = (int)(item % heads), run = (int)(item / heads % eights), b = (int)(item / heads / eights);
+  const int pos = (pos0 & ~7) + 8 * run + (lane >> 2), tok = pos - pos0;
+  const bool in = tok >= 0 && tok < a.S;
   const bool is_q = head < a.n_q, is_v = head >= a.n_q + a.n_kv;
   const int h = is_q ? head : is_v ? head - a.n_q - a.n_kv : head - a.n_q;
-  const T *src = is_q ? reinterpret_cast<const T *>(a.q) + b * a.k_batch + t * a.k_tok
-                 : is_v ? reinterpret_cast<const T *>(a.v) + b * a.v_batch + t * a.v_tok : reinterpret_cast<const T *>(a.k) + b * a.k_batch + t * a.k_tok;
-  uint4 raw = *reinterpret_cast<const uint4 *>(src + (size_t)h * HD + 8 * u);
-  float x[8];
-  unpack8<T>(raw, x);
-  const T *nw = is_v ? nullptr : reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
-  float ss = 0.f;
+  const T *src = is_q ? reinterpret_cast<const T *>(a.q) + b * a.k_batch + tok * a.k_tok
+                 : is_v ? reinterpret_cast<const T *>(a.v) + b * a.v_batch + tok * a.v_tok : reinterpret_cast<const T *>(a.k) + b * a.k_batch + tok * a.k_tok;
+  src += (size_t)h * HD + 8 * t;
+  uint32_t c[NG][4];
 #pragma unroll
-  for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (nw) {
-    const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
-    float w[8];
-    unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * u), w);
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = rnd<T>(x[i] * inv * w[i]);
+  for (int j = 0; j < NG; j++) {
+    const uint4 v = in ? *reinterpret_cast<const uint4 *>(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+    c[j][0] = v.x; c[j][1] = v.y; c[j][2] = v.z; c[j][3] = v.w;
   }
-  if (a.cos_t) {   // pairs (i, i + rot / 2); rot is a multiple of 16: a lane's entries are all of one half
-    const int half = a.rot / 2, at8 = 8 * u;
-    const bool turned = !is_v && at8 < a.rot, low = at8 < half;
-    const int other = (lane & ~(LPR - 1)) + (turned ? (low ? u + half / 8 : u - half / 8) : u);
-    float y[8], c[8], s[8];
+  if (!is_v && (a.cos_t || a.q_norm || a.k_norm)) {   // (a warp's head is one)
+    const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
+    float inv = 0.f;
+    if (nw) {
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other);
-    if (turned) {
-      const size_t o = (size_t)pos * half + (low ? at8 : at8 - half);
-      unpack8<T>(*reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.cos_t) + o), c);
-      unpack8<T>(*reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.sin_t) + o), s);
+      for (int j = 0; j < NG; j++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = low ? rnd<T>(rnd<T>(x[i] * c[i]) - rnd<T>(y[i] * s[i])) : rnd<T>(rnd<T>(x[i] * c[i]) + rnd<T>(y[i] * s[i]));
+        for (int e = 0; e < 4; e++) {
+          const float2 x = DT<T>::unpack2(c[j][e]);
+          ss += x.x * x.x + x.y * x.y;
+        }
+      ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+      ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+      inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+    }
+    auto normed = [&](uint32_t (&x)[4], int at) {   // entries at .. at + 7 of the head
+      if (!nw) return;
+      const uint4 w = *reinterpret_cast<const uint4 *>(nw + at);
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float2 y = DT<T>::unpack2(x[e]), g = DT<T>::unpack2(ww[e]);
+        x[e] = pack2x<T>(y.x * inv * g.x, y.y * inv * g.y);
+      }
+    };
+    const int half = a.rot / 2;   // pairs (i, i + half), a multiple of 8: a lane's 8 entries are all of one half
+    // the other ones of the pairs: this lane's, or, where half is no whole number of groups, read again
+    const bool same = half == HD / 2;
+    uint32_t far[NG][4];
+    if (a.cos_t && !same)
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        const int at = 32 * j + 8 * t, other = at < half ? at + half : at - half;
+        const uint4 v = in && at < a.rot ? *reinterpret_cast<const uint4 *>(src - 8 * t + other) : make_uint4(0u, 0u, 0u, 0u);
+        far[j][0] = v.x; far[j][1] = v.y; far[j][2] = v.z; far[j][3] = v.w;
+        if (at < a.rot) normed(far[j], other);
+      }
+#pragma unroll
+    for (int j = 0; j < NG; j++) normed(c[j], 32 * j + 8 * t);
+    if (a.cos_t) {
+      auto turn = [&](uint32_t x, uint32_t y, uint32_t cw, uint32_t sw, bool low) {
+        const float2 xf = DT<T>::unpack2(x), yf = DT<T>::unpack2(y), cf = DT<T>::unpack2(cw), sf = DT<T>::unpack2(sw);
+        return low ? pack2x<T>(rnd<T>(xf.x * cf.x) - rnd<T>(yf.x * sf.x), rnd<T>(xf.y * cf.y) - rnd<T>(yf.y * sf.y))
+                   : pack2x<T>(rnd<T>(xf.x * cf.x) + rnd<T>(yf.x * sf.x), rnd<T>(xf.y * cf.y) + rnd<T>(yf.y * sf.y));
+      };
+      const T *cr = reinterpret_cast<const T *>(a.cos_t) + (size_t)(in ? pos : pos0) * half, *sr = reinterpret_cast<const T *>(a.sin_t) + (size_t)(in ? pos : pos0) * half;
+      if (same) {
+#pragma unroll
+        for (int j = 0; j < NG / 2; j++) {
+          const uint4 cv = *reinterpret_cast<const uint4 *>(cr + 32 * j + 8 * t), sv = *reinterpret_cast<const uint4 *>(sr + 32 * j + 8 * t);
+          const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t x = c[j][e], y = c[j + NG / 2][e];
+            c[j][e] = turn(x, y, cw[e], sw[e], true);
+            c[j + NG / 2][e] = turn(y, x, cw[e], sw[e], false);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+          const int at = 32 * j + 8 * t;
+          if (at < a.rot) {
+            const int o = at < half ? at : at - half;
+            const uint4 cv = *reinterpret_cast<const uint4 *>(cr + o), sv = *reinterpret_cast<const uint4 *>(sr + o);
+            const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[j][e] = turn(c[j][e], far[j][e], cw[e], sw[e], at < half);
+          }
+        }
+      }
+    }
+    if (is_q) {
+      __syncwarp();   // (every lane has read what it needs of the row)
+      if (in)
+#pragma unroll
+        for (int j = 0; j < NG; j++) *reinterpret_cast<uint4 *>(const_cast<T *>(src) + 32 * j) = make_uint4(c[j][0], c[j][1], c[j][2], c[j][3]);
     }
   }
-  uint32_t pair, w = encode8<T>(x, &pair);
-  if (is_q) {
-    if (in)
-      *reinterpret_cast<uint4 *>(const_cast<T *>(src) + (size_t)h * HD + 8 * u) =
-          make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+  if (is_q) return;
+  uint32_t ends[NG];   // a group's minimum and negated maximum
+#pragma unroll
+  for (int j = 0; j < NG; j++) {
+    uint32_t lo = min2<T>(min2<T>(c[j][0], c[j][1]), min2<T>(c[j][2], c[j][3])), hi = max2<T>(max2<T>(c[j][0], c[j][1]), max2<T>(c[j][2], c[j][3]));
+    lo = min2<T>(lo, __byte_perm(lo, lo, 0x1032));
+    hi = max2<T>(hi, __byte_perm(hi, hi, 0x1032));
+    uint32_t e = __byte_perm(lo, hi ^ 0x80008000u, 0x5410);
+    e = min2<T>(e, __shfl_xor_sync(0xffffffffu, e, 1));
+    ends[j] = min2<T>(e, __shfl_xor_sync(0xffffffffu, e, 2));
   }
-  if (is_q || !in) return;
   char *blk = reinterpret_cast<char *>(a.cache) + ((size_t)(b * a.n_kv + h) * a.blocks + (pos >> 4)) * block_bytes(HD);
-  const int r = pos & 15, j = u >> 2, q = u & 3;
+  const int r = pos & 15;
+  float invs[(NG + 3) / 4];   // of groups t, t + 4
+#pragma unroll
+  for (int i = 0; i < (NG + 3) / 4; i++) {
+    uint32_t e = ends[4 * i];
+#pragma unroll
+    for (int j = 1; j < 4 && j < NG; j++) e = t == j ? ends[4 * i + j] : e;
+    const float2 x = DT<T>::unpack2(e);
+    const float span = -x.y - x.x;   // NaN or infinite: the group has no code
+    const bool fine = span <= 3.402823466e38f;
+    T st = round_up<T>(fine ? span / 15.f : 0.f);
+    if (DT<T>::to_f(st) < 1.17549435e-38f && span > 0.f) st = DT<T>::from_f(1.17549435e-38f);
+    const float step = DT<T>::to_f(st);
+    invs[i] = fine && step > 0.f ? 1.f / step : 0.f;
+    if (in && 4 * i + t < NG)
+      reinterpret_cast<uint32_t *>(blk + (is_v ? v_pairs(HD) : k_pairs(HD)))[pair_word(HD, r, 4 * i + t)] = fine ? bits(st) | e << 16 : 0x7fff7fffu;
+  }
+  uint32_t w[NG];
+#pragma unroll
+  for (int j = 0; j < NG; j++) {
+    const float inv = __shfl_sync(0xffffffffu, invs[j / 4], (lane & ~3) | (j & 3)), lo = DT<T>::unpack2(ends[j]).x;
+    w[j] = is_v ? encode8<T, false>(c[j], lo, inv) : encode8<T, true>(c[j], lo, inv);
+  }
+  auto store = [](char *p, const uint32_t *x) {
+    if (NG == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(x[0], x[1]);
+    else *reinterpret_cast<uint4 *>(p) = make_uint4(x[0], x[1], x[2 % NG], x[3 % NG]);
+  };
   if (!is_v) {
-    // entry 2i to nibble i, entry 2i + 1 to nibble 4 + i
-    uint32_t k = 0;
+    if (in)
 #pragma unroll
-    for (int i = 0; i < 4; i++) k |= (w >> (8 * i) & 15u) << (4 * i) | (w >> (8 * i + 4) & 15u) << (16 + 4 * i);
-    reinterpret_cast<uint32_t *>(blk)[k_word(HD, r, u)] = k;
-    if (q == 0) reinterpret_cast<uint32_t *>(blk + k_pairs(HD))[pair_word(HD, r, j)] = pair;
-  } else {
-    uint16_t *v = reinterpret_cast<uint16_t *>(blk + v_codes(HD));
-    v[v_half(HD, r, 2 * q, j)] = (uint16_t)w;
-    v[v_half(HD, r, 2 * q + 1, j)] = (uint16_t)(w >> 16);
-    if (q == 0) reinterpret_cast<uint32_t *>(blk + v_pairs(HD))[pair_word(HD, r, j)] = pair;
+      for (int j = 0; j < NG; j += 4) store(blk + k_word(HD, r, t) * 4 + j * 4, w + j);
+    return;
   }
+  // V: an even position's lane has word g = 2 t, an odd one's g = 2 t + 1, of both positions
+  const bool odd = r & 1, pair_in = __shfl_xor_sync(0xffffffffu, (int)in, 4) && in;
+  const int g = 2 * t + (odd ? 1 : 0);
+#pragma unroll
+  for (int j = 0; j < NG; j++) {
+    const uint32_t theirs = __shfl_xor_sync(0xffffffffu, w[j], 4);
+    if (!pair_in) {   // the neighbour stays as it is
+      if (in) {
+        uint16_t *v = reinterpret_cast<uint16_t *>(blk + v_codes(HD));
+        v[v_half(HD, r, 2 * t, j)] = (uint16_t)w[j];
+        v[v_half(HD, r, 2 * t + 1, j)] = (uint16_t)(w[j] >> 16);
+      }
+    }
+    w[j] = odd ? __byte_perm(theirs, w[j], 0x7632) : __byte_perm(w[j], theirs, 0x5410);
+  }
+  if (pair_in)
+#pragma unroll
+    for (int j = 0; j < NG; j += 4) store(blk + v_codes(HD) + v_half(HD, r & ~1, g, j) * 2, w + j);
 }
 
-template <typename T> __device__ __forceinline__ float2 open_pair(uint32_t p) { return DT<T>::unpack2(p); }   // (step, lo)
-
-// entry i's code in nibble i of what is returned: entries 8u .. 8u + 7 of position r
-template <int HD> __device__ __forceinline__ uint32_t codes8(const char *blk, int which, int r, int u) {
-  if (!which) {
-    const uint32_t k = reinterpret_cast<const uint32_t *>(blk)[k_word(HD, r, u)];
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) w |= (k >> (4 * i) & 15u) << (8 * i) | (k >> (16 + 4 * i) & 15u) << (8 * i + 4);
-    return w;
+// ------------------------------------------------------------------------------------------ rows out of the cache
+// Bound by memory too: 5 bits read and 16 written an entry.  A warp takes a block: K's words as they lie (a row's four lanes write 64 bytes of it
+// together), V's likewise (8 lanes write 64 bytes of a row).  A value is one fma in pairs of D on exact codes: one rounding.
+// 32768 positions of 8 heads of 128, K and V: 71 us with 2-byte reads of V and 64-bit divisions a lane; so 30 (5.85 TB/s).
+// As operands of matrix products (a.nan): a group that reads as NaN becomes zero, so that it counts for no row that does not see it, and the
+// block's word says where: byte 0 the first position (in the block) whose K has such a group, byte 1 + j that of V's group j, 255 none.
+template <typename T> struct Codes;   // n as pairs of D, nibbles i and 4 + i of w
+template <> struct Codes<__half> {
+  static __device__ __forceinline__ void open(uint32_t w, uint32_t (&r)[4]) {
+    const uint32_t v = w >> 8;
+    r[0] = fma2<__half>(and_or(w, 0x000f000fu, 0x64006400u), 0x3c003c00u, 0xe400e400u);   // (1024 + n) - 1024
+    r[1] = fma2<__half>(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);   // (1024 + 16 n) / 16 - 64
+    r[2] = fma2<__half>(and_or(v, 0x000f000fu, 0x64006400u), 0x3c003c00u, 0xe400e400u);
+    r[3] = fma2<__half>(and_or(v, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);
   }
-  const uint16_t *v = reinterpret_cast<const uint16_t *>(blk + v_codes(HD));
-  return v[v_half(HD, r, 2 * (u & 3), u >> 2)] | (uint32_t)v[v_half(HD, r, 2 * (u & 3) + 1, u >> 2)] << 16;
-}
-
+};
+template <> struct Codes<__nv_bfloat16> {
+  static __device__ __forceinline__ void open(uint32_t w, uint32_t (&r)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = fma2<__nv_bfloat16>(and_or(w >> (4 * i), 0x000f000fu, 0x43004300u), 0x3f803f80u, 0xc300c300u);   // (128 + n) - 128
+  }
+};
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) read_kernel(const Read a) {
   pdl_launch_dependents();
+  constexpr int NG = HD / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int blk0 = a.first >> 4, n_blk = ((a.first + a.n - 1) >> 4) - blk0 + 1;
+  const unsigned item = blockIdx.x * 4 + (threadIdx.x >> 5);
   pdl_wait();
-  constexpr int LPR = HD / 8;
-  const int lane = threadIdx.x & 31, u = lane % LPR;
-  const long long row = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * (32 / LPR) + lane / LPR;
-  if (row >= (long long)a.B * a.n_kv * a.n) return;
-  const int i = (int)(row % a.n), slab = (int)(row / a.n), pos = a.first + i, r = pos & 15;
-  const char *blk = reinterpret_cast<const char *>(a.cache) + ((size_t)slab * a.blocks + (pos >> 4)) * block_bytes(HD);
-  const uint32_t w = codes8<HD>(blk, a.which, r, u);
-  const float2 p = open_pair<T>(reinterpret_cast<const uint32_t *>(blk + (a.which ? v_pairs(HD) : k_pairs(HD)))[pair_word(HD, r, u >> 2)]);
-  uint32_t o[4];
+  if (item >= (unsigned)a.B * a.n_kv * n_blk) return;
+  const int i = (int)(item % n_blk), slab = (int)(item / n_blk);
+  const char *blk = reinterpret_cast<const char *>(a.cache) + ((size_t)slab * a.blocks + blk0 + i) * block_bytes(HD);
+  const int row0 = 16 * (blk0 + i) - a.first;   // the output row of the block's first position
+  bool any_nan = false;
+  auto pair_of = [&](uint32_t p, uint32_t (&q)[2]) {   // step and lo, twice each
+    if (a.nan && (p & 0x7fffu) > (sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u)) {
+      any_nan = true;
+      p = 0;
+    }
+    q[0] = __byte_perm(p, p, 0x1010);
+    q[1] = __byte_perm(p, p, 0x3232);
+  };
+  if (a.k) {
+    T *out = reinterpret_cast<T *>(a.k) + ((size_t)slab * a.out_rows + row0) * HD;
 #pragma unroll
-  for (int e = 0; e < 4; e++)
-    o[e] = pack2x<T>(fmaf(p.x, (float)(w >> (8 * e) & 15u), p.y), fmaf(p.x, (float)(w >> (8 * e + 4) & 15u), p.y));
-  *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + ((size_t)slab * a.out_rows + i) * HD + 8 * u) = make_uint4(o[0], o[1], o[2], o[3]);
+    for (int half = 0; half < 2; half++) {
+      const int r = g + 8 * half, row = row0 + r;
+      uint32_t w[NG], p[NG];
+      lds_words<NG>(blk + (half * 32 + lane) * NG * 4, w);
+      lds_words<NG>(blk + k_pairs(HD) + r * NG * 4, p);
+      const bool in = row >= 0 && row < a.n;
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        uint32_t c[4], q[2];
+        Codes<T>::open(w[j], c);
+        if (in) pair_of(p[(j & 1) * (NG / 2) + j / 2], q);
+        else q[0] = q[1] = 0u;
+        if (in)
+          *reinterpret_cast<uint4 *>(out + (size_t)r * HD + 32 * j + 8 * t) =
+              make_uint4(fma2<T>(c[0], q[0], q[1]), fma2<T>(c[1], q[0], q[1]), fma2<T>(c[2], q[0], q[1]), fma2<T>(c[3], q[0], q[1]));
+      }
+    }
+  }
+  if (a.v) {
+    T *out = reinterpret_cast<T *>(a.v) + ((size_t)slab * a.out_rows + row0) * HD;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {   // positions 8 half + 2 t and its neighbour
+      const int r = 8 * half + 2 * t;
+      uint32_t p0[NG], p1[NG];
+      lds_words<NG>(blk + v_pairs(HD) + r * NG * 4, p0);
+      lds_words<NG>(blk + v_pairs(HD) + (r + 1) * NG * 4, p1);
+      const bool in0 = row0 + r >= 0 && row0 + r < a.n, in1 = row0 + r + 1 >= 0 && row0 + r + 1 < a.n;
+#pragma unroll
+      for (int j = 0; j < NG; j++) {
+        // entries 4 g .. + 3 of the group: nibbles 0 .. 3 of either half; as pairs of neighbouring entries
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(blk + v_codes(HD) + v_half(HD, r, g, j) * 2);
+        uint32_t c[4], q[2];
+        Codes<T>::open(w, c);   // c[e]: entry e of both positions
+        const uint32_t a0 = __byte_perm(c[0], c[1], 0x5410), a1 = __byte_perm(c[2], c[3], 0x5410), b0 = __byte_perm(c[0], c[1], 0x7632),
+                       b1 = __byte_perm(c[2], c[3], 0x7632);
+        if (in0) {
+          pair_of(p0[(j & 1) * (NG / 2) + j / 2], q);
+          *reinterpret_cast<uint2 *>(out + (size_t)r * HD + 32 * j + 4 * g) = make_uint2(fma2<T>(a0, q[0], q[1]), fma2<T>(a1, q[0], q[1]));
+        }
+        if (in1) {
+          pair_of(p1[(j & 1) * (NG / 2) + j / 2], q);
+          *reinterpret_cast<uint2 *>(out + (size_t)(r + 1) * HD + 32 * j + 4 * g) = make_uint2(fma2<T>(b0, q[0], q[1]), fma2<T>(b1, q[0], q[1]));
+        }
+      }
+    }
+  }
+  if (HD <= 128 && a.nan) {   // (heads of 256 entries have more groups than a word has bytes, and no such products)
+    unsigned long long word = ~0ull;
+    if (__any_sync(0xffffffffu, any_nan)) {
+      const int r = lane & 15;   // lanes 0 .. 15: positions
+      const bool in = lane < 16 && row0 + r >= 0 && row0 + r < a.n;
+      for (int j = -1; j < NG; j++) {
+        bool bad = false;
+        for (int k = max(j, 0); k <= (j < 0 ? NG - 1 : j); k++) {
+          const float step = open_pair<T>(reinterpret_cast<const uint32_t *>(blk + (j < 0 ? k_pairs(HD) : v_pairs(HD)))[pair_word(HD, r, k)]).x;
+          bad = bad || step != step;
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, in && bad);
+        if (who) word = (word & ~(0xffull << (8 * (j + 1)))) | (unsigned long long)(__ffs(who) - 1) << (8 * (j + 1));
+      }
+    }
+    if (lane == 0) a.nan[(size_t)slab * n_blk + i] = word;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ attention of a few rows, keys split
@@ -232,11 +434,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t c) {   // (as two constants the compiler takes two operations)
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(m), "r"(c));
-  return r;
-}
 // nibbles i and 4 + i of w as a pair of fp16: 1024 + n for even i, 1024 + 16 n for odd i
 __device__ __forceinline__ void open_codes(uint32_t w, uint32_t (&r)[4]) {
   const uint32_t v = w >> 8;
@@ -249,20 +446,6 @@ __device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t c) {   // pairs of
   const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
-template <int N> __device__ __forceinline__ void lds_words(const void *p, uint32_t (&w)[N]) {   // in pieces of up to 16 bytes
-  if (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
-  else if (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x; w[1 % N] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 4; i++) {
-      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-      w[(4 * i) % N] = v.x; w[(4 * i + 1) % N] = v.y; w[(4 * i + 2) % N] = v.z; w[(4 * i + 3) % N] = v.w;
-    }
-  }
-}
-
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -738,14 +921,15 @@ template <typename F> static int by_type(int dtype, int hd, F &&f) {
 int write(cudaStream_t s, int dtype, const Write &a, uint64_t *launches) {
   return by_type(dtype, a.hd, [&](auto t, auto hd) {
     typedef decltype(t) T;
-    const long long warps = ((long long)a.B * a.S * (a.n_q + 2 * a.n_kv) * (a.hd / 8) + 31) / 32;
+    const int eights = a.d_pos ? (a.S + 14) / 8 : ((a.pos0 & 7) + a.S + 7) / 8;   // (at any position on the device)
+    const long long warps = (long long)a.B * eights * (a.n_q + 2 * a.n_kv);
     return launch(s, launches, write_kernel<T, hd.value>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, 1, a);
   });
 }
 int read(cudaStream_t s, int dtype, const Read &a, uint64_t *launches) {
   return by_type(dtype, a.hd, [&](auto t, auto hd) {
     typedef decltype(t) T;
-    const long long warps = ((long long)a.B * a.n_kv * a.n * (a.hd / 8) + 31) / 32;
+    const long long warps = (long long)a.B * a.n_kv * read_blocks(a.first, a.n);
     return launch(s, launches, read_kernel<T, hd.value>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, 1, a);
   });
 }

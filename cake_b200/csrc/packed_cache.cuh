@@ -55,13 +55,15 @@ struct Write {
 };
 int write(cudaStream_t, int dtype, const Write &, uint64_t *launches);
 
-// positions [first, first + n) of K (which 0) or V (1) -> out [B, n_kv, n, hd] in D, a (batch row, head) every out_rows rows
+// positions [first, first + n) of K and V (either may be nullptr) -> [B, n_kv, n, hd] in D, a (batch row, head) every out_rows rows
 struct Read {
   const void *cache;
-  void *out;
-  int B, n_kv, hd, blocks, which, first, n;
+  void *k, *v;
+  int B, n_kv, hd, blocks, first, n;
   long long out_rows;
+  unsigned long long *nan = nullptr;   // as operands of products: [B n_kv][read_blocks], see nan_groups
 };
+inline int read_blocks(int first, int n) { return ((first + n - 1) >> 4) - (first >> 4) + 1; }
 int read(cudaStream_t, int dtype, const Read &, uint64_t *launches);
 
 // Row t of S (position pos0 + t) of q attends to the positions first <= j <= pos0 + t; a row without any is zero.
@@ -84,6 +86,14 @@ size_t scratch_floats(int sms);
 size_t scratch_tickets(int sms);
 int prepare(int dtype, int hd);   // once per device and kind of cache, in front of the first call
 int attend(cudaStream_t, int dtype, const Attend &, const Scratch &, uint64_t *launches);
+// Whether keys and values expanded once, for the kernel of prompts, are the faster way: where the pieces of 16 rows are more than the SMs, or their
+// blocks (0.48 us a quarter SM each) take longer than expanding and reading the rows in D (8 key heads: 3.5 us per 1000 positions and 20).  32 / 8 heads,
+// on codes and expanded: 64 rows at 0 7.5, 9.0 us, at 2000 22, 28, at 30000 201, 122; 128 rows at 0 14.0, 9.9; 32 rows at 30000 109, 126.
+inline bool many_rows(const Attend &a, int sms) {
+  const long long cols = (long long)a.S * (a.n_heads / a.n_kv), pieces = (long long)a.B * a.n_kv * ((cols + 15) / 16);
+  const double keys = a.pos0 + 0.5 * a.S - a.first;
+  return a.hd == 128 && cols > 16 && (pieces > sms || 0.48 * pieces * (keys / BLOCK) / (4.0 * sms) > 20 + 3.5e-3 * keys);
+}
 
 }  // namespace pc
 }  // namespace cake

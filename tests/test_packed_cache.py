@@ -320,6 +320,35 @@ def test_what_no_row_sees_may_be_anything(hd, s):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("b,s,at,first", [(1, 150, 100, 0), (1, 150, 100, 37), (1, 150, 2000, 1003), (2, 260, 0, 0), (1, 77, 3000, 16)])
+def test_nan_in_a_prompt_reaches_the_rows_that_see_it(b, s, at, first, dtype):
+    """Rows enough for keys and values to be expanded for the prompt's kernel, in one piece and with the keys cut: a NaN of K makes the rows from its
+    position on NaN, one of V its group's entries of theirs; nothing else, whatever lies in front of `first` and behind the rows."""
+    ctx = ctx_for(32, 8, 128, dtype)
+    n = at + s + 5
+    q = queries(b, s, 32, 128, dtype, 3)
+    k0, v0 = rows(b, n, 8, 128, dtype, 1), rows(b, n, 8, 128, dtype, 2)
+    k0[:, :first], v0[:, at + s:] = torch.inf, torch.nan
+    cache = Cache(ctx, b, n, bits=4)
+    for spots in ([], [("v", 0, 2, 70, at + s // 2)], [("k", 0, 0, 5, at + s - 1), ("v", b - 1, 7, 127, first)], [("v", 0, 3, 0, at + 16), ("v", 0, 3, 40, at + 31), ("k", 0, 4, 9, at + 47)]):
+        k, v = k0.clone(), v0.clone()
+        bad = torch.zeros((b, s, 32, 128), dtype=torch.bool)
+        for which, bi, h, d, pos in spots:
+            (k if which == "k" else v)[bi, pos, h, d] = torch.nan
+            d0, d1 = (0, 128) if which == "k" else (d // 32 * 32, d // 32 * 32 + 32)
+            bad[bi, max(0, pos - at):, 4 * h:4 * h + 4, d0:d1] = True
+        cache.write(0, k, v, 0)
+        got = cache.attend(0, q, at, first=first).cpu()
+        assert torch.equal(got.isnan(), bad), spots
+        if not spots:
+            check_attention(got, q, k, v, at, first, dtype)
+        clean = got if not spots else clean
+        assert torch.equal(got[~bad], clean[~bad])
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_scales_and_sizes_of_entries(dtype):
     """Sharp and flat softmaxes; values so small or large that weights times steps leave fp16; a step that grows by 2^12 on the way."""
     ctx = ctx_for(8, 2, 128, dtype)
