@@ -162,9 +162,9 @@ SYMBOLS += [
 # caches in four bits
 SYMBOLS += [
     ("cake_b200_cache_create_packed", _I, [_VP, _I, _I, _I, POINTER(_VP)]),
-    ("cake_b200_cache_write", _I, [_VP, _I, _VP, c_size_t, c_size_t, _VP, c_size_t, c_size_t, _I, _I]),
-    ("cake_b200_cache_unpack", _I, [_VP, _I, _I, _I, _I, _VP]),
-    ("cake_b200_cache_attend", _I, [_VP, _I, _VP, c_size_t, c_size_t, _VP, _I, _I, _I, c_float]),
+    ("cake_b200_cache_write", _I, [_VP, _I, _VP, c_size_t, c_size_t, _VP, c_size_t, c_size_t, _I, _I, _VP]),
+    ("cake_b200_cache_unpack", _I, [_VP, _I, _I, _I, _I, _VP, _VP]),
+    ("cake_b200_cache_attend", _I, [_VP, _I, _VP, c_size_t, c_size_t, _VP, _I, _I, _I, c_float, _VP]),
 ]
 
 

@@ -154,6 +154,7 @@ struct cake_b200_ctx {
   void *pc_rows = nullptr;   // rows of such caches in D, for the kernels of prompts
   size_t pc_rows_cap = 0;
   unsigned *pc_tickets = nullptr;
+  cudaEvent_t pc_in = nullptr, pc_out = nullptr;   // a caller's stream in front of this one's work, and behind it
   // head of a batch: its logits where the caller keeps none, its tokens
   void *hd_logits = nullptr;
   size_t hd_logits_rows = 0;
@@ -677,6 +678,8 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
     if (c->stage_free[i]) cudaEventDestroy(c->stage_free[i]);
   }
   if (c->load_done) cudaEventDestroy(c->load_done);
+  for (cudaEvent_t ev : {c->pc_in, c->pc_out})
+    if (ev) cudaEventDestroy(ev);
   if (c->ev_fork) cudaEventDestroy(c->ev_fork);
   if (c->ev_join) cudaEventDestroy(c->ev_join);
   if (c->side_stream) { cudaStreamSynchronize(c->side_stream); cudaStreamDestroy(c->side_stream); }
@@ -953,6 +956,8 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
   CU(cudaSetDevice(c->device));
   if (!c->pc_tickets) {
     CU((cudaError_t)pc::prepare(c->cfg.dtype, c->cfg.head_dim));
+    for (cudaEvent_t *ev : {&c->pc_in, &c->pc_out})
+      if (!*ev) CU(cudaEventCreateWithFlags(ev, cudaEventDisableTiming));
     if (!c->pc_ws) CU(cudaMalloc(&c->pc_ws, pc::scratch_floats(c->sm_count) * sizeof(float)));
     const size_t n = pc::scratch_tickets(c->sm_count) * sizeof(unsigned);
     unsigned *tickets = nullptr;
@@ -1045,7 +1050,7 @@ extern "C" int cake_b200_cache_read(cake_b200_cache *k, int block_idx, int which
     if (!len) return CAKE_B200_OK;
     void *rows = nullptr;
     CU(cudaMalloc(&rows, need));
-    int rc = cake_b200_cache_unpack(k, block_idx, which, 0, len, rows);
+    int rc = cake_b200_cache_unpack(k, block_idx, which, 0, len, rows, nullptr);
     if (rc == CAKE_B200_OK) rc = sync_results(c);
     if (rc == CAKE_B200_OK) {
       const cudaError_t e = cudaMemcpy(out_host, rows, need, cudaMemcpyDeviceToHost);
@@ -1070,8 +1075,21 @@ static int packed_call(const cake_b200_cache *k, int block_idx, const char *what
   return check_cache(k);
 }
 static bool unaligned(const void *p, size_t s0 = 0, size_t s1 = 0) { return ((uintptr_t)p & 15) || s0 % 8 || s1 % 8; }
+// work of the ctx's stream in the order of the caller's
+template <typename F> static int in_order_of(cake_b200_ctx *c, void *stream, F &&call) {
+  if (!stream || stream == (void *)c->stream) return call();
+  CU(cudaEventRecord(c->pc_in, (cudaStream_t)stream));
+  CU(cudaStreamWaitEvent(c->stream, c->pc_in, 0));
+  const int rc = call();
+  const std::string said = rc == CAKE_B200_OK ? "" : g_err;   // (the message that stays is the call's)
+  cudaError_t e = cudaEventRecord(c->pc_out, c->stream);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent((cudaStream_t)stream, c->pc_out, 0);
+  if (rc != CAKE_B200_OK) return fail(rc, "%s", said.c_str());
+  CU(e);
+  return CAKE_B200_OK;
+}
 extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const void *k_dev, size_t k_tok, size_t k_batch, const void *v_dev,
-                                     size_t v_tok, size_t v_batch, int seq, int index_pos) {
+                                     size_t v_tok, size_t v_batch, int seq, int index_pos, void *stream) {
   RC(packed_call(k, block_idx, "cache_write"));
   if (!k_dev || !v_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
   if (unaligned(k_dev, k_tok, k_batch) || unaligned(v_dev, v_tok, v_batch))
@@ -1083,11 +1101,13 @@ extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const vo
   const cake_b200_config &f = k->ctx->cfg;
   pc::Write a{k->k[block_idx], k_dev, v_dev, (long long)k_tok, (long long)k_batch, (long long)v_tok, (long long)v_batch};
   a.B = k->batch; a.S = seq; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(k->cap); a.pos0 = index_pos;
-  CU((cudaError_t)pc::write(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
-  k->len[block_idx] = index_pos + seq;
-  return CAKE_B200_OK;
+  return in_order_of(k->ctx, stream, [&]() -> int {
+    CU((cudaError_t)pc::write(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
+    k->len[block_idx] = index_pos + seq;
+    return CAKE_B200_OK;
+  });
 }
-extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int which, int first, int n, void *out_dev) {
+extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int which, int first, int n, void *out_dev, void *stream) {
   RC(packed_call(k, block_idx, "cache_unpack"));
   if (which != 0 && which != 1) return fail(CAKE_B200_EINVAL, "which is 0 (K) or 1 (V), not %d", which);
   if (first < 0 || n < 1 || (long long)first + n > k->len[block_idx])
@@ -1095,8 +1115,10 @@ extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int whi
   if (!out_dev || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "cache_unpack writes to a 16-byte boundary");
   const cake_b200_config &f = k->ctx->cfg;
   pc::Read a{k->k[block_idx], which ? nullptr : out_dev, which ? out_dev : nullptr, k->batch, f.n_kv_heads, f.head_dim, pc::cap_blocks(k->cap), first, n, n};
-  CU((cudaError_t)pc::read(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
-  return CAKE_B200_OK;
+  return in_order_of(k->ctx, stream, [&]() -> int {
+    CU((cudaError_t)pc::read(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
+    return CAKE_B200_OK;
+  });
 }
 template <typename T>
 static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_t q_batch, const void *k, const void *v, int cap, void *y, int B, int S, int pos0,
@@ -1142,7 +1164,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq,
-                                      int index_pos, int first, float scale) {
+                                      int index_pos, int first, float scale, void *stream) {
   RC(packed_call(k, block_idx, "cache_attend"));
   if (!q_dev || !out_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
   if (unaligned(q_dev, q_tok, q_batch) || unaligned(out_dev))
@@ -1150,8 +1172,10 @@ extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const v
   if (index_pos < 0 || (long long)index_pos + seq > k->len[block_idx])
     return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, index_pos, seq, k->len[block_idx]);
   if (first < 0 || !(scale >= 0.f && scale <= 3.402823466e38f)) return fail(CAKE_B200_EINVAL, "first %d or scale %g out of range", first, (double)scale);
-  return attend_packed(k->ctx, k, block_idx, q_dev, q_tok, q_batch, out_dev, seq, index_pos, first,
-                       scale > 0.f ? scale : (float)(1.0 / sqrt((double)k->ctx->cfg.head_dim)));
+  return in_order_of(k->ctx, stream, [&]() -> int {
+    return attend_packed(k->ctx, k, block_idx, q_dev, q_tok, q_batch, out_dev, seq, index_pos, first,
+                         scale > 0.f ? scale : (float)(1.0 / sqrt((double)k->ctx->cfg.head_dim)));
+  });
 }
 // a step's rows of a fused projection [tokens, heads + 2 kv heads, hd]: norms and rotation, q in place, k and v into the cache
 static int write_packed(cake_b200_ctx *c, const cake_b200_block *b, const cake_b200_cache *kc, int l, void *qkv, const void *qn, const void *kn, int S, int pos0,

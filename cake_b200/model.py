@@ -91,52 +91,46 @@ class Cache:
     # -- the operators of a cache in four bits -----------------------------------------------------
     def _rows(self, t: torch.Tensor, name: str, seq: Optional[int], heads: int) -> torch.Tensor:
         """(batch, seq, heads, hd) rows as the library takes them: heads side by side on 16-byte boundaries (copied where they are not)."""
-        want = (self.batch, t.shape[1] if seq is None and t.dim() == 4 else seq, heads, self.ctx.config.hd)
-        if tuple(t.shape) != want:
-            raise ValueError(f"{name} has shape {list(t.shape)}, expected (batch, seq, heads, head_dim) = {list(want)}")
-        if t.dtype != self.ctx.torch_dtype or t.device.type != "cuda" or t.device.index != self.ctx.device:
+        hd = self.ctx.config.hd
+        if t.dim() != 4 or t.shape != (self.batch, t.shape[1] if seq is None else seq, heads, hd):
+            raise ValueError(f"{name} has shape {list(t.shape)}, expected (batch, seq, heads, head_dim) = {[self.batch, seq or 'seq', heads, hd]}")
+        if t.dtype != self.ctx.torch_dtype or not t.is_cuda or t.get_device() != self.ctx.device:
             raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self.ctx.torch_dtype} on cuda:{self.ctx.device}")
         sb, st, sh, sd = t.stride()
-        if sd != 1 or (sh != want[3] and heads > 1) or st % 8 or sb % 8 or t.data_ptr() % 16:
-            t = t.contiguous() if not t.is_contiguous() else t.clone()
+        if sd != 1 or (sh != hd and heads > 1) or st % 8 or sb % 8 or t.data_ptr() % 16:
+            t = t.clone() if t.is_contiguous() else t.contiguous()
         return t
 
-    def _on_stream(self, call) -> None:
-        """``call`` on the context's stream, in the order of the current one."""
-        cur, own = torch.cuda.current_stream(self.ctx.device), self.ctx.torch_stream
-        if cur == own:
-            return check(call())
-        own.wait_stream(cur)
-        try:
-            check(call())
-        finally:
-            cur.wait_stream(own)
+    def _stream(self) -> Optional[int]:
+        """The current stream as the library's calls take it: they keep their order with its work."""
+        s = torch._C._cuda_getCurrentRawStream(self.ctx.device)
+        return s or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's own
 
     def write(self, block_idx: int, k: torch.Tensor, v: torch.Tensor, index_pos: int) -> None:
         """Rows k, v (batch, seq, n_kv, head_dim) in D (any stride of batch rows and tokens) become the positions index_pos .. of the block's cache, whose
         length is then index_pos + seq: index_pos is the length so far, or an earlier position from which on the cache is written anew."""
         n_kv = self.ctx.config.num_key_value_heads
         k = self._rows(k, "k", None, n_kv)
-        v = self._rows(v, "v", k.shape[1], n_kv)
-        ks, vs = k.stride(), v.stride()
-        self._on_stream(lambda: self._lib.cake_b200_cache_write(self.h, block_idx, k.data_ptr(), ks[1], ks[0], v.data_ptr(), vs[1], vs[0], k.shape[1], index_pos))
+        seq = k.shape[1]
+        v = self._rows(v, "v", seq, n_kv)
+        check(self._lib.cake_b200_cache_write(self.h, block_idx, k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1), v.stride(0), seq, index_pos,
+                                              self._stream()))
 
     def read(self, block_idx: int, which: int, first: int = 0, n: Optional[int] = None) -> torch.Tensor:
         """Positions [first, first + n) (to the end without n) of the block's K (which 0) or V (1) rows: (batch, n_kv, n, head_dim) in D."""
         c = self.ctx.config
         n = max(0, self.len(block_idx) - first) if n is None else n
-        out = torch.empty((self.batch, c.num_key_value_heads, max(n, 0), c.hd), dtype=self.ctx.torch_dtype, device=f"cuda:{self.ctx.device}")
-        self._on_stream(lambda: self._lib.cake_b200_cache_unpack(self.h, block_idx, which, first, n, out.data_ptr()))
+        out = torch.empty((self.batch, c.num_key_value_heads, max(n, 0), c.hd), dtype=self.ctx.torch_dtype, device=self.ctx.torch_device)
+        check(self._lib.cake_b200_cache_unpack(self.h, block_idx, which, first, n, out.data_ptr(), self._stream()))
         return out
 
     def attend(self, block_idx: int, q: torch.Tensor, index_pos: int, first: int = 0, scale: float = 0.0) -> torch.Tensor:
         """Attention of the rows q (batch, seq, n_heads, head_dim) in D at positions index_pos .., which the cache holds: row t sees the positions
         first <= j <= index_pos + t (one that sees none is zero).  scale 0: head_dim^-1/2.  (batch, seq, n_heads, head_dim) in D."""
         q = self._rows(q, "q", None, self.ctx.config.num_attention_heads)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qs = q.stride()
-        self._on_stream(lambda: self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), qs[1], qs[0], out.data_ptr(), q.shape[1], index_pos,
-                                                                 first, scale))
+        out = torch.empty(q.shape, dtype=q.dtype, device=self.ctx.torch_device)
+        check(self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), q.shape[1], index_pos, first, scale,
+                                               self._stream()))
         return out
 
     def __del__(self):
@@ -156,6 +150,7 @@ class Context:
         self.config, self.var_builder, self.dtype, self.device = config, var_builder, dtype, device
         self.max_seq = max_seq or config.max_seq_len
         self.cache_bits = cache_bits  # of the caches made for this context: 0 rows in D, 4 packed
+        self.torch_device = torch.device("cuda", device)
         self.topology = topology or {}
         self.ccfg = CConfig.from_config(config, dtype, self.max_seq)
         self.h = c_void_p()

@@ -393,21 +393,24 @@ int cake_b200_cache_fill_synthetic(cake_b200_cache *, const int *block_idx, int 
  * Llama-family blocks with head_dim 64, 128 or 256 and rotated parts of a multiple of 16 entries; bits = 4.  cake_b200_forward_batch,
  * cake_b200_decode_build and the other calls on caches take such a cache like any other (every rank of a sharded decode then has one); attention reads
  * what the cache holds, the rows of the same call included, so that a prompt may be cut anywhere.  cake_b200_cache_read returns the entries' values
- * rounded to D. */
+ * rounded to D.
+ * The three calls below run on the ctx's stream.  stream: NULL, or the cudaStream_t that their tensors belong to (cudaStreamLegacy for the default
+ * stream): the call waits for what that stream holds so far, and the stream goes on behind the call; it may be capturing, once the same call has run
+ * outside a capture (memory grows on first use). */
 int cake_b200_cache_create_packed(cake_b200_ctx *, int batch, int max_seq, int bits, cake_b200_cache **out);
 /* Rows k, v (batch, seq, n_kv, head_dim) in D, as they are, join block_idx's part of the cache at index_pos, which is its length or less: what is behind
  * index_pos is dropped and the length becomes index_pos + seq (CAKE_B200_ESTATE where index_pos is beyond the length or the rows beyond the
  * capacity).  *_tok, *_batch: strides of tokens and batch rows in entries, multiples of 8; heads lie side by side; pointers on 16 bytes.  The first
  * write of a block allocates its part. */
 int cake_b200_cache_write(cake_b200_cache *, int block_idx, const void *k_dev, size_t k_tok, size_t k_batch, const void *v_dev, size_t v_tok,
-                          size_t v_batch, int seq, int index_pos);
+                          size_t v_batch, int seq, int index_pos, void *stream);
 /* Positions [first, first + n) of K (which 0) or V (1), rounded to D -> out (batch, n_kv, n, head_dim), device memory on 16 bytes. */
-int cake_b200_cache_unpack(cake_b200_cache *, int block_idx, int which, int first, int n, void *out_dev);
+int cake_b200_cache_unpack(cake_b200_cache *, int block_idx, int which, int first, int n, void *out_dev, void *stream);
 /* Attention of the rows q (batch, seq, n_heads, head_dim) in D at positions index_pos .., which the cache holds: row t sees the positions first <= j <=
  * index_pos + t;  out = softmax(scale q . k_j) weighted sum of v_j, in fp32 up to one rounding to D; a row that sees no position is zero.
  * q_tok, q_batch: strides as above; out (batch, seq, n_heads, head_dim) contiguous; scale 0: head_dim^-1/2. */
 int cake_b200_cache_attend(cake_b200_cache *, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq, int index_pos,
-                           int first, float scale);
+                           int first, float scale, void *stream);
 
 /* ---- the block forward ------------------------------------------------------------------------ */
 /* == Forwarder::forward_batch over `n_blocks` consecutive local layers (n_blocks == 1 == forward).

@@ -93,9 +93,9 @@ extern "C" {
     pub fn cake_b200_cache_len(c: *const cake_b200_cache, block_idx: c_int) -> c_int;
     pub fn cake_b200_cache_read(c: *mut cake_b200_cache, block_idx: c_int, which: c_int, out_host: *mut c_void, bytes: usize) -> c_int;
     pub fn cake_b200_cache_create_packed(c: *mut cake_b200_ctx, batch: c_int, max_seq: c_int, bits: c_int, out: *mut *mut cake_b200_cache) -> c_int;
-    pub fn cake_b200_cache_write(c: *mut cake_b200_cache, block_idx: c_int, k_dev: *const c_void, k_tok: usize, k_batch: usize, v_dev: *const c_void, v_tok: usize, v_batch: usize, seq: c_int, index_pos: c_int) -> c_int;
-    pub fn cake_b200_cache_unpack(c: *mut cake_b200_cache, block_idx: c_int, which: c_int, first: c_int, n: c_int, out_dev: *mut c_void) -> c_int;
-    pub fn cake_b200_cache_attend(c: *mut cake_b200_cache, block_idx: c_int, q_dev: *const c_void, q_tok: usize, q_batch: usize, out_dev: *mut c_void, seq: c_int, index_pos: c_int, first: c_int, scale: f32) -> c_int;
+    pub fn cake_b200_cache_write(c: *mut cake_b200_cache, block_idx: c_int, k_dev: *const c_void, k_tok: usize, k_batch: usize, v_dev: *const c_void, v_tok: usize, v_batch: usize, seq: c_int, index_pos: c_int, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_cache_unpack(c: *mut cake_b200_cache, block_idx: c_int, which: c_int, first: c_int, n: c_int, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_cache_attend(c: *mut cake_b200_cache, block_idx: c_int, q_dev: *const c_void, q_tok: usize, q_batch: usize, out_dev: *mut c_void, seq: c_int, index_pos: c_int, first: c_int, scale: f32, stream: *mut c_void) -> c_int;
     pub fn cake_b200_cache_fill_synthetic(c: *mut cake_b200_cache, block_idx: *const c_int, n_blocks: c_int, len: c_int, seed: u32) -> c_int;
     pub fn cake_b200_bench_kernel(ctx: *mut cake_b200_ctx, blocks: *const *mut cake_b200_block, block_idx: *const c_int,
         n_blocks: c_int, cache: *mut cake_b200_cache, which: c_int, reps: c_int, ms_per_launch: *mut f32) -> c_int;

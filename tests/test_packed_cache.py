@@ -510,11 +510,11 @@ def test_refusals():
     for w, first, n in ((0, 0, 5), (0, 4, 1), (1, -1, 2), (1, 0, 0), (0, 2, -1)):
         refused(ESTATE, lambda: cache.read(0, w, first, n))
     refused(EINVAL, lambda: cache.read(0, 2, 0, 1))
-    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k) + 2, 128, 512, ptr(k), 128, 512, 1, 0)))
-    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 127, 512, ptr(k), 128, 512, 1, 0)))
-    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 128, 512, None, 128, 512, 1, 0)))
-    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 128, 512, ptr(k), 128, 512, 0, 0)))
-    refused(EINVAL, lambda: check(lib().cake_b200_cache_attend(cache.h, 0, ptr(q), 512, 2048, ptr(q) + 8, 1, 0, 0, 0.0)))
+    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k) + 2, 128, 512, ptr(k), 128, 512, 1, 0, None)))
+    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 127, 512, ptr(k), 128, 512, 1, 0, None)))
+    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 128, 512, None, 128, 512, 1, 0, None)))
+    refused(EINVAL, lambda: check(lib().cake_b200_cache_write(cache.h, 0, ptr(k), 128, 512, ptr(k), 128, 512, 0, 0, None)))
+    refused(EINVAL, lambda: check(lib().cake_b200_cache_attend(cache.h, 0, ptr(q), 512, 2048, ptr(q) + 8, 1, 0, 0, 0.0, None)))
     for bad in (k.float(), k.cpu(), k[..., :32], k[:, :, :1], k[0], k.expand(2, -1, -1, -1)):
         with pytest.raises(ValueError):
             cache.write(0, bad, k, 0)
