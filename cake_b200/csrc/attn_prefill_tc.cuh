@@ -134,7 +134,10 @@ struct FtParams {
 };
 
 // SPLIT: clusters that cut the keys; without it every CTA sees its rows' first key in its first tile.
-template <typename T, bool SPLIT>
+// LO: P is kept to ~16 bits as P_hi + P_lo.  Without it P is rounded to D once: for keys and values that come from a packed cache, which are rounded to D
+// from four bits themselves: a prompt of 4096 (32 / 8 heads) takes 163 us for 190, and its distance to 64 bits stays 0.0017 of the result's norm, that of
+// rounding the result to bf16.
+template <typename T, bool SPLIT, bool LO = true>
 __global__ void __launch_bounds__(FT_THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FtParams p) {
@@ -247,7 +250,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint64_t vt = ft_desc_mn(v_s, FT_KV_BYTES / 2) + (uint64_t)(st * (FT_KV_BYTES >> 4));
         if (one) {
 #pragma unroll
-          for (int half = 0; half < 2; half++)
+          for (int half = 0; half < (LO ? 2 : 1); half++)
 #pragma unroll
             for (int ks = 0; ks < FT_BN / 16; ks++) {  // keys 16ks..16ks+15 = 8 packed columns of P_hi (0..31) or P_lo (32..63)
               const uint32_t ta = tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8);
@@ -338,11 +341,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int i = 0; i < 32; i++) {
           const float p0 = sv[2 * i], p1 = sv[2 * i + 1];
           hi[i] = pack2x<T>(p0, p1);
-          const float2 hf = DT<T>::unpack2(hi[i]);
-          lo[i] = pack2x<T>(p0 - hf.x, p1 - hf.y);
+          if (LO) {
+            const float2 hf = DT<T>::unpack2(hi[i]);
+            lo[i] = pack2x<T>(p0 - hf.x, p1 - hf.y);
+          }
         }
         tc_st32(tmem_sp, hi);
-        tc_st32(tmem_sp + 32u, lo);
+        if (LO) tc_st32(tmem_sp + 32u, lo);
       }
       tc_wait_st();
       tc_fence_before();

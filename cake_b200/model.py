@@ -46,6 +46,8 @@ class Cache:
         self.h = c_void_p()
         self._lib = lib()  # a handle is only ever given back to the library that made it
         if self.bits:
+            c = ctx.config
+            self._heads, self._kv, self._hd = c.num_attention_heads, c.num_key_value_heads, c.hd
             check(self._lib.cake_b200_cache_create_packed(ctx.h, batch, self.max_seq, self.bits, byref(self.h)))
         else:
             check(self._lib.cake_b200_cache_create(ctx.h, batch, self.max_seq, byref(self.h)))
@@ -89,48 +91,53 @@ class Cache:
         check(lib().cake_b200_cache_fill_synthetic(self.h, int_array(list(block_idx)), len(block_idx), length, seed))
 
     # -- the operators of a cache in four bits -----------------------------------------------------
-    def _rows(self, t: torch.Tensor, name: str, seq: Optional[int], heads: int) -> torch.Tensor:
+    def _rows(self, t: torch.Tensor, name: str, heads: int) -> torch.Tensor:
         """(batch, seq, heads, hd) rows as the library takes them: heads side by side on 16-byte boundaries (copied where they are not)."""
-        hd = self.ctx.config.hd
-        if t.dim() != 4 or t.shape != (self.batch, t.shape[1] if seq is None else seq, heads, hd):
-            raise ValueError(f"{name} has shape {list(t.shape)}, expected (batch, seq, heads, head_dim) = {[self.batch, seq or 'seq', heads, hd]}")
-        if t.dtype != self.ctx.torch_dtype or not t.is_cuda or t.get_device() != self.ctx.device:
-            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self.ctx.torch_dtype} on cuda:{self.ctx.device}")
+        ctx, shape = self.ctx, t.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[2] != heads or shape[3] != self._hd:
+            raise ValueError(f"{name} has shape {list(shape)}, expected (batch, seq, heads, head_dim) = {[self.batch, 'seq', heads, self._hd]}")
+        if t.dtype != ctx.torch_dtype or t.get_device() != ctx.device:   # (-1: not on a GPU)
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {ctx.torch_dtype} on cuda:{ctx.device}")
         sb, st, sh, sd = t.stride()
-        if sd != 1 or (sh != hd and heads > 1) or st % 8 or sb % 8 or t.data_ptr() % 16:
+        if sd != 1 or (sh != self._hd and heads > 1) or st % 8 or sb % 8 or t.data_ptr() % 16:
             t = t.clone() if t.is_contiguous() else t.contiguous()
         return t
 
-    def _stream(self) -> Optional[int]:
+    def _packed(self) -> None:
+        if not self.bits:
+            raise capi.CakeB200Error(-1, "write, read and attend are for caches in four bits (Cache(..., bits=4))")
+
+    def _stream(self) -> int:
         """The current stream as the library's calls take it: they keep their order with its work."""
-        s = torch._C._cuda_getCurrentRawStream(self.ctx.device)
-        return s or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's own
+        return torch._C._cuda_getCurrentRawStream(self.ctx.device) or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's
 
     def write(self, block_idx: int, k: torch.Tensor, v: torch.Tensor, index_pos: int) -> None:
         """Rows k, v (batch, seq, n_kv, head_dim) in D (any stride of batch rows and tokens) become the positions index_pos .. of the block's cache, whose
         length is then index_pos + seq: index_pos is the length so far, or an earlier position from which on the cache is written anew."""
-        n_kv = self.ctx.config.num_key_value_heads
-        k = self._rows(k, "k", None, n_kv)
+        self._packed()
+        k, v = self._rows(k, "k", self._kv), self._rows(v, "v", self._kv)
         seq = k.shape[1]
-        v = self._rows(v, "v", seq, n_kv)
-        check(self._lib.cake_b200_cache_write(self.h, block_idx, k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1), v.stride(0), seq, index_pos,
-                                              self._stream()))
+        if v.shape[1] != seq:
+            raise ValueError(f"v has {v.shape[1]} rows, k {seq}")
+        ks, vs = k.stride(), v.stride()
+        check(self._lib.cake_b200_cache_write(self.h, block_idx, k.data_ptr(), ks[1], ks[0], v.data_ptr(), vs[1], vs[0], seq, index_pos, self._stream()))
 
     def read(self, block_idx: int, which: int, first: int = 0, n: Optional[int] = None) -> torch.Tensor:
         """Positions [first, first + n) (to the end without n) of the block's K (which 0) or V (1) rows: (batch, n_kv, n, head_dim) in D."""
-        c = self.ctx.config
-        n = max(0, self.len(block_idx) - first) if n is None else n
-        out = torch.empty((self.batch, c.num_key_value_heads, max(n, 0), c.hd), dtype=self.ctx.torch_dtype, device=self.ctx.torch_device)
+        self._packed()
+        n = self.len(block_idx) - first if n is None else n
+        out = torch.empty((self.batch, self._kv, max(n, 0), self._hd), dtype=self.ctx.torch_dtype, device=self.ctx.torch_device)
         check(self._lib.cake_b200_cache_unpack(self.h, block_idx, which, first, n, out.data_ptr(), self._stream()))
         return out
 
     def attend(self, block_idx: int, q: torch.Tensor, index_pos: int, first: int = 0, scale: float = 0.0) -> torch.Tensor:
         """Attention of the rows q (batch, seq, n_heads, head_dim) in D at positions index_pos .., which the cache holds: row t sees the positions
         first <= j <= index_pos + t (one that sees none is zero).  scale 0: head_dim^-1/2.  (batch, seq, n_heads, head_dim) in D."""
-        q = self._rows(q, "q", None, self.ctx.config.num_attention_heads)
-        out = torch.empty(q.shape, dtype=q.dtype, device=self.ctx.torch_device)
-        check(self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), q.shape[1], index_pos, first, scale,
-                                               self._stream()))
+        self._packed()
+        q = self._rows(q, "q", self._heads)
+        out = q.new_empty(q.shape)
+        qs = q.stride()
+        check(self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), qs[1], qs[0], out.data_ptr(), q.shape[1], index_pos, first, scale, self._stream()))
         return out
 
     def __del__(self):
