@@ -154,6 +154,7 @@ struct cake_b200_ctx {
   void *pc_rows = nullptr;   // rows of such caches in D, for the kernels of prompts
   size_t pc_rows_cap = 0;
   unsigned *pc_tickets = nullptr;
+  cudaMemPool_t pc_pool = nullptr;   // the caches' memory: a closed cache's is the next one's (a new cache of 67 MB: 20 us, 3 ms from the driver)
   cudaEvent_t pc_in = nullptr, pc_out = nullptr;   // a caller's stream in front of this one's work, and behind it
   // head of a batch: its logits where the caller keeps none, its tokens
   void *hd_logits = nullptr;
@@ -679,6 +680,7 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
     if (c->stage_free[i]) cudaEventDestroy(c->stage_free[i]);
   }
   if (c->load_done) cudaEventDestroy(c->load_done);
+  if (c->pc_pool) cudaMemPoolDestroy(c->pc_pool);   // (what caches still hold goes when they do)
   for (cudaEvent_t ev : {c->pc_in, c->pc_out})
     if (ev) cudaEventDestroy(ev);
   if (c->ev_fork) cudaEventDestroy(c->ev_fork);
@@ -957,6 +959,15 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
   CU(cudaSetDevice(c->device));
   if (!c->pc_tickets) {
     CU((cudaError_t)pc::prepare(c->cfg.dtype, c->cfg.head_dim));
+    if (!c->pc_pool) {
+      cudaMemPoolProps props{};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = c->device;
+      CU(cudaMemPoolCreate(&c->pc_pool, &props));
+      uint64_t keep = ~0ull;
+      CU(cudaMemPoolSetAttribute(c->pc_pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    }
     for (cudaEvent_t *ev : {&c->pc_in, &c->pc_out})
       if (!*ev) CU(cudaEventCreateWithFlags(ev, cudaEventDisableTiming));
     if (!c->pc_ws) CU(cudaMalloc(&c->pc_ws, pc::scratch_floats(c->sm_count) * sizeof(float)));
@@ -974,7 +985,12 @@ static int cache_ensure(cake_b200_cache *k, int layer) {
   if (k->k[layer]) return CAKE_B200_OK;
   if (k->bits) {
     const int hd = k->ctx->cfg.head_dim;
-    CU(cudaMalloc(&k->k[layer], (size_t)k->batch * k->ctx->cfg.n_kv_heads * pc::cap_blocks(k->cap) * pc::block_bytes(hd)));
+    cudaStreamCaptureStatus st;
+    CU(cudaStreamIsCapturing(k->ctx->stream, &st));
+    if (st != cudaStreamCaptureStatusNone)   // (the memory would be the graph's)
+      return fail(CAKE_B200_ESTATE, "block %d has no cache memory yet and a capture cannot make it: run the call once before", layer);
+    CU(cudaMallocFromPoolAsync(&k->k[layer], (size_t)k->batch * k->ctx->cfg.n_kv_heads * pc::cap_blocks(k->cap) * pc::block_bytes(hd), k->ctx->pc_pool,
+                               k->ctx->stream));
     return CAKE_B200_OK;
   }
   const size_t bytes = (size_t)k->batch * k->ctx->cfg.n_kv_heads * k->cap * k->ctx->cfg.head_dim * k->ctx->es;
@@ -1006,8 +1022,12 @@ extern "C" void cake_b200_cache_free(cake_b200_cache *k) {
       }
     }
   }
-  for (void *p : k->k)
-    if (p) cudaFree(p);
+  {
+    std::lock_guard<std::mutex> lk(g_live_mu);
+    const bool pool = k->bits && g_live_ctx.count(k->ctx);
+    for (void *p : k->k)
+      if (p) (void)(pool ? cudaFreeAsync(p, k->ctx->stream) : cudaFree(p));
+  }
   for (void *p : k->v)
     if (p) cudaFree(p);
   for (auto &v : k->shift_state)
