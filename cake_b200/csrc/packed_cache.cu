@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t c) {
 // fma, add with rounding down (the integer in the lowest bits) and a multiply-add that moves it to its place: n = floor((x - lo) / step + 1/2) exactly,
 // since (x - lo) inv is exact but for 2^-22 relative and (x - lo) / step is k + 1/2 or at least the last place of x, lo or step away from
 // it: 2^-19 decides the former and leaves the latter, where x's last place is above step 2^-19.
-// 8 x 4096 rows of 8 heads of 128, written and read back: a row per 16 lanes, V in 16-bit stores 102 + 71 us on the device; so 41 + 30.
+// 8 x 4096 rows of 8 heads of 128, written and read back: a row per 16 lanes, V in 16-bit stores 102 + 71 us on the device; so 39 + 30 (29 without the arithmetic).
 template <typename T, bool ODDS_LAST> __device__ __forceinline__ uint32_t encode8(const uint32_t (&c)[4], float lo, float inv) {
   uint32_t w = 0;
 #pragma unroll
@@ -95,7 +95,8 @@ template <typename T, bool ODDS_LAST> __device__ __forceinline__ uint32_t encode
   }
   return w - 0xfb000000u;   // the exponents: 0x4b000000 (1 + 16 + 16^2 ..) mod 2^32
 }
-template <typename T, int HD>
+// BARE: rows as they are, without norm and rotation (41.5 us with their code beside it, unused).
+template <typename T, int HD, bool BARE>
 __global__ void __launch_bounds__(128) write_kernel(const Write a) {
   pdl_launch_dependents();
   constexpr int NG = HD / 32;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(128) write_kernel(const Write a) {
     const uint4 v = in ? *reinterpret_cast<const uint4 *>(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
     c[j][0] = v.x; c[j][1] = v.y; c[j][2] = v.z; c[j][3] = v.w;
   }
-  if (!is_v && (a.cos_t || a.q_norm || a.k_norm)) {   // (a warp's head is one)
+  if (!BARE && !is_v) {   // (a warp's head is one)
     const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
     float inv = 0.f;
     if (nw) {
@@ -923,7 +924,9 @@ int write(cudaStream_t s, int dtype, const Write &a, uint64_t *launches) {
     typedef decltype(t) T;
     const int eights = a.d_pos ? (a.S + 14) / 8 : ((a.pos0 & 7) + a.S + 7) / 8;   // (at any position on the device)
     const long long warps = (long long)a.B * eights * (a.n_q + 2 * a.n_kv);
-    return launch(s, launches, write_kernel<T, hd.value>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, 1, a);
+    const dim3 grid((unsigned)((warps + 3) / 4)), block(128);
+    if (!a.n_q && !a.cos_t && !a.k_norm) return launch(s, launches, write_kernel<T, hd.value, true>, grid, block, 0, 1, a);
+    return launch(s, launches, write_kernel<T, hd.value, false>, grid, block, 0, 1, a);
   });
 }
 int read(cudaStream_t s, int dtype, const Read &a, uint64_t *launches) {
