@@ -303,6 +303,7 @@ struct cake_b200_cache {
   std::vector<uint32_t> last_tok;
   int embed_len = 0;
   unsigned wait_failures = 0;  // the context's count when the cache was created or cleared: another one, and its rows may be no results
+  bool moved = false;  // by cake_b200_cache_write: the decode graph's position is another one until cake_b200_decode_begin
   int bits = 0;  // 4: k holds K and V rows in four bits (packed_cache.cuh), v nothing; 0: rows in D
 };
 
@@ -980,15 +981,20 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
   }
   return cache_create(c, batch, max_seq, bits, out);
 }
+// memory that a captured call would need and does not have: made inside the capture it would be the graph's, if that is allowed at all
+static int no_capture(cudaStream_t s, const char *what) {
+  cudaStreamCaptureStatus st;
+  const cudaError_t e = cudaStreamIsCapturing(s, &st);
+  if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) return CAKE_B200_OK;
+  (void)cudaGetLastError();   // (the default stream while another one captures: an error that ends no capture)
+  return fail(CAKE_B200_ESTATE, "%s is not there yet and a capture cannot make it: run the call once before", what);
+}
 static int cache_ensure(cake_b200_cache *k, int layer) {
   if (layer < 0 || layer >= (int)k->k.size()) return fail(CAKE_B200_EINVAL, "block_idx %d out of range", layer);
   if (k->k[layer]) return CAKE_B200_OK;
   if (k->bits) {
     const int hd = k->ctx->cfg.head_dim;
-    cudaStreamCaptureStatus st;
-    CU(cudaStreamIsCapturing(k->ctx->stream, &st));
-    if (st != cudaStreamCaptureStatusNone)   // (the memory would be the graph's)
-      return fail(CAKE_B200_ESTATE, "block %d has no cache memory yet and a capture cannot make it: run the call once before", layer);
+    RC(no_capture(k->ctx->stream, "a block's part of the cache"));
     CU(cudaMallocFromPoolAsync(&k->k[layer], (size_t)k->batch * k->ctx->cfg.n_kv_heads * pc::cap_blocks(k->cap) * pc::block_bytes(hd), k->ctx->pc_pool,
                                k->ctx->stream));
     return CAKE_B200_OK;
@@ -1086,12 +1092,19 @@ extern "C" int cake_b200_cache_read(cake_b200_cache *k, int block_idx, int which
   return CAKE_B200_OK;
 }
 // ---- caches in four bits (packed_cache.cuh)
+struct OnDevice {   // the calling thread's device is another one's business again afterwards
+  int was = -1;
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&was) != cudaSuccess || was == device) was = -1;
+    else cudaSetDevice(device);
+  }
+  ~OnDevice() { if (was >= 0) cudaSetDevice(was); }
+};
 static uint64_t *launch_counter(cake_b200_ctx *c) { return c->capturing ? &c->g_kernels : &c->launches; }
 static int packed_call(const cake_b200_cache *k, int block_idx, const char *what) {
   if (!k) return fail(CAKE_B200_EINVAL, "null argument");
   if (!k->bits) return fail(CAKE_B200_EINVAL, "%s is for caches of cake_b200_cache_create_packed", what);
   if (block_idx < 0 || block_idx >= (int)k->len.size()) return fail(CAKE_B200_EINVAL, "block_idx %d out of range", block_idx);
-  CU(cudaSetDevice(k->device));
   RC(check_waits(k->ctx));
   return check_cache(k);
 }
@@ -1112,12 +1125,14 @@ template <typename F> static int in_order_of(cake_b200_ctx *c, void *stream, F &
 extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const void *k_dev, size_t k_tok, size_t k_batch, const void *v_dev,
                                      size_t v_tok, size_t v_batch, int seq, int index_pos, void *stream) {
   RC(packed_call(k, block_idx, "cache_write"));
+  const OnDevice dev(k->device);
   if (!k_dev || !v_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
   if (unaligned(k_dev, k_tok, k_batch) || unaligned(v_dev, v_tok, v_batch))
     return fail(CAKE_B200_EINVAL, "cache_write takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
   if (index_pos < 0 || index_pos > k->len[block_idx])
     return fail(CAKE_B200_ESTATE, "block %d: index_pos %d is not within the cache's %d positions", block_idx, index_pos, k->len[block_idx]);
   if ((long long)index_pos + seq > k->cap) return fail(CAKE_B200_ESTATE, "index_pos %d + seq %d exceeds cache capacity %d", index_pos, seq, k->cap);
+  if (!k->k[block_idx] && stream) RC(no_capture((cudaStream_t)stream, "a block's part of the cache"));
   RC(cache_ensure(k, block_idx));
   const cake_b200_config &f = k->ctx->cfg;
   pc::Write a{k->k[block_idx], k_dev, v_dev, (long long)k_tok, (long long)k_batch, (long long)v_tok, (long long)v_batch};
@@ -1125,11 +1140,13 @@ extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const vo
   return in_order_of(k->ctx, stream, [&]() -> int {
     CU((cudaError_t)pc::write(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
     k->len[block_idx] = index_pos + seq;
+    k->moved = true;
     return CAKE_B200_OK;
   });
 }
 extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int which, int first, int n, void *out_dev, void *stream) {
   RC(packed_call(k, block_idx, "cache_unpack"));
+  const OnDevice dev(k->device);
   if (which != 0 && which != 1) return fail(CAKE_B200_EINVAL, "which is 0 (K) or 1 (V), not %d", which);
   if (first < 0 || n < 1 || (long long)first + n > k->len[block_idx])
     return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, first, n, k->len[block_idx]);
@@ -1161,6 +1178,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
     const int group = (int)std::max<size_t>(1, std::min<size_t>(kc->batch, PC_EXPAND_MOST / (2 * slab)));
     const size_t need = group * (2 * slab + marks);
     if (need > c->pc_rows_cap) {
+      RC(no_capture(c->stream, "memory for the rows that a call of many rows expands"));
       CU(cudaStreamSynchronize(c->stream));
       if (c->pc_rows) { cudaFree(c->pc_rows); c->pc_rows = nullptr; c->pc_rows_cap = 0; }
       CU(cudaMalloc(&c->pc_rows, need));
@@ -1187,6 +1205,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
 extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq,
                                       int index_pos, int first, float scale, void *stream) {
   RC(packed_call(k, block_idx, "cache_attend"));
+  const OnDevice dev(k->device);
   if (!q_dev || !out_dev || seq < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
   if (unaligned(q_dev, q_tok, q_batch) || unaligned(out_dev))
     return fail(CAKE_B200_EINVAL, "cache_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
@@ -4380,6 +4399,7 @@ extern "C" int cake_b200_decode_begin(cake_b200_ctx *c, uint32_t first_token, in
     if (kc->len[l] != index_pos)
       return fail(CAKE_B200_ESTATE, "block %d: index_pos %d != cache length %d", l, index_pos, kc->len[l]);
   if (index_pos >= kc->cap) return fail(CAKE_B200_ESTATE, "cache full");
+  kc->moved = false;
   if (c->g_rank == 0 && first_token >= (uint32_t)c->cfg.vocab)  // candle's index_select fails on an out-of-range id (text_model.rs:271)
     return fail(CAKE_B200_EINVAL, "token id %u out of range (vocab %d)", first_token, c->cfg.vocab);
   set_int_kernel<<<1, 1, 0, c->stream>>>(kc->d_pos, index_pos);
@@ -4397,6 +4417,7 @@ extern "C" int cake_b200_decode_run(cake_b200_ctx *c, int n_steps) {
   cake_b200_cache *kc = c->g_cache;
   RC(check_waits(c));
   RC(check_cache(kc));
+  if (kc->moved) return fail(CAKE_B200_ESTATE, "rows have been written into the cache: cake_b200_decode_begin first");
   int cur = c->g_block_idx.empty() ? 0 : kc->len[c->g_block_idx[0]];
   if (!c->g_block_idx.empty() && cur + n_steps > kc->cap)
     return fail(CAKE_B200_ESTATE, "decode_run: %d steps from position %d exceed cache capacity %d", n_steps, cur, kc->cap);

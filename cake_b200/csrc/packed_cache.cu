@@ -401,7 +401,7 @@ constexpr int SP_STAGES = 4, SP_WARPS = 8, SP_CLUSTER = 8;
 constexpr int sp_per_sm(int hd, int nt) { return hd * nt <= 128 ? 2 : 1; }   // CTAs that 128 or 255 registers a thread leave room for
 struct Split {
   Attend a;
-  int cols, units, n_blk;        // rows of a (batch row, key head); blocks of a unit (0: the device knows)
+  int cols, units;               // rows of a (batch row, key head); units in all
   int cluster;                   // CTAs of a cluster, 0: the line
   float *ws;                     // [2 CTA + (part that begins behind the CTA's first block)] of {O [col][hd], m [col], l [col]}
   unsigned *tickets;             // [first CTA of a cut unit], zero between launches
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        s[nt][i] = ex2(fmaf(s[nt][i], sc[nt][i & 1], ce - m[nt][i & 1]));
+        s[nt][i] = EDGE && s[nt][i] == -INFINITY ? 0.f : ex2(fmaf(s[nt][i], sc[nt][i & 1], ce - m[nt][i & 1]));   // (sc may have become 0)
         l[nt][i & 1] += s[nt][i];
       }
     auto times = [](float w, float x) { return EDGE && w == 0.f ? 0.f : w * x; };   // a key that a row does not see may be anything
@@ -975,7 +975,6 @@ size_t scratch_tickets(int sms) { return (size_t)sms * 2; }
 template <typename T, int HD, int NT, int PK> static int big_smem() {
   cudaError_t e = cudaFuncSetAttribute(attend_split_kernel<T, HD, NT, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(sp_smem<HD, NT>(), 120 * 1024));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_split_kernel<T, HD, NT, PK>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_split_kernel<T, HD, NT, PK>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return (int)e;
 }
 int prepare(int dtype, int hd) {

@@ -486,12 +486,14 @@ class Cache {  // cache.rs:9
  public:
   cake_b200_cache *h = nullptr;
   cake_b200_ctx *ctx;
-  int batch, max_seq;
-  Cache(cake_b200_ctx *c, int b, int ms) : ctx(c), batch(b), max_seq(ms) { check(cake_b200_cache_create(c, b, ms, &h), "cache"); }
+  int batch, max_seq, bits;  // bits 4: K and V rows in four bits, 0: in D
+  Cache(cake_b200_ctx *c, int b, int ms, int bits_ = 0) : ctx(c), batch(b), max_seq(ms), bits(bits_) {
+    check(bits ? cake_b200_cache_create_packed(c, b, ms, bits, &h) : cake_b200_cache_create(c, b, ms, &h), "cache");
+  }
   ~Cache() { cake_b200_cache_free(h); }
   Cache(const Cache &) = delete;
   void clear() { check(cake_b200_cache_clear(h), "cache.clear"); }                          // cache.rs:247-253
-  std::unique_ptr<Cache> as_new() const { return std::make_unique<Cache>(ctx, batch, max_seq); }  // cache.rs:241-245
+  std::unique_ptr<Cache> as_new() const { return std::make_unique<Cache>(ctx, batch, max_seq, bits); }  // cache.rs:241-245
   int len(int block_idx) const { return cake_b200_cache_len(h, block_idx); }
 };
 
@@ -502,12 +504,12 @@ struct Context {  // cake/mod.rs:41-65
   std::unique_ptr<Cache> cache;
   std::string dtype_name;
   // `worker_layers`: non-empty on a worker — only the shards that hold those layers are mapped
-  Context(const std::string &model_dir, int device, int dtype, int max_seq = 0, const std::vector<std::string> &worker_layers = {})
+  Context(const std::string &model_dir, int device, int dtype, int max_seq = 0, const std::vector<std::string> &worker_layers = {}, int cache_bits = 0)
       : config(Config::from_path(model_dir + "/config.json", dtype, max_seq)), var_builder(new VarBuilder(model_dir, worker_layers)) {
     config.model_prefix = VarBuilder::detect_model_prefix(model_dir, config.model_prefix);
     dtype_name = dtype == CAKE_B200_BF16 ? "BF16" : "F16";
     check(cake_b200_ctx_create(device, &config.c, &h), "ctx_create");
-    cache.reset(new Cache(h, 1, config.c.max_seq));
+    cache.reset(new Cache(h, 1, config.c.max_seq, cache_bits));
   }
   ~Context() {
     cache.reset();

@@ -2,6 +2,7 @@
 // cake's interface) and libcake_b200.so.  It takes token ids instead of text (tokenizer / chat template are outside
 // the path):   cake_run <model_dir> --prompt-ids 1,2,3 [-n 32] [--dtype bf16|f16] [--repeat-penalty 1.0]
 // <model_dir> holds config.json + model.safetensors (or model.safetensors.index.json + shards), HF layout.
+// --cache-bits 4: the conversation's K and V rows in four bits (cake_b200_cache_create_packed).
 // Prints one line:  tokens: t0 t1 ...   and   tok/s as the reference defines it (master.rs:160-166).
 // --show-config: parse config.json only and print the resolved block configuration (needs no GPU).
 #include <cstdio>
@@ -13,13 +14,13 @@ using namespace cake_host;
 
 int main(int argc, char **argv) {
   if (argc < 2) {
-    fprintf(stderr, "usage: %s <model_dir> --prompt-ids a,b,c [-n N] [--dtype bf16|f16] [--repeat-penalty P] [--max-seq S]\n", argv[0]);
+    fprintf(stderr, "usage: %s <model_dir> --prompt-ids a,b,c [-n N] [--dtype bf16|f16] [--repeat-penalty P] [--max-seq S] [--cache-bits 4]\n", argv[0]);
     return 2;
   }
   std::string dir = argv[1];
   std::vector<uint32_t> prompt;
   size_t n = 32;
-  int dtype = CAKE_B200_BF16, max_seq = 0;
+  int dtype = CAKE_B200_BF16, max_seq = 0, cache_bits = 0;
   float rp = 1.0f;
   bool show_config = false;
   for (int i = 2; i < argc; i++) {
@@ -33,6 +34,7 @@ int main(int argc, char **argv) {
     else if (a == "--dtype") dtype = (next() == "f16") ? CAKE_B200_F16 : CAKE_B200_BF16;
     else if (a == "--repeat-penalty") rp = std::stof(next());
     else if (a == "--max-seq") max_seq = std::stoi(next());
+    else if (a == "--cache-bits") cache_bits = std::stoi(next());
     else if (a == "--show-config") show_config = true;
   }
   try {
@@ -49,7 +51,7 @@ int main(int argc, char **argv) {
              [&]() { std::string g; for (bool b : k.global_layers) g += b ? '1' : '0'; return g.empty() ? std::string("-") : g; }().c_str());
       return 0;
     }
-    Context ctx(dir, 0, dtype, max_seq);
+    Context ctx(dir, 0, dtype, max_seq, {}, cache_bits);
     auto model = TextModelBase::load(ctx);
     model->repeat_penalty = rp;
     Master master(*model);

@@ -182,7 +182,7 @@ struct B200Backend : cw::Backend {
 int main(int argc, char **argv) {
   std::string dir, layers, address = "127.0.0.1:10128", key, topology, name;
   bool echo = false, reflect = false, has_key = false, list_tensors = false;
-  int dtype = CAKE_B200_BF16, max_seq = 0, device = 0, connections = -1;
+  int dtype = CAKE_B200_BF16, max_seq = 0, device = 0, connections = -1, cache_bits = 0;
   for (int i = 1; i < argc; i++) {
     std::string a = argv[i];
     auto next = [&]() -> std::string { return i + 1 < argc ? std::string(argv[++i]) : std::string(); };
@@ -191,6 +191,7 @@ int main(int argc, char **argv) {
     else if (a == "--cluster-key") { key = next(); has_key = true; }
     else if (a == "--dtype") dtype = (next() == "f16") ? CAKE_B200_F16 : CAKE_B200_BF16;
     else if (a == "--max-seq") max_seq = std::stoi(next());
+    else if (a == "--cache-bits") cache_bits = std::stoi(next());
     else if (a == "--device") device = std::stoi(next());
     else if (a == "--connections") connections = std::stoi(next());
     else if (a == "--topology") topology = next();
@@ -243,7 +244,7 @@ int main(int argc, char **argv) {
   }
   if (!echo && (dir.empty() || layers.empty())) {
     fprintf(stderr, "usage: %s <model_dir> --layers model.layers.A-B [--address host:port] [--cluster-key K] [--dtype bf16|f16] "
-                    "[--max-seq S] [--device N] [--connections N]\n       %s --echo [--reflect] [--address host:port] [--cluster-key K]\n", argv[0], argv[0]);
+                    "[--max-seq S] [--cache-bits 4] [--device N] [--connections N]\n       %s --echo [--reflect] [--address host:port] [--cluster-key K]\n", argv[0], argv[0]);
     return 2;
   }
   try {
@@ -257,7 +258,7 @@ int main(int argc, char **argv) {
       be.reset(new cw::EchoBackend());
     } else {
       const std::vector<std::string> names = expand_layers(layers);
-      ctx.reset(new Context(dir, device, dtype, max_seq, names));
+      ctx.reset(new Context(dir, device, dtype, max_seq, names, cache_bits));
       be.reset(new B200Backend(*ctx, names, device));
     }
     cw::WireWorker w(*be, host, port, has_key ? &key : nullptr);

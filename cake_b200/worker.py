@@ -58,6 +58,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--cluster-key")
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "f16"])
     ap.add_argument("--max-seq", type=int, default=0)
+    ap.add_argument("--cache-bits", type=int, default=0, choices=[0, 4], help="4: the sessions' K and V rows in four bits")
     ap.add_argument("--device", type=int, default=0)
     ap.add_argument("--echo", action="store_true")
     a = ap.parse_args(argv)
@@ -73,7 +74,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         from .model import B200Transformer, Context
         from .wire import B200Backend
         cfg, vb = open_model(a.model_dir, {"self": {"layers": names}}, worker="self")
-        ctx = Context(cfg, vb, a.dtype, device=a.device, max_seq=a.max_seq or None)
+        ctx = Context(cfg, vb, a.dtype, device=a.device, max_seq=a.max_seq or None, cache_bits=a.cache_bits)
         backend = B200Backend(ctx, {n: B200Transformer.load(n, ctx) for n in names})
     w = WireWorker(backend, host, int(port), a.cluster_key)
     print(f"listening on {w.address}", flush=True)

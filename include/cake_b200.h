@@ -395,8 +395,9 @@ int cake_b200_cache_fill_synthetic(cake_b200_cache *, const int *block_idx, int 
  * what the cache holds, the rows of the same call included, so that a prompt may be cut anywhere.  cake_b200_cache_read returns the entries' values
  * rounded to D.
  * The three calls below run on the ctx's stream.  stream: NULL, or the cudaStream_t that their tensors belong to (cudaStreamLegacy for the default
- * stream): the call waits for what that stream holds so far, and the stream goes on behind the call; it may be capturing, once the same call has run
- * outside a capture (memory grows on first use). */
+ * stream): the call waits for what that stream holds so far, and the stream goes on behind the call.  It may be capturing, once the same call has run
+ * outside a capture (memory is made on first use; CAKE_B200_ESTATE otherwise); graphs captured from calls of one ctx share its scratch like the calls
+ * themselves and are not replayed at the same time. */
 int cake_b200_cache_create_packed(cake_b200_ctx *, int batch, int max_seq, int bits, cake_b200_cache **out);
 /* Rows k, v (batch, seq, n_kv, head_dim) in D, as they are, join block_idx's part of the cache at index_pos, which is its length or less: what is behind
  * index_pos is dropped and the length becomes index_pos + seq (CAKE_B200_ESTATE where index_pos is beyond the length or the rows beyond the

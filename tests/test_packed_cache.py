@@ -358,7 +358,7 @@ def test_scales_and_sizes_of_entries(dtype):
     cache = Cache(ctx, 1, n, bits=4)
     sizes = (1.0, 2.0 ** -9, 2.0 ** 9) if dtype == "f16" else (1.0, 2.0 ** -60, 2.0 ** 60)
     for size in sizes:
-        for scale in (None, 1e-3, 1.0):
+        for scale in (None, 1e-3, 1.0, 1e-30):
             w = v * size
             cache.write(0, k, w, 0)
             check_attention(cache.attend(0, q / 4 if scale == 1.0 else q, n - 1, scale=scale or 0.0) / size, q / 4 if scale == 1.0 else q, k, w / size, n - 1, 0, dtype, scale)
@@ -470,6 +470,78 @@ def test_captured_calls_share_a_context():
             check_attention(caches[i].attend(0, q, 1500 - s), q, k, v, 1500 - s, 0, "bf16")
     torch.cuda.synchronize()
     del graphs, g
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture():
+    """Memory that a call has to make cannot come in a capture: the call is refused, and the refusal leaves the capture usable."""
+    ctx = ctx_for(32, 8, 128, "bf16")
+    cache = Cache(ctx, 1, 600, bits=4)
+    k, v = rows(1, 600, 8, 128, "bf16", 1), rows(1, 600, 8, 128, "bf16", 2)
+    q = queries(1, 600, 32, 128, "bf16", 3)
+    cache.write(1, k[:, :1], v[:, :1], 0)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(CakeB200Error) as e:
+            cache.write(0, k, v, 0)
+        assert e.value.code == ESTATE and cache.len(0) == 0
+        cache.write(1, k, v, 0)
+        one = cache.attend(1, q[:, 599:], 599)
+        with pytest.raises(CakeB200Error) as e:
+            cache.attend(1, q, 0)
+        assert e.value.code == ESTATE
+    g.replay()
+    check_attention(one, q[:, 599:], k, v, 599, 0, "bf16")
+    check_attention(cache.attend(1, q, 0), q, k, v, 0, 0, "bf16")
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        many = cache.attend(1, q, 0)
+    q.copy_(queries(1, 600, 32, 128, "bf16", 4))
+    g2.replay()
+    check_attention(many, q, k, v, 0, 0, "bf16")
+    torch.cuda.synchronize()
+    del g, g2
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_closed_caches_and_contexts():
+    """A closed cache's memory is the next one's; caches may outlive their context; the calling thread keeps its device and stream."""
+    ctx = ctx_for(8, 2, 128, "bf16")
+    for i in range(6):
+        cache, k, v = filled(ctx, 1 + i % 2, 700, i, "bf16")
+        q = queries(1 + i % 2, 1, 8, 128, "bf16", i)
+        check_attention(cache.attend(0, q, 699), q, k, v, 699, 0, "bf16")
+        cache.close()
+    left, k, v = filled(ctx, 1, 50, 9, "bf16")
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+    h, left.h = left.h, None                     # the library's own order: the context first
+    ctx._children = []
+    ctx.sync()
+    lib().cake_b200_ctx_destroy(ctx.h)
+    lib().cake_b200_cache_free(h)
+    ctx.h = None
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_decode_graph_asks_for_its_position_after_rows_were_written():
+    cfg = medium_config(num_hidden_layers=1)
+    ctx = Context(cfg, checkpoint(cfg, "bf16", std=0.05, peaked=True), "bf16", cache_bits=4)
+    m = TextModelBase.load(ctx)
+    m.forward([[1, 2, 3, 4, 5, 6, 7, 8]], 0)
+    m.index_pos = 8
+    m.decode_build()
+    m.decode_greedy(5, 2)
+    k = rows(1, 3, 2, 64, "bf16", 1)
+    ctx.cache.write(0, k, k, 6)
+    with pytest.raises(CakeB200Error) as e:
+        check(lib().cake_b200_decode_run(ctx.h, 1))
+    assert e.value.code == ESTATE
+    m.index_pos = 9
+    assert len(m.decode_greedy(5, 2)) == 2 and ctx.cache.len(0) == 11
     ctx.close()
 
 
@@ -658,7 +730,26 @@ def test_batch_rows_are_their_own():
     ctx.close()
 
 
-def test_command_line_names_the_choice():
-    from cake_b200 import run
-    with pytest.raises(SystemExit):
-        run.main(["x", "--cache-bits", "3"])
+def test_command_lines_name_the_choice():
+    from cake_b200 import run, worker
+    for main in (run.main, worker.main):
+        with pytest.raises(SystemExit):
+            main(["x", "--cache-bits", "3"])
+
+
+@pytest.mark.gpu
+def test_compiled_host_gives_the_same_tokens(tmp_path):
+    from tests.test_cpp_host import RUN, _write_model
+    from cake_b200.build import build
+    build()
+    cfg = medium_config(num_hidden_layers=2)
+    sd = checkpoint(cfg, "bf16", std=0.05, peaked=True)
+    _write_model(tmp_path, cfg, sd)
+    prompt = np.random.default_rng(5).integers(0, cfg.vocab_size - 1, 21).tolist()
+    out = [subprocess.run([RUN, str(tmp_path), "--prompt-ids", ",".join(map(str, prompt)), "-n", "10", "--cache-bits", bits], capture_output=True, text=True,
+                          timeout=120) for bits in ("4", "3")]
+    assert out[0].returncode == 0, out[0].stderr
+    assert out[1].returncode == 1 and "4 bits" in out[1].stderr
+    ctx = Context(cfg, sd, "bf16", cache_bits=4)
+    assert [int(t) for t in out[0].stdout.splitlines()[0].split(":")[1].split()] == Master(TextModelBase.load(ctx)).generate_text(prompt, 10)["tokens"]
+    ctx.close()
