@@ -396,19 +396,22 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 //
 // Who takes which blocks: a unit is 8 NT / PK rows of a (batch row, key head).  Short caches: the CTAs of a cluster cut a unit's blocks between them and
 // join over the cluster's shared memory.  Else all units' blocks lie in one line that the grid, two CTAs per SM, cuts into equal parts; a CTA's part of
-// a unit that others have parts of goes to ws, and the last one to come joins them, in the order of the line.
-constexpr int SP_STAGES = 4, SP_WARPS = 8, SP_CLUSTER = 8;
+// a unit that others have parts of goes to ws, and the last one to come joins them, in the order of the line.  (A cluster's CTAs send their sums to
+// the one that joins them: one barrier behind, where reading them there takes a second one before anybody leaves.)
+constexpr int SP_STAGES = 4, SP_WARPS = 8, SP_CLUSTER_LOG2 = 3;
 constexpr int sp_per_sm(int hd, int nt) { return hd * nt <= 128 ? 2 : 1; }   // CTAs that 128 or 255 registers a thread leave room for
 struct Split {
   Attend a;
-  int cols, units;               // rows of a (batch row, key head); units in all
-  int cluster;                   // CTAs of a cluster, 0: the line
+  int cols, col_blocks, units;   // rows of a (batch row, key head), pieces that they are cut into; units in all
+  int cluster_log2;              // CTAs of a cluster, a unit for each of the grid's (y, z); -1: the line
   float *ws;                     // [2 CTA + (part that begins behind the CTA's first block)] of {O [col][hd], m [col], l [col]}
   unsigned *tickets;             // [first CTA of a cut unit], zero between launches
 };
+// what a CTA of a cluster is sent: for its share of the results, from every CTA, four sums and their m and l
+template <int HD, int NT> __host__ __device__ constexpr int sp_recv() { return 8 * NT * (HD / 4) * 32; }
 template <int HD, int NT> __host__ __device__ constexpr int sp_smem() {
   const int w = SP_WARPS, ring = w * SP_STAGES * block_bytes(HD), out = w * 8 * NT * (HD * 4 + 16) + w * 8 * NT * 8;
-  return (ring > out ? ring : out) + 8 * NT * (HD + 4) * 4 + 16;
+  return (ring > out ? ring : out) + sp_recv<HD, NT>() + 16;
 }
 // a block into a stage, by the whole warp
 template <int HD> __device__ __forceinline__ void copy_block(uint32_t dst, const char *src, int lane) {
@@ -447,13 +450,8 @@ __device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t c) {   // pairs of
   const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void ld_cluster4(uint32_t addr, float (&v)[4]) {
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
 template <typename T, int HD, int NT, int PK>
@@ -466,18 +464,18 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
   const int half = PK == 2 ? t >> 1 : 0, tc = PK == 2 ? t & 1 : t;
   unsigned char *ring = sp_raw + warp * SP_STAGES * block_bytes(HD);
   int *last = reinterpret_cast<int *>(sp_raw + sp_smem<HD, NT>() - 16);
-  float *sr = reinterpret_cast<float *>(last) - 8 * NT * (HD + 4);   // the CTA's sums [col][hd], m, l and 1 / l [col]
+  float *recv = reinterpret_cast<float *>(last) - sp_recv<HD, NT>() / 4;   // [item of mine][CTA of the cluster][8]
+  const bool in_line = p.cluster_log2 < 0;
+  if (p.cluster_log2 > 0) cluster_arrive_relaxed();   // (waited for where the first sums go to another CTA: it has begun by then)
   pdl_launch_dependents();
   pdl_wait();
-  const int G = a.n_heads / a.n_kv, col_blocks = (p.cols + COLS - 1) / COLS;
+  const int G = a.n_heads / a.n_kv;
   const int pos0 = a.d_pos ? *a.d_pos : a.pos0;
   const int first = a.d_pos ? (a.window > 0 ? max(0, pos0 + 1 - a.window) : 0) : a.first;
   const int blk0 = first >> 4, n_blk = max(0, ((pos0 + a.S - 1) >> 4) - blk0 + 1);   // of a unit (its own rows may see fewer)
-  const long long line = (long long)p.units * n_blk;
-  // this CTA's blocks of the line, or of its unit
-  const int rank = p.cluster ? (int)(blockIdx.x % (unsigned)p.cluster) : 0;
+  const long long line = in_line ? (long long)p.units * n_blk : 0;
   const long long ctas = min((long long)gridDim.x, (line + WARPS - 1) / WARPS);   // that the line is cut between: none of them without a block
-  if (!p.cluster && blockIdx.x >= ctas) return;
+  if (in_line && blockIdx.x >= ctas) return;
   // first block of a CTA, CTA of a block (whole CTAs for a unit where their number divides: a part of its own costs a CTA some 3 us)
   auto start_of = [&](int cta) {
     return line * ctas >> 32 ? line * cta / ctas : (long long)((unsigned)line * (unsigned)cta / (unsigned)ctas);
@@ -485,16 +483,20 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
   auto cta_of = [&](long long x) {
     return line * ctas >> 32 ? (int)(((x + 1) * ctas - 1) / line) : (int)(((unsigned)(x + 1) * (unsigned)ctas - 1u) / (unsigned)line);
   };
-  const long long unit_at = (long long)(blockIdx.x / (unsigned)max(1, p.cluster)) * n_blk;
-  long long at = p.cluster ? unit_at + n_blk * rank / p.cluster : start_of(blockIdx.x);
-  const long long end = p.cluster ? unit_at + n_blk * (rank + 1) / p.cluster : start_of(blockIdx.x + 1);
+  const int rank = in_line ? 0 : (int)blockIdx.x, lg = max(0, p.cluster_log2);
+  // this CTA's blocks of the line, or of its unit
+  long long at = in_line ? start_of(blockIdx.x) : n_blk * rank >> lg;
+  const long long end = in_line ? start_of(blockIdx.x + 1) : n_blk * (rank + 1) >> lg;
   // ---- one unit's blocks
 #pragma unroll 1
   for (bool again = true; again;) {
-  const int unit = p.cluster ? (int)(blockIdx.x / (unsigned)p.cluster) : n_blk ? (int)(at / n_blk) : 0;
+  const int unit = in_line ? (int)(at / n_blk) : 0;
+  const int heads_at = in_line ? unit : (int)blockIdx.y, piece = p.col_blocks == 1 ? 0 : heads_at % p.col_blocks;
+  const int kvh_b = p.col_blocks == 1 ? heads_at : heads_at / p.col_blocks;
+  const int c0 = piece * COLS, kvh = in_line ? kvh_b % a.n_kv : kvh_b, b = in_line ? kvh_b / a.n_kv : (int)blockIdx.z;
   const long long unit0 = (long long)unit * n_blk, stop = min(end, unit0 + n_blk);
-  const int c0 = unit % col_blocks * COLS, kvh = unit / col_blocks % a.n_kv, b = unit / col_blocks / a.n_kv;
-  const int n_cols = min(COLS, p.cols - c0), pos_lo = pos0 + c0 / G, pos_hi = pos0 + (c0 + n_cols - 1) / G;   // the rows' first and last position
+  auto tok_of = [&](int c) { return a.S == 1 ? 0 : c / G; };
+  const int n_cols = min(COLS, p.cols - c0), pos_lo = pos0 + tok_of(c0), pos_hi = pos0 + tok_of(c0 + n_cols - 1);   // the rows' first and last position
   const int mine0 = blk0 + (int)(at - unit0), n_here = (int)(stop - at);
   const int n_mine = max(0, (n_here - warp + WARPS - 1) / WARPS);   // this warp's blocks: mine0 + warp, + WARPS, ...
   const char *src = reinterpret_cast<const char *>(a.cache) + ((size_t)(b * a.n_kv + kvh) * a.blocks + mine0 + warp) * block_bytes(HD) + lane * 16;
@@ -511,7 +513,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
   int cpos[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    const int c = c0 + (PK == 2 ? g & 3 : nt * 8 + g), tok = c / G;
+    const int c = c0 + (PK == 2 ? g & 3 : nt * 8 + g), tok = tok_of(c);
     const bool in = c < p.cols;
     const T *q = reinterpret_cast<const T *>(a.q) + b * a.q_batch + (long long)tok * a.q_tok + (size_t)(kvh * G + c - tok * G) * HD + 8 * t;
     uint4 raw[NG];
@@ -528,7 +530,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = min(141 - (int)(__float_as_uint(top) >> 23), 100);   // 2^14 <= top 2^e < 2^15
-    const float up = ldexpf(1.f, e), down = ldexpf(a.scale * 1.4426950408889634f, -e);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23), down = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e) << 23);
     sc[nt][0] = __shfl_sync(0xffffffffu, down, 8 * tc);
     sc[nt][1] = __shfl_sync(0xffffffffu, down, 8 * tc + 4);
 #pragma unroll
@@ -559,7 +561,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       }
     }
 #pragma unroll
-    for (int e2 = 0; e2 < 2; e2++) cpos[nt][e2] = pos0 + min(c0 + nt * 8 + 2 * tc + e2, p.cols - 1) / G;
+    for (int e2 = 0; e2 < 2; e2++) cpos[nt][e2] = pos0 + tok_of(min(c0 + nt * 8 + 2 * tc + e2, p.cols - 1));
   }
   float o[NT][2 * NG][4] = {}, mid[NT][MG][2] = {}, m[NT][2], l[NT][2] = {};
   float ce = 0.f, step_lim = 0.f;
@@ -778,77 +780,71 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       }
     }
   __syncthreads();
-  const bool whole = p.cluster ? p.cluster == 1 : n_here == n_blk;   // nobody else has a part
-  if (threadIdx.x < COLS) {
-    const int col = threadIdx.x;
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm[w * COLS + col]);
-    for (int w = 0; w < WARPS; w++) {
-      const float f = sm[w * COLS + col] == -INFINITY ? 0.f : ex2(sm[w * COLS + col] - M);
-      L += f * sl[w * COLS + col];
-      sm[w * COLS + col] = f;
-    }
-    sr[COLS * HD + col] = M;
-    sr[COLS * HD + COLS + col] = L;
-    sr[COLS * HD + 2 * COLS + col] = L == 0.f ? 0.f : 1.f / L;
-  }
-  __syncthreads();
-  auto put = [&](int col, int d, const float (&v)[4], float f) {
-    const int c = c0 + col, tok = c / G;
+  const bool whole = in_line ? n_here == n_blk : lg == 0;   // nobody else has a part
+  auto put = [&](int col, int d, const float (&v)[4], float L) {
+    const int c = c0 + col, tok = tok_of(c);
+    const float f = L == 0.f ? 0.f : 1.f / L;   // 0: the row sees nothing
     T *y = reinterpret_cast<T *>(a.out) + ((size_t)(b * (long long)a.S + tok) * a.n_heads + kvh * G + c - tok * G) * HD + d;
     *reinterpret_cast<uint2 *>(y) = make_uint2(pack2x<T>(v[0] * f, v[1] * f), pack2x<T>(v[2] * f, v[3] * f));
   };
   // parts of this unit, where there are several: CTAs first_cta .., in the line
-  const int first_cta = whole || p.cluster ? 0 : cta_of(unit0), parts = whole || p.cluster ? 1 : cta_of(unit0 + n_blk - 1) - first_cta + 1;
-  const bool behind = !whole && start_of(first_cta) < unit0;   // the first CTA has blocks of another unit in front
+  const bool parted = in_line && !whole;
+  const int first_cta = parted ? cta_of(unit0) : 0, parts = parted ? cta_of(unit0 + n_blk - 1) - first_cta + 1 : 1;
+  const bool behind = parted && start_of(first_cta) < unit0;   // the first CTA has blocks of another unit in front
   auto slot_of = [&](int cta) { return p.ws + (size_t)(2 * cta + (cta == first_cta && behind ? 1 : 0)) * PART; };
-  float *part = whole || p.cluster ? sr : slot_of(blockIdx.x);
   const int items = n_cols * (HD / 4);
+  if (lg) cluster_wait();   // every CTA of the cluster has begun
   for (int i = threadIdx.x; i < items; i += WARPS * 32) {
     const int col = i / (HD / 4), d = i % (HD / 4) * 4;
-    float v[4] = {};
+    float mw[WARPS], M = -INFINITY, L = 0.f, v[4] = {};
 #pragma unroll
     for (int w = 0; w < WARPS; w++) {
-      const float f = sm[w * COLS + col];
+      mw[w] = sm[w * COLS + col];
+      M = fmaxf(M, mw[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
       const float4 x = *reinterpret_cast<const float4 *>(&so[(w * COLS + col) * OUT_LD + d]);
+      L = fmaf(f, sl[w * COLS + col], L);
       if (f != 0.f) {
         v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
       }
     }
-    if (whole) put(col, d, v, sr[COLS * HD + 2 * COLS + col]);
-    else *reinterpret_cast<float4 *>(&part[col * HD + d]) = make_float4(v[0], v[1], v[2], v[3]);
+    if (whole) put(col, d, v, L);
+    else if (parted) {
+      float *part = slot_of(blockIdx.x);
+      *reinterpret_cast<float4 *>(&part[col * HD + d]) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) {
+        part[COLS * HD + col] = M;
+        part[COLS * HD + COLS + col] = L;
+      }
+    } else {   // result i is CTA i mod 2^lg's
+      const uint32_t to = cluster_map(smem_u32(recv + ((size_t)(i >> lg << lg) + rank) * 8), (uint32_t)(i & ((1 << lg) - 1)));
+      st_cluster4(to, v[0], v[1], v[2], v[3]);
+      st_cluster4(to + 16, M, L, 0.f, 0.f);
+    }
   }
-  if (p.cluster > 1) {
-    // ---- the cluster's CTAs take an equal share of the results each; neighbouring lanes read the parts of one ---------------
+  if (lg) {
+    // ---- the cluster's CTAs join an equal share of the results each, from what they were sent: nobody reads another's memory ----
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    const int P = p.cluster, who = lane & (P - 1);
-    const uint32_t theirs = cluster_map(smem_u32(sr), (uint32_t)who);
-    for (int i0 = 0; i0 < items; i0 += WARPS * 32) {   // (the same trips for every lane)
-      const int i = i0 + (int)threadIdx.x / P * P + rank, at_col = min(i, items - 1) / (HD / 4), d = min(i, items - 1) % (HD / 4) * 4;
-      const float mm = ld_cluster(theirs + (COLS * HD + at_col) * 4);
-      float L = ld_cluster(theirs + (COLS * HD + COLS + at_col) * 4), v[4];
-      ld_cluster4(theirs + (at_col * HD + d) * 4, v);
-      float M = mm;
-      for (int o2 = 1; o2 < P; o2 <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o2));
-      const float f = mm == -INFINITY ? 0.f : ex2(mm - M);
-      L *= f;
+    for (int i = ((int)threadIdx.x << lg) + rank; i < items; i += WARPS * 32 << lg) {
+      const float *x = recv + (size_t)(i - rank) * 8;
+      float M = -INFINITY, L = 0.f, v[4] = {};
+      for (int s = 0; s < 1 << lg; s++) M = fmaxf(M, x[8 * s + 4]);
+      for (int s = 0; s < 1 << lg; s++) {
+        const float f = x[8 * s + 4] == -INFINITY ? 0.f : ex2(x[8 * s + 4] - M);
+        L = fmaf(f, x[8 * s + 5], L);
+        if (f != 0.f)
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = f == 0.f ? 0.f : v[e] * f;
-      for (int o2 = 1; o2 < P; o2 <<= 1) {
-        L += __shfl_xor_sync(0xffffffffu, L, o2);
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o2);
+          for (int e = 0; e < 4; e++) v[e] = fmaf(f, x[8 * s + e], v[e]);
       }
-      if (who == 0 && i < items) put(at_col, d, v, L == 0.f ? 0.f : 1.f / L);
+      put(i / (HD / 4), i % (HD / 4) * 4, v, L);
     }
-    __syncwarp();
-    cluster_arrive();   // nobody leaves while its parts are read
-    cluster_wait();
-  } else if (!whole) {
+  } else if (parted) {
     // ---- the last CTA of a unit joins its parts, in their order -----------------------------------------------------------
-    if (threadIdx.x < 2 * COLS) part[COLS * HD + threadIdx.x] = sr[COLS * HD + threadIdx.x];
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) *last = atomicAdd(&p.tickets[first_cta], 1u) == (unsigned)parts - 1;
@@ -874,7 +870,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
             v[0] = v[0] * f0 + y.x * f1; v[1] = v[1] * f0 + y.y * f1; v[2] = v[2] * f0 + y.z * f1; v[3] = v[3] * f0 + y.w * f1;
           }
         }
-        if (teams == 1) put(col, d, v, L == 0.f ? 0.f : 1.f / L);
+        if (teams == 1) put(col, d, v, L);
         else {
           float *x = so + (size_t)(team * items + i1) * 8;
           *reinterpret_cast<float4 *>(x) = make_float4(v[0], v[1], v[2], v[3]);
@@ -896,14 +892,14 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = fmaf(f, x[e], v[e]);
           }
-          put(col, d, v, L == 0.f ? 0.f : 1.f / L);
+          put(col, d, v, L);
         }
       }
       if (threadIdx.x == 0) p.tickets[first_cta] = 0;   // for the next launch
     }
   }
   at = stop;
-  again = !p.cluster && at < end;
+  again = in_line && at < end;
   if (again) __syncthreads();   // the ring takes copies again
   }
 }
@@ -942,22 +938,26 @@ template <typename T, int HD, int NT, int PK> static int attend_split(cudaStream
   constexpr int COLS = 8 * NT / PK;
   Split p{a};
   p.cols = a.S * (a.n_heads / a.n_kv);
+  p.col_blocks = (p.cols + COLS - 1) / COLS;
   p.ws = x.ws; p.tickets = x.tickets;
-  const long long units = (long long)a.B * a.n_kv * ((p.cols + COLS - 1) / COLS), slots = (long long)x.sms * sp_per_sm(HD, NT);
+  const long long units = (long long)a.B * a.n_kv * p.col_blocks, slots = (long long)x.sms * sp_per_sm(HD, NT);
   const int n_blk = a.d_pos ? a.blocks : std::max(1, (a.pos0 + a.S - 1) / BLOCK - a.first / BLOCK + 1);
   p.units = (int)units;
-  int cluster = 1;
-  while (cluster < SP_CLUSTER && cluster * SP_WARPS < n_blk && units * 2 * cluster <= slots) cluster *= 2;
+  int lg = 0;
+  while (lg < SP_CLUSTER_LOG2 && SP_WARPS << lg < n_blk && units << (lg + 1) <= slots) lg++;
+  const int cluster = 1 << lg;
   // Microseconds of either way behind what both cost: a block takes a quarter of an SM 0.3 (hd 128, 8 columns), a CTA alone twice as long a warp; parts
   // in the line cost 8, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 8.8,
   // 11.2 us, at 16384 16.3, 14.4; batch 4 at 16384 24.9, 27.9; batch 16 at 4096 24.1, 28.6, at 16384 75, 73)
   const double each = 0.3 * std::max(1.0, HD * NT / 128.0), ctas = (double)((units * cluster + x.sms - 1) / x.sms);
-  const bool line = each * units * n_blk / (4.0 * x.sms) + (slots % units ? 8 : 5) < 2 * each * ctas * n_blk / (SP_WARPS * cluster);
-  if (!line) p.cluster = cluster;
-  const long long grid = line ? std::min<long long>(slots, (units * n_blk + SP_WARPS - 1) / SP_WARPS) : units * cluster;
-  return launch(s, launches, attend_split_kernel<T, HD, NT, PK>, dim3((unsigned)grid), dim3(SP_WARPS * 32),
-                // (few clusters: so much shared memory that their CTAs come to lie on an SM each; 16384 positions 20.2 -> 16.8 us)
-                !line && 2 * grid <= x.sms ? (size_t)std::max(sp_smem<HD, NT>(), 120 * 1024) : (size_t)sp_smem<HD, NT>(), line ? 1 : cluster, p);
+  const bool line = (long long)a.n_kv * p.col_blocks > 65535 || a.B > 65535 ||
+                    each * units * n_blk / (4.0 * x.sms) + (slots % units ? 8 : 5) < 2 * each * ctas * n_blk / (SP_WARPS * cluster);
+  p.cluster_log2 = line ? -1 : lg;
+  const dim3 grid = line ? dim3((unsigned)std::min<long long>(slots, (units * n_blk + SP_WARPS - 1) / SP_WARPS))
+                         : dim3((unsigned)cluster, (unsigned)(a.n_kv * p.col_blocks), (unsigned)a.B);
+  // (few clusters: so much shared memory that their CTAs come to lie on an SM each; 16384 positions 20.2 -> 16.8 us)
+  const int smem = !line && 2 * units * cluster <= x.sms ? std::max(sp_smem<HD, NT>(), 120 * 1024) : sp_smem<HD, NT>();
+  return launch(s, launches, attend_split_kernel<T, HD, NT, PK>, grid, dim3(SP_WARPS * 32), (size_t)smem, line ? 1 : cluster, p);
 }
 int attend(cudaStream_t s, int dtype, const Attend &a, const Scratch &x, uint64_t *launches) {
   return by_type(dtype, a.hd, [&](auto t, auto hd) {
