@@ -963,9 +963,15 @@ int attend(cudaStream_t s, int dtype, const Attend &a, const Scratch &x, uint64_
   return by_type(dtype, a.hd, [&](auto t, auto hd) {
     typedef decltype(t) T;
     constexpr int HD = hd.value;
-    const long long cols = (long long)a.S * (a.n_heads / a.n_kv);
-    if (cols <= 4) return attend_split<T, HD, 1, 2>(s, a, x, launches);
-    if (HD == 256 || cols <= 8) return attend_split<T, HD, 1, 1>(s, a, x, launches);
+    const long long cols = (long long)a.S * (a.n_heads / a.n_kv), heads = (long long)a.B * a.n_kv;
+    // more rows are cut into smaller pieces while their clusters leave a third of the SMs without work and a warp has few blocks (4 rows of 8 / 2
+    // heads of 64 at 1000 positions 7.3 -> 5.2 us, 4 of 32 / 8 of 128 at 500 8.7 -> 6.7; on all SMs it costs more than it saves: 3 at 2000 9.6 -> 10.3)
+    const int n_blk = a.d_pos ? a.blocks : (a.pos0 + a.S - 1) / BLOCK - a.first / BLOCK + 1;
+    int lg = 0;
+    while (lg < SP_CLUSTER_LOG2 && SP_WARPS << lg < n_blk) lg++;
+    auto room = [&](int rows) { return n_blk <= 8 * SP_WARPS << lg && 3 * (heads * ((cols + rows - 1) / rows) << lg) <= 2 * x.sms; };
+    if (cols <= 4 || room(4)) return attend_split<T, HD, 1, 2>(s, a, x, launches);
+    if (HD == 256 || cols <= 8 || room(8)) return attend_split<T, HD, 1, 1>(s, a, x, launches);
     return attend_split<T, HD, HD == 256 ? 1 : 2, 1>(s, a, x, launches);
   });
 }
