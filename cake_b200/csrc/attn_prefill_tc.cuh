@@ -287,18 +287,19 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int i = 0; i < 32; i++) sv[32 + i] = __uint_as_float(r[i]);
       }
       // causal mask (attention.rs:314-341) — only tiles reaching past the first row's position need the compare
-      float mx = -INFINITY;
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (one maximum behind the other is 64 times an operation's latency)
       const int k0 = (j0 + j) * FT_BN;
       if (k0 + FT_BN - 1 > pos0 + t0) {
 #pragma unroll
         for (int i = 0; i < FT_BN; i++) {
           if (k0 + i > qp) sv[i] = -INFINITY;
-          mx = fmaxf(mx, sv[i]);
+          mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < FT_BN; i++) mx = fmaxf(mx, sv[i]);
+        for (int i = 0; i < FT_BN; i++) mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
       }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       // running max with lazy update: keep the old reference while the new max exceeds it by at most tau
       float fac = 1.f;
       bool resc = false;
@@ -312,13 +313,15 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       // p = exp((s - m) / sqrt(hd)) = 2^(s c - m c), c = log2(e) / sqrt(hd): one FFMA + one MUFU.EX2 per score; 2^-inf = 0 masks
       // (a row that has seen no key of this CTA's range yet keeps m = -inf: its scores count from 0)
       const float mc = SPLIT && m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
-      float rs = 0.f;
+      float rs = 0.f, rs4[4] = {};
 #pragma unroll
       for (int i = 0; i < FT_BN; i++) {
         const float e = ft_ex2(fmaf(sv[i], p.scale_log2, -mc));
         sv[i] = e;
-        rs += e;
+        if (LO) rs += e;
+        else rs4[i & 3] += e;
       }
+      if (!LO) rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
       l_run = l_run * fac + rs;
       if (j > 0) {
         mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, p.err, left);  // P V of the previous tile is complete: O stable

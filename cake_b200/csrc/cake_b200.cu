@@ -65,6 +65,7 @@ static int round_up(int v, int m);
 static int wait_loads(cake_b200_ctx *c);
 static int check_waits(cake_b200_ctx *c);
 static int sync_results(cake_b200_ctx *c);
+static int settle(cake_b200_ctx *c);
 extern "C" const char *cake_b200_last_error(void) { return g_err; }
 extern "C" const char *cake_b200_version(void) { return "cake_b200 0.1 (sm_100a)"; }
 
@@ -155,7 +156,11 @@ struct cake_b200_ctx {
   size_t pc_rows_cap = 0;
   unsigned *pc_tickets = nullptr;
   cudaMemPool_t pc_pool = nullptr;   // the caches' memory: a closed cache's is the next one's (a new cache of 67 MB: 20 us, 3 ms from the driver)
-  cudaEvent_t pc_in = nullptr, pc_out = nullptr;   // a caller's stream in front of this one's work, and behind it
+  // The operators of such caches may run on a caller's stream: `stream` then is that one for the call.  pc_out: behind the last of them, waited for by
+  // this ctx's stream (settle) or another caller's when it goes on; pc_in: the ctx's stream as it was, waited for by a caller's while pc_behind
+  cudaEvent_t pc_in = nullptr, pc_out = nullptr;
+  unsigned long long pc_on = 0;   // the id of the stream that pc_out was recorded on last and nobody has waited for yet; 0: none
+  bool pc_behind = true;
   // head of a batch: its logits where the caller keeps none, its tokens
   void *hd_logits = nullptr;
   size_t hd_logits_rows = 0;
@@ -656,6 +661,7 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
     g_live_ctx.erase(c);
   }
   cudaSetDevice(c->device);
+  (void)settle(c);
   cudaStreamSynchronize(c->stream);
   if (c->gexec) cudaGraphExecDestroy(c->gexec);
   if (c->graph) cudaGraphDestroy(c->graph);
@@ -808,7 +814,19 @@ static int check_waits(cake_b200_ctx *c) {
   c->wait_failures++;
   return fail(CAKE_B200_ECUDA, "a kernel gave up a wait (for its copies, or for other parts of its grid): this call and the ones before it since the last synchronisation have no results");
 }
+// the ctx's stream goes on behind operators that ran on a caller's
+static int settle(cake_b200_ctx *c) {
+  c->pc_behind = true;
+  if (!c->pc_on) return CAKE_B200_OK;
+  cudaStreamCaptureStatus st;
+  CU(cudaStreamIsCapturing(c->stream, &st));
+  if (st != cudaStreamCaptureStatusNone) return CAKE_B200_OK;   // (a graph's order with what ran before is its user's)
+  CU(cudaStreamWaitEvent(c->stream, c->pc_out, 0));
+  c->pc_on = 0;
+  return CAKE_B200_OK;
+}
 static int sync_results(cake_b200_ctx *c) {
+  RC(settle(c));
   CU(cudaStreamSynchronize(c->stream));
   return check_waits(c);
 }
@@ -818,6 +836,7 @@ static int check_cache(const cake_b200_cache *k) {
 }
 static int wait_loads(cake_b200_ctx *c) {
   RC(check_waits(c));
+  RC(settle(c));
   if (c->load_pending) {
     CU(cudaStreamWaitEvent(c->stream, c->load_done, 0));
     c->load_pending = false;
@@ -997,6 +1016,7 @@ static int cache_ensure(cake_b200_cache *k, int layer) {
     RC(no_capture(k->ctx->stream, "a block's part of the cache"));
     CU(cudaMallocFromPoolAsync(&k->k[layer], (size_t)k->batch * k->ctx->cfg.n_kv_heads * pc::cap_blocks(k->cap) * pc::block_bytes(hd), k->ctx->pc_pool,
                                k->ctx->stream));
+    k->ctx->pc_behind = true;
     return CAKE_B200_OK;
   }
   const size_t bytes = (size_t)k->batch * k->ctx->cfg.n_kv_heads * k->cap * k->ctx->cfg.head_dim * k->ctx->es;
@@ -1018,6 +1038,7 @@ extern "C" void cake_b200_cache_free(cake_b200_cache *k) {
     std::lock_guard<std::mutex> lk(g_live_mu);
     if (g_live_ctx.count(k->ctx)) {
       cake_b200_ctx *c = k->ctx;
+      (void)settle(c);
       cudaStreamSynchronize(c->stream);
       c->mk_sig.clear();
       if (c->g_cache == k) {
@@ -1109,18 +1130,36 @@ static int packed_call(const cake_b200_cache *k, int block_idx, const char *what
   return check_cache(k);
 }
 static bool unaligned(const void *p, size_t s0 = 0, size_t s1 = 0) { return ((uintptr_t)p & 15) || s0 % 8 || s1 % 8; }
-// work of the ctx's stream in the order of the caller's
-template <typename F> static int in_order_of(cake_b200_ctx *c, void *stream, F &&call) {
-  if (!stream || stream == (void *)c->stream) return call();
-  CU(cudaEventRecord(c->pc_in, (cudaStream_t)stream));
-  CU(cudaStreamWaitEvent(c->stream, c->pc_in, 0));
+// An operator on the caller's stream, behind the ctx's work so far and the operators before it (calls on one ctx are not made at the same time).  Handing
+// it to the ctx's stream and waiting for it takes two events and two crossings of streams a call: 8 x 4096 rows written and read back 81 us, so 72.
+template <typename F> static int on_stream(cake_b200_ctx *c, void *stream, F &&call) {
+  const cudaStream_t s = (cudaStream_t)stream, own = c->stream;
+  if (!s || s == own) {
+    RC(settle(c));
+    return call();
+  }
+  cudaStreamCaptureStatus st;
+  unsigned long long id = 0;
+  CU(cudaStreamIsCapturing(s, &st));
+  const bool eager = st == cudaStreamCaptureStatusNone;   // (a graph's order with what runs beside it is its user's)
+  if (eager) {
+    CU(cudaStreamGetId(s, &id));
+    if (c->pc_behind) {
+      CU(cudaEventRecord(c->pc_in, own));
+      CU(cudaStreamWaitEvent(s, c->pc_in, 0));
+      c->pc_behind = false;
+    }
+    if (c->pc_on && c->pc_on != id) CU(cudaStreamWaitEvent(s, c->pc_out, 0));
+  }
+  c->stream = s;
   const int rc = call();
-  const std::string said = rc == CAKE_B200_OK ? "" : g_err;   // (the message that stays is the call's)
-  cudaError_t e = cudaEventRecord(c->pc_out, c->stream);
-  if (e == cudaSuccess) e = cudaStreamWaitEvent((cudaStream_t)stream, c->pc_out, 0);
-  if (rc != CAKE_B200_OK) return fail(rc, "%s", said.c_str());
-  CU(e);
-  return CAKE_B200_OK;
+  c->stream = own;
+  if (eager) {
+    const cudaError_t e = cudaEventRecord(c->pc_out, s);
+    c->pc_on = id;
+    if (e != cudaSuccess && rc == CAKE_B200_OK) return fail(CAKE_B200_ECUDA, "event behind an operator: %s", cudaGetErrorString(e));
+  }
+  return rc;
 }
 extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const void *k_dev, size_t k_tok, size_t k_batch, const void *v_dev,
                                      size_t v_tok, size_t v_batch, int seq, int index_pos, void *stream) {
@@ -1137,7 +1176,7 @@ extern "C" int cake_b200_cache_write(cake_b200_cache *k, int block_idx, const vo
   const cake_b200_config &f = k->ctx->cfg;
   pc::Write a{k->k[block_idx], k_dev, v_dev, (long long)k_tok, (long long)k_batch, (long long)v_tok, (long long)v_batch};
   a.B = k->batch; a.S = seq; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(k->cap); a.pos0 = index_pos;
-  return in_order_of(k->ctx, stream, [&]() -> int {
+  return on_stream(k->ctx, stream, [&]() -> int {
     CU((cudaError_t)pc::write(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
     k->len[block_idx] = index_pos + seq;
     k->moved = true;
@@ -1153,7 +1192,7 @@ extern "C" int cake_b200_cache_unpack(cake_b200_cache *k, int block_idx, int whi
   if (!out_dev || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "cache_unpack writes to a 16-byte boundary");
   const cake_b200_config &f = k->ctx->cfg;
   pc::Read a{k->k[block_idx], which ? nullptr : out_dev, which ? out_dev : nullptr, k->batch, f.n_kv_heads, f.head_dim, pc::cap_blocks(k->cap), first, n, n};
-  return in_order_of(k->ctx, stream, [&]() -> int {
+  return on_stream(k->ctx, stream, [&]() -> int {
     CU((cudaError_t)pc::read(k->ctx->stream, f.dtype, a, launch_counter(k->ctx)));
     return CAKE_B200_OK;
   });
@@ -1212,7 +1251,7 @@ extern "C" int cake_b200_cache_attend(cake_b200_cache *k, int block_idx, const v
   if (index_pos < 0 || (long long)index_pos + seq > k->len[block_idx])
     return fail(CAKE_B200_ESTATE, "block %d: positions %d .. + %d are not within the cache's %d", block_idx, index_pos, seq, k->len[block_idx]);
   if (first < 0 || !(scale >= 0.f && scale <= 3.402823466e38f)) return fail(CAKE_B200_EINVAL, "first %d or scale %g out of range", first, (double)scale);
-  return in_order_of(k->ctx, stream, [&]() -> int {
+  return on_stream(k->ctx, stream, [&]() -> int {
     return attend_packed(k->ctx, k, block_idx, q_dev, q_tok, q_batch, out_dev, seq, index_pos, first,
                          scale > 0.f ? scale : (float)(1.0 / sqrt((double)k->ctx->cfg.head_dim)));
   });
@@ -1258,6 +1297,7 @@ extern "C" int cake_b200_cache_fill_synthetic(cake_b200_cache *k, const int *blo
   CU(cudaSetDevice(c->device));
   if (len > k->cap) return fail(CAKE_B200_EINVAL, "len %d > cache capacity %d", len, k->cap);
   if (c->cfg.layer_list) return fail(CAKE_B200_EINVAL, "cache_fill_synthetic is for the Llama-family blocks");
+  RC(settle(c));
   for (int i = 0; i < n_blocks; i++) {
     const int l = block_idx[i];
     RC(cache_ensure(k, l));
@@ -4418,6 +4458,7 @@ extern "C" int cake_b200_decode_run(cake_b200_ctx *c, int n_steps) {
   RC(check_waits(c));
   RC(check_cache(kc));
   if (kc->moved) return fail(CAKE_B200_ESTATE, "rows have been written into the cache: cake_b200_decode_begin first");
+  RC(settle(c));
   int cur = c->g_block_idx.empty() ? 0 : kc->len[c->g_block_idx[0]];
   if (!c->g_block_idx.empty() && cur + n_steps > kc->cap)
     return fail(CAKE_B200_ESTATE, "decode_run: %d steps from position %d exceed cache capacity %d", n_steps, cur, kc->cap);

@@ -36,8 +36,8 @@ class Cache:
     """KV cache of one session (cache.rs:9).  RoPE tables live in the ctx (computed once per model).
 
     ``bits`` 4 (None: the context's ``cache_bits``; 0: rows in D): K and V rows in four bits, ``cake_b200_cache_create_packed``.  Such a cache serves the
-    blocks like any other and has three operators of its own, ``write``, ``read`` and ``attend``: they run on the context's stream, behind what the calling
-    thread's current stream holds, which in turn goes on behind them."""
+    blocks like any other and has three operators of its own, ``write``, ``read`` and ``attend``: they run on the calling thread's current stream, in
+    order with the context's work."""
 
     def __init__(self, ctx: "Context", batch: int = 1, max_seq: Optional[int] = None, bits: Optional[int] = None):
         self.ctx, self.batch = ctx, batch
@@ -108,7 +108,7 @@ class Cache:
             raise capi.CakeB200Error(-1, "write, read and attend are for caches in four bits (Cache(..., bits=4))")
 
     def _stream(self) -> int:
-        """The current stream as the library's calls take it: they keep their order with its work."""
+        """The current stream as the library's calls take it."""
         return torch._C._cuda_getCurrentRawStream(self.ctx.device) or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's
 
     def write(self, block_idx: int, k: torch.Tensor, v: torch.Tensor, index_pos: int) -> None:
