@@ -126,7 +126,7 @@ class Cache:
         """Positions [first, first + n) (to the end without n) of the block's K (which 0) or V (1) rows: (batch, n_kv, n, head_dim) in D."""
         self._packed()
         n = self.len(block_idx) - first if n is None else n
-        out = torch.empty((self.batch, self._kv, max(n, 0), self._hd), dtype=self.ctx.torch_dtype, device=self.ctx.torch_device)
+        out = torch.empty(self.batch, self._kv, max(n, 0), self._hd, dtype=self.ctx.torch_dtype, device=self.ctx.torch_device)
         check(self._lib.cake_b200_cache_unpack(self.h, block_idx, which, first, n, out.data_ptr(), self._stream()))
         return out
 
@@ -135,9 +135,9 @@ class Cache:
         first <= j <= index_pos + t (one that sees none is zero).  scale 0: head_dim^-1/2.  (batch, seq, n_heads, head_dim) in D."""
         self._packed()
         q = self._rows(q, "q", self._heads)
-        out = q.new_empty(q.shape)
-        qs = q.stride()
-        check(self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), qs[1], qs[0], out.data_ptr(), q.shape[1], index_pos, first, scale, self._stream()))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        sb, st, _, _ = q.stride()
+        check(self._lib.cake_b200_cache_attend(self.h, block_idx, q.data_ptr(), st, sb, out.data_ptr(), q.shape[1], index_pos, first, scale, self._stream()))
         return out
 
     def __del__(self):

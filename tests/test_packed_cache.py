@@ -697,6 +697,7 @@ def test_generation_steps_and_graph_agree(dtype):
     ctx.cache.clear()
     m.forward([prompt[:20]], 0)
     lg = m.forward([prompt[20:]], 20)
+    ctx.sync()
     first = int(lg.float().argmax())
     m.index_pos = 37
     m.decode_build()
@@ -706,6 +707,52 @@ def test_generation_steps_and_graph_agree(dtype):
     s = Sessions(m)
     assert s.cache_of("a").bits == 4
     ctx.close()
+
+
+@pytest.mark.gpu
+def test_graph_and_steps_agree_where_capacity_is_large():
+    """The graph cuts keys as the capacity asks, steps as the length does."""
+    cfg = medium_config(num_hidden_layers=2, max_seq_len=40000, head_dim=128, num_attention_heads=4, num_key_value_heads=2)
+    ctx = Context(cfg, checkpoint(cfg, "bf16", std=0.05, peaked=True), "bf16", cache_bits=4)
+    m = TextModelBase.load(ctx)
+    for n in (5, 130, 1500):
+        ids = np.random.default_rng(n).integers(0, cfg.vocab_size, n).tolist()
+        want = Master(m).generate_text(ids, 8)["tokens"]
+        ctx.cache.clear()
+        logits = m.forward([ids], 0)
+        ctx.sync()
+        first = int(logits.float().argmax())
+        m.index_pos = n
+        m.decode_build()
+        assert [first] + m.decode_greedy(first, len(want) - 1) == want
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["olmo2", "gemma3", "exaone4"])
+def test_sibling_blocks(kind):
+    """Per layer: norms, rotation or none and the layer's window are those of the plain cache.  Rows as there, in four bits; what lies in front of a local
+    layer's window changes nothing, of a global layer's something."""
+    from tests.test_gpu_parity import SIBLINGS
+    cfg = medium_config(num_hidden_layers=4, **SIBLINGS[kind])
+    (pc, plain), (qc, packed) = _model_pair(cfg, "bf16")
+    xs = [torch.randn((1, 14, cfg.hidden_size), generator=torch.Generator().manual_seed(s)).bfloat16().cuda() for s in (1, 2)]
+    xs[1][:, 4:] = xs[0][:, 4:]                          # the first four tokens differ
+    for layer in range(4):
+        last = []
+        for x in xs:
+            for ctx, m in ((pc, plain), (qc, packed)):
+                ctx.cache.clear()
+                for at, n in ((0, 4), (4, 3), (7, 1), (8, 1), (9, 4), (13, 1)):
+                    y = m.blocks[layer].forward(x[:, at:at + n], at, layer, ctx)
+                ctx.sync()
+            last.append(y.clone())
+            for which in (0, 1):
+                got, ref = qc.cache.read(layer, which).cpu().double(), stands_for(pc.cache.kv(layer)[which])
+                assert ((got - ref).abs() <= ref.abs() * (HALF["bf16"] + 2.0 ** -23) + 2.0 ** -25).float().mean() > 0.99
+        local = bool(cfg.sliding_window) and not cfg.global_layers[layer]
+        assert torch.equal(last[0], last[1]) == local, layer
+    pc.close(), qc.close()
 
 
 @pytest.mark.gpu
@@ -719,12 +766,18 @@ def test_batch_rows_are_their_own():
     for r in range(3):
         ctx.cache.clear()
         m.forward([ids[r, :25].tolist()], 0)
-        alone.append([m.forward([[int(t)]], 25 + i).float()[0].cpu() for i, t in enumerate(ids[r, 25:])])
+        alone.append([])
+        for i, t in enumerate(ids[r, 25:]):
+            lg = m.forward([[int(t)]], 25 + i)
+            ctx.sync()
+            alone[-1].append(lg.float()[0].cpu())
     ctx.cache = Cache(ctx, 3, 64)
     assert ctx.cache.bits == 4
     m.forward(ids[:, :25], 0)
     for i in range(5):
-        lg = m.forward(ids[:, 25 + i:26 + i], 25 + i).float().cpu()
+        lg = m.forward(ids[:, 25 + i:26 + i], 25 + i)
+        ctx.sync()
+        lg = lg.float().cpu()
         for r in range(3):
             assert torch.nn.functional.cosine_similarity(lg[r], alone[r][i], dim=0) > 0.999
     ctx.close()
