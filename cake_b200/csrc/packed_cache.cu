@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 // Four bits become fp16 by one logic operation a pair: n under the exponent of 1024 is 1024 + n in the lowest four bits, 1024 + 16 n in the next.
 // The 16 stays in: K's queries are divided by it, V's sums at the end.  K's 1024 is what the accumulators start from (-1024 sum of q), a sum that
 // cancels to 2^-24 of 1024 sum |q|; from V's codes 1024 + 8 (1024 + 128) is subtracted, which also centres them: a weight's rounding counts for 8
-// steps at most.  (The codes are what binds the kernel: ALU operations at half rate, 130 of 340 a block.)
+// steps at most.  (What binds the kernel is issue: 340 instructions a block and warp, 150 of them on the ALU at half rate.)
 // PK = 2, up to 4 rows: columns 0 .. 3 of an operand belong to a group and columns 4 .. 7 to its neighbour (the queries of the other are zero there),
 // so that no lane works for columns without a row; a row's two halves join by a shuffle.
 // A row's reference m moves when a score exceeds it by 2^6 (TAU), and 2^ce is kept so that steps times 2^ce are at most 512, the first ones about 8:
@@ -947,11 +947,11 @@ template <typename T, int HD, int NT, int PK> static int attend_split(cudaStream
   while (lg < SP_CLUSTER_LOG2 && SP_WARPS << lg < n_blk && units << (lg + 1) <= slots) lg++;
   const int cluster = 1 << lg;
   // Microseconds of either way behind what both cost: a block takes a quarter of an SM 0.3 (hd 128, 8 columns), a CTA alone twice as long a warp; parts
-  // in the line cost 8, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 8.8,
-  // 11.2 us, at 16384 16.3, 14.4; batch 4 at 16384 24.9, 27.9; batch 16 at 4096 24.1, 28.6, at 16384 75, 73)
+  // in the line cost 6, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 7.4,
+  // 10.8 us, at 16384 14.6, 14.1, at 32768 24.2, 18.0; batch 4 at 16384 25.4, 26.9; batch 16 at 8192 40.2, 43.9, at 16384 72.4, 71.5)
   const double each = 0.3 * std::max(1.0, HD * NT / 128.0), ctas = (double)((units * cluster + x.sms - 1) / x.sms);
   const bool line = (long long)a.n_kv * p.col_blocks > 65535 || a.B > 65535 ||
-                    each * units * n_blk / (4.0 * x.sms) + (slots % units ? 8 : 5) < 2 * each * ctas * n_blk / (SP_WARPS * cluster);
+                    each * units * n_blk / (4.0 * x.sms) + (slots % units ? 6 : 5) < 2 * each * ctas * n_blk / (SP_WARPS * cluster);
   p.cluster_log2 = line ? -1 : lg;
   const dim3 grid = line ? dim3((unsigned)std::min<long long>(slots, (units * n_blk + SP_WARPS - 1) / SP_WARPS))
                          : dim3((unsigned)cluster, (unsigned)(a.n_kv * p.col_blocks), (unsigned)a.B);
