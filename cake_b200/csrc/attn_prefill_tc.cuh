@@ -155,8 +155,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = p.S, pos0 = p.pos0, G = p.G, tpt = p.tpt, lg = SPLIT ? p.splits_log2 : 0, splits = 1 << lg;
   const int rank = (int)blockIdx.x & (splits - 1);                        // the cluster's CTAs are neighbours along x
-  const int mt = (int)(gridDim.x >> lg) - 1 - (int)(blockIdx.x >> lg);  // heavy (late) query tiles first
-  const int kvh = blockIdx.y, b = blockIdx.z, t0 = mt * tpt;
+  // heavy (late) query tiles first, those of every key head before the next: CTAs start in the order of x, y, z
+  // (one head behind the other, the SMs are without work for a sixth of a prompt of 4096, 32 / 8 heads: 157 us for 138)
+  const int nth = (int)blockIdx.y * (int)(gridDim.x >> lg) + (int)(blockIdx.x >> lg);
+  const int mt = (int)(gridDim.x >> lg) - 1 - nth / (int)gridDim.y, kvh = nth % (int)gridDim.y, b = blockIdx.z, t0 = mt * tpt;
   const int kv_end = pos0 + min(S, t0 + tpt);  // keys visible to the last query of this tile
   const int all_tiles = (kv_end + FT_BN - 1) / FT_BN;
   const int j0 = (all_tiles * rank) >> lg, n_tiles = ((all_tiles * (rank + 1)) >> lg) - j0;  // 0: fewer tiles than CTAs
