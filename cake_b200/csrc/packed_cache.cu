@@ -851,49 +851,62 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     __syncthreads();
     if (*last) {
       __threadfence();
-      // a share of the parts for each of `teams` threads of a result
-      int teams = 1;
-      while (2 * teams * items <= WARPS * 32 && 2 * teams <= parts) teams *= 2;
-      const int i = threadIdx.x % items, team = threadIdx.x / items;
-      for (int i1 = i; i1 < items && team < teams; i1 += teams == 1 ? WARPS * 32 : items) {
-        const int col = i1 / (HD / 4), d = i1 % (HD / 4) * 4, p0 = parts * team / teams, p1 = parts * (team + 1) / teams;
-        float M = -INFINITY, L = 0.f, v[4] = {};
-#pragma unroll 4
-        for (int s = p0; s < p1; s++) {   // (the running maximum keeps the loads of four parts on their way together)
-          const float *x = slot_of(first_cta + s);
-          const float mm = __ldcg(x + COLS * HD + col), ll = __ldcg(x + COLS * HD + COLS + col);
-          const float4 y = __ldcg(reinterpret_cast<const float4 *>(x + col * HD + d));
-          const float mn = fmaxf(M, mm), f0 = M == -INFINITY ? 0.f : ex2(M - mn), f1 = mm == -INFINITY ? 0.f : ex2(mm - mn);
-          M = mn;
-          L = L * f0 + ll * f1;
-          if (f1 != 0.f) {
-            v[0] = v[0] * f0 + y.x * f1; v[1] = v[1] * f0 + y.y * f1; v[2] = v[2] * f0 + y.z * f1; v[3] = v[3] * f0 + y.w * f1;
-          }
+      // Into shared memory, as many as it holds at a time, then weights by a warp a column and sums by a thread a result: short code, as it comes from memory
+      // once per launch (131072 positions: straight from memory, unrolled, 42.6 us of which it is 5.3; so 40.7).
+      constexpr int ROOM = (sp_smem<HD, NT>() - 16 - COLS * 8) / (PART * 4);
+      static_assert(ROOM >= 2, "");
+      float *held = reinterpret_cast<float *>(sp_raw), *ml = reinterpret_cast<float *>(last) - 2 * COLS;   // [part][results, m, l]
+      for (int s0 = 0; s0 < parts;) {   // after the first time, held[0] is what came before
+        const int from = s0 > 0, n = min(ROOM, from + parts - s0);
+#pragma unroll 1
+        for (int x = threadIdx.x; x < (n - from) * (PART / 4); x += WARPS * 32) {
+          const int e = x / (PART / 4), r = x - e * (PART / 4);
+          const float *src = slot_of(first_cta + s0 + e) + r * 4;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + (from + e) * PART + r * 4)), "l"(src) : "memory");
         }
-        if (teams == 1) put(col, d, v, L);
-        else {
-          float *x = so + (size_t)(team * items + i1) * 8;
-          *reinterpret_cast<float4 *>(x) = make_float4(v[0], v[1], v[2], v[3]);
-          x[4] = M;
-          x[5] = L;
-        }
-      }
-      if (teams > 1) {
+        copies_commit();
+        copies_wait<0>();
+        if (from && (int)threadIdx.x < 2 * COLS) held[COLS * HD + threadIdx.x] = ml[threadIdx.x];
         __syncthreads();
-        if ((int)threadIdx.x < items) {
-          const int col = threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
-          float M = -INFINITY, L = 0.f, v[4] = {};
-          for (int s = 0; s < teams; s++) M = fmaxf(M, so[(size_t)(s * items + threadIdx.x) * 8 + 4]);
-          for (int s = 0; s < teams; s++) {
-            const float *x = so + (size_t)(s * items + threadIdx.x) * 8;
-            if (x[4] == -INFINITY) continue;
-            const float f = ex2(x[4] - M);
-            L = fmaf(f, x[5], L);
+#pragma unroll 1
+        for (int col = warp; col < n_cols; col += WARPS) {
+          float *x = held + COLS * HD + col, M = -INFINITY, L = 0.f;
+#pragma unroll 1
+          for (int e = lane; e < n; e += 32) M = fmaxf(M, x[e * PART]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = fmaf(f, x[e], v[e]);
+          for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 1
+          for (int e = lane; e < n; e += 32) {
+            const float f = x[e * PART] == -INFINITY ? 0.f : ex2(x[e * PART] - M);
+            L = fmaf(f, x[e * PART + COLS], L);
+            x[e * PART] = f;
           }
-          put(col, d, v, L);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+          if (lane == 0) {
+            ml[col] = M;
+            ml[COLS + col] = L;
+          }
         }
+        __syncthreads();
+        s0 += n - from;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < n_cols * (HD / 4); i += WARPS * 32) {
+          const int col = i / (HD / 4), d = i % (HD / 4) * 4;
+          float *x = held + col * HD + d, v[4] = {};
+          const float *f = held + COLS * HD + col;
+#pragma unroll 4
+          for (int e = 0; e < n; e++) {
+            const float w = f[e * PART];
+            const float4 y = *reinterpret_cast<const float4 *>(x + e * PART);
+            if (w != 0.f) {
+              v[0] = fmaf(w, y.x, v[0]); v[1] = fmaf(w, y.y, v[1]); v[2] = fmaf(w, y.z, v[2]); v[3] = fmaf(w, y.w, v[3]);
+            }
+          }
+          if (s0 == parts) put(col, d, v, ml[COLS + col]);
+          else *reinterpret_cast<float4 *>(x) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        if (s0 < parts) __syncthreads();
       }
       if (threadIdx.x == 0) p.tickets[first_cta] = 0;   // for the next launch
     }
@@ -946,17 +959,20 @@ template <typename T, int HD, int NT, int PK> static int attend_split(cudaStream
   int lg = 0;
   while (lg < SP_CLUSTER_LOG2 && SP_WARPS << lg < n_blk && units << (lg + 1) <= slots) lg++;
   const int cluster = 1 << lg;
+  // few clusters: so much shared memory that their CTAs come to lie on an SM each (16384 positions 20.2 -> 16.8 us); of more, two come to lie on one
+  const bool apart = 2 * units * cluster <= x.sms;
   // Microseconds of either way behind what both cost: a block takes a quarter of an SM 0.3 (hd 128, 8 columns), a CTA alone twice as long a warp; parts
   // in the line cost 6, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 7.4,
-  // 10.8 us, at 16384 14.6, 14.1, at 32768 24.2, 18.0; batch 4 at 16384 25.4, 26.9; batch 16 at 8192 40.2, 43.9, at 16384 72.4, 71.5)
-  const double each = 0.3 * std::max(1.0, HD * NT / 128.0), ctas = (double)((units * cluster + x.sms - 1) / x.sms);
+  // 9.9 us, at 12000 12.2, 12.2, at 32768 24.2, 16.9; batch 2 at 8192 14.1, 15.6, at 12000 18.0, 17.4, at 16384 22.2, 19.1; batch 4 at 16384 24.2, 26.6;
+  // batch 16 at 8192 40.1, 43.0)
+  const double each = 0.3 * std::max(1.0, HD * NT / 128.0);
+  const double ctas = apart ? 1. : std::max((double)sp_per_sm(HD, NT), (double)((units * cluster + x.sms - 1) / x.sms));
   const bool line = (long long)a.n_kv * p.col_blocks > 65535 || a.B > 65535 ||
                     each * units * n_blk / (4.0 * x.sms) + (slots % units ? 6 : 5) < 2 * each * ctas * n_blk / (SP_WARPS * cluster);
   p.cluster_log2 = line ? -1 : lg;
   const dim3 grid = line ? dim3((unsigned)std::min<long long>(slots, (units * n_blk + SP_WARPS - 1) / SP_WARPS))
                          : dim3((unsigned)cluster, (unsigned)(a.n_kv * p.col_blocks), (unsigned)a.B);
-  // (few clusters: so much shared memory that their CTAs come to lie on an SM each; 16384 positions 20.2 -> 16.8 us)
-  const int smem = !line && 2 * units * cluster <= x.sms ? std::max(sp_smem<HD, NT>(), 120 * 1024) : sp_smem<HD, NT>();
+  const int smem = !line && apart ? std::max(sp_smem<HD, NT>(), 120 * 1024) : sp_smem<HD, NT>();
   return launch(s, launches, attend_split_kernel<T, HD, NT, PK>, grid, dim3(SP_WARPS * 32), (size_t)smem, line ? 1 : cluster, p);
 }
 int attend(cudaStream_t s, int dtype, const Attend &a, const Scratch &x, uint64_t *launches) {

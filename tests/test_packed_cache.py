@@ -419,6 +419,27 @@ def test_a_long_cache():
     ctx.close()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd", [(4, 1, 128), (8, 1, 64), (2, 1, 256), (6, 2, 128), (5, 5, 64)])
+def test_a_few_heads_over_many_positions(heads, kv, hd):
+    """A head's keys are cut between many CTAs: more parts than shared memory holds at a time, and CTAs with parts of two heads.
+    (Up to 157 parts are added one behind the other, 230 + 2.3 * 157 < 600 halves of 2^-23 V; the bound's mass * 2 h, mass > 0.5 here, is 2^-11, V < 5.)"""
+    n = 20011
+    ctx = ctx_for(heads, kv, hd, "f16", max_seq=n)
+    cache, k, v = filled(ctx, 1, n, 5, "f16")
+    for s, at, first in ((1, n - 1, 3), (2, 17003, 17), (5, 15001, 0)):
+        q = queries(1, s, heads, hd, "f16", at)
+        got = cache.attend(0, q, at, first=first)
+        check_attention(got, q, k, v, at, first, "f16")
+        assert torch.equal(cache.attend(0, q, at, first=first), got)
+    v[:, 11000, 0, :32] = float("nan")          # one part's
+    cache.write(0, k[:, 11000:], v[:, 11000:], 11000)     # (a write ends the cache behind its rows)
+    q = queries(1, 1, heads, hd, "f16", 1)
+    got = cache.attend(0, q, n - 1)
+    assert got[..., :heads // kv, :32].isnan().all() and not got[..., :heads // kv, 32:].isnan().any() and not got[..., heads // kv:, :].isnan().any()
+    ctx.close()
+
+
 # ---------------------------------------------------------------------------------------------- streams and graphs
 @pytest.mark.gpu
 def test_rows_made_and_read_on_another_stream():
