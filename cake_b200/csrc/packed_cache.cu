@@ -79,17 +79,17 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t c) {
 // position r for all groups j: that is K's words of the lane as the cache has them, so that codes leave as one piece of 16 bytes a lane (hd 128);
 // V's words take a 16-bit half from the neighbouring position's lane.  Minimum and maximum of a group are taken in pairs (D's own comparisons, which
 // keep a NaN), minimum and negated maximum together over its four lanes; each lane then has the division of one group in four.  A code is
-// fma, add with rounding down (the integer in the lowest bits) and a multiply-add that moves it to its place: n = floor((x - lo) / step + 1/2) exactly,
-// since (x - lo) inv is exact but for 2^-22 relative and (x - lo) / step is k + 1/2 or at least the last place of x, lo or step away from
-// it: 2^-19 decides the former and leaves the latter, where x's last place is above step 2^-19.
+// fma, add with rounding down (the integer in the lowest bits) and a multiply-add that moves it to its place: n = floor((x - lo) / step + 1/2).
+// inv is 1 / step rounded up and the fma rounds down: a tie (common, with eight bits an entry) is never taken for less, and what is below one only where
+// it lies closer than 2^-23 of the quotient, fp32's own step.  (Ties by a constant 2^-19 on top: an entry near zero, 2^-20 steps below a tie, went up.)
 // 8 x 4096 rows of 8 heads of 128, written and read back: a row per 16 lanes, V in 16-bit stores 102 + 71 us on the device; so 39 + 30 (29 without the arithmetic).
 template <typename T, bool ODDS_LAST> __device__ __forceinline__ uint32_t encode8(const uint32_t (&c)[4], float lo, float inv) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const float2 x = DT<T>::unpack2(c[i]);
-    const uint32_t a = __float_as_uint(__fadd_rd(fmaf(x.x - lo, inv, 0.5f + 1.9073486328125e-6f), 8388608.f));
-    const uint32_t b = __float_as_uint(__fadd_rd(fmaf(x.y - lo, inv, 0.5f + 1.9073486328125e-6f), 8388608.f));
+    const uint32_t a = __float_as_uint(__fadd_rd(__fmaf_rd(x.x - lo, inv, 0.5f), 8388608.f));
+    const uint32_t b = __float_as_uint(__fadd_rd(__fmaf_rd(x.y - lo, inv, 0.5f), 8388608.f));
     w += a * (1u << (4 * (ODDS_LAST ? i : 2 * i)));
     w += b * (1u << (4 * (ODDS_LAST ? 4 + i : 2 * i + 1)));
   }
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(128) write_kernel(const Write a) {
     T st = round_up<T>(fine ? span / 15.f : 0.f);
     if (DT<T>::to_f(st) < 1.17549435e-38f && span > 0.f) st = DT<T>::from_f(1.17549435e-38f);
     const float step = DT<T>::to_f(st);
-    invs[i] = fine && step > 0.f ? 1.f / step : 0.f;
+    invs[i] = fine && step > 0.f ? __frcp_ru(step) : 0.f;
     if (in && 4 * i + t < NG)
       reinterpret_cast<uint32_t *>(blk + (is_v ? v_pairs(HD) : k_pairs(HD)))[pair_word(HD, r, 4 * i + t)] = fine ? bits(st) | e << 16 : 0x7fff7fffu;
   }

@@ -191,6 +191,9 @@ def test_rows_of_every_kind(dtype):
     x[0, 9, 0, :32] = torch.inf
     x[0, 10, 0, 2], x[0, 10, 0, 3] = torch.inf, -torch.inf
     x[0, 11] += 300.0
+    for row, unit in ((13, 1.0), (14, 3.0), (15, 0.8125)):       # entries just below, on and above a tie: the ends are 7.5 steps from zero
+        x[0, row, :, :32] = torch.tensor([-2.0, -1.0, 0.0, 1.0, 2.0, -4.0, 4.0, 8.0] * 4) * 2.0 ** -20 * unit
+        x[0, row, :, 0], x[0, row, :, 1] = -7.5 * unit, 7.5 * unit
     x = x.to(D).cuda()
     if dtype == "bf16":
         x[0, 12, :, 0], x[0, 12, :, 1] = torch.finfo(D).max, -torch.finfo(D).max   # a span beyond fp32
