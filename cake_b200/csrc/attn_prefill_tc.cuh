@@ -134,10 +134,7 @@ struct FtParams {
 };
 
 // SPLIT: clusters that cut the keys; without it every CTA sees its rows' first key in its first tile.
-// LO: P is kept to ~16 bits as P_hi + P_lo.  Without it P is rounded to D once: for keys and values that come from a packed cache, which are rounded to D
-// from four bits themselves: a prompt of 4096 (32 / 8 heads) took 163 us for 190 (138 now), and its distance to 64 bits stays 0.0017 of the result's norm, that of
-// rounding the result to bf16.
-template <typename T, bool SPLIT, bool LO = true>
+template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(FT_THREADS, 2)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FtParams p) {
@@ -252,7 +249,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const uint64_t vt = ft_desc_mn(v_s, FT_KV_BYTES / 2) + (uint64_t)(st * (FT_KV_BYTES >> 4));
         if (one) {
 #pragma unroll
-          for (int half = 0; half < (LO ? 2 : 1); half++)
+          for (int half = 0; half < 2; half++)
 #pragma unroll
             for (int ks = 0; ks < FT_BN / 16; ks++) {  // keys 16ks..16ks+15 = 8 packed columns of P_hi (0..31) or P_lo (32..63)
               const uint32_t ta = tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8);
@@ -315,15 +312,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       // p = exp((s - m) / sqrt(hd)) = 2^(s c - m c), c = log2(e) / sqrt(hd): one FFMA + one MUFU.EX2 per score; 2^-inf = 0 masks
       // (a row that has seen no key of this CTA's range yet keeps m = -inf: its scores count from 0)
       const float mc = SPLIT && m_run == -INFINITY ? 0.f : m_run * p.scale_log2;
-      float rs = 0.f, rs4[4] = {};
+      float rs = 0.f;
 #pragma unroll
       for (int i = 0; i < FT_BN; i++) {
         const float e = ft_ex2(fmaf(sv[i], p.scale_log2, -mc));
         sv[i] = e;
-        if (LO) rs += e;
-        else rs4[i & 3] += e;
+        rs += e;
       }
-      if (!LO) rs = (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
       l_run = l_run * fac + rs;
       if (j > 0) {
         mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, p.err, left);  // P V of the previous tile is complete: O stable
@@ -346,13 +341,11 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         for (int i = 0; i < 32; i++) {
           const float p0 = sv[2 * i], p1 = sv[2 * i + 1];
           hi[i] = pack2x<T>(p0, p1);
-          if (LO) {
-            const float2 hf = DT<T>::unpack2(hi[i]);
-            lo[i] = pack2x<T>(p0 - hf.x, p1 - hf.y);
-          }
+          const float2 hf = DT<T>::unpack2(hi[i]);
+          lo[i] = pack2x<T>(p0 - hf.x, p1 - hf.y);
         }
         tc_st32(tmem_sp, hi);
-        if (LO) tc_st32(tmem_sp + 32u, lo);
+        tc_st32(tmem_sp + 32u, lo);
       }
       tc_wait_st();
       tc_fence_before();

@@ -438,11 +438,10 @@ template <typename T> static int set_smem_attrs_T() {
 #undef SETB
   CU(cudaFuncSetAttribute(attn_prefill_mma_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * FA_BN * 128 * 2));
   CU(cudaFuncSetAttribute(attn_prefill_mma_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * FA_BN * 64 * 2));
-#define SETP(SPLIT, LO)                                                                                                                     \
-  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, SPLIT, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, FT_SMEM_BYTES));              \
-  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, SPLIT, LO>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-  SETP(false, true) SETP(true, true) SETP(false, false) SETP(true, false)
-#undef SETP
+  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, FT_SMEM_BYTES));
+  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, FT_SMEM_BYTES));
+  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, false>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  CU(cudaFuncSetAttribute(attn_prefill_tc_kernel<T, true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
 #define SETT(EPI)                                                                                                                  \
   CU(cudaFuncSetAttribute(gemm_tc_kernel<T, EPI, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<128>::SMEM_BYTES));      \
   CU(cudaFuncSetAttribute(gemm_tc_kernel<T, EPI, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<256>::SMEM_BYTES));      \
@@ -1843,10 +1842,6 @@ static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_
   while (lg < 3 && ((long)tiles * f.n_kv_heads * B << (lg + 1)) <= 2 * c->sm_count && key_tiles >= 6 << lg) lg++;
   FtParams fp{y, S, f.n_heads, f.n_kv_heads, pos0, G, tpt, lg, sc * 1.4426950408889634f, fa_tau * 1.4426950408889634f, c->wait_err, nan};
   const dim3 ga((unsigned)(tiles << lg), f.n_kv_heads, B), ta(FT_THREADS);
-  if (nan.words) {   // expanded from a packed cache
-    if (lg) return launch_cluster_pdl(c, attn_prefill_tc_kernel<T, true, false>, ga, ta, (size_t)FT_SMEM_BYTES, 1u << lg, mq, mk, mv, fp);
-    return launch_pdl(c, attn_prefill_tc_kernel<T, false, false>, ga, ta, (size_t)FT_SMEM_BYTES, mq, mk, mv, fp);
-  }
   if (lg) return launch_cluster_pdl(c, attn_prefill_tc_kernel<T, true>, ga, ta, (size_t)FT_SMEM_BYTES, 1u << lg, mq, mk, mv, fp);
   return launch_pdl(c, attn_prefill_tc_kernel<T, false>, ga, ta, (size_t)FT_SMEM_BYTES, mq, mk, mv, fp);
 }
