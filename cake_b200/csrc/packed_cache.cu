@@ -391,8 +391,9 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 // steps at most.  (What binds the kernel is issue: 340 instructions a block and warp, 150 of them on the ALU at half rate.)
 // PK = 2, up to 4 rows: columns 0 .. 3 of an operand belong to a group and columns 4 .. 7 to its neighbour (the queries of the other are zero there),
 // so that no lane works for columns without a row; a row's two halves join by a shuffle.
-// A row's reference m moves when a score exceeds it by 2^6 (TAU), and 2^ce is kept so that steps times 2^ce are at most 512, the first ones about 8:
-// weights times steps then use fp16's range whatever the size of V's entries.
+// A row's reference m moves when a score exceeds it by 2^6 (TAU).  Every row and group has a power of two `up` that keeps the steps which the row sees at
+// 512 at most, the first ones at 8 to 16: weights times steps then use fp16's range whatever the size of V's entries, of other groups' (one power for all
+// groups took a group 2^24 times smaller than its neighbour for one value) and of those in places that only other rows of the call see.
 //
 // Who takes which blocks: a unit is 8 NT / PK rows of a (batch row, key head).  Short caches: the CTAs of a cluster cut a unit's blocks between them and
 // join over the cluster's shared memory.  Else all units' blocks lie in one line that the grid, two CTAs per SM, cuts into equal parts; a CTA's part of
@@ -564,10 +565,17 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int e2 = 0; e2 < 2; e2++) cpos[nt][e2] = pos0 + tok_of(min(c0 + nt * 8 + 2 * tc + e2, p.cols - 1));
   }
   float o[NT][2 * NG][4] = {}, mid[NT][MG][2] = {}, m[NT][2], l[NT][2] = {};
-  float ce = 0.f, step_lim = 0.f;
-  constexpr float TAU = 6.f;
+  float up[NT][MG][2], lim[MG];   // lim: the step of the pairs' i-th word from which on `up` has to change for one of the lane's columns
+  constexpr float TAU = 6.f, UP0 = 8.50705917e37f;   // 2^126
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -3.402823466e38f;
+#pragma unroll
+  for (int j = 0; j < MG; j++) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) up[nt][j][0] = up[nt][j][1] = UP0;
+    lim[j] = 512.f / UP0;
+  }
+  auto group_of = [](int i) { return PK == 1 ? 2 * (i % (NG / 2)) + i / (NG / 2) : i; };   // the lane's group that its i-th word of pairs belongs to
 
   auto body = [&](auto edge_, const unsigned char *blk, int key0) {
     constexpr bool EDGE = decltype(edge_)::value;
@@ -592,7 +600,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
           const uint32_t(&q0)[4] = qf[nt][2 * w], (&q1)[4] = qf[nt][2 * w + 1];
           auto join = [&](int i, float(&d)[4]) {   // d: sums of the group that is the lane's i-th word of pairs
             const float2 p0 = open_pair<T>(kp[0][i]), p1 = open_pair<T>(kp[1][i]);
-            const int jj = PK == 1 ? 2 * (i % (NG / 2)) + i / (NG / 2) : i;
+            const int jj = group_of(i);
             s[nt][0] = fmaf(p0.x, d[0], fmaf(p0.y, qs[nt][jj][0], s[nt][0]));
             s[nt][1] = fmaf(p0.x, d[1], fmaf(p0.y, qs[nt][jj][1], s[nt][1]));
             s[nt][2] = fmaf(p1.x, d[2], fmaf(p1.y, qs[nt][jj][0], s[nt][2]));
@@ -620,16 +628,17 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
         for (int i = 0; i < 4; i++) s[0][i] += __shfl_xor_sync(0xffffffffu, s[0][i], 2);
     }
     uint32_t vp[2][MG];
-    uint32_t step_bits = 0;
 #pragma unroll
     for (int r = 0; r < 2; r++) {
       lds_words<MG>(blk + v_pairs(HD) + ((g + 8 * r) * NG + half * MG) * 4, vp[r]);
       const bool seen = !EDGE || (key0 + g + 8 * r >= first && key0 + g + 8 * r <= pos_hi);   // by any row: the others' steps say nothing
 #pragma unroll
       for (int i = 0; i < MG; i++) vp[r][i] = seen ? vp[r][i] : 0u;
-#pragma unroll
-      for (int i = 0; i < MG; i++) step_bits = max(step_bits, __float_as_uint(open_pair<T>(vp[r][i]).x));   // no step is negative; NaN is the largest
     }
+    bool more = false;   // steps beyond what `up` is for
+#pragma unroll
+    for (int i = 0; i < MG; i++)   // no step is negative; NaN is the largest
+      more = more || max(__float_as_uint(open_pair<T>(vp[0][i]).x), __float_as_uint(open_pair<T>(vp[1][i]).x)) > __float_as_uint(lim[i]);
     // scores less their reference, in powers of two
     float far = -INFINITY;
 #pragma unroll
@@ -642,39 +651,49 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
         }
         far = fmaxf(far, fmaf(s[nt][i], sc[nt][i & 1], -m[nt][i & 1]));
       }
-    if (__any_sync(0xffffffffu, far > TAU || step_bits > __float_as_uint(step_lim))) {
-      uint32_t top = 0;
+    if (__any_sync(0xffffffffu, far > TAU || more)) {
+      float f[NT][2];
 #pragma unroll
-      for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int i = 0; i < MG; i++) {
-          const uint32_t st = __float_as_uint(open_pair<T>(vp[r][i]).x);
-          if (st < 0x7f800000u) top = max(top, st);
-        }
-      top = __reduce_max_sync(0xffffffffu, top);
-      float up = 0.f;   // change of ce
-      if (top > __float_as_uint(step_lim)) {
-        const float e = fminf(fmaxf(130.f - (float)(top >> 23), -100.f), 100.f);   // 8 <= top 2^e < 16
-        up = e - ce;
-        ce = e;
-        step_lim = ex2(9.f - e);
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           float mx = fmaxf(s[nt][e], s[nt][2 + e]) * sc[nt][e];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-          const float mn = fmaxf(m[nt][e], mx), f = ex2(m[nt][e] - mn + up);
+          const float mn = fmaxf(m[nt][e], mx);
+          f[nt][e] = ex2(m[nt][e] - mn);
           m[nt][e] = mn;
-          l[nt][e] *= f;
+          l[nt][e] *= f[nt][e];
+        }
 #pragma unroll
-          for (int j = 0; j < MG; j++) mid[nt][j][e] *= f;
+      for (int i = 0; i < MG; i++) {
+        const int j = group_of(i);
+        lim[i] = INFINITY;
 #pragma unroll
-          for (int j = 0; j < 2 * NG; j++) {
-            o[nt][j][e] *= f;
-            o[nt][j][2 + e] *= f;
+        for (int nt = 0; nt < NT; nt++) {
+          uint32_t top = 0;   // the largest finite step that column 0 sees, in the low half, that column 1 sees in the high one
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const uint32_t st = vp[r][i] & 0xffffu, fine = st < bits(DT<T>::from_f(INFINITY)) ? st : 0u;
+            const int key = key0 + g + 8 * r;
+            top = __vmaxu2(top, EDGE ? (key <= cpos[nt][0] ? fine : 0u) | (key <= cpos[nt][1] ? fine << 16 : 0u) : fine * 0x10001u);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float2 most = open_pair<T>(top);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint32_t was = __float_as_uint(up[nt][j][e]), t2 = __float_as_uint(e ? most.y : most.x);
+            const uint32_t now = (e ? most.y : most.x) * up[nt][j][e] > 512.f ? (257u - (t2 >> 23)) << 23 : was;   // 8 <= top up < 16
+            const float change = now + 0x3f800000u > was ? __uint_as_float(now + 0x3f800000u - was) * f[nt][e] : 0.f;   // now / was, a power of two
+            up[nt][j][e] = __uint_as_float(now);
+            lim[i] = fminf(lim[i], 512.f * __uint_as_float(0x7f000000u - now));
+            mid[nt][j][e] *= f[nt][e];
+#pragma unroll
+            for (int k = 2 * PK * j; k < 2 * PK * (j + 1); k++) {   // the group's sums (PK 2: and the neighbour's, which the lane's columns don't have)
+              o[nt][k][e] *= change;
+              o[nt][k][2 + e] *= change;
+            }
           }
         }
       }
@@ -689,7 +708,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        s[nt][i] = EDGE && s[nt][i] == -INFINITY ? 0.f : ex2(fmaf(s[nt][i], sc[nt][i & 1], ce - m[nt][i & 1]));   // (sc may have become 0)
+        s[nt][i] = EDGE && s[nt][i] == -INFINITY ? 0.f : ex2(fmaf(s[nt][i], sc[nt][i & 1], -m[nt][i & 1]));   // (sc may have become 0)
         l[nt][i & 1] += s[nt][i];
       }
     auto times = [](float w, float x) { return EDGE && w == 0.f ? 0.f : w * x; };   // a key that a row does not see may be anything
@@ -705,12 +724,12 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
             b1[1] = b1[0];
             continue;
           }
-          const int i = PK == 2 ? w : h * (NG / 2) + w;   // the pair's word; its sums' place
-          const int jj = PK == 2 ? w : 2 * w + h;
+          const int i = PK == 2 ? w : h * (NG / 2) + w, jj = group_of(i);   // the pair's word; its sums' place
+          const float u0 = up[nt][jj][0], u1 = up[nt][jj][1];
           const float2 p0 = open_pair<T>(vp[0][i]), p1 = open_pair<T>(vp[1][i]);
           const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y);
-          b0[h] = turn8x8(pack2x<__half>(times(s[nt][0], p0.x), times(s[nt][1], p0.x)));
-          b1[h] = turn8x8(pack2x<__half>(times(s[nt][2], p1.x), times(s[nt][3], p1.x)));
+          b0[h] = turn8x8(pack2x<__half>(times(s[nt][0], p0.x * u0), times(s[nt][1], p0.x * u1)));
+          b1[h] = turn8x8(pack2x<__half>(times(s[nt][2], p1.x * u0), times(s[nt][3], p1.x * u1)));
           mid[nt][jj][0] += times(s[nt][0], m0);
           mid[nt][jj][0] += times(s[nt][2], m1);
           mid[nt][jj][1] += times(s[nt][1], m0);
@@ -768,15 +787,16 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int e = 0; e < 2; e++) {
       const int col = nt * 8 + 2 * tc + e;
       if (g == 0 && half == 0) {
-        sm[warp * COLS + col] = l[nt][e] == 0.f ? -INFINITY : m[nt][e] - ce;
+        sm[warp * COLS + col] = l[nt][e] == 0.f ? -INFINITY : m[nt][e];
         sl[warp * COLS + col] = l[nt][e];
       }
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        const float z = mid[nt][j / PK][e];
+        const float z = mid[nt][j / PK][e], down = __uint_as_float((254u << 23) - __float_as_uint(up[nt][j / PK][e]));   // 1 / up
         if (PK == 1 || (j & 1) == half)
           *reinterpret_cast<float4 *>(&so[(warp * COLS + col) * OUT_LD + 32 * j + 4 * g]) =
-              make_float4(o[nt][2 * j][e] + z, fmaf(0.0625f, o[nt][2 * j][2 + e], z), o[nt][2 * j + 1][e] + z, fmaf(0.0625f, o[nt][2 * j + 1][2 + e], z));
+              make_float4(fmaf(down, o[nt][2 * j][e], z), fmaf(0.0625f * down, o[nt][2 * j][2 + e], z), fmaf(down, o[nt][2 * j + 1][e], z),
+                          fmaf(0.0625f * down, o[nt][2 * j + 1][2 + e], z));
       }
     }
   __syncthreads();
