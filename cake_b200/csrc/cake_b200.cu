@@ -33,6 +33,7 @@
 #include "gemm_skinny.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
+#include "kept_memory.cuh"
 #include "packed_cache.cuh"
 #include "prefill.cuh"
 #include "sample.cuh"
@@ -152,8 +153,7 @@ struct cake_b200_ctx {
   size_t io_x_cap = 0;
   // attention over caches in four bits: sums of keys cut over several CTAs, CTAs that have come
   float *pc_ws = nullptr;
-  void *pc_rows = nullptr;   // rows of such caches in D, for the kernels of prompts
-  size_t pc_rows_cap = 0;
+  KeptMemory pc_rows;   // rows of such caches in D, for the kernels of prompts
   unsigned *pc_tickets = nullptr;
   cudaMemPool_t pc_pool = nullptr;   // the caches' memory: a closed cache's is the next one's (a new cache of 67 MB: 20 us, 3 ms from the driver)
   // The operators of such caches may run on a caller's stream: `stream` then is that one for the call.  pc_out: behind the last of them, waited for by
@@ -671,9 +671,10 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
                   c->token_ring, c->d_ids, c->d_pen, c->pf_h, c->pf_qkv, c->pf_y, c->pf_x1, c->pf_gu, c->pf_mm, c->io_x,
                   c->gbar, c->mk_pk, c->mk_part, c->mk_tab_dev, c->g_tab_dev, c->tickets, c->ring_seq, c->inbox, c->step_trace, c->trace,
                   c->samp_p, c->samp_noise, c->hd_logits, c->hd_tokens, c->x0, c->sp_h, c->sp_hs, c->sp_in, c->sp_a, c->sp_hn, c->sp_logits, c->sp_rows_idx, c->mx_ws,
-                  c->pc_ws, c->pc_tickets, c->pc_rows};
+                  c->pc_ws, c->pc_tickets};
   for (void *b : bufs)
     if (b) cudaFree(b);
+  c->pc_rows.release_all([](void *p) { cudaFree(p); });
   if (c->bigram) cudaFree(c->bigram);
   if (c->pos_tab) cudaFree(c->pos_tab);
   for (void *b : {c->side_tab, c->ln_f_b, c->proj_w, c->proj_ws, c->embed_norm})
@@ -1201,7 +1202,7 @@ static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_
                             float sc, const NanMarks &nan);
 // Attention of S rows a batch row over a packed cache; the rows' own positions are in it.  Many rows of heads of 128 entries take the kernel of
 // prompts, whose operands are rows in D: the keys and values that the call sees are expanded once (each entry rounded to D) into memory of the ctx, which
-// grows on first use; above PC_EXPAND_MOST a few batch rows at a time.  (Heads of 64: their prompt kernel, on mma.sync, does not cut the keys: 1024 rows of
+// grows on first use (what a captured call has used stays); above PC_EXPAND_MOST a few batch rows at a time.  (Heads of 64: their prompt kernel, on mma.sync, does not cut the keys: 1024 rows of
 // 8 / 2 heads at 2000 positions 190 us, 58 on codes.)
 constexpr size_t PC_EXPAND_MOST = (size_t)1 << 30;
 static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, const void *q, size_t q_tok, size_t q_batch, void *out, int S, int pos0,
@@ -1215,16 +1216,23 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
     const size_t slab = (size_t)f.n_kv_heads * cap * hd * c->es, marks = (size_t)f.n_kv_heads * blocks * 8;   // of a batch row
     const int group = (int)std::max<size_t>(1, std::min<size_t>(kc->batch, PC_EXPAND_MOST / (2 * slab)));
     const size_t need = group * (2 * slab + marks);
-    if (need > c->pc_rows_cap) {
+    cudaStreamCaptureStatus st;
+    CU(cudaStreamIsCapturing(c->stream, &st));
+    if (c->pc_rows.short_of(need, st != cudaStreamCaptureStatusNone)) {
       RC(no_capture(c->stream, "memory for the rows that a call of many rows expands"));
       CU(cudaStreamSynchronize(c->stream));
-      if (c->pc_rows) { cudaFree(c->pc_rows); c->pc_rows = nullptr; c->pc_rows_cap = 0; }
-      CU(cudaMalloc(&c->pc_rows, need));
-      c->pc_rows_cap = need;
+      cudaError_t e = cudaSuccess;
+      c->pc_rows.grow(need, PC_EXPAND_MOST, [&](size_t bytes) -> void * {
+        void *p = nullptr;
+        e = cudaMalloc(&p, bytes);
+        if (e != cudaSuccess) (void)cudaGetLastError();
+        return e == cudaSuccess ? p : nullptr;
+      }, [](void *p) { cudaFree(p); });
+      CU(e);
     }
     for (int b0 = 0; b0 < kc->batch; b0 += group) {
       const int nb = std::min(group, kc->batch - b0);
-      char *kr = (char *)c->pc_rows, *vr = kr + group * slab;
+      char *kr = (char *)c->pc_rows.now, *vr = kr + group * slab;
       unsigned long long *nan = (unsigned long long *)(vr + group * slab);
       const char *from = (const char *)kc->k[l] + (size_t)b0 * f.n_kv_heads * a.blocks * pc::block_bytes(hd);
       pc::Read r{from, kr, vr, nb, f.n_kv_heads, hd, a.blocks, first, n, cap, nan};

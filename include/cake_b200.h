@@ -397,7 +397,8 @@ int cake_b200_cache_fill_synthetic(cake_b200_cache *, const int *block_idx, int 
  * The three calls below run on `stream`, the cudaStream_t that their tensors belong to (cudaStreamLegacy for the default stream; NULL: the ctx's own),
  * behind what the ctx's other calls have enqueued, which in turn go on behind them.  It may be capturing, once the same call has run outside a
  * capture (memory is made on first use; CAKE_B200_ESTATE otherwise).  A captured call takes its place in the graph alone: graphs captured from calls of one
- * ctx share its scratch and are replayed neither at the same time nor beside its calls. */
+ * ctx share its scratch and are replayed neither at the same time nor beside its calls; before and after them they may be, whatever the calls, until the cache is
+ * closed. */
 int cake_b200_cache_create_packed(cake_b200_ctx *, int batch, int max_seq, int bits, cake_b200_cache **out);
 /* Rows k, v (batch, seq, n_kv, head_dim) in D, as they are, join block_idx's part of the cache at index_pos, which is its length or less: what is behind
  * index_pos is dropped and the length becomes index_pos + seq (CAKE_B200_ESTATE where index_pos is beyond the length or the rows beyond the
