@@ -31,6 +31,7 @@ static int launch(cudaStream_t s, uint64_t *launches, void (*kern)(KArgs...), di
 template <typename T> __device__ __forceinline__ T round_up(float f);
 template <> __device__ __forceinline__ __nv_bfloat16 round_up<__nv_bfloat16>(float f) { return __float2bfloat16_ru(f); }
 template <> __device__ __forceinline__ __half round_up<__half>(float f) { return __float2half_ru(f); }
+template <typename T> __device__ __forceinline__ uint32_t most2() { return std::is_same<T, __half>::value ? 0x7bff7bffu : 0x7f7f7f7fu; }   // D's largest number, twice
 template <typename T> __device__ __forceinline__ uint32_t bits(T v) { return *reinterpret_cast<const uint16_t *>(&v); }
 template <typename T> __device__ __forceinline__ float2 open_pair(uint32_t p) { return DT<T>::unpack2(p); }   // (step, lo)
 
@@ -267,7 +268,9 @@ __global__ void __launch_bounds__(128) write_kernel(const Write a) {
 
 // ------------------------------------------------------------------------------------------ rows out of the cache
 // Bound by memory too: 5 bits read and 16 written an entry.  A warp takes a block: K's words as they lie (a row's four lanes write 64 bytes of it
-// together), V's likewise (8 lanes write 64 bytes of a row).  A value is one fma in pairs of D on exact codes: one rounding.
+// together), V's likewise (8 lanes write 64 bytes of a row).  A value is one fma in pairs of D on exact codes: one rounding; as step is rounded up, the
+// highest codes of a group that reaches D's end may lie beyond it: they become D's largest number (an infinity would be one that nobody wrote, and NaN for
+// every row whose weight for it is zero).
 // 32768 positions of 8 heads of 128, K and V: 71 us with 2-byte reads of V and 64-bit divisions a lane; so 30 (5.85 TB/s).
 // As operands of matrix products (a.nan): a group that reads as NaN becomes zero, so that it counts for no row that does not see it, and the
 // block's word says where: byte 0 the first position (in the block) whose K has such a group, byte 1 + j that of V's group j, 255 none.
@@ -300,6 +303,7 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
   const char *blk = reinterpret_cast<const char *>(a.cache) + ((size_t)slab * a.blocks + blk0 + i) * block_bytes(HD);
   const int row0 = 16 * (blk0 + i) - a.first;   // the output row of the block's first position
   bool any_nan = false;
+  auto value = [](uint32_t n, const uint32_t (&q)[2]) { return min2<T>(fma2<T>(n, q[0], q[1]), most2<T>()); };   // (keeps a NaN)
   auto pair_of = [&](uint32_t p, uint32_t (&q)[2]) {   // step and lo, twice each
     if (a.nan && (p & 0x7fffu) > (sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u)) {
       any_nan = true;
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
         else q[0] = q[1] = 0u;
         if (in)
           *reinterpret_cast<uint4 *>(out + (size_t)r * HD + 32 * j + 8 * t) =
-              make_uint4(fma2<T>(c[0], q[0], q[1]), fma2<T>(c[1], q[0], q[1]), fma2<T>(c[2], q[0], q[1]), fma2<T>(c[3], q[0], q[1]));
+              make_uint4(value(c[0], q), value(c[1], q), value(c[2], q), value(c[3], q));
       }
     }
   }
@@ -348,11 +352,11 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
                        b1 = __byte_perm(c[2], c[3], 0x7632);
         if (in0) {
           pair_of(p0[(j & 1) * (NG / 2) + j / 2], q);
-          *reinterpret_cast<uint2 *>(out + (size_t)r * HD + 32 * j + 4 * g) = make_uint2(fma2<T>(a0, q[0], q[1]), fma2<T>(a1, q[0], q[1]));
+          *reinterpret_cast<uint2 *>(out + (size_t)r * HD + 32 * j + 4 * g) = make_uint2(value(a0, q), value(a1, q));
         }
         if (in1) {
           pair_of(p1[(j & 1) * (NG / 2) + j / 2], q);
-          *reinterpret_cast<uint2 *>(out + (size_t)(r + 1) * HD + 32 * j + 4 * g) = make_uint2(fma2<T>(b0, q[0], q[1]), fma2<T>(b1, q[0], q[1]));
+          *reinterpret_cast<uint2 *>(out + (size_t)(r + 1) * HD + 32 * j + 4 * g) = make_uint2(value(b0, q), value(b1, q));
         }
       }
     }
@@ -804,8 +808,12 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
   auto put = [&](int col, int d, const float (&v)[4], float L) {
     const int c = c0 + col, tok = tok_of(c);
     const float f = L == 0.f ? 0.f : 1.f / L;   // 0: the row sees nothing
+    auto held = [](float x) {   // the highest codes' values may lie beyond D's end, see read_kernel
+      const float most = DT<T>::unpack2(most2<T>()).x;
+      return x > most ? most : x < -most ? -most : x;
+    };
     T *y = reinterpret_cast<T *>(a.out) + ((size_t)(b * (long long)a.S + tok) * a.n_heads + kvh * G + c - tok * G) * HD + d;
-    *reinterpret_cast<uint2 *>(y) = make_uint2(pack2x<T>(v[0] * f, v[1] * f), pack2x<T>(v[2] * f, v[3] * f));
+    *reinterpret_cast<uint2 *>(y) = make_uint2(pack2x<T>(held(v[0] * f), held(v[1] * f)), pack2x<T>(held(v[2] * f), held(v[3] * f)));
   };
   // parts of this unit, where there are several: CTAs first_cta .., in the line
   const bool parted = in_line && !whole;
