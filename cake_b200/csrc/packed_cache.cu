@@ -1004,6 +1004,8 @@ template <typename T, int HD, int NT, int PK> static int attend_split(cudaStream
   return launch(s, launches, attend_split_kernel<T, HD, NT, PK>, grid, dim3(SP_WARPS * 32), (size_t)smem, line ? 1 : cluster, p);
 }
 int attend(cudaStream_t s, int dtype, const Attend &a, const Scratch &x, uint64_t *launches) {
+  if (!a.d_pos && a.first >= (long long)a.pos0 + a.S)   // no row sees anything (and a line of no blocks would have no CTA to say so)
+    return (int)cudaMemsetAsync(a.out, 0, (size_t)a.B * a.S * a.n_heads * a.hd * 2, s);
   return by_type(dtype, a.hd, [&](auto t, auto hd) {
     typedef decltype(t) T;
     constexpr int HD = hd.value;
