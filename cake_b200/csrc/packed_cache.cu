@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
         s[nt][i] = EDGE && s[nt][i] == -INFINITY ? 0.f : ex2(fmaf(s[nt][i], sc[nt][i & 1], -m[nt][i & 1]));   // (sc may have become 0)
         l[nt][i & 1] += s[nt][i];
       }
-    auto times = [](float w, float x) { return EDGE && w == 0.f ? 0.f : w * x; };   // a key that a row does not see may be anything
+    // weight i of a row times a number of its key: a key that the row does not see may be anything (one that it does may be NaN, whatever the weight)
+    auto times = [&](int nt, int i, float x) { return EDGE && key0 + g + 8 * (i >> 1) > cpos[nt][i & 1] ? 0.f : s[nt][i] * x; };
 #pragma unroll
     for (int w = 0; w < NG / 2; w++)
 #pragma unroll
@@ -732,12 +733,12 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
           const float u0 = up[nt][jj][0], u1 = up[nt][jj][1];
           const float2 p0 = open_pair<T>(vp[0][i]), p1 = open_pair<T>(vp[1][i]);
           const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y);
-          b0[h] = turn8x8(pack2x<__half>(times(s[nt][0], p0.x * u0), times(s[nt][1], p0.x * u1)));
-          b1[h] = turn8x8(pack2x<__half>(times(s[nt][2], p1.x * u0), times(s[nt][3], p1.x * u1)));
-          mid[nt][jj][0] += times(s[nt][0], m0);
-          mid[nt][jj][0] += times(s[nt][2], m1);
-          mid[nt][jj][1] += times(s[nt][1], m0);
-          mid[nt][jj][1] += times(s[nt][3], m1);
+          b0[h] = turn8x8(pack2x<__half>(times(nt, 0, p0.x * u0), times(nt, 1, p0.x * u1)));
+          b1[h] = turn8x8(pack2x<__half>(times(nt, 2, p1.x * u0), times(nt, 3, p1.x * u1)));
+          mid[nt][jj][0] += times(nt, 0, m0);
+          mid[nt][jj][0] += times(nt, 2, m1);
+          mid[nt][jj][1] += times(nt, 1, m0);
+          mid[nt][jj][1] += times(nt, 3, m1);
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -835,9 +836,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
       const float4 x = *reinterpret_cast<const float4 *>(&so[(w * COLS + col) * OUT_LD + d]);
       L = fmaf(f, sl[w * COLS + col], L);
-      if (f != 0.f) {
-        v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
-      }
+      v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);   // (NaN also where f is too small for a number)
     }
     if (whole) put(col, d, v, L);
     else if (parted) {
@@ -865,9 +864,8 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       for (int s = 0; s < 1 << lg; s++) {
         const float f = x[8 * s + 4] == -INFINITY ? 0.f : ex2(x[8 * s + 4] - M);
         L = fmaf(f, x[8 * s + 5], L);
-        if (f != 0.f)
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = fmaf(f, x[8 * s + e], v[e]);
+        for (int e = 0; e < 4; e++) v[e] = fmaf(f, x[8 * s + e], v[e]);
       }
       put(i / (HD / 4), i % (HD / 4) * 4, v, L);
     }
@@ -927,9 +925,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
           for (int e = 0; e < n; e++) {
             const float w = f[e * PART];
             const float4 y = *reinterpret_cast<const float4 *>(x + e * PART);
-            if (w != 0.f) {
-              v[0] = fmaf(w, y.x, v[0]); v[1] = fmaf(w, y.y, v[1]); v[2] = fmaf(w, y.z, v[2]); v[3] = fmaf(w, y.w, v[3]);
-            }
+            v[0] = fmaf(w, y.x, v[0]); v[1] = fmaf(w, y.y, v[1]); v[2] = fmaf(w, y.z, v[2]); v[3] = fmaf(w, y.w, v[3]);
           }
           if (s0 == parts) put(col, d, v, ml[COLS + col]);
           else *reinterpret_cast<float4 *>(x) = make_float4(v[0], v[1], v[2], v[3]);

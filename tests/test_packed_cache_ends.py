@@ -74,3 +74,31 @@ def test_rows_do_not_see_what_lies_behind_them(s, at, dtype):
     got = cache.attend(0, q, at)
     assert torch.equal(got[:, :s - late], clean[:, :s - late])
     ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,hd,s,n", [(4, 2, 128, 1, 10), (4, 2, 128, 1, 700), (4, 2, 128, 1, 20000), (8, 2, 64, 3, 100), (8, 1, 128, 3, 40), (4, 2, 256, 1, 3000), (32, 8, 128, 150, 400)])
+def test_nan_reaches_a_row_through_any_weight(heads, kv, hd, s, n, dtype):
+    """A key whose score is 700 below the others': its weight is no number of fp32, but a value that is NaN still is one that the rows see."""
+    ctx = ctx_for(heads, kv, hd, dtype, max_seq=n)
+    k, v = torch.zeros((1, n, kv, hd)), rows(1, n, kv, hd, dtype, 2)
+    at = n - s
+    q = torch.ones((1, s, heads, hd)).to(TORCH_DTYPES[dtype]).cuda()
+    for far in {0, at // 2, at - 1, at}:
+        kf, vf = k.clone(), v.clone()
+        kf[:, far] = -700.0 * hd ** -0.5
+        kf = kf.to(v.dtype).cuda()
+        cache = Cache(ctx, 1, n, bits=4)
+        cache.write(0, kf, vf, 0)
+        clean = cache.attend(0, q, at)
+        assert torch.isfinite(clean).all()
+        vf[:, far, 0, 40] = torch.nan
+        cache.write(0, kf, vf, 0)
+        got = cache.attend(0, q, at)
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[:, :, :heads // kv, 32:64] = True
+        assert torch.equal(got.isnan(), bad), far
+        assert torch.equal(got[~bad], clean[~bad])
+        cache.close()
+    ctx.close()
