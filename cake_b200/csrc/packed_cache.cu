@@ -395,9 +395,11 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 // steps at most.  (What binds the kernel is issue: 340 instructions a block and warp, 150 of them on the ALU at half rate.)
 // PK = 2, up to 4 rows: columns 0 .. 3 of an operand belong to a group and columns 4 .. 7 to its neighbour (the queries of the other are zero there),
 // so that no lane works for columns without a row; a row's two halves join by a shuffle.
-// A row's reference m moves when a score exceeds it by 2^6 (TAU).  Every row and group has a power of two `up` that keeps the steps which the row sees at
-// 512 at most, the first ones at 8 to 16: weights times steps then use fp16's range whatever the size of V's entries, of other groups' (one power for all
-// groups took a group 2^24 times smaller than its neighbour for one value) and of those in places that only other rows of the call see.
+// A row's reference m moves when a score exceeds it by 2^6 (TAU).  Every group has a power of two `up` that keeps its steps at 512 at most, the first ones at
+// 8 to 16: weights times steps then use fp16's range whatever the size of V's entries and of other groups' (one power for all groups took a
+// group 2^24 times smaller than its neighbour for one value).  It is the same for all rows; a block with positions that only later rows of the call see, and
+// much larger steps there, is taken in the order of those positions, so that a row's own weights meet the power of what it sees.  (A power per row
+// and group: 32 sequences of 2 rows at 4000 positions 62.6 us, 46.7 with one power in all.)
 //
 // Who takes which blocks: a unit is 8 NT / PK rows of a (batch row, key head).  Short caches: the CTAs of a cluster cut a unit's blocks between them and
 // join over the cluster's shared memory.  Else all units' blocks lie in one line that the grid, two CTAs per SM, cuts into equal parts; a CTA's part of
@@ -569,19 +571,18 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int e2 = 0; e2 < 2; e2++) cpos[nt][e2] = pos0 + tok_of(min(c0 + nt * 8 + 2 * tc + e2, p.cols - 1));
   }
   float o[NT][2 * NG][4] = {}, mid[NT][MG][2] = {}, m[NT][2], l[NT][2] = {};
-  float up[NT][MG][2], lim[MG];   // lim: the step of the pairs' i-th word from which on `up` has to change for one of the lane's columns
-  constexpr float TAU = 6.f, UP0 = 8.50705917e37f;   // 2^126
+  float up[MG];   // of the group of the lane's i-th word of pairs
+  constexpr float TAU = 6.f;
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -3.402823466e38f;
 #pragma unroll
-  for (int j = 0; j < MG; j++) {
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) up[nt][j][0] = up[nt][j][1] = UP0;
-    lim[j] = 512.f / UP0;
-  }
+  for (int i = 0; i < MG; i++) up[i] = 8.50705917e37f;   // 2^126
   auto group_of = [](int i) { return PK == 1 ? 2 * (i % (NG / 2)) + i / (NG / 2) : i; };   // the lane's group that its i-th word of pairs belongs to
 
-  auto body = [&](auto edge_, const unsigned char *blk, int key0) {
+  // the finite one of a pair's step, as the 16 bits of D that it is (no step is negative: as integers they have their order)
+  auto step_bits = [](uint32_t pair) { return (pair & 0xffffu) < bits(DT<T>::from_f(INFINITY)) ? pair & 0xffffu : 0u; };
+  // EDGE: of the block's positions from .. to, those that a row sees
+  auto body = [&](auto edge_, const unsigned char *blk, int key0, int from, int to) {
     constexpr bool EDGE = decltype(edge_)::value;
     float s[NT][4] = {};
     {
@@ -635,14 +636,13 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
 #pragma unroll
     for (int r = 0; r < 2; r++) {
       lds_words<MG>(blk + v_pairs(HD) + ((g + 8 * r) * NG + half * MG) * 4, vp[r]);
-      const bool seen = !EDGE || (key0 + g + 8 * r >= first && key0 + g + 8 * r <= pos_hi);   // by any row: the others' steps say nothing
+      const bool seen = !EDGE || (key0 + g + 8 * r >= from && key0 + g + 8 * r <= to);   // by any row: the others' steps say nothing
 #pragma unroll
       for (int i = 0; i < MG; i++) vp[r][i] = seen ? vp[r][i] : 0u;
     }
     bool more = false;   // steps beyond what `up` is for
 #pragma unroll
-    for (int i = 0; i < MG; i++)   // no step is negative; NaN is the largest
-      more = more || max(__float_as_uint(open_pair<T>(vp[0][i]).x), __float_as_uint(open_pair<T>(vp[1][i]).x)) > __float_as_uint(lim[i]);
+    for (int i = 0; i < MG; i++) more = more || fmaxf(open_pair<T>(vp[0][i]).x, open_pair<T>(vp[1][i]).x) * up[i] > 512.f;
     // scores less their reference, in powers of two
     float far = -INFINITY;
 #pragma unroll
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       for (int i = 0; i < 4; i++) {
         if (EDGE) {
           const int key = key0 + g + 8 * (i >> 1);
-          if (key < first || key > cpos[nt][i & 1]) s[nt][i] = -INFINITY;
+          if (key < from || key > to || key > cpos[nt][i & 1]) s[nt][i] = -INFINITY;
         }
         far = fmaxf(far, fmaf(s[nt][i], sc[nt][i & 1], -m[nt][i & 1]));
       }
@@ -672,34 +672,25 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
 #pragma unroll
       for (int i = 0; i < MG; i++) {
         const int j = group_of(i);
-        lim[i] = INFINITY;
+        uint32_t top = max(step_bits(vp[0][i]), step_bits(vp[1][i]));
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          uint32_t top = 0;   // the largest finite step that column 0 sees, in the low half, that column 1 sees in the high one
+        for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float most = open_pair<T>(top).x;
+        const uint32_t was = __float_as_uint(up[i]), now = most * up[i] > 512.f ? (257u - (__float_as_uint(most) >> 23)) << 23 : was;   // 8 <= most up < 16
+        const float change = now + 0x3f800000u > was ? __uint_as_float(now + 0x3f800000u - was) : 0.f;   // now / was, a power of two
+        up[i] = __uint_as_float(now);
 #pragma unroll
-          for (int r = 0; r < 2; r++) {
-            const uint32_t st = vp[r][i] & 0xffffu, fine = st < bits(DT<T>::from_f(INFINITY)) ? st : 0u;
-            const int key = key0 + g + 8 * r;
-            top = __vmaxu2(top, EDGE ? (key <= cpos[nt][0] ? fine : 0u) | (key <= cpos[nt][1] ? fine << 16 : 0u) : fine * 0x10001u);
-          }
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const float2 most = open_pair<T>(top);
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const uint32_t was = __float_as_uint(up[nt][j][e]), t2 = __float_as_uint(e ? most.y : most.x);
-            const uint32_t now = (e ? most.y : most.x) * up[nt][j][e] > 512.f ? (257u - (t2 >> 23)) << 23 : was;   // 8 <= top up < 16
-            const float change = now + 0x3f800000u > was ? __uint_as_float(now + 0x3f800000u - was) * f[nt][e] : 0.f;   // now / was, a power of two
-            up[nt][j][e] = __uint_as_float(now);
-            lim[i] = fminf(lim[i], 512.f * __uint_as_float(0x7f000000u - now));
             mid[nt][j][e] *= f[nt][e];
+            const float fc = f[nt][e] * change;
 #pragma unroll
             for (int k = 2 * PK * j; k < 2 * PK * (j + 1); k++) {   // the group's sums (PK 2: and the neighbour's, which the lane's columns don't have)
-              o[nt][k][e] *= change;
-              o[nt][k][2 + e] *= change;
+              o[nt][k][e] *= fc;
+              o[nt][k][2 + e] *= fc;
             }
           }
-        }
       }
     }
     uint32_t vw[2 * NG];
@@ -716,7 +707,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
         l[nt][i & 1] += s[nt][i];
       }
     // weight i of a row times a number of its key: a key that the row does not see may be anything (one that it does may be NaN, whatever the weight)
-    auto times = [&](int nt, int i, float x) { return EDGE && key0 + g + 8 * (i >> 1) > cpos[nt][i & 1] ? 0.f : s[nt][i] * x; };
+    auto times = [&](int nt, int i, float x) { return EDGE && key0 + g + 8 * (i >> 1) > min(cpos[nt][i & 1], to) ? 0.f : s[nt][i] * x; };
 #pragma unroll
     for (int w = 0; w < NG / 2; w++)
 #pragma unroll
@@ -730,11 +721,10 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
             continue;
           }
           const int i = PK == 2 ? w : h * (NG / 2) + w, jj = group_of(i);   // the pair's word; its sums' place
-          const float u0 = up[nt][jj][0], u1 = up[nt][jj][1];
           const float2 p0 = open_pair<T>(vp[0][i]), p1 = open_pair<T>(vp[1][i]);
-          const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y);
-          b0[h] = turn8x8(pack2x<__half>(times(nt, 0, p0.x * u0), times(nt, 1, p0.x * u1)));
-          b1[h] = turn8x8(pack2x<__half>(times(nt, 2, p1.x * u0), times(nt, 3, p1.x * u1)));
+          const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y), x0 = p0.x * up[i], x1 = p1.x * up[i];
+          b0[h] = turn8x8(pack2x<__half>(times(nt, 0, x0), times(nt, 1, x0)));
+          b1[h] = turn8x8(pack2x<__half>(times(nt, 2, x1), times(nt, 3, x1)));
           mid[nt][jj][0] += times(nt, 0, m0);
           mid[nt][jj][0] += times(nt, 2, m1);
           mid[nt][jj][1] += times(nt, 1, m0);
@@ -766,8 +756,34 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     st = st == SP_STAGES - 1 ? 0 : st + 1;
     const int key0 = (mine0 + warp + i * WARPS) * 16;
     if (key0 > pos_hi) ;   // only later rows of the call see it
-    else if (key0 < first || key0 + 15 > pos_lo) body(std::true_type{}, blk, key0);
-    else body(std::false_type{}, blk, key0);
+    else if (key0 < first || key0 + 15 > pos_lo) {
+      // positions that not all rows see and whose steps are far beyond what `up` is for and the others have: one after the other
+      const int all = max(pos_lo, max(key0, first));   // those up to here come first
+      bool far = false;
+      if (all < pos_hi) {
+#pragma unroll
+        for (int i = 0; i < MG; i++) {
+          uint32_t top = 0;   // the largest step of the first ones in the low half, of the others in the high one
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            const uint32_t st = step_bits(reinterpret_cast<const uint32_t *>(blk + v_pairs(HD) + ((g + 8 * r) * NG + half * MG) * 4)[i]);
+            const int key = key0 + g + 8 * r;
+            top = __vmaxu2(top, key < first || key > pos_hi ? 0u : key <= all ? st : st << 16);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float2 most = open_pair<T>(top);
+          far = far || (most.y > 64.f * most.x && most.y * up[i] > 512.f);
+        }
+        far = __any_sync(0xffffffffu, far);
+      }
+      const int end = min(pos_hi, key0 + 15);
+      for (int from = first, to = far ? min(all, end) : end;; from = ++to) {
+        body(std::true_type{}, blk, key0, from, to);
+        if (to == end) break;
+      }
+    }
+    else body(std::false_type{}, blk, key0, 0, 0);
   }
   copies_wait<0>();
 
@@ -797,7 +813,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
       }
 #pragma unroll
       for (int j = 0; j < NG; j++) {
-        const float z = mid[nt][j / PK][e], down = __uint_as_float((254u << 23) - __float_as_uint(up[nt][j / PK][e]));   // 1 / up
+        const float z = mid[nt][j / PK][e], down = __uint_as_float((254u << 23) - __float_as_uint(up[PK == 2 ? j / 2 : (j & 1) * (NG / 2) + j / 2]));   // 1 / up
         if (PK == 1 || (j & 1) == half)
           *reinterpret_cast<float4 *>(&so[(warp * COLS + col) * OUT_LD + 32 * j + 4 * g]) =
               make_float4(fmaf(down, o[nt][2 * j][e], z), fmaf(0.0625f * down, o[nt][2 * j][2 + e], z), fmaf(down, o[nt][2 * j + 1][e], z),

@@ -68,7 +68,7 @@ def few_rows(q, kx, vx, at, first, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("heads,kv,hd,s", [(4, 2, 128, 1), (8, 2, 64, 1), (8, 1, 128, 1), (4, 1, 128, 4), (4, 1, 64, 5), (2, 1, 256, 1), (2, 1, 256, 4)])
+@pytest.mark.parametrize("heads,kv,hd,s", [(4, 2, 128, 1), (8, 2, 64, 1), (8, 1, 128, 1), (4, 1, 128, 4), (4, 1, 64, 5), (2, 1, 256, 1), (2, 1, 256, 4), (1, 1, 128, 12), (2, 2, 64, 16), (8, 8, 128, 7)])
 def test_groups_of_values_keep_their_bits_whatever_else_there_is(heads, kv, hd, s, dtype):
     """Values of one head whose groups differ in size by 2^30 (f16: 2^24, which is most of its range); positions whose values are far larger than those in
     front of them, which the rows in front do not see.  Keys of one value per group, so that scores are all but exact."""
@@ -82,7 +82,8 @@ def test_groups_of_values_keep_their_bits_whatever_else_there_is(heads, kv, hd, 
         exps = torch.tensor([0, 30, 15, 3] * 2 if dtype == "bf16" else [-10, 13, 0, 7] * 2)[:hd // 32]
         sizes = v * torch.exp2(exps.double()).float().repeat_interleave(32)
         later = v * torch.exp2(torch.where(torch.arange(n) > n - s, 40.0 if dtype == "bf16" else 13.0, 0.0))[None, :, None, None] * (1.0 if dtype == "bf16" else 2.0 ** -8)
-        for x in (sizes, sizes.flip(3), later):
+        rising = v * torch.exp2((torch.arange(n) - (n - s)).clamp(min=0) * (7.0 if dtype == "bf16" else 1.3))[None, :, None, None] * (1.0 if dtype == "bf16" else 2.0 ** -8)
+        for x in (sizes, sizes.flip(3), later, later.flip(1), rising, rising.flip(1)):
             x = x.clamp(-60000, 60000).to(D).cuda() if dtype == "f16" else x.to(D).cuda()
             cache = Cache(ctx, 1, n, bits=4)
             cache.write(0, k, x, 0)
