@@ -87,13 +87,19 @@ size_t scratch_floats(int sms);
 size_t scratch_tickets(int sms);
 int prepare(int dtype, int hd);   // once per device and kind of cache, in front of the first call
 int attend(cudaStream_t, int dtype, const Attend &, const Scratch &, uint64_t *launches);
-// Whether keys and values expanded once, for the kernel of prompts, are the faster way: where the pieces of 16 rows are more than the SMs, or their
-// blocks (0.48 us a quarter SM each) take longer than expanding and reading the rows in D (8 key heads: 3.5 us per 1000 positions and 20).  32 / 8 heads,
-// on codes and expanded: 64 rows at 0 7.5, 9.0 us, at 2000 22, 28, at 30000 201, 122; 128 rows at 0 14.0, 9.9; 32 rows at 30000 109, 126.
+// Whether keys and values expanded once, for the kernel of prompts, are the faster way for heads of 128.  Microseconds of either:
+//   on codes   a wave of pieces of 16 rows over the SMs 7, and 0.15 for each of their blocks
+//   expanded   12, 2 per 1000 positions (a tile's steps) and 0.21 per 1000 positions and (batch row, key head): five bits read, 16 written and 16 read
+//              again an entry
+// Codes / expanded, by (batch row, key head)s in all, rows of each, and positions: 8, 64 rows: at 0 5.5 / 7.8, at 1000 11 / 16, at 16000 42 / 64;
+// 8, 256: 8.3 / 8.7, 16 / 21, 131 / 75; 64, 32: 7.6 / 8.1, 16 / 24, 133 / 230; 64, 128: 28 / 10, 58 / 31, 496 / 236; 256, 20: 24 / 9, 55 / 61, 492 / 867;
+// 256, 64: 47 / 11, 100 / 63, 975 / 876; 1024, 32: 105 / 28, 209 / 229, 1960 / 3740.  Of 810 such pairs (1 to 1024 of them, 17 to 256 rows, 0 to 16000
+// positions, 1 to 8 query heads a key head) 27 go a way that takes over a tenth longer, 31 % at most: those of 16 clusters, which the SMs have no room for at once.
 inline bool many_rows(const Attend &a, int sms) {
-  const long long cols = (long long)a.S * (a.n_heads / a.n_kv), pieces = (long long)a.B * a.n_kv * ((cols + 15) / 16);
+  const long long cols = (long long)a.S * (a.n_heads / a.n_kv), heads = (long long)a.B * a.n_kv, pieces = heads * ((cols + 15) / 16);
   const double keys = a.pos0 + 0.5 * a.S - a.first;
-  return a.hd == 128 && cols > 16 && (pieces > sms || 0.48 * pieces * (keys / BLOCK) / (4.0 * sms) > 20 + 3.5e-3 * keys);
+  const double codes = 7 * (double)((pieces + sms - 1) / sms) + 0.15 * (double)pieces / sms * keys / BLOCK;
+  return a.hd == 128 && cols > 16 && codes > 12 + (2 + 0.21 * (double)heads) * keys / 1000;
 }
 
 }  // namespace pc
