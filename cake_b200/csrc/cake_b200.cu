@@ -115,6 +115,8 @@ static int nccl_load() {
   } while (0)
 
 // ------------------------------------------------------------------------------------------ handles
+constexpr unsigned long long PC_POOL_KEEPS = 1ull << 30;   // bytes of closed caches in four bits that stay for the next ones; more goes back to the device
+
 struct cake_b200_ctx {
   int device = 0;
   cake_b200_config cfg{};
@@ -155,7 +157,7 @@ struct cake_b200_ctx {
   float *pc_ws = nullptr;
   KeptMemory pc_rows;   // rows of such caches in D, for the kernels of prompts
   unsigned *pc_tickets = nullptr;
-  cudaMemPool_t pc_pool = nullptr;   // the caches' memory: a closed cache's is the next one's (a new cache of 67 MB: 20 us, 3 ms from the driver)
+  cudaMemPool_t pc_pool = nullptr;   // the caches' memory: a closed cache's is the next one's (a new cache of 67 MB: 20 us, 3 ms from the driver), up to PC_POOL_KEEPS
   // The operators of such caches may run on a caller's stream: `stream` then is that one for the call.  pc_out: behind the last of them, waited for by
   // this ctx's stream (settle) or another caller's when it goes on; pc_in: the ctx's stream as it was, waited for by a caller's while pc_behind
   cudaEvent_t pc_in = nullptr, pc_out = nullptr;
@@ -985,7 +987,7 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
       props.location.type = cudaMemLocationTypeDevice;
       props.location.id = c->device;
       CU(cudaMemPoolCreate(&c->pc_pool, &props));
-      uint64_t keep = ~0ull;
+      uint64_t keep = PC_POOL_KEEPS;
       CU(cudaMemPoolSetAttribute(c->pc_pool, cudaMemPoolAttrReleaseThreshold, &keep));
     }
     for (cudaEvent_t *ev : {&c->pc_in, &c->pc_out})
@@ -1054,6 +1056,7 @@ extern "C" void cake_b200_cache_free(cake_b200_cache *k) {
     const bool pool = k->bits && g_live_ctx.count(k->ctx);
     for (void *p : k->k)
       if (p) (void)(pool ? cudaFreeAsync(p, k->ctx->stream) : cudaFree(p));
+    if (pool && cudaStreamSynchronize(k->ctx->stream) == cudaSuccess) (void)cudaMemPoolTrimTo(k->ctx->pc_pool, PC_POOL_KEEPS);
   }
   for (void *p : k->v)
     if (p) cudaFree(p);

@@ -394,6 +394,8 @@ int cake_b200_cache_fill_synthetic(cake_b200_cache *, const int *block_idx, int 
  * cake_b200_decode_build and the other calls on caches take such a cache like any other (every rank of a sharded decode then has one); attention reads
  * what the cache holds, the rows of the same call included, so that a prompt may be cut anywhere.  cake_b200_cache_read returns the entries' values
  * rounded to D.
+ * Up to 1 GiB of closed caches' memory stays with the ctx for the next ones; so does, at its largest so far, the memory that calls of many rows of 128-entry heads
+ * expand keys and values in (1 GiB at most unless one batch row needs more, and what captured calls have used).
  * The three calls below run on `stream`, the cudaStream_t that their tensors belong to (cudaStreamLegacy for the default stream; NULL: the ctx's own),
  * behind what the ctx's other calls have enqueued, which in turn go on behind them.  It may be capturing, once the same call has run outside a
  * capture (memory is made on first use; CAKE_B200_ESTATE otherwise).  A captured call takes its place in the graph alone: graphs captured from calls of one
