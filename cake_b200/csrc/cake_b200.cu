@@ -4445,7 +4445,6 @@ extern "C" int cake_b200_decode_begin(cake_b200_ctx *c, uint32_t first_token, in
     if (kc->len[l] != index_pos)
       return fail(CAKE_B200_ESTATE, "block %d: index_pos %d != cache length %d", l, index_pos, kc->len[l]);
   if (index_pos >= kc->cap) return fail(CAKE_B200_ESTATE, "cache full");
-  kc->moved = false;
   if (c->g_rank == 0 && first_token >= (uint32_t)c->cfg.vocab)  // candle's index_select fails on an out-of-range id (text_model.rs:271)
     return fail(CAKE_B200_EINVAL, "token id %u out of range (vocab %d)", first_token, c->cfg.vocab);
   set_int_kernel<<<1, 1, 0, c->stream>>>(kc->d_pos, index_pos);
@@ -4454,6 +4453,7 @@ extern "C" int cake_b200_decode_begin(cake_b200_ctx *c, uint32_t first_token, in
   c->launches += 3;
   c->steps_done = 0;
   CU(cudaGetLastError());
+  kc->moved = false;
   return CAKE_B200_OK;
 }
 
