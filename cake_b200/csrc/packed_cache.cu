@@ -384,15 +384,17 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 // A CTA serves up to 8 NT / PK query rows (row = token G + head of one key head) and a range of blocks; its warps take the blocks in turn, each through
 // a ring of its own (cp.async, 16 bytes a lane; a bulk copy and an mbarrier a block took a fifth of the loop), so that no warp waits for another
 // until the end.  Per block, with m16n8k16 products in fp16:
-//   S^T = K Q^T   A: 16 keys' codes, B: the rows' queries, kept in registers.  A group's sum is taken apart from the others', then
-//                 s += step sum + lo (sum of the group's q): the codes go in exactly, and no entry is formed.  Queries are scaled by a power of two
-//                 that puts a row's largest below 2^15: an entry down to 2^-29 of it keeps its bits.
-//   O^T += V^T P  A: 16 entries' codes, B: weights times steps in fp16 (11 bits), one operand per group; what is left of the value, lo + 8
-//                 step, is a number per key and group and is summed in fp32.  P^T turns into an operand by movmatrix.
-// Four bits become fp16 by one logic operation a pair: n under the exponent of 1024 is 1024 + n in the lowest four bits, 1024 + 16 n in the next.
-// The 16 stays in: K's queries are divided by it, V's sums at the end.  K's 1024 is what the accumulators start from (-1024 sum of q), a sum that
-// cancels to 2^-24 of 1024 sum |q|; from V's codes 1024 + 8 (1024 + 128) is subtracted, which also centres them: a weight's rounding counts for 8
-// steps at most.  (What binds the kernel is issue: 340 instructions a block and warp, 150 of them on the ALU at half rate.)
+//   S^T = K Q^T   A: 16 keys' codes less 8, B: the rows' queries, kept in registers.  A group's sum is taken apart from the others', then
+//                 s += step sum + (lo + 8 step) (sum of the group's q): the codes go in exactly, and no entry is formed.  Queries are scaled by a power of
+//                 two that puts a row's largest below 2^15: an entry down to 2^-29 of it keeps its bits, or 2^-25 where it meets an odd nibble.
+//   O^T += V^T P  A: 16 entries' codes less 8, B: weights times steps in fp16 (11 bits: what a call in f16 may be off by beside the result's own rounding,
+//                 0.000223 for 0.000201 of the norm over 31 positions, 0.000199 for 0.000197 over 1000), one operand per group; what is left of the value,
+//                 lo + 8 step, is a number per key and group and is summed in fp32.  P^T turns into an operand by movmatrix.
+// Four bits become fp16 by one logic operation a pair (Kim, Henry, Fahim and Hassan 2022): n under the exponent of 1024 is 1024 + n in the lowest four bits, 1024 + 16 n
+// in the next.  The 16 stays in: K's queries are divided by it, V's sums at the end.  1024 + 8 (1024 + 128) is subtracted, exactly: left in K's sums,
+// which then start from -1024 sum of q, it took their last ten bits; V's weights would count for all of 1024 + n, and so for 8 steps at most.  (K's
+// codes cost 16 of 340 instructions a block and warp: one token at 131072 39.8 -> 40.7 us; the registers of the sums that they started from are
+// free again, 32 sequences of 2 rows at 4000 51.0 -> 47.4.)
 // PK = 2, up to 4 rows: columns 0 .. 3 of an operand belong to a group and columns 4 .. 7 to its neighbour (the queries of the other are zero there),
 // so that no lane works for columns without a row; a row's two halves join by a shuffle.
 // A row's reference m moves when a score exceeds it by 2^6 (TAU).  Every group has a power of two `up` that keeps its steps at 512 at most, the first ones at
@@ -445,17 +447,17 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// nibbles i and 4 + i of w as a pair of fp16: 1024 + n for even i, 1024 + 16 n for odd i
-__device__ __forceinline__ void open_codes(uint32_t w, uint32_t (&r)[4]) {
-  const uint32_t v = w >> 8;
-  r[0] = and_or(w, 0x000f000fu, 0x64006400u);
-  r[1] = and_or(w, 0x00f000f0u, 0x64006400u);
-  r[2] = and_or(v, 0x000f000fu, 0x64006400u);
-  r[3] = and_or(v, 0x00f000f0u, 0x64006400u);
-}
 __device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t c) {   // pairs of fp16; exact here
   const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
+}
+// nibbles i and 4 + i of w as a pair of fp16: n - 8 for even i, 16 (n - 8) for odd i
+__device__ __forceinline__ void open_centred(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t v = w >> 8;
+  r[0] = add2(and_or(w, 0x000f000fu, 0x64006400u), 0xe408e408u);   // 1024 + n less 1024 + 8
+  r[1] = add2(and_or(w, 0x00f000f0u, 0x64006400u), 0xe480e480u);   // 1024 + 16 n less 1024 + 16 * 8
+  r[2] = add2(and_or(v, 0x000f000fu, 0x64006400u), 0xe408e408u);
+  r[3] = add2(and_or(v, 0x00f000f0u, 0x64006400u), 0xe480e480u);
 }
 __device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
   }
   // the rows' queries as operands: column g of n-tile nt, entries 32 j + 8 t .. (PK 2: column g & 3, group j's where g / 4 is j's half and else 0)
   uint32_t qf[NT][NG][4];
-  float qs[NT][MG][2], qn[NT][MG][2], sc[NT][2];   // a group's sums of q, and what the products start from; scale log2(e) and the power of two back
+  float qs[NT][MG][2], sc[NT][2];   // a group's sums of q; scale log2(e) and the power of two back
   int cpos[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     sc[nt][1] = __shfl_sync(0xffffffffu, down, 8 * tc + 4);
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-      float f[8], sum = 0.f, off = 0.f;
+      float f[8], sum = 0.f;
       unpack8<T>(raw[j], f);
 #pragma unroll
       for (int i = 0; i < 8; i++) sum += f[i] *= up;
@@ -550,21 +552,14 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
 #pragma unroll
       for (int h = 0; h < 4; h++) {
         const uint32_t x = pack2x<__half>(f[2 * h] * (h & 1 ? 0.0625f : 1.f), f[2 * h + 1] * (h & 1 ? 0.0625f : 1.f));
-        const float2 y = DT<__half>::unpack2(x);
-        off += y.x + y.y;
         qf[nt][j][h] = here ? x : 0u;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      off += __shfl_xor_sync(0xffffffffu, off, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      off += __shfl_xor_sync(0xffffffffu, off, 2);
 #pragma unroll
       for (int e2 = 0; e2 < 2; e2++) {
-        const float s2 = __shfl_sync(0xffffffffu, sum, 8 * tc + 4 * e2), o2 = -1024.f * __shfl_sync(0xffffffffu, off, 8 * tc + 4 * e2);
-        if (PK == 1 || (j & 1) == half) {
-          qs[nt][j / PK][e2] = s2;
-          qn[nt][j / PK][e2] = o2;
-        }
+        const float s2 = __shfl_sync(0xffffffffu, sum, 8 * tc + 4 * e2);
+        if (PK == 1 || (j & 1) == half) qs[nt][j / PK][e2] = s2;
       }
     }
 #pragma unroll
@@ -597,8 +592,8 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
         uint32_t x[2][4], y[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          open_codes(kw[0][2 * w + h], x[h]);
-          open_codes(kw[1][2 * w + h], y[h]);
+          open_centred(kw[0][2 * w + h], x[h]);
+          open_centred(kw[1][2 * w + h], y[h]);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -606,22 +601,23 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
           auto join = [&](int i, float(&d)[4]) {   // d: sums of the group that is the lane's i-th word of pairs
             const float2 p0 = open_pair<T>(kp[0][i]), p1 = open_pair<T>(kp[1][i]);
             const int jj = group_of(i);
-            s[nt][0] = fmaf(p0.x, d[0], fmaf(p0.y, qs[nt][jj][0], s[nt][0]));
-            s[nt][1] = fmaf(p0.x, d[1], fmaf(p0.y, qs[nt][jj][1], s[nt][1]));
-            s[nt][2] = fmaf(p1.x, d[2], fmaf(p1.y, qs[nt][jj][0], s[nt][2]));
-            s[nt][3] = fmaf(p1.x, d[3], fmaf(p1.y, qs[nt][jj][1], s[nt][3]));
+            const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y);
+            s[nt][0] = fmaf(p0.x, d[0], fmaf(m0, qs[nt][jj][0], s[nt][0]));
+            s[nt][1] = fmaf(p0.x, d[1], fmaf(m0, qs[nt][jj][1], s[nt][1]));
+            s[nt][2] = fmaf(p1.x, d[2], fmaf(m1, qs[nt][jj][0], s[nt][2]));
+            s[nt][3] = fmaf(p1.x, d[3], fmaf(m1, qs[nt][jj][1], s[nt][3]));
           };
           if constexpr (PK == 2) {   // 8 entries of either group a product
-            float d[4] = {qn[nt][w][0], qn[nt][w][1], qn[nt][w][0], qn[nt][w][1]};
+            float d[4] = {};
 #pragma unroll
             for (int h = 0; h < 4; h++) mma16(d, x[0][h], y[0][h], x[1][h], y[1][h], q0[h], q1[h]);
             join(w, d);
           } else {
-            float d[4] = {qn[nt][2 * w][0], qn[nt][2 * w][1], qn[nt][2 * w][0], qn[nt][2 * w][1]};
+            float d[4] = {};
             mma16(d, x[0][0], y[0][0], x[0][1], y[0][1], q0[0], q0[1]);
             mma16(d, x[0][2], y[0][2], x[0][3], y[0][3], q0[2], q0[3]);
             join(w, d);
-            float f[4] = {qn[nt][2 * w + 1][0], qn[nt][2 * w + 1][1], qn[nt][2 * w + 1][0], qn[nt][2 * w + 1][1]};
+            float f[4] = {};
             mma16(f, x[1][0], y[1][0], x[1][1], y[1][1], q1[0], q1[1]);
             mma16(f, x[1][2], y[1][2], x[1][3], y[1][3], q1[2], q1[3]);
             join(NG / 2 + w, f);
@@ -733,13 +729,8 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           uint32_t x[4], y[4];
-          open_codes(vw[2 * w + h], x);
-          open_codes(vw[NG + 2 * w + h], y);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            x[e] = add2(x[e], e & 1 ? 0xe480e480u : 0xe408e408u);   // -(1024 + 16 * 8), -(1024 + 8)
-            y[e] = add2(y[e], e & 1 ? 0xe480e480u : 0xe408e408u);
-          }
+          open_centred(vw[2 * w + h], x);
+          open_centred(vw[NG + 2 * w + h], y);
           float(&u)[4] = o[nt][2 * (2 * w + h)], (&v)[4] = o[nt][2 * (2 * w + h) + 1];
           mma16(u, x[0], x[1], y[0], y[1], b0[h], b1[h]);
           mma16(v, x[2], x[3], y[2], y[3], b0[h], b1[h]);

@@ -128,3 +128,29 @@ def test_a_row_of_many_and_the_row_alone(dtype):
         wide = 1.01 * h * ref.abs() + mass * (torch.expm1(2 * mag * (h + 2.0 ** -18)) + 1.01 * h + 2.0 ** -14) + 2.0 ** -25
         assert ((many[:, t:t + 1] - ref).abs() <= wide).all(), t
     ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,hd,s", [(32, 8, 128, 1), (64, 8, 64, 1), (8, 4, 256, 1), (32, 4, 128, 1), (4, 4, 128, 3), (8, 8, 64, 12)])
+def test_scores_whose_sums_cancel(heads, kv, hd, s, dtype):
+    """Keys of one size and both signs against queries whose neighbours are alike: the codes' sums come to little, the scores to the steps' roundings.  Values of one number
+    per group, so that nothing but scores and the result is rounded.  With S = scale times the sum of step |q|, a group's sum has four products behind one another
+    and two additions, each off by 2^-24 of 8 times its share of S at most (n - 8 and 8 steps), rms 1 / sqrt 3 of that, half of it on the way: sqrt 6 / 2 / sqrt 3 * 8 * 2^-24
+    S / sqrt groups < 1.5 * 2^-21 S / sqrt groups, and half of that where one of few keys' weights p moves by p (1 - p) <= 1 / 4 of it, to either side of |v|."""
+    ctx = ctx_for(heads, kv, hd, dtype)
+    D, b, n, groups = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype], 8, 2 + s, hd // 32
+    g = torch.Generator().manual_seed(hd + s)
+    size = 500 + 1000 * torch.rand((b, n, kv, 1), generator=g)
+    k = (size * (1 - 2 * (torch.arange(hd) % 2))).to(D).cuda()
+    q = torch.randn((b, s, heads, hd // 2, 1), generator=g).expand(-1, -1, -1, -1, 2).flatten(-2).to(D).cuda()
+    v = torch.randn((b, n, kv, groups, 1), generator=g).expand(-1, -1, -1, -1, 32).flatten(-2).to(D).cuda()
+    cache = Cache(ctx, b, n, bits=4)
+    cache.write(0, k, v, 0)
+    ref, _ = few_rows(q, k, v, n - s, 0, dtype)
+    S = hd ** -0.5 * q.double().abs().sum(-1, keepdim=True).cpu() * (2 * float(size.max()) / 15 * (1 + 2 * HALF[dtype]))
+    rms = lambda t: float(t.square().mean().sqrt())
+    own = rms(ref.to(D).double() - ref)
+    err = rms(cache.attend(0, q, n - s).double().cpu() - ref)
+    assert err ** 2 <= 1.2 * own ** 2 + rms(float(v.abs().max()) * 0.75 * 2.0 ** -21 * S / groups ** 0.5) ** 2, (err, own)
+    ctx.close()
