@@ -91,10 +91,10 @@ int attend(cudaStream_t, int dtype, const Attend &, const Scratch &, uint64_t *l
 //   on codes   a wave of pieces of 16 rows over the SMs 7, and 0.15 for each of their blocks
 //   expanded   12, 2 per 1000 positions (a tile's steps) and 0.21 per 1000 positions and (batch row, key head): five bits read, 16 written and 16 read
 //              again an entry
-// Codes / expanded, by (batch row, key head)s in all, rows of each, and positions: 8, 64 rows: at 0 5.5 / 7.8, at 1000 11 / 16, at 16000 42 / 64;
-// 8, 256: 8.3 / 8.7, 16 / 21, 131 / 75; 64, 32: 7.6 / 8.1, 16 / 24, 133 / 230; 64, 128: 28 / 10, 58 / 31, 496 / 236; 256, 20: 24 / 9, 55 / 61, 492 / 867;
-// 256, 64: 47 / 11, 100 / 63, 975 / 876; 1024, 32: 105 / 28, 209 / 229, 1960 / 3740.  Of 810 such pairs (1 to 1024 of them, 17 to 256 rows, 0 to 16000
-// positions, 1 to 8 query heads a key head) 27 go a way that takes over a tenth longer, 31 % at most: those of 16 clusters, which the SMs have no room for at once.
+// Codes / expanded, by (batch row, key head)s in all, rows of each, and positions: 8, 64 rows: at 0 5.2 / 7.7, at 1000 10 / 16, at 16000 40 / 65;
+// 8, 256: 7.6 / 8.7, 15 / 21, 122 / 75; 64, 32: 7.1 / 8.0, 15 / 24, 123 / 230; 64, 128: 26 / 10, 54 / 31, 460 / 236; 256, 20: 23 / 9, 51 / 61, 456 / 849;
+// 256, 64: 45 / 11, 94 / 63, 901 / 861; 1024, 32: 94 / 26, 201 / 229, 1790 / 3600.  Of 810 such pairs (1 to 1024 of them, 17 to 256 rows, 0 to 16000
+// positions, 1 to 8 query heads a key head) 19 go a way that takes over a tenth longer, 25 % at most: those of 16 clusters, which the SMs have no room for at once.
 inline bool many_rows(const Attend &a, int sms) {
   const long long cols = (long long)a.S * (a.n_heads / a.n_kv), heads = (long long)a.B * a.n_kv, pieces = heads * ((cols + 15) / 16);
   const double keys = a.pos0 + 0.5 * a.S - a.first;

@@ -3,8 +3,8 @@ import pytest
 import torch
 
 from cake_b200.capi import CakeB200Error, check, lib
-from cake_b200.model import Context, TextModelBase
-from tests.test_packed_cache import EINVAL, ESTATE, rows
+from cake_b200.model import Cache, Context, TextModelBase
+from tests.test_packed_cache import EINVAL, ESTATE, check_attention, ctx_for, filled, queries, rows
 from tests.util import checkpoint, medium_config
 
 
@@ -29,4 +29,62 @@ def test_a_refused_begin_leaves_the_graph_refused():
         assert e.value.code == ESTATE
     m.index_pos = 9
     assert len(m.decode_greedy(5, 2)) == 2 and ctx.cache.len(0) == 11
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,s", [(8, 2, 128, 1), (8, 2, 64, 6), (4, 2, 256, 3), (32, 8, 128, 150)])
+def test_values_of_any_size_of_bf16(heads, kv, hd, s):
+    """Powers of two on V alone change nothing but the result's exponent."""
+    ctx = ctx_for(heads, kv, hd, "bf16")
+    n = s + 50
+    k, v, q = rows(1, n, kv, hd, "bf16", 1), rows(1, n, kv, hd, "bf16", 2), queries(1, s, heads, hd, "bf16", 3)
+    cache, want = Cache(ctx, 1, n, bits=4), None
+    for e in (0, -100, 60, 114):
+        cache.write(0, k, v * 2.0 ** e, 0)
+        got = cache.attend(0, q, n - s) * 2.0 ** -e
+        if want is None:
+            want = got
+            check_attention(got, q, k, v, n - s, 0, "bf16")
+        assert torch.equal(got, want), e
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s", [1, 5, 200])
+def test_queries_of_any_stride(s):
+    """Tokens and batch rows on any multiple of 8 entries, one over another, and one for all."""
+    ctx = ctx_for(32, 8, 128, "bf16")
+    cache, k, v = filled(ctx, 2, 400, 3, "bf16")
+    row = 32 * 128
+    buf = queries(1, 2 * s + 2, 40, 128, "bf16", 4).reshape(-1)
+    for tok, batch in ((row + 8, (row + 8) * s + 16), (row, row * s + 8), (row, 0), (0, row), (8, 24), (1032, 8)):
+        q = buf.as_strided((2, s, 32, 128), (batch, tok, 128, 1))
+        check_attention(cache.attend(0, q, 400 - s), q.clone(), k, v, 400 - s, 0, "bf16")
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_the_context_in_turn():
+    """Writes on one stream, attention on another, blocks on the context's own, without a wait of the host between them."""
+    ctx = ctx_for(32, 8, 128, "f16")
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    cache, k, v = filled(ctx, 1, 900, 3, "f16")
+    q = queries(1, 300, 32, 128, "f16", 4)
+    torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(a):
+            for _ in range(3):
+                cache.write(0, k, v if i % 2 else -v, 0)
+        with torch.cuda.stream(b):
+            got.append((cache.attend(0, q, 600), cache.attend(0, q[:, 299:], 899)))
+        with torch.cuda.stream(ctx.torch_stream):
+            got[-1] += (cache.attend(0, q, 600),)
+    torch.cuda.synchronize()
+    for i, (many, one, again) in enumerate(got):
+        assert torch.equal(many, again) and torch.equal(many, got[i % 2][0]) and torch.equal(one, got[i % 2][1])
+    check_attention(got[1][0], q, k, v, 600, 0, "f16")
+    check_attention(got[1][1], q[:, 299:], k, v, 899, 0, "f16")
+    check_attention(got[0][0], q, k, -v, 600, 0, "f16")
     ctx.close()

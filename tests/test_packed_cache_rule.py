@@ -5,13 +5,13 @@ import subprocess
 from tests.test_packed_cache import ROOT
 
 # query heads a key head, key heads, batch rows, rows a call, position, device microseconds on codes and expanded
-MEASURED = [(4, 8, 1, 5, 0, 4.5, 7.2), (4, 8, 1, 16, 16000, 42.4, 64.3), (4, 8, 1, 64, 16000, 131.2, 74.9), (4, 8, 1, 64, 4000, 40.7, 34.2),
-            (8, 1, 1, 16, 4000, 13.3, 21.5), (8, 1, 8, 32, 16000, 130.9, 75.8), (4, 32, 1, 5, 16000, 73.8, 152.9), (4, 32, 1, 64, 1000, 58.5, 30.4),
-            (4, 8, 8, 5, 4000, 40.2, 65.9), (8, 8, 8, 3, 16000, 132.3, 229.6), (4, 8, 8, 32, 4000, 150.0, 72.1), (4, 8, 8, 32, 0, 27.5, 10.1),
-            (4, 8, 32, 5, 4000, 149.2, 217.2), (4, 8, 32, 5, 16000, 492.5, 861.9), (4, 8, 32, 5, 0, 25.4, 9.6), (4, 8, 32, 16, 4000, 283.2, 218.7),
-            (1, 8, 32, 17, 16000, 494.3, 869.8), (4, 32, 32, 5, 16000, 1922.6, 3662.0), (4, 32, 32, 8, 250, 118.6, 78.9), (4, 32, 32, 16, 1000, 410.2, 234.0),
-            (4, 32, 32, 64, 16000, 15407.8, 5578.6), (4, 8, 1, 16, 2000, 13.1, 16.4), (4, 8, 32, 64, 1000, 420.8, 92.6), (8, 32, 8, 16, 2000, 320.0, 119.5),
-            (4, 1, 1, 32, 4000, 13.1, 21.6)]
+MEASURED = [(4, 8, 1, 5, 0, 4.1, 7.2), (4, 8, 1, 16, 16000, 39.7, 64.3), (4, 8, 1, 64, 16000, 121.8, 75.7), (4, 8, 1, 64, 4000, 37.8, 34.4),
+            (8, 1, 1, 16, 4000, 12.3, 21.6), (8, 1, 8, 32, 16000, 121.6, 76.3), (4, 32, 1, 5, 16000, 69.2, 155.4), (4, 32, 1, 64, 1000, 55.2, 30.4),
+            (4, 8, 8, 5, 4000, 37.6, 66.4), (8, 8, 8, 3, 16000, 122.3, 230.3), (4, 8, 8, 32, 4000, 139.6, 72.4), (4, 8, 8, 32, 0, 25.9, 10.0),
+            (4, 8, 32, 5, 4000, 139.0, 217.2), (4, 8, 32, 5, 16000, 455.8, 849.1), (4, 8, 32, 5, 0, 22.8, 9.1), (4, 8, 32, 16, 4000, 259.5, 218.2),
+            (1, 8, 32, 17, 16000, 456.5, 856.2), (4, 32, 32, 5, 16000, 1780.5, 3577.6), (4, 32, 32, 8, 250, 113.0, 80.0), (4, 32, 32, 16, 1000, 394.0, 235.3),
+            (4, 32, 32, 64, 16000, 14236.0, 5374.5), (4, 8, 1, 16, 2000, 12.5, 16.5), (4, 8, 32, 64, 1000, 392.4, 92.2), (8, 32, 8, 16, 2000, 300.1, 119.5),
+            (4, 1, 1, 32, 4000, 12.3, 21.6)]
 
 
 def test_the_faster_way_is_taken(tmp_path):
