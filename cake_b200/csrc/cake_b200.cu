@@ -1211,13 +1211,14 @@ constexpr size_t PC_EXPAND_MOST = (size_t)1 << 30;
 static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, const void *q, size_t q_tok, size_t q_batch, void *out, int S, int pos0,
                          int first, float scale, const int *d_pos = nullptr, int window = 0) {
   const cake_b200_config &f = c->cfg;
-  pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, kc->batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
+  const int batch = d_pos ? 1 : kc->batch;   // (the decode chain's rows are the first batch row's)
+  pc::Attend a{kc->k[l], q, (long long)q_tok, (long long)q_batch, out, batch, S, f.n_heads, f.n_kv_heads, f.head_dim, pc::cap_blocks(kc->cap), pos0, first};
   a.scale = scale; a.d_pos = d_pos; a.window = window;
-  const bool strides = q_tok > 0 && (q_batch > 0 || kc->batch == 1);   // (a tensor map has none of zero)
+  const bool strides = q_tok > 0 && (q_batch > 0 || batch == 1);   // (a tensor map has none of zero)
   if (!d_pos && first <= pos0 && strides && pc::many_rows(a, c->sm_count)) {
     const int hd = f.head_dim, n = pos0 + S - first, cap = round_up(n, 64), blocks = pc::read_blocks(first, n);
     const size_t slab = (size_t)f.n_kv_heads * cap * hd * c->es, marks = (size_t)f.n_kv_heads * blocks * 8;   // of a batch row
-    const int group = (int)std::max<size_t>(1, std::min<size_t>(kc->batch, PC_EXPAND_MOST / (2 * slab)));
+    const int group = (int)std::max<size_t>(1, std::min<size_t>(batch, PC_EXPAND_MOST / (2 * slab)));
     const size_t need = group * (2 * slab + marks);
     cudaStreamCaptureStatus st;
     CU(cudaStreamIsCapturing(c->stream, &st));
@@ -1233,8 +1234,8 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
       }, [](void *p) { cudaFree(p); });
       CU(e);
     }
-    for (int b0 = 0; b0 < kc->batch; b0 += group) {
-      const int nb = std::min(group, kc->batch - b0);
+    for (int b0 = 0; b0 < batch; b0 += group) {
+      const int nb = std::min(group, batch - b0);
       char *kr = (char *)c->pc_rows.now, *vr = kr + group * slab;
       unsigned long long *nan = (unsigned long long *)(vr + group * slab);
       const char *from = (const char *)kc->k[l] + (size_t)b0 * f.n_kv_heads * a.blocks * pc::block_bytes(hd);
@@ -1242,7 +1243,7 @@ static int attend_packed(cake_b200_ctx *c, const cake_b200_cache *kc, int l, con
       CU((cudaError_t)pc::read(c->stream, f.dtype, r, launch_counter(c)));
       RC(DISPATCH_T(f.dtype, T_LAMBDA {
         typedef typename decltype(tag_)::type T;
-        return prompt_attention<T>(c, (const T *)q + (size_t)b0 * q_batch, q_tok, kc->batch == 1 ? (size_t)S * q_tok : q_batch, kr, vr, cap,
+        return prompt_attention<T>(c, (const T *)q + (size_t)b0 * q_batch, q_tok, batch == 1 ? (size_t)S * q_tok : q_batch, kr, vr, cap,
                                    (T *)out + (size_t)b0 * S * f.n_heads * hd, nb, S, pos0 - first, scale, NanMarks{nan, blocks, first & 15});
       }));
     }
@@ -1275,7 +1276,7 @@ static int write_packed(cake_b200_ctx *c, const cake_b200_block *b, const cake_b
               c->nqkv, (long long)S * c->nqkv};
   a.q = qkv; a.q_norm = qn; a.k_norm = kn; a.n_q = f.n_heads; a.rot = c->rot; a.eps = f.rms_eps; a.d_pos = d_pos;
   if (b->use_rope && c->rot > 0) { a.cos_t = c->cos_t; a.sin_t = c->sin_t; }
-  a.B = kc->batch; a.S = S; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(kc->cap); a.pos0 = pos0;
+  a.B = d_pos ? 1 : kc->batch; a.S = S; a.n_kv = f.n_kv_heads; a.hd = f.head_dim; a.blocks = pc::cap_blocks(kc->cap); a.pos0 = pos0;
   CU((cudaError_t)pc::write(c->stream, f.dtype, a, launch_counter(c)));
   return CAKE_B200_OK;
 }

@@ -1,4 +1,6 @@
 """Caches in four bits: calls one after another that no other test makes."""
+from ctypes import byref, c_float, c_int, c_void_p
+
 import pytest
 import torch
 
@@ -87,4 +89,23 @@ def test_calls_on_two_streams_and_the_context_in_turn():
     check_attention(got[1][0], q, k, v, 600, 0, "f16")
     check_attention(got[1][1], q[:, 299:], k, v, 899, 0, "f16")
     check_attention(got[0][0], q, k, -v, 600, 0, "f16")
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_the_attention_kernel_timed_over_a_batch():
+    """cake_b200_bench_kernel times one token's attention: it has one row, whatever the cache's batch, and that row is the first batch row's."""
+    cfg = medium_config(num_hidden_layers=2)
+    ctx = Context(cfg, checkpoint(cfg, "bf16", std=0.05), "bf16", cache_bits=4)
+    m = TextModelBase.load(ctx)
+    cache = Cache(ctx, 3, 100)
+    cache.fill_synthetic([0, 1], 50)
+    before = [cache.read(l, w).clone() for l in (0, 1) for w in (0, 1)]
+    n, ms = len(m.blocks), c_float()
+    hs, ix = (c_void_p * n)(*[b.h for b in m.blocks]), (c_int * n)(*range(n))
+    check(lib().cake_b200_bench_kernel(ctx.h, hs, ix, n, cache.h, 4, 3, byref(ms)))
+    assert 0 < ms.value < 10 and cache.len(0) == 50
+    after = [cache.read(l, w) for l in (0, 1) for w in (0, 1)]
+    for a, b in zip(after, before):
+        assert torch.equal(a[1:], b[1:]) and torch.equal(a[0, :, :49], b[0, :, :49])
     ctx.close()
