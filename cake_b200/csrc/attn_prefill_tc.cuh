@@ -153,7 +153,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int S = p.S, pos0 = p.pos0, G = p.G, tpt = p.tpt, lg = SPLIT ? p.splits_log2 : 0, splits = 1 << lg;
   const int rank = (int)blockIdx.x & (splits - 1);                        // the cluster's CTAs are neighbours along x
   // heavy (late) query tiles first, those of every key head before the next: CTAs start in the order of x, y, z
-  // (one head behind the other, the SMs are without work for a sixth of a prompt of 4096, 32 / 8 heads: 157 us for 138)
+  // (one head behind the other, the SMs are without work for an eighth of a prompt of 4096, 32 / 8 heads: 188 us for 165)
   const int nth = (int)blockIdx.y * (int)(gridDim.x >> lg) + (int)(blockIdx.x >> lg);
   const int mt = (int)(gridDim.x >> lg) - 1 - nth / (int)gridDim.y, kvh = nth % (int)gridDim.y, b = blockIdx.z, t0 = mt * tpt;
   const int kv_end = pos0 + min(S, t0 + tpt);  // keys visible to the last query of this tile

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(128) write_kernel(const Write a) {
 // together), V's likewise (8 lanes write 64 bytes of a row).  A value is one fma in pairs of D on exact codes: one rounding; as step is rounded up, the
 // highest codes of a group that reaches D's end may lie beyond it: they become D's largest number (an infinity would be one that nobody wrote, and NaN for
 // every row whose weight for it is zero).
-// 32768 positions of 8 heads of 128, K and V: 71 us with 2-byte reads of V and 64-bit divisions a lane; so 30 (5.85 TB/s).
+// 32768 positions of 8 heads of 128, K and V: 71 us with 2-byte reads of V and 64-bit divisions a lane; so 30 (5.8 TB/s).
 // As operands of matrix products (a.nan): a group that reads as NaN becomes zero, so that it counts for no row that does not see it, and the
 // block's word says where: byte 0 the first position (in the block) whose K has such a group, byte 1 + j that of V's group j, 255 none.
 template <typename T> struct Codes;   // n as pairs of D, nibbles i and 4 + i of w
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 // Four bits become fp16 by one logic operation a pair (Kim, Henry, Fahim and Hassan 2022): n under the exponent of 1024 is 1024 + n in the lowest four bits, 1024 + 16 n
 // in the next.  The 16 stays in: K's queries are divided by it, V's sums at the end.  1024 + 8 (1024 + 128) is subtracted, exactly: left in K's sums,
 // which then start from -1024 sum of q, it took their last ten bits; V's weights would count for all of 1024 + n, and so for 8 steps at most.  (K's
-// codes cost 16 of 340 instructions a block and warp: one token at 131072 39.8 -> 40.7 us; the registers of the sums that they started from are
+// codes cost 32 of 376 instructions a block and warp: one token at 131072 39.8 -> 40.7 us; the registers of the sums that they started from are
 // free again, 32 sequences of 2 rows at 4000 51.0 -> 47.4.)
 // PK = 2, up to 4 rows: columns 0 .. 3 of an operand belong to a group and columns 4 .. 7 to its neighbour (the queries of the other are zero there),
 // so that no lane works for columns without a row; a row's two halves join by a shuffle.
@@ -993,9 +993,9 @@ template <typename T, int HD, int NT, int PK> static int attend_split(cudaStream
   // few clusters: so much shared memory that their CTAs come to lie on an SM each (16384 positions 20.2 -> 16.8 us); of more, two come to lie on one
   const bool apart = 2 * units * cluster <= x.sms;
   // Microseconds of either way behind what both cost: a block takes a quarter of an SM 0.3 (hd 128, 8 columns), a CTA alone twice as long a warp; parts
-  // in the line cost 6, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 7.4,
-  // 9.9 us, at 12000 12.2, 12.2, at 32768 24.2, 16.9; batch 2 at 8192 14.1, 15.6, at 12000 18.0, 17.4, at 16384 22.2, 19.1; batch 4 at 16384 24.2, 26.6;
-  // batch 16 at 8192 40.1, 43.0)
+  // in the line cost 6, or 5 where no CTA has parts of two units (one token, 32 / 8 heads, 128 entries, cluster and line: batch 1 at 4096 positions 7.2,
+  // 9.4 us, at 12000 12.6, 11.8, at 32768 26.0, 16.6; batch 2 at 8192 14.2, 15.2, at 12000 18.3, 17.0, at 16384 22.7, 19.0; batch 4 at 16384 25.0, 26.6;
+  // batch 16 at 8192 40.9, 43.4)
   const double each = 0.3 * std::max(1.0, HD * NT / 128.0);
   const double ctas = apart ? 1. : std::max((double)sp_per_sm(HD, NT), (double)((units * cluster + x.sms - 1) / x.sms));
   const bool line = (long long)a.n_kv * p.col_blocks > 65535 || a.B > 65535 ||

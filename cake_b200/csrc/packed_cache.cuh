@@ -4,8 +4,9 @@
 // Format.  A row of hd entries (K: after norm and rotation) is cut into hd / 32 groups of neighbours.  With lo = min x (a D number) and step the
 // smallest D number that is not below (max x - lo) / 15 (D = bf16: and not below 2^-126 where the span is not 0), entry x is held as
 // n = floor((x - lo) / step + 1/2), 0 <= n <= 15, and stands for lo + step n.  A pair (step, lo) in D and 32 codes are 20 bytes for 32 entries.
-// step is rounded up so that 15 steps reach the maximum; lo and step are D numbers, so that n step and the codes' distances to their borders are
-// exact in fp32.  A group whose span is not finite (an infinity, a NaN) has the pair (NaN, NaN): all of it reads as NaN.  What lies beyond D's
+// step is rounded up so that 15 steps reach the maximum; lo and step are D numbers, so that n step is exact in fp32.  Span and distances are formed in
+// fp32 and exact there unless the exponents lie so far apart that 24 bits do not hold a difference of two D numbers: step can then be its neighbour (f16,
+// lo = -2^-24, max = 15360: 1024 for 1025).  A group whose span is not finite (an infinity, a NaN) has the pair (NaN, NaN): all of it reads as NaN.  What lies beyond D's
 // largest number, as 15 steps may, is rounded to it.
 //
 // Place.  16 positions of one (batch row, key head) are one block of 20 hd bytes: K's codes, K's pairs, V's codes, V's pairs; the blocks of a

@@ -388,7 +388,7 @@ int cake_b200_cache_fill_synthetic(cake_b200_cache *, const int *block_idx, int 
 /* ---- caches in four bits ----------------------------------------------------------------------
  * A cache whose K and V rows (after norm and rotation) are held in 4 bits an entry and a pair of D numbers for every 32 neighbouring entries of a row: 5 bits an entry
  * instead of 16.  For a group of 32 entries x:  lo = min x;  step = the smallest D number that is not below (max x - lo) / 15 (bf16: nor below
- * 2^-126 where max x != lo);  n = floor((x - lo) / step + 1/2), 0 <= n <= 15;  the entry stands for lo + step n.  A group whose max x - lo is no
+ * 2^-126 where max x != lo);  n = floor((x - lo) / step + 1/2), 0 <= n <= 15 (differences formed in fp32);  the entry stands for lo + step n.  A group whose max x - lo is no
  * finite number reads as NaN; a value that lies beyond D's largest number (step is rounded up) is rounded to that number.
  * Llama-family blocks with head_dim 64, 128 or 256 and rotated parts of a multiple of 16 entries; bits = 4.  cake_b200_forward_batch,
  * cake_b200_decode_build and the other calls on caches take such a cache like any other (every rank of a sharded decode then has one); attention reads
