@@ -387,9 +387,10 @@ __global__ void __launch_bounds__(128) read_kernel(const Read a) {
 //   S^T = K Q^T   A: 16 keys' codes less 8, B: the rows' queries, kept in registers.  A group's sum is taken apart from the others', then
 //                 s += step sum + (lo + 8 step) (sum of the group's q): the codes go in exactly, and no entry is formed.  Queries are scaled by a power of
 //                 two that puts a row's largest below 2^15: an entry down to 2^-29 of it keeps its bits, or 2^-25 where it meets an odd nibble.
-//   O^T += V^T P  A: 16 entries' codes less 8, B: weights times steps in fp16 (11 bits: what a call in f16 may be off by beside the result's own rounding,
-//                 0.000223 for 0.000201 of the norm over 31 positions, 0.000199 for 0.000197 over 1000), one operand per group; what is left of the value,
-//                 lo + 8 step, is a number per key and group and is summed in fp32.  P^T turns into an operand by movmatrix.
+//   O^T += V^T P  A: 16 entries' codes less 8, B: weights times steps in fp16, an operand per group; what is left of the value, lo + 8 step, is a number
+//                 per key and group and is summed in fp32.  P^T turns into an operand by movmatrix.  One operand has 11 bits, three more than a result in
+//                 bf16; in f16 a second one takes what rounding the first one left (with one, 31 positions: 0.000223 of the norm from 64 bits, rounding
+//                 the result alone is 0.000200; 32 sequences at 4000 positions 39.7 -> 44.4 us).
 // Four bits become fp16 by one logic operation a pair (Kim, Henry, Fahim and Hassan 2022): n under the exponent of 1024 is 1024 + n in the lowest four bits, 1024 + 16 n
 // in the next.  The 16 stays in: K's queries are divided by it, V's sums at the end.  1024 + 8 (1024 + 128) is subtracted, exactly: left in K's sums,
 // which then start from -1024 sum of q, it took their last ten bits; V's weights would count for all of 1024 + n, and so for 8 steps at most.  (K's
@@ -467,6 +468,7 @@ template <typename T, int HD, int NT, int PK>
 __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split_kernel(const Split p) {
   // a lane's groups: all (PK 1), or those of its half of the columns (PK 2); its heads: columns 2 t and 2 t + 1, of the half
   constexpr int WARPS = SP_WARPS, NG = HD / 32, MG = NG / PK, COLS = 8 * NT / PK, OUT_LD = HD + 4;
+  constexpr bool TWO = std::is_same<T, __half>::value;   // operands of a weight times a step
   const Attend &a = p.a;
   extern __shared__ __align__(128) unsigned char sp_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -708,19 +710,29 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
     for (int w = 0; w < NG / 2; w++)
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        uint32_t b0[2], b1[2];
+        uint32_t b0[2], b1[2], r0[2], r1[2];   // weights times steps, and what rounding them left
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           if (PK == 2 && h) {
             b0[1] = b0[0];
             b1[1] = b1[0];
+            r0[1] = r0[0];
+            r1[1] = r1[0];
             continue;
           }
           const int i = PK == 2 ? w : h * (NG / 2) + w, jj = group_of(i);   // the pair's word; its sums' place
           const float2 p0 = open_pair<T>(vp[0][i]), p1 = open_pair<T>(vp[1][i]);
           const float m0 = fmaf(8.f, p0.x, p0.y), m1 = fmaf(8.f, p1.x, p1.y), x0 = p0.x * up[i], x1 = p1.x * up[i];
-          b0[h] = turn8x8(pack2x<__half>(times(nt, 0, x0), times(nt, 1, x0)));
-          b1[h] = turn8x8(pack2x<__half>(times(nt, 2, x1), times(nt, 3, x1)));
+          auto operand = [&](float v0, float v1, uint32_t &b, uint32_t &r) {
+            b = pack2x<__half>(v0, v1);
+            if (TWO) {
+              const float2 y = DT<__half>::unpack2(b);
+              r = turn8x8(pack2x<__half>(v0 - y.x, v1 - y.y));
+            }
+            b = turn8x8(b);
+          };
+          operand(times(nt, 0, x0), times(nt, 1, x0), b0[h], r0[h]);
+          operand(times(nt, 2, x1), times(nt, 3, x1), b1[h], r1[h]);
           mid[nt][jj][0] += times(nt, 0, m0);
           mid[nt][jj][0] += times(nt, 2, m1);
           mid[nt][jj][1] += times(nt, 1, m0);
@@ -734,6 +746,10 @@ __global__ void __launch_bounds__(SP_WARPS * 32, sp_per_sm(HD, NT)) attend_split
           float(&u)[4] = o[nt][2 * (2 * w + h)], (&v)[4] = o[nt][2 * (2 * w + h) + 1];
           mma16(u, x[0], x[1], y[0], y[1], b0[h], b1[h]);
           mma16(v, x[2], x[3], y[2], y[3], b0[h], b1[h]);
+          if (TWO) {
+            mma16(u, x[0], x[1], y[0], y[1], r0[h], r1[h]);
+            mma16(v, x[2], x[3], y[2], y[3], r0[h], r1[h]);
+          }
         }
       }
   };

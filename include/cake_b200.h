@@ -412,7 +412,7 @@ int cake_b200_cache_write(cake_b200_cache *, int block_idx, const void *k_dev, s
 int cake_b200_cache_unpack(cake_b200_cache *, int block_idx, int which, int first, int n, void *out_dev, void *stream);
 /* Attention of the rows q (batch, seq, n_heads, head_dim) in D at positions index_pos .., which the cache holds: row t sees the positions first <= j <=
  * index_pos + t;  out = softmax(scale q . k_j) weighted sum of v_j, with sums, maxima and weights in fp32 and one rounding to D; a row that sees no
- * position is zero.  What is rounded before: a call of a few rows takes the codes themselves and rounds a weight times a group's step to fp16 (11 bits); one of many
+ * position is zero.  What is rounded before: a call of a few rows takes the codes themselves and rounds a weight times a group's step to fp16 (bf16: 11 bits; f16: two operands, 22 bits); one of many
  * rows of 128-entry heads rounds the entries to D as cache_read does and keeps a weight to two operands in D (16 bits and more).  A row may come out one
  * way or the other as the number of rows beside it has it.
  * q_tok, q_batch: strides as above; out (batch, seq, n_heads, head_dim) contiguous; scale 0: head_dim^-1/2. */

@@ -34,10 +34,10 @@ def test_many_rows_round_entries_and_the_result_only(b, s, at, first, dtype):
 
 def few_rows(q, kx, vx, at, first, dtype):
     """In 64 bits: the attention of q [b, s, heads, hd] over what rows kx, vx [b, n, kv, hd] stand for, and how far a call on codes may be from it.  With u = step |n - 8|
-    of an entry, a row of `keys` keys rounds: the result, h; a weight times a step to fp16, 2^-11 of p u, or, where it has fp16's last bits, 2^-25 of
-    the power of two that puts the largest step of the group which the row sees at 8 or more: 2^-25 / 8 of that step, times 8; the sums of u and of lo + 8 step, 230 * 2^-24
-    of V, the largest entry of the group that the row sees; scores: four products behind one another of at most 1040 steps times the sum of |q|, 2^-22
-    each, and 2^-20 of mag for the rest; a weight changes by e^(2 ds)."""
+    of an entry, a row of `keys` keys rounds: the result, h; a weight times a step to one operand of fp16 (bf16: 2^-11 of p u) or to two (f16: 2^-22), or, where it has
+    fp16's last bits, 2^-25 of the power of two that puts the largest step of the group which the row sees at 8 or more: 2^-25 / 8 of that step, times 8;
+    the sums of u and of lo + 8 step, 230 * 2^-24 of V, the largest entry of the group that the row sees; scores: four products behind one another of at
+    most 8 steps times the sum of |q|, 2^-22 each, eight additions of them of 2^-24 each, and 2^-20 of mag for lo + 8 step and the exponent; a weight changes by e^(2 ds)."""
     b, s, heads, hd = q.shape
     n, G, scale, h = kx.shape[1], heads // kx.shape[2], hd ** -0.5, HALF[dtype]
 
@@ -56,13 +56,13 @@ def few_rows(q, kx, vx, at, first, dtype):
     j, i = torch.arange(n)[None], torch.arange(at, at + s)[:, None]
     seen = (j >= first) & (j <= i)
     p = torch.softmax(torch.where(seen, q @ k.transpose(2, 3) * scale, -torch.inf), -1)
-    ds = scale * 2.0 ** -10 * q.abs() @ ks.transpose(2, 3) + scale * 2.0 ** -20 * q.abs() @ k.abs().transpose(2, 3)
+    ds = scale * (4 * 2.0 ** -22 * 8 + 8 * 2.0 ** -24 * 8) * q.abs() @ ks.transpose(2, 3) + scale * 2.0 ** -20 * q.abs() @ k.abs().transpose(2, 3)
     ds = torch.where(seen, ds, 0.0).amax(-1, keepdim=True)
     group = lambda t: t.unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(*t.shape[:-1], t.shape[-1] // 32, 32).flatten(-2)
     most = lambda t: torch.stack([group(t[:, :, first:at + r + 1].amax(2)) for r in range(s)], 2)   # of what row r sees
     keys = (i + 1 - first).double()
     ref, mass = p @ v, p @ v.abs()
-    bound = 1.01 * h * ref.abs() + 2.0 ** -11 * 1.01 * (p @ u) + keys * 2.0 ** -25 * most(vs) + 2.0 ** -16 * most(v.abs()) + mass * torch.expm1(2 * ds) + 2.0 ** -25
+    bound = 1.01 * h * ref.abs() + 1.01 * (2.0 ** -11 if dtype == "bf16" else 2.0 ** -22) * (p @ u) + keys * 2.0 ** -25 * most(vs) + 2.0 ** -16 * most(v.abs()) + mass * torch.expm1(2 * ds) + 2.0 ** -25
     return ref.transpose(1, 2), bound.transpose(1, 2)
 
 
@@ -105,6 +105,20 @@ def test_few_rows_keep_the_codes(heads, kv, hd, dtype):
         ref, bound = few_rows(q, k, v, at, first, dtype)
         err = (cache.attend(0, q, at, first=first).double().cpu() - ref).abs()
         assert (err <= bound).all(), (at, float((err / bound).max()))
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,s,at", [(32, 8, 128, 1, 30), (8, 2, 64, 3, 100), (5, 5, 128, 5, 60), (4, 2, 256, 2, 400), (8, 1, 128, 4, 20)])
+def test_few_rows_in_f16_are_off_by_the_result(heads, kv, hd, s, at):
+    """All but the result keeps 20 bits and more (few_rows), so the distance to 64 bits is that of rounding the result once, up to 2^-8 of it for what falls to the other side."""
+    ctx = ctx_for(heads, kv, hd, "f16")
+    cache, k, v = filled(ctx, 4, at + s, at, "f16")
+    q = queries(4, s, heads, hd, "f16", at + 1)
+    ref, _ = few_rows(q, k, v, at, 0, "f16")
+    rms = lambda t: float(t.square().mean().sqrt())
+    own, err = rms(ref.half().double() - ref), rms(cache.attend(0, q, at).double().cpu() - ref)
+    assert err <= (1 + 2.0 ** -8) * own, (err, own)
     ctx.close()
 
 
