@@ -28,7 +28,7 @@ def _nccl_include() -> str:
 
 def sources():
     d = os.path.join(HERE, "csrc")
-    return [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith((".cu", ".cuh"))] + \
+    return [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith((".cu", ".cuh", ".hpp"))] + \
            [os.path.join(ROOT, "include", "cake_b200.h")]
 
 
@@ -48,6 +48,7 @@ UNITS = {
     "mixers_window.o": ("mixers_window.cu", ("mixers.cuh", "common.cuh")),
     "mixers_streams.o": ("mixers_streams.cu", ("mixers.cuh", "common.cuh")),
     "packed_cache.o": ("packed_cache.cu", ("packed_cache.cuh", "common.cuh")),
+    "paged_cache.o": ("paged_cache.cu", ("paged_cache.cuh", "paged_plan.hpp", "gemm_tc.cuh", "attn_prefill_tc.cuh", "common.cuh")),
 }
 
 

@@ -167,6 +167,22 @@ SYMBOLS += [
     ("cake_b200_cache_attend", _I, [_VP, _I, _VP, c_size_t, c_size_t, _VP, _I, _I, _I, c_float, _VP]),
 ]
 
+# caches in pages
+SYMBOLS += [
+    ("cake_b200_pages_create", _I, [_VP, _I, _I, _I, _I, _VP, _VP, _I, POINTER(_VP)]),
+    ("cake_b200_pages_free", None, [_VP]),
+    ("cake_b200_pages_add", _I, [_VP, POINTER(_I)]),
+    ("cake_b200_pages_drop", _I, [_VP, _I]),
+    ("cake_b200_pages_truncate", _I, [_VP, _I, _I]),
+    ("cake_b200_pages_len", _I, [_VP, _I]),
+    ("cake_b200_pages_available", _I, [_VP]),
+    ("cake_b200_pages_step", _I, [_VP, POINTER(_I), POINTER(_I), _I, _VP]),
+    ("cake_b200_pages_append", _I, [_VP, _I, _VP, c_size_t, _VP, c_size_t, _VP, c_size_t, _VP, _I, _VP]),
+    ("cake_b200_pages_attend", _I, [_VP, _I, _VP, c_size_t, _VP, _I, c_float, _VP]),
+    ("cake_b200_pages_read", _I, [_VP, _I, _I, _I, _I, _VP, _VP, _VP]),
+    ("cake_b200_forward_paged", _I, [_VP, POINTER(_VP), POINTER(_I), _I, _VP, _VP, _VP, _I]),
+]
+
 
 class CakeB200Error(RuntimeError):
     def __init__(self, code: int, msg: str):

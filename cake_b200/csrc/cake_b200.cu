@@ -35,6 +35,7 @@
 #include "gemv.cuh"
 #include "kept_memory.cuh"
 #include "packed_cache.cuh"
+#include "paged_cache.cuh"
 #include "prefill.cuh"
 #include "sample.cuh"
 
@@ -161,6 +162,10 @@ struct cake_b200_ctx {
   // The operators of such caches may run on a caller's stream: `stream` then is that one for the call.  pc_out: behind the last of them, waited for by
   // this ctx's stream (settle) or another caller's when it goes on; pc_in: the ctx's stream as it was, waited for by a caller's while pc_behind
   cudaEvent_t pc_in = nullptr, pc_out = nullptr;
+  // caches in pages (paged_host.cuh): host data on its way to the device, the rotation tables in fp32
+  struct Staging { void *p = nullptr; size_t cap = 0; cudaEvent_t done = nullptr; bool busy = false; } pg_stage[4];
+  unsigned pg_next = 0;
+  float *pg_cos = nullptr, *pg_sin = nullptr;   // (one piece)
   unsigned long long pc_on = 0;   // the id of the stream that pc_out was recorded on last and nobody has waited for yet; 0: none
   bool pc_behind = true;
   // head of a batch: its logits where the caller keeps none, its tokens
@@ -677,6 +682,11 @@ extern "C" void cake_b200_ctx_destroy(cake_b200_ctx *c) {
   for (void *b : bufs)
     if (b) cudaFree(b);
   c->pc_rows.release_all([](void *p) { cudaFree(p); });
+  if (c->pg_cos) cudaFree(c->pg_cos);
+  for (auto &t : c->pg_stage) {
+    if (t.p) cudaFreeHost(t.p);
+    if (t.done) cudaEventDestroy(t.done);
+  }
   if (c->bigram) cudaFree(c->bigram);
   if (c->pos_tab) cudaFree(c->pos_tab);
   for (void *b : {c->side_tab, c->ln_f_b, c->proj_w, c->proj_ws, c->embed_norm})
@@ -970,6 +980,21 @@ static int cache_create(cake_b200_ctx *c, int batch, int max_seq, int bits, cake
   *out = k;
   return CAKE_B200_OK;
 }
+// what caches with operators of their own (in four bits, in pages) need first: a pool for their memory, events for their callers' streams
+static int ops_ready(cake_b200_ctx *c) {
+  if (!c->pc_pool) {
+    cudaMemPoolProps props{};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = c->device;
+    CU(cudaMemPoolCreate(&c->pc_pool, &props));
+    uint64_t keep = PC_POOL_KEEPS;
+    CU(cudaMemPoolSetAttribute(c->pc_pool, cudaMemPoolAttrReleaseThreshold, &keep));
+  }
+  for (cudaEvent_t *ev : {&c->pc_in, &c->pc_out})
+    if (!*ev) CU(cudaEventCreateWithFlags(ev, cudaEventDisableTiming));
+  return CAKE_B200_OK;
+}
 extern "C" int cake_b200_cache_create(cake_b200_ctx *c, int batch, int max_seq, cake_b200_cache **out) { return cache_create(c, batch, max_seq, 0, out); }
 extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int max_seq, int bits, cake_b200_cache **out) {
   if (!c || !out) return fail(CAKE_B200_EINVAL, "null argument");
@@ -981,17 +1006,7 @@ extern "C" int cake_b200_cache_create_packed(cake_b200_ctx *c, int batch, int ma
   CU(cudaSetDevice(c->device));
   if (!c->pc_tickets) {
     CU((cudaError_t)pc::prepare(c->cfg.dtype, c->cfg.head_dim));
-    if (!c->pc_pool) {
-      cudaMemPoolProps props{};
-      props.allocType = cudaMemAllocationTypePinned;
-      props.location.type = cudaMemLocationTypeDevice;
-      props.location.id = c->device;
-      CU(cudaMemPoolCreate(&c->pc_pool, &props));
-      uint64_t keep = PC_POOL_KEEPS;
-      CU(cudaMemPoolSetAttribute(c->pc_pool, cudaMemPoolAttrReleaseThreshold, &keep));
-    }
-    for (cudaEvent_t *ev : {&c->pc_in, &c->pc_out})
-      if (!*ev) CU(cudaEventCreateWithFlags(ev, cudaEventDisableTiming));
+    RC(ops_ready(c));
     if (!c->pc_ws) CU(cudaMalloc(&c->pc_ws, pc::scratch_floats(c->sm_count) * sizeof(float)));
     const size_t n = pc::scratch_tickets(c->sm_count) * sizeof(unsigned);
     unsigned *tickets = nullptr;
@@ -1329,6 +1344,8 @@ extern "C" int cake_b200_cache_fill_synthetic(cake_b200_cache *k, const int *blo
   CU(cudaGetLastError());
   return CAKE_B200_OK;
 }
+
+#include "paged_host.cuh"
 
 // ------------------------------------------------------------------------------------------ decode path (batch 1, seq 1)
 // x_in -> x_out through `n` blocks; position comes from cache->d_pos (device).  5 kernels per layer.
@@ -1859,8 +1876,8 @@ static int prompt_attention(cake_b200_ctx *c, const void *q, size_t q_tok, size_
 }
 
 static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *blocks, const int *block_idx, int n,
-                                  cake_b200_cache *kc, const void *x_in, void *x_out, int B, int S, int pos0) {
-  const cake_b200_config &f = c->cfg;
+                                  cake_b200_cache *kc, const void *x_in, void *x_out, int B, int S, int pos0, cake_b200_pages *pages = nullptr) {
+  const cake_b200_config &f = c->cfg;   // (with pages: B = 1, the S rows are the present step's, kc is nullptr)
   const int H = f.hidden, I = f.inter, hd = f.head_dim, sq = f.n_heads * hd, M = B * S;
   RC(pf_reserve(c, (size_t)M));
   // cache.rs:173-205: a call on a non-empty cache sees the last `window` positions of cat(cache, new) — every query of
@@ -1902,7 +1919,9 @@ static int enqueue_prefill_layers(cake_b200_ctx *c, cake_b200_block *const *bloc
         qn = kn = nullptr;
       }
       const int rope_on = b->use_rope ? 1 : 0;
-      if (kc->bits) {
+      if (pages) {
+        RC(pages_layer(c, b, pages, l, c->pf_qkv, qn, kn, c->pf_y));
+      } else if (kc->bits) {
         RC(write_packed(c, b, kc, l, c->pf_qkv, qn, kn, S, pos0));
         RC(attend_packed(c, kc, l, c->pf_qkv, c->nqkv, (size_t)S * c->nqkv, c->pf_y, S, pos0, ws, (float)(1.0 / sqrt((double)hd))));
       } else {
@@ -3872,6 +3891,31 @@ static int io_reserve(cake_b200_ctx *c, size_t bytes) {
   return CAKE_B200_OK;
 }
 
+// == forward_batch over the present step of a cache in pages
+extern "C" int cake_b200_forward_paged(cake_b200_ctx *c, cake_b200_block *const *blocks, const int *block_idx, int n_blocks, cake_b200_pages *g,
+                                       const void *x_dev, void *y_dev, int n_rows) {
+  if (!c || !blocks || !block_idx || !g || !x_dev || !y_dev || n_blocks < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
+  if (g->ctx != c) return fail(CAKE_B200_EINVAL, "the cache belongs to another context");
+  CU(cudaSetDevice(c->device));
+  RC(wait_loads(c));
+  for (int i = 0; i < n_blocks; i++) {
+    if (!blocks[i]) return fail(CAKE_B200_EINVAL, "blocks[%d] is null", i);
+    if (blocks[i]->listed || blocks[i]->mixer) return fail(CAKE_B200_EINVAL, "caches in pages are for the Llama-family blocks");
+    RC(pages_block(g, block_idx[i], "forward_paged", true));
+    for (int j = 0; j < i; j++)
+      if (block_idx[j] == block_idx[i]) return fail(CAKE_B200_EINVAL, "block_idx %d is twice in the call", block_idx[i]);
+    RC(pages_written(g, block_idx[i], false));
+    const int w = blocks[i]->window >= 0 ? blocks[i]->window : c->cfg.sliding_window;
+    for (const pg::SeqRow &s : g->book.step)   // (as forward_batch has it)
+      if (w > 0 && s.pos0 > 0 && s.count > w) return fail(CAKE_B200_EINVAL, "a chunk of %d tokens on a non-empty cache exceeds the sliding window %d", s.count, w);
+  }
+  if (n_rows != g->book.n_rows) return fail(CAKE_B200_EINVAL, "x has %d rows, the step %d", n_rows, g->book.n_rows);
+  RC(settle(c));
+  RC(enqueue_prefill_layers(c, blocks, block_idx, n_blocks, nullptr, x_dev, y_dev, 1, n_rows, 0, g));
+  c->pc_behind = true;
+  CU(cudaGetLastError());
+  return CAKE_B200_OK;
+}
 extern "C" int cake_b200_forward_batch_host(cake_b200_ctx *c, cake_b200_block *const *blocks, const int *block_idx,
                                             int n_blocks, cake_b200_cache *kc, const void *x_host, void *y_host,
                                             int batch, int seq, int index_pos) {

@@ -1,0 +1,218 @@
+// paged_cache.cu — kernels of the cache in pages (format and interface: paged_cache.cuh)
+#include "paged_cache.cuh"
+#include "common.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace cake {
+namespace pg {
+
+template <typename... KArgs, typename... Args>
+static int launch(cudaStream_t s, uint64_t *launches, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  if (e == cudaSuccess) ++*launches;
+  return (int)e;
+}
+template <typename T> struct Tag { typedef T type; };
+template <typename F> static int by_type(int dtype, F &&f) { return dtype == 1 ? f(Tag<__half>{}) : f(Tag<__nv_bfloat16>{}); }
+
+// whether this call is the present step's; a replayed call of another one does nothing
+__device__ __forceinline__ bool same_step(const Pool &p) {
+  if (__ldg(&p.step->shape) == p.shape) return true;
+  if (threadIdx.x == 0) *p.bad = 1;
+  return false;
+}
+__device__ __forceinline__ char *rows_of(const Pool &p, int page, int kvh, int which) {
+  return p.pages + ((size_t)page * p.n_kv + kvh) * (rows_bytes(p.hd, 2) << p.page_log2) + (which ? rows_bytes(p.hd, 1) << p.page_log2 : (size_t)0);
+}
+__device__ __forceinline__ int page_of(const Pool &p, int slot, int pos) { return __ldg(p.table + (size_t)slot * p.per_seq + (pos >> p.page_log2)); }
+
+// ------------------------------------------------------------------------------------------ a step's sequences and rows
+__global__ void __launch_bounds__(256) spread_kernel(const StepHead *step, int max_seqs, int n_seqs, int *table, int2 *rows) {
+  const SeqRow *seqs = reinterpret_cast<const SeqRow *>(step + 1);
+  const int at = blockIdx.y * 256 + threadIdx.x, by = gridDim.y * 256;
+  if ((int)blockIdx.x == n_seqs) {
+    const int2 *u = reinterpret_cast<const int2 *>(seqs + max_seqs);
+    for (int i = at; i < step->n_updates; i += by) table[u[i].x] = u[i].y;
+    return;
+  }
+  const SeqRow s = seqs[blockIdx.x];
+  for (int i = at; i < s.count; i += by) rows[s.row0 + i] = make_int2(s.slot, s.pos0 + i);
+}
+int spread(cudaStream_t s, const StepHead *step, int max_seqs, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches) {
+  const int most = std::max(most_rows, n_updates);
+  // (launched without the early start of the others: what runs behind it reads the table before it waits)
+  spread_kernel<<<dim3((unsigned)n_seqs + 1, (unsigned)std::min(64, (most + 255) / 256)), 256, 0, s>>>(step, max_seqs, n_seqs, table, rows);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) ++*launches;
+  return (int)e;
+}
+
+// ------------------------------------------------------------------------------------------ rows into the pages
+// Bound by memory: what comes in goes out.  A lane has 16 bytes of a row, hd / 8 lanes a head, a warp 32 / (hd / 8) heads of a token at once and, where the
+// tokens alone do not fill the chip, a part of its heads; the row of the tables is read once a warp.  A pair's other entry comes from the lane that has it.
+// Norm and rotation in fp32 and one rounding; in a block's step they are rounded where the blocks' other paths round them (the normed entries, the products),
+// so that its rows are those that any other cache would hold: logits of three layers within 4 units in the last place of the oracle, else up to 6.
+template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
+template <typename T>
+__global__ void __launch_bounds__(128) append_kernel(const Pool p, const Append a, int parts) {
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cph = p.hd >> 3, at_once = 32 / cph, c = lane & (cph - 1), sub = lane / cph;
+  const int row = blockIdx.x * 4 + warp, heads = a.n_q + 2 * p.n_kv;
+  pdl_wait();
+  if (!same_step(p) || row >= a.n_rows) return;
+  const int2 at = __ldg(a.rows + row);
+  const int page = page_of(p, at.x, at.y), r = at.y & ((1 << p.page_log2) - 1);
+  const int h8 = a.rot >> 4;   // chunks of the pairs' first entries
+  const bool turns = a.cos_t && c < 2 * h8, low = c < h8;
+  const int other = lane - c + (turns ? (low ? c + h8 : c - h8) : c);
+  float cs[8], sn[8];
+  if (turns) {
+    const size_t o = (size_t)at.y * (8 * h8) + 8 * (low ? c : c - h8);
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(a.cos_t + o + i)), y = __ldg(reinterpret_cast<const float4 *>(a.sin_t + o + i));
+      cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
+      sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
+    }
+  }
+#pragma unroll 2
+  for (int g = blockIdx.y; g * at_once < heads; g += parts) {
+    const int head = g * at_once + sub;
+    const bool in = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + p.n_kv;
+    const int h = is_q ? head : is_v ? head - a.n_q - p.n_kv : head - a.n_q;
+    const T *src = is_q ? reinterpret_cast<const T *>(a.q) + (size_t)row * a.q_tok
+                   : is_v ? reinterpret_cast<const T *>(a.v) + (size_t)row * a.v_tok : reinterpret_cast<const T *>(a.k) + (size_t)row * a.k_tok;
+    uint4 w = in ? *reinterpret_cast<const uint4 *>(src + (size_t)h * p.hd + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+    const bool dirty = in && is_v && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w));
+    const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
+    if (a.cos_t || a.q_norm || a.k_norm) {   // (the same for all lanes, as the exchanges have to be)
+      float x[8], y[8];
+      unpack8<T>(w, x);
+      if (a.q_norm || a.k_norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+        for (int o = 1; o < cph; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (nw && !is_v) {
+          const float inv = 1.0f / sqrtf(ss / (float)p.hd + a.eps);
+          float g8[8];
+          unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c), g8);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = a.as_blocks ? rnd<T>(x[i] * inv * g8[i]) : x[i] * inv * g8[i];
+        }
+      }
+      if (a.cos_t) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other);
+        if (turns && !is_v)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float f = x[i] * cs[i], s = low ? -y[i] * sn[i] : y[i] * sn[i];
+            x[i] = a.as_blocks ? rnd<T>(f) + rnd<T>(s) : f + s;
+          }
+      }
+      if (!is_v) w = make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+    }
+    if (in) {
+      void *to = is_q ? (void *)(reinterpret_cast<T *>(a.q_out) + (size_t)row * a.out_tok + (size_t)h * p.hd + 8 * c) : (void *)(rows_of(p, page, h, is_v) + chunk_at(p.hd, r, c));
+      *reinterpret_cast<uint4 *>(to) = w;
+      if (dirty) p.marks[(size_t)page * p.n_kv + h] = 1u;
+    }
+  }
+}
+int append(cudaStream_t s, int dtype, const Pool &p, const Append &a, int sms, uint64_t *launches) {
+  const int at_once = 256 / p.hd, groups = (a.n_q + 2 * p.n_kv + at_once - 1) / at_once;
+  int parts = 1;
+  while (parts < groups && (long)a.n_rows * parts < 16l * sms) parts++;
+  return by_type(dtype, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    return launch(s, launches, append_kernel<T>, dim3((unsigned)((a.n_rows + 3) / 4), (unsigned)parts), dim3(128), 0, p, a, parts);
+  });
+}
+
+// ------------------------------------------------------------------------------------------ rows out of the pages
+__global__ void __launch_bounds__(256) read_kernel(const Pool p, const Read a) {
+  pdl_launch_dependents();
+  const int cph = p.hd >> 3;
+  const size_t n = (size_t)a.n * p.n_kv * cph;
+  pdl_wait();
+  if (a.rows && !same_step(p)) return;
+  for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
+    const int c = (int)(i % cph), h = (int)(i / cph % p.n_kv), row = (int)(i / cph / p.n_kv);
+    const int2 at = a.rows ? __ldg(a.rows + row) : make_int2(a.slot, a.first + row);
+    const int page = page_of(p, at.x, at.y), r = at.y & ((1 << p.page_log2) - 1);
+    if (a.k) reinterpret_cast<uint4 *>(a.k)[i] = *reinterpret_cast<const uint4 *>(rows_of(p, page, h, 0) + chunk_at(p.hd, r, c));
+    if (a.v) reinterpret_cast<uint4 *>(a.v)[i] = *reinterpret_cast<const uint4 *>(rows_of(p, page, h, 1) + chunk_at(p.hd, r, c));
+  }
+}
+int read(cudaStream_t s, int, const Pool &p, const Read &a, uint64_t *launches) {
+  const size_t n = (size_t)a.n * p.n_kv * (p.hd >> 3);
+  return launch(s, launches, read_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 148 * 32)), dim3(256), 0, p, a);
+}
+
+// ------------------------------------------------------------------------------------------ attention
+// A warp per row and head, a key after the other.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) attend_kernel(const Pool p, const Attend a) {
+  pdl_launch_dependents();
+  constexpr int E = HD / 32;   // entries of a lane: E lane .. E lane + E - 1
+  const int lane = threadIdx.x & 31;
+  const long item = blockIdx.x * 4l + (threadIdx.x >> 5);
+  pdl_wait();
+  if (!same_step(p) || item >= (long)a.n_rows * a.n_heads) return;
+  const int row = (int)(item / a.n_heads), head = (int)(item % a.n_heads), kvh = head / (a.n_heads / p.n_kv);
+  const int2 at = a.rows[row];
+  int lo = 0;
+  if (a.win.w > 0 && !a.win.by_call) lo = max(0, at.y + 1 - a.win.w);
+  if (a.win.w > 0 && a.win.by_call)
+    for (int i = 0; i < p.step->n_seqs; i++)
+      if (a.seqs[i].slot == at.x) lo = a.seqs[i].pos0 > 0 ? max(0, a.seqs[i].pos0 + a.seqs[i].count - a.win.w) : 0;
+  float q[E], o[E], m = -INFINITY, l = 0.f;
+  for (int e = 0; e < E; e++) {
+    q[e] = DT<T>::to_f(reinterpret_cast<const T *>(a.q)[(size_t)row * a.q_tok + head * HD + lane * E + e]) * a.scale * 1.4426950408889634f;
+    o[e] = 0.f;
+  }
+  const int c = lane * E / 8, e0 = lane * E % 8;
+  for (int j = lo; j <= at.y; j++) {
+    const int page = page_of(p, at.x, j), r = j & ((1 << p.page_log2) - 1);
+    const T *k = reinterpret_cast<const T *>(rows_of(p, page, kvh, 0) + chunk_at(HD, r, c)) + e0, *v = reinterpret_cast<const T *>(rows_of(p, page, kvh, 1) + chunk_at(HD, r, c)) + e0;
+    float s = 0.f;
+    for (int e = 0; e < E; e++) s += q[e] * DT<T>::to_f(k[e]);
+    s = warp_sum(s);
+    const float mn = fmaxf(m, s), f = m == mn ? 1.f : exp2f(m - mn), w = exp2f(s - mn);
+    m = mn;
+    l = l * f + w;
+    for (int e = 0; e < E; e++) o[e] = o[e] * f + w * DT<T>::to_f(v[e]);
+  }
+  for (int e = 0; e < E; e++) reinterpret_cast<T *>(a.out)[((size_t)row * a.n_heads + head) * HD + lane * E + e] = DT<T>::from_f(o[e] / l);
+}
+int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, uint64_t *launches) {
+  const dim3 grid((unsigned)(((long)a.n_rows * a.n_heads + 3) / 4));
+  return by_type(dtype, [&](auto t) {
+    typedef typename decltype(t)::type T;
+    switch (p.hd) {
+      case 64: return launch(s, launches, attend_kernel<T, 64>, grid, dim3(128), 0, p, a);
+      case 128: return launch(s, launches, attend_kernel<T, 128>, grid, dim3(128), 0, p, a);
+      default: return launch(s, launches, attend_kernel<T, 256>, grid, dim3(128), 0, p, a);
+    }
+  });
+}
+
+}  // namespace pg
+}  // namespace cake

@@ -1,0 +1,316 @@
+// paged_host.cuh — the C ABI of caches in pages (include/cake_b200.h, cake_b200_pages_*), part of cake_b200.cu
+#pragma once
+
+struct cake_b200_pages {
+  cake_b200_ctx *ctx;
+  int device = 0;
+  pg::Book book;
+  // device memory, one piece of the ctx's pool: the step, the page table, the rows' places
+  char *arena = nullptr;
+  pg::StepHead *step = nullptr;
+  int *table = nullptr;
+  int2 *rows = nullptr;
+  std::vector<void *> pool;          // of each block: the pages and, behind them, their marks
+  std::vector<std::vector<int>> len; // positions written, of each block and sequence
+  std::vector<char> in_graph;        // a captured call writes this block's rows: how far, only its user knows
+  const float *cos_t = nullptr, *sin_t = nullptr;
+  int rot = 0;
+  int *bad = nullptr;                // pinned: a replayed call met a step of another shape
+  size_t page_bytes() const { return (size_t)2 * book.page * ctx->cfg.n_kv_heads * ctx->cfg.head_dim * 2; }
+};
+
+static int pages_call(const cake_b200_pages *g, const char *what) {
+  if (!g) return fail(CAKE_B200_EINVAL, "null argument");
+  RC(check_waits(g->ctx));
+  if (*(volatile int *)g->bad) {
+    *(volatile int *)g->bad = 0;
+    return fail(CAKE_B200_ESTATE, "%s: a replayed graph's calls were made for steps of other counts than the present one and did nothing", what);
+  }
+  return CAKE_B200_OK;
+}
+static bool is_capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus st;
+  const cudaError_t e = cudaStreamIsCapturing(s, &st);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e != cudaSuccess || st != cudaStreamCaptureStatusNone;
+}
+// host data on its way to the device: pinned buffers in turn
+static int pages_upload(cake_b200_ctx *c, void *dst, const void *src, size_t bytes) {
+  cake_b200_ctx::Staging &t = c->pg_stage[c->pg_next++ % (sizeof c->pg_stage / sizeof c->pg_stage[0])];
+  if (!t.done) CU(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming));
+  if (t.busy) CU(cudaEventSynchronize(t.done));
+  t.busy = false;
+  if (bytes > t.cap) {
+    if (t.p) cudaFreeHost(t.p);
+    t.p = nullptr; t.cap = 0;
+    const size_t cap = std::max<size_t>(bytes, 1 << 16);
+    CU(cudaMallocHost(&t.p, cap));
+    t.cap = cap;
+  }
+  memcpy(t.p, src, bytes);
+  CU(cudaMemcpyAsync(dst, t.p, bytes, cudaMemcpyHostToDevice, c->stream));
+  CU(cudaEventRecord(t.done, c->stream));
+  t.busy = true;
+  return CAKE_B200_OK;
+}
+template <typename T> __global__ void widen_kernel(const T *x, float *y, size_t n) {
+  for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) y[i] = DT<T>::to_f(x[i]);
+}
+
+extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_size, int max_seqs, int max_seq, const float *cos_dev, const float *sin_dev,
+                                      int rot, cake_b200_pages **out) {
+  if (!c || !out) return fail(CAKE_B200_EINVAL, "null argument");
+  const cake_b200_config &f = c->cfg;
+  if (f.layer_list) return fail(CAKE_B200_EINVAL, "caches in pages are for the Llama-family blocks");
+  if (!pg::head_dim_ok(f.head_dim)) return fail(CAKE_B200_EINVAL, "caches in pages hold heads of 64, 128 or 256 entries, not %d", f.head_dim);
+  if (!pg::page_ok(page_size)) return fail(CAKE_B200_EINVAL, "a page holds 16, 32, .. 1024 positions (a power of two), not %d", page_size);
+  if (n_pages < 1 || max_seqs < 1 || max_seq < 1) return fail(CAKE_B200_EINVAL, "pages, max_seqs and max_seq are 1 or more");
+  if ((long long)n_pages * page_size > (1ll << 30) || (long long)max_seqs * ((max_seq + page_size - 1) / page_size) > (1ll << 28))
+    return fail(CAKE_B200_EINVAL, "%d pages of %d positions, %d sequences of %d: more than a cache in pages counts", n_pages, page_size, max_seqs, max_seq);
+  const bool own = !cos_dev && !sin_dev;
+  if (!own && (!cos_dev || !sin_dev)) return fail(CAKE_B200_EINVAL, "cos without sin");
+  if (own) {
+    rot = c->rot;
+    if (max_seq > f.max_seq) return fail(CAKE_B200_EINVAL, "max_seq %d exceeds config max_seq %d (RoPE table rows)", max_seq, f.max_seq);
+  }
+  if (rot < 0 || rot > f.head_dim || rot % 16) return fail(CAKE_B200_EINVAL, "caches in pages rotate multiples of 16 entries of a head, not %d", rot);
+  if (!own && (((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15)) return fail(CAKE_B200_EINVAL, "rotation tables start on 16-byte boundaries");
+  const OnDevice dev(c->device);
+  RC(ops_ready(c));
+  RC(settle(c));
+  if (own && rot && !c->pg_cos) {
+    const size_t n = (size_t)f.max_seq * (c->rot / 2);
+    float *both = nullptr;
+    CU(cudaMalloc(&both, 2 * n * sizeof(float)));
+    const int rc = DISPATCH_T(f.dtype, T_LAMBDA {
+      typedef typename decltype(tag_)::type T;
+      widen_kernel<T><<<592, 256, 0, c->stream>>>((const T *)c->cos_t, both, n);
+      widen_kernel<T><<<592, 256, 0, c->stream>>>((const T *)c->sin_t, both + n, n);
+      CU(cudaGetLastError());
+      return CAKE_B200_OK;
+    });
+    if (rc != CAKE_B200_OK) { cudaFree(both); return rc; }
+    c->launches += 2;
+    c->pg_cos = both; c->pg_sin = both + n;
+    c->pc_behind = true;
+  }
+  auto *g = new cake_b200_pages{c, c->device};
+  struct Guard { cake_b200_pages *g; ~Guard() { if (g) cake_b200_pages_free(g); } } guard{g};
+  g->book.init(n_pages, page_size, max_seqs, max_seq);
+  g->pool.assign((size_t)f.n_layers, nullptr);
+  g->len.assign((size_t)f.n_layers, std::vector<int>((size_t)max_seqs, 0));
+  g->in_graph.assign((size_t)f.n_layers, 0);
+  g->rot = rot;
+  if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
+  CU(cudaMallocHost(&g->bad, 4));
+  *g->bad = 0;
+  const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
+               s_rows = (size_t)n_pages * page_size * 8;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  void *arena = nullptr;
+  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + s_rows, c->pc_pool, c->stream));
+  g->arena = (char *)arena;
+  g->step = (pg::StepHead *)g->arena;
+  g->table = (int *)(g->arena + up(s_step));
+  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table));
+  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table), c->stream));
+  c->pc_behind = true;
+  guard.g = nullptr;
+  *out = g;
+  return CAKE_B200_OK;
+}
+extern "C" void cake_b200_pages_free(cake_b200_pages *g) {
+  if (!g) return;
+  const OnDevice dev(g->device);
+  {
+    std::lock_guard<std::mutex> lk(g_live_mu);
+    const bool live = g_live_ctx.count(g->ctx) != 0;
+    if (live) {
+      (void)settle(g->ctx);
+      cudaStreamSynchronize(g->ctx->stream);
+    }
+    for (void *p : g->pool)
+      if (p) (void)(live ? cudaFreeAsync(p, g->ctx->stream) : cudaFree(p));
+    if (g->arena) (void)(live ? cudaFreeAsync(g->arena, g->ctx->stream) : cudaFree(g->arena));
+    if (live && cudaStreamSynchronize(g->ctx->stream) == cudaSuccess) (void)cudaMemPoolTrimTo(g->ctx->pc_pool, PC_POOL_KEEPS);
+  }
+  if (g->bad) cudaFreeHost(g->bad);
+  (void)cudaGetLastError();
+  delete g;
+}
+
+extern "C" int cake_b200_pages_add(cake_b200_pages *g, int *seq) {
+  if (!g || !seq) return fail(CAKE_B200_EINVAL, "null argument");
+  const int s = g->book.add();
+  if (s < 0) return fail(CAKE_B200_ESTATE, "all %d sequences are taken", g->book.max_seqs);
+  for (auto &l : g->len) l[(size_t)s] = 0;
+  *seq = s;
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_pages_truncate(cake_b200_pages *g, int seq, int len) {
+  if (!g) return fail(CAKE_B200_EINVAL, "null argument");
+  if (!g->book.has(seq)) return fail(CAKE_B200_EINVAL, "there is no sequence %d", seq);
+  if (len < 0 || len > g->book.seqs[(size_t)seq].len) return fail(CAKE_B200_ESTATE, "sequence %d has %d positions, not %d", seq, g->book.seqs[(size_t)seq].len, len);
+  g->book.cut(seq, len);
+  for (auto &l : g->len) l[(size_t)seq] = std::min(l[(size_t)seq], len);
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_pages_drop(cake_b200_pages *g, int seq) {
+  if (!g) return fail(CAKE_B200_EINVAL, "null argument");
+  if (!g->book.has(seq)) return fail(CAKE_B200_EINVAL, "there is no sequence %d", seq);
+  g->book.drop(seq);
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_pages_len(const cake_b200_pages *g, int seq) { return !g || !g->book.has(seq) ? -1 : g->book.seqs[(size_t)seq].len; }
+extern "C" int cake_b200_pages_available(const cake_b200_pages *g) { return g ? (int)g->book.free_pages.size() : -1; }
+
+extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const int *counts, int n, void *stream) {
+  RC(pages_call(g, "pages_step"));
+  if (!seqs || !counts || n < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
+  if (n > g->book.max_seqs) return fail(CAKE_B200_EINVAL, "a step of %d sequences, the cache has %d", n, g->book.max_seqs);
+  cake_b200_ctx *c = g->ctx;
+  const OnDevice dev(g->device);
+  if (is_capturing(stream ? (cudaStream_t)stream : c->stream)) return fail(CAKE_B200_ESTATE, "a step is planned outside captures; its calls may be captured");
+  pg::Book &k = g->book;
+  int i = 0;
+  switch (k.plan(seqs, counts, n, c->cfg.n_heads / c->cfg.n_kv_heads, &i)) {
+    case pg::Book::OK: break;
+    case pg::Book::NOT_LIVE: return fail(CAKE_B200_EINVAL, "there is no sequence %d", seqs[i]);
+    case pg::Book::TWICE: return fail(CAKE_B200_EINVAL, "sequence %d is twice in the step", seqs[i]);
+    case pg::Book::COUNT: return fail(CAKE_B200_EINVAL, "sequence %d brings %d rows", seqs[i], counts[i]);
+    case pg::Book::TOO_LONG: return fail(CAKE_B200_ESTATE, "sequence %d: %d + %d positions exceed max_seq %d", seqs[i], k.seqs[(size_t)seqs[i]].len, counts[i], k.max_seq);
+    case pg::Book::NO_PAGES: return fail(CAKE_B200_ENOMEM, "the step needs more pages than the %d that are free", (int)k.free_pages.size());
+  }
+  return on_stream(c, stream, [&]() -> int {
+    const size_t at = sizeof(pg::StepHead) + (size_t)k.max_seqs * sizeof(pg::SeqRow), bytes = at + k.updates.size() * 4;
+    std::vector<char> blob(bytes, 0);
+    pg::StepHead h{};
+    h.shape = k.shape; h.n_seqs = n; h.n_rows = k.n_rows; h.n_updates = (int)k.updates.size() / 2;
+    memcpy(blob.data(), &h, sizeof h);
+    memcpy(blob.data() + sizeof h, k.step.data(), k.step.size() * sizeof(pg::SeqRow));
+    if (!k.updates.empty()) memcpy(blob.data() + at, k.updates.data(), k.updates.size() * 4);
+    RC(pages_upload(c, g->step, blob.data(), bytes));
+    int most = 1;
+    for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
+    CU((cudaError_t)pg::spread(c->stream, g->step, k.max_seqs, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
+    return CAKE_B200_OK;
+  });
+}
+
+static int pages_block(cake_b200_pages *g, int block_idx, const char *what, bool wants_step) {
+  RC(pages_call(g, what));
+  if (block_idx < 0 || block_idx >= (int)g->pool.size()) return fail(CAKE_B200_EINVAL, "block_idx %d out of range", block_idx);
+  if (wants_step && g->book.step.empty()) return fail(CAKE_B200_ESTATE, "%s: there is no step (or one of its sequences was cut or dropped)", what);
+  return CAKE_B200_OK;
+}
+static int pages_ensure(cake_b200_pages *g, int l) {
+  if (g->pool[(size_t)l]) return CAKE_B200_OK;
+  cake_b200_ctx *c = g->ctx;
+  RC(no_capture(c->stream, "a block's pages"));
+  const size_t bytes = (size_t)g->book.n_pages * (g->page_bytes() + (size_t)c->cfg.n_kv_heads * 4);
+  void *p = nullptr;
+  CU(cudaMallocFromPoolAsync(&p, bytes, c->pc_pool, c->stream));
+  const cudaError_t e = cudaMemsetAsync(p, 0, bytes, c->stream);
+  if (e != cudaSuccess) { (void)cudaFreeAsync(p, c->stream); return fail(CAKE_B200_ECUDA, "pages: %s", cudaGetErrorString(e)); }
+  g->pool[(size_t)l] = p;
+  return CAKE_B200_OK;
+}
+static pg::Pool pages_pool(const cake_b200_pages *g, int l) {
+  const cake_b200_config &f = g->ctx->cfg;
+  int log2 = 0;
+  while (1 << log2 < g->book.page) log2++;
+  char *p = (char *)g->pool[(size_t)l];
+  return pg::Pool{p, (uint32_t *)(p + (size_t)g->book.n_pages * g->page_bytes()), g->table, g->step, g->book.shape, g->bad, f.n_kv_heads, f.head_dim, log2, g->book.per_seq};
+}
+// the rows that the step's follow are there (append), and its own (attend, read)
+static int pages_written(const cake_b200_pages *g, int l, bool own) {
+  if (g->in_graph[(size_t)l]) return CAKE_B200_OK;
+  for (const pg::SeqRow &s : g->book.step) {
+    const int have = g->len[(size_t)l][(size_t)s.slot], need = own ? s.pos0 + s.count : s.pos0;
+    if (have < need) return fail(CAKE_B200_ESTATE, "block %d has %d positions of sequence %d, not %d", l, have, s.slot, need);
+  }
+  return CAKE_B200_OK;
+}
+static int pages_append_on(cake_b200_pages *g, int l, const pg::Append &a) {   // on the ctx's stream of the moment
+  cake_b200_ctx *c = g->ctx;
+  CU((cudaError_t)pg::append(c->stream, c->cfg.dtype, pages_pool(g, l), a, c->sm_count, launch_counter(c)));
+  if (is_capturing(c->stream)) g->in_graph[(size_t)l] = 1;
+  for (const pg::SeqRow &s : g->book.step) g->len[(size_t)l][(size_t)s.slot] = s.pos0 + s.count;
+  return CAKE_B200_OK;
+}
+static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_tok, void *out, const pg::Window &win, float scale) {
+  cake_b200_ctx *c = g->ctx;
+  const pg::Attend a{g->rows, q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), g->book.n_rows, c->cfg.n_heads, scale, win};
+  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, launch_counter(c)));
+  return CAKE_B200_OK;
+}
+extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,
+                                      size_t v_tok, void *q_out, int rotate, void *stream) {
+  RC(pages_block(g, block_idx, "pages_append", true));
+  const OnDevice dev(g->device);
+  if (!k_dev || !v_dev || !q_dev != !q_out) return fail(CAKE_B200_EINVAL, "null argument");
+  if (unaligned(k_dev, k_tok) || unaligned(v_dev, v_tok) || unaligned(q_dev, q_tok) || unaligned(q_out))
+    return fail(CAKE_B200_EINVAL, "pages_append takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
+  RC(pages_written(g, block_idx, false));
+  cake_b200_ctx *c = g->ctx;
+  if (!g->pool[(size_t)block_idx] && stream) RC(no_capture((cudaStream_t)stream, "a block's pages"));
+  const cake_b200_config &f = c->cfg;
+  return on_stream(c, stream, [&]() -> int {
+    RC(pages_ensure(g, block_idx));
+    pg::Append a{};
+    a.rows = g->rows; a.q = q_dev; a.k = k_dev; a.v = v_dev; a.q_out = q_out; a.q_tok = (long long)q_tok; a.k_tok = (long long)k_tok; a.v_tok = (long long)v_tok;
+    a.out_tok = (long long)f.n_heads * f.head_dim;
+    if (rotate) { a.cos_t = g->cos_t; a.sin_t = g->sin_t; a.rot = g->rot; }
+    a.n_rows = g->book.n_rows; a.n_q = q_dev ? f.n_heads : 0;
+    return pages_append_on(g, block_idx, a);
+  });
+}
+extern "C" int cake_b200_pages_attend(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, void *out_dev, int window, float scale, void *stream) {
+  RC(pages_block(g, block_idx, "pages_attend", true));
+  const OnDevice dev(g->device);
+  if (!q_dev || !out_dev) return fail(CAKE_B200_EINVAL, "null argument");
+  if (unaligned(q_dev, q_tok) || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "pages_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
+  if (window < 0 || !(scale >= 0.f && scale <= 3.402823466e38f)) return fail(CAKE_B200_EINVAL, "window %d or scale %g out of range", window, (double)scale);
+  if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);
+  RC(pages_written(g, block_idx, true));
+  return on_stream(g->ctx, stream, [&]() -> int {
+    return pages_attend_on(g, block_idx, q_dev, q_tok, out_dev, pg::Window{window, false}, scale > 0.f ? scale : (float)(1.0 / sqrt((double)g->ctx->cfg.head_dim)));
+  });
+}
+extern "C" int cake_b200_pages_read(cake_b200_pages *g, int block_idx, int seq, int first, int n, void *k_dev, void *v_dev, void *stream) {
+  RC(pages_block(g, block_idx, "pages_read", seq < 0));
+  const OnDevice dev(g->device);
+  if (!k_dev && !v_dev) return fail(CAKE_B200_EINVAL, "null argument");
+  if (unaligned(k_dev) || unaligned(v_dev)) return fail(CAKE_B200_EINVAL, "pages_read writes to 16-byte boundaries");
+  if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);
+  pg::Read a{nullptr, seq, first, n, k_dev, v_dev};
+  if (seq < 0) {
+    RC(pages_written(g, block_idx, true));
+    a = pg::Read{g->rows, 0, 0, g->book.n_rows, k_dev, v_dev};
+  } else {
+    if (!g->book.has(seq)) return fail(CAKE_B200_EINVAL, "there is no sequence %d", seq);
+    const int have = g->in_graph[(size_t)block_idx] ? g->book.seqs[(size_t)seq].len : g->len[(size_t)block_idx][(size_t)seq];
+    if (first < 0 || n < 1 || (long long)first + n > have)
+      return fail(CAKE_B200_ESTATE, "block %d, sequence %d: positions %d .. + %d are not within %d", block_idx, seq, first, n, have);
+  }
+  return on_stream(g->ctx, stream, [&]() -> int {
+    CU((cudaError_t)pg::read(g->ctx->stream, g->ctx->cfg.dtype, pages_pool(g, block_idx), a, launch_counter(g->ctx)));
+    return CAKE_B200_OK;
+  });
+}
+// a layer's attention in a step of rows in pages: qkv [rows, heads + 2 kv heads, hd] as the projection left them (q is normed and rotated in place) -> y
+static int pages_layer(cake_b200_ctx *c, const cake_b200_block *b, cake_b200_pages *g, int l, void *qkv, const void *qn, const void *kn, void *y) {
+  const cake_b200_config &f = c->cfg;
+  RC(pages_ensure(g, l));
+  char *p = (char *)qkv;
+  pg::Append a{};
+  a.rows = g->rows; a.q = p; a.q_out = p;
+  a.k = p + (size_t)f.n_heads * f.head_dim * c->es;
+  a.v = p + (size_t)(f.n_heads + f.n_kv_heads) * f.head_dim * c->es;
+  a.q_tok = a.k_tok = a.v_tok = a.out_tok = c->nqkv;
+  a.q_norm = qn; a.k_norm = kn; a.eps = f.rms_eps;
+  if (b->use_rope) { a.cos_t = g->cos_t; a.sin_t = g->sin_t; a.rot = g->rot; }
+  a.n_rows = g->book.n_rows; a.n_q = f.n_heads; a.as_blocks = true;
+  RC(pages_append_on(g, l, a));
+  return pages_attend_on(g, l, qkv, c->nqkv, y, pg::Window{b->window >= 0 ? b->window : f.sliding_window, true}, (float)(1.0 / sqrt((double)f.head_dim)));
+}

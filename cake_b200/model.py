@@ -147,6 +147,124 @@ class Cache:
             pass
 
 
+class PagedCache:
+    """K and V rows of many sequences of different lengths in pages of one pool (``cake_b200_pages_*``): ``pages`` pages of ``page_size`` positions, up to
+    ``max_seqs`` sequences of up to ``max_seq`` positions.  A step brings new rows of some sequences: ``step`` plans it, then every block ``append``s its
+    rows and ``attend``s over them, on the calling thread's current stream, in order with the context's work; ``TextModelBase.forward_paged`` does all of it.
+    ``rotation``: (cos, sin), fp32 (max_seq, rotated entries / 2) on the context's device, instead of the context's tables."""
+
+    def __init__(self, ctx: "Context", pages: int, page_size: int = 64, max_seqs: int = 64, max_seq: Optional[int] = None,
+                 rotation: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+        self.ctx, self.pages, self.page_size, self.max_seqs = ctx, pages, page_size, max_seqs
+        self.max_seq = max_seq or ctx.max_seq
+        c = ctx.config
+        self._heads, self._kv, self._hd, self._dtype = c.num_attention_heads, c.num_key_value_heads, c.hd, ctx.torch_dtype
+        self._rows = 0   # of the present step
+        self.h = c_void_p()
+        self._lib = lib()
+        cos = sin = None
+        rot = 0
+        if rotation is not None:
+            cos, sin = rotation
+            if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < self.max_seq or not cos.shape[1]:
+                raise ValueError(f"rotation tables have shapes {list(cos.shape)} and {list(sin.shape)}, expected ({self.max_seq} or more, rotated entries / 2)")
+            for t in (cos, sin):
+                if t.dtype != torch.float32 or t.get_device() != ctx.device:
+                    raise ValueError(f"a rotation table is {t.dtype} on {t.device}, expected {torch.float32} on cuda:{ctx.device}")
+            cos, sin = cos.contiguous(), sin.contiguous()
+            rot = 2 * cos.shape[1]
+        self.rotation = (cos, sin)   # read by the library as long as the cache lives
+        check(self._lib.cake_b200_pages_create(ctx.h, pages, page_size, max_seqs, self.max_seq, ptr(cos), ptr(sin), rot, byref(self.h)))
+        ctx._children.append(weakref.ref(self))
+
+    def close(self):
+        if self.h:
+            self._lib.cake_b200_pages_free(self.h)
+            self.h = None
+
+    def add(self) -> int:
+        """A new sequence without positions."""
+        seq = ctypes.c_int()
+        check(self._lib.cake_b200_pages_add(self.h, byref(seq)))
+        return seq.value
+
+    def drop(self, seq: int) -> None:
+        """The sequence goes, its pages are free again; ends a step that it is part of."""
+        check(self._lib.cake_b200_pages_drop(self.h, seq))
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Back to the sequence's first ``length`` positions; ends a step that it is part of."""
+        check(self._lib.cake_b200_pages_truncate(self.h, seq, length))
+
+    def len(self, seq: int) -> int:
+        return self._lib.cake_b200_pages_len(self.h, seq)
+
+    @property
+    def available(self) -> int:
+        """Pages that no sequence has."""
+        return self._lib.cake_b200_pages_available(self.h)
+
+    def _stream(self) -> int:
+        return torch._C._cuda_getCurrentRawStream(self.ctx.device) or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's
+
+    def step(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
+        """The next step: counts[i] new rows of sequence seqs[i], packed in this order."""
+        if len(seqs) != len(counts):
+            raise ValueError(f"{len(seqs)} sequences and {len(counts)} counts")
+        check(self._lib.cake_b200_pages_step(self.h, int_array(seqs), int_array(counts), len(seqs), self._stream()))
+        self._rows = sum(counts)
+
+    def _in(self, t: torch.Tensor, name: str, heads: int) -> torch.Tensor:
+        """(rows, heads, hd) as the library takes them: heads side by side on 16-byte boundaries (copied where they are not)."""
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != self._rows or shape[1] != heads or shape[2] != self._hd:
+            raise ValueError(f"{name} has shape {list(shape)}, expected (the step's rows, heads, head_dim) = {[self._rows, heads, self._hd]}")
+        if t.dtype != self._dtype or t.get_device() != self.ctx.device:   # (-1: not on a GPU)
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self._dtype} on cuda:{self.ctx.device}")
+        st, sh, sd = t.stride()
+        if sd != 1 or (sh != self._hd and heads > 1) or st % 8 or t.data_ptr() % 16:
+            t = t.clone() if t.is_contiguous() else t.contiguous()
+        return t
+
+    def append(self, block_idx: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rotate: bool = True) -> Optional[torch.Tensor]:
+        """The step's rows k, v (rows, n_kv, head_dim) in D join the block's pages, k rotated by its position; the result is q (rows, n_heads, head_dim), rotated
+        likewise (None without q)."""
+        k, v = self._in(k, "k", self._kv), self._in(v, "v", self._kv)
+        out, at, tok = None, 0, 0
+        if q is not None:
+            q = self._in(q, "q", self._heads)
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            at, tok = q.data_ptr(), q.stride(0)
+        check(self._lib.cake_b200_pages_append(self.h, block_idx, at, tok, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                                               out.data_ptr() if at else 0, 1 if rotate else 0, self._stream()))
+        return out
+
+    def attend(self, block_idx: int, q: torch.Tensor, window: int = 0, scale: float = 0.0) -> torch.Tensor:
+        """Attention of the step's rows q (rows, n_heads, head_dim) in D over their sequences: a row at position p sees the positions up to p, with a window
+        only the last ``window`` of them.  scale 0: head_dim^-1/2.  (rows, n_heads, head_dim) in D."""
+        q = self._in(q, "q", self._heads)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        check(self._lib.cake_b200_pages_attend(self.h, block_idx, q.data_ptr(), q.stride(0), out.data_ptr(), window, scale, self._stream()))
+        return out
+
+    def read(self, block_idx: int, seq: Optional[int] = None, first: int = 0, n: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(K, V), each (rows, n_kv, head_dim) in D, as the block's pages hold them: the step's rows, or positions [first, first + n) (to the end without n)
+        of one sequence."""
+        if seq is None:
+            n = self._rows
+        elif n is None:
+            n = self.len(seq) - first
+        k, v = (torch.empty(max(n, 0), self._kv, self._hd, dtype=self._dtype, device=self.ctx.torch_device) for _ in range(2))
+        check(self._lib.cake_b200_pages_read(self.h, block_idx, -1 if seq is None else seq, first, n, k.data_ptr(), v.data_ptr(), self._stream()))
+        return k, v
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Context:
     """cake/mod.rs:41-65: shared state handed to Forwarder::load / forward."""
 
@@ -634,6 +752,29 @@ class TextModelBase:
         check(lib().cake_b200_logits(ctx.h, ptr(x), b, s, ptr(logits), None))
         return logits
 
+    def forward_paged(self, pages: PagedCache, requests: Sequence[Tuple[int, Sequence[int]]]) -> torch.Tensor:
+        """One step of many sequences: requests [(sequence of ``pages``, its next token ids)] -> logits (len(requests), vocab) of their last tokens, a device
+        tensor in D.  All blocks are local ones."""
+        ctx, L = self.ctx, lib()
+        run = self._local_run()
+        if run is None:
+            raise ValueError("forward_paged takes blocks of this process (B200Transformer)")
+        counts = [len(t) for _, t in requests]
+        ids = np.ascontiguousarray([i for _, t in requests for i in t], dtype=np.uint32)
+        n = len(ids)
+        with torch.cuda.stream(ctx.torch_stream):
+            if n and (ids >= ctx.config.vocab_size).any():   # in front of the step, which takes its pages
+                raise ValueError(f"token id {ids.max()} out of range (vocab {ctx.config.vocab_size})")
+            pages.step([s for s, _ in requests], counts)
+            x, y = (torch.empty(n, ctx.config.stream_width, dtype=ctx.stream_dtype, device=ctx.torch_device) for _ in range(2))
+            check(L.cake_b200_embed(ctx.h, ids.ctypes.data_as(ctypes.POINTER(c_uint32)), 1, n, ptr(x)))
+            check(L.cake_b200_forward_paged(ctx.h, run[0], run[1], run[2], pages.h, ptr(x), ptr(y), n))
+            if n > len(counts):   # the last row of each
+                y = y.index_select(0, torch.from_numpy(np.cumsum(counts) - 1).to(y.device))
+            logits = torch.empty(len(counts), ctx.config.vocab_size, dtype=ctx.logits_dtype, device=ctx.torch_device)
+            check(L.cake_b200_logits(ctx.h, ptr(y), len(counts), 1, ptr(logits), None))
+        return logits
+
     def _local_run(self):
         """All blocks as one run of this process: (handles, cache slots, count), or None where a block lives elsewhere, is of another make, or has a
         method of its own or a wrapped one (a tracer's) on its class or on itself, which then is to be asked."""
@@ -776,6 +917,43 @@ class Sessions:
         c = self.live.pop(rid, None)
         if c is not None:
             self.free.append(c)
+
+
+class PagedSessions:
+    """Requests that run together over ONE model: every step takes the next tokens of any of them, prompts and single tokens side by side, through the blocks
+    as one batch; their keys and values are pages of one pool."""
+
+    def __init__(self, model: TextModelBase, pages: int, page_size: int = 64, max_requests: int = 64, max_seq: Optional[int] = None):
+        self.model = model
+        self.cache = PagedCache(model.ctx, pages, page_size, max_requests, max_seq)
+        self.live: Dict[str, int] = {}
+
+    def step(self, tokens: Dict[str, Sequence[int]]) -> Dict[str, torch.Tensor]:
+        """{request: its next token ids} -> {request: logits (vocab) of the last of them}.  A request that is not live begins with these.  Where the pages do not
+        suffice (CakeB200Error, CAKE_B200_ENOMEM) nothing has happened: another request has to end, or fewer to go on."""
+        new = []
+        held = {rid: self.cache.len(self.live[rid]) for rid in tokens if rid in self.live}
+        try:
+            for rid in tokens:
+                if rid not in self.live:
+                    self.live[rid] = self.cache.add()
+                    new.append(rid)
+            logits = self.model.forward_paged(self.cache, [(self.live[rid], ids) for rid, ids in tokens.items()])
+        except BaseException:
+            for rid, n in held.items():
+                self.cache.truncate(self.live[rid], n)
+            for rid in new:
+                self.end(rid)
+            raise
+        return dict(zip(tokens, logits))
+
+    def len(self, rid: str) -> int:
+        return self.cache.len(self.live[rid]) if rid in self.live else 0
+
+    def end(self, rid: str) -> None:
+        seq = self.live.pop(rid, None)
+        if seq is not None:
+            self.cache.drop(seq)
 
 
 def sampling_from_args(temperature: float, top_k: Optional[int], top_p: Optional[float], seed: int) -> "capi.CSampling":

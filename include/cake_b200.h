@@ -56,6 +56,7 @@ extern "C" {
 
 typedef struct cake_b200_ctx cake_b200_ctx;     /* per (process, device): stream, workspaces, graphs, NCCL comm, head weights */
 typedef struct cake_b200_block cake_b200_block; /* immutable weights of one transformer layer */
+typedef struct cake_b200_pages cake_b200_pages; /* K and V rows of many sequences in pages of one pool */
 typedef struct cake_b200_cache cake_b200_cache; /* KV cache of one session (== reference Cache); RoPE tables live in the ctx */
 
 /* models/common/config.rs:87-150, the fields the dense Llama-family block reads */
@@ -418,6 +419,49 @@ int cake_b200_cache_unpack(cake_b200_cache *, int block_idx, int which, int firs
  * q_tok, q_batch: strides as above; out (batch, seq, n_heads, head_dim) contiguous; scale 0: head_dim^-1/2. */
 int cake_b200_cache_attend(cake_b200_cache *, int block_idx, const void *q_dev, size_t q_tok, size_t q_batch, void *out_dev, int seq, int index_pos,
                            int first, float scale, void *stream);
+
+/* ---- caches in pages ----------------------------------------------------------------------------
+ * K and V rows of many sequences of different lengths in pages of one pool: a page holds page_size consecutive positions (16, 32, .. 1024) of one sequence,
+ * for every block.  A sequence takes pages as it grows and gives them back when it is dropped or truncated.  Llama-family blocks with head_dim 64, 128 or
+ * 256 and rotated parts of a multiple of 16 entries.  The pool of a block (n_pages pages) is made at its first append.
+ * A STEP brings counts[i] new rows (1 or more) of each of some sequences, packed one sequence behind another in the order given: row r of a sequence that held
+ * n positions stands at position n + r.  cake_b200_pages_step plans it (pages are taken, lengths grow, tables go to the device) and then, for every
+ * block, _append puts the step's k and v into the pages and _attend attends over them; both may be repeated while the step stands, and every block of a
+ * sequence has to have the rows in front of a step's (CAKE_B200_ESTATE otherwise).  cake_b200_forward_paged does all of it for blocks.
+ * stream, as for caches in four bits: the cudaStream_t that the call's tensors belong to (cudaStreamLegacy for the default stream; NULL: the ctx's own), behind
+ * what the ctx's other calls have enqueued.  It may be capturing for _append, _attend and _read, once the same call has run outside a capture for a step of
+ * the same counts and the present step (CAKE_B200_ESTATE otherwise).  A graph then does the captured calls for whatever step stands when it is replayed: steps of other sequences
+ * and lengths, but the same counts in the same order; the step is planned in front of the replay, outside the graph, on the stream of the replay or before it.
+ * A replay for a step of other counts does nothing and makes the next call on the cache fail with CAKE_B200_ESTATE.  Whether a block that a graph appends
+ * to has its rows is its user's to know.  Graphs that share a cache are replayed neither at the same time nor beside its calls. */
+/* rot, cos_dev, sin_dev: rows [max_seq][rot / 2] fp32 in device memory, pairs (e, e + rot / 2), to rotate by instead of the ctx's tables; they stay the
+ * caller's and are read while the cache lives.  Both NULL: the ctx's (rot is not read). */
+int cake_b200_pages_create(cake_b200_ctx *, int n_pages, int page_size, int max_seqs, int max_seq, const float *cos_dev, const float *sin_dev, int rot,
+                           cake_b200_pages **out);
+void cake_b200_pages_free(cake_b200_pages *);
+int cake_b200_pages_add(cake_b200_pages *, int *seq);              /* a new sequence without positions; CAKE_B200_ESTATE when max_seqs are there */
+int cake_b200_pages_drop(cake_b200_pages *, int seq);
+int cake_b200_pages_truncate(cake_b200_pages *, int seq, int len); /* back to its first len positions; ends a step that it is part of */
+int cake_b200_pages_len(const cake_b200_pages *, int seq);         /* positions, the step's included, or < 0 */
+int cake_b200_pages_available(const cake_b200_pages *);            /* pages that no sequence has */
+/* CAKE_B200_ENOMEM where the free pages do not suffice, CAKE_B200_ESTATE beyond max_seq, CAKE_B200_EINVAL for a sequence that is not there or is there
+ * twice: nothing has changed then. */
+int cake_b200_pages_step(cake_b200_pages *, const int *seqs, const int *counts, int n, void *stream);
+/* Rows k, v (rows, n_kv, head_dim) and q (rows, n_heads, head_dim) in D, *_tok entries (a multiple of 8) from row to row, heads side by side, pointers on 16
+ * bytes.  k and v join the pages, k rotated by its position's row of the tables; q, rotated likewise, goes to q_out (rows, n_heads, head_dim) contiguous, which
+ * may be q where that is contiguous.  q and q_out NULL: keys and values alone.  rotate 0: all as they are.  Products and sums in fp32, one rounding to D. */
+int cake_b200_pages_append(cake_b200_pages *, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev, size_t v_tok,
+                           void *q_out, int rotate, void *stream);
+/* out (rows, n_heads, head_dim): softmax(scale q . k_j) weighted sum of v_j over the positions j of a row's sequence up to its own position p, with window > 0
+ * only p - window < j.  Scores, maxima and sums in fp32, weights as two operands of D (16 bits and more), one rounding to D; what a row does not see counts for
+ * nothing, infinities and NaN included.  scale 0: head_dim^-1/2. */
+int cake_b200_pages_attend(cake_b200_pages *, int block_idx, const void *q_dev, size_t q_tok, void *out_dev, int window, float scale, void *stream);
+/* Rows as the pages hold them -> k, v (rows, n_kv, head_dim), either may be NULL: the step's (seq < 0), or positions [first, first + n) of a sequence. */
+int cake_b200_pages_read(cake_b200_pages *, int block_idx, int seq, int first, int n, void *k_dev, void *v_dev, void *stream);
+/* == cake_b200_forward_batch over the step: x_dev, y_dev (n_rows, hidden) in D.  A block's sliding window is that of forward_batch: all of a sequence's rows see
+ * the last `window` positions that its last row does, and a first call everything. */
+int cake_b200_forward_paged(cake_b200_ctx *, cake_b200_block *const *blocks, const int *block_idx, int n_blocks, cake_b200_pages *, const void *x_dev,
+                            void *y_dev, int n_rows);
 
 /* ---- the block forward ------------------------------------------------------------------------ */
 /* == Forwarder::forward_batch over `n_blocks` consecutive local layers (n_blocks == 1 == forward).

@@ -8,6 +8,7 @@ use std::os::raw::{c_char, c_int, c_void};
 #[repr(C)] pub struct cake_b200_ctx { _p: [u8; 0] }
 #[repr(C)] pub struct cake_b200_block { _p: [u8; 0] }
 #[repr(C)] pub struct cake_b200_cache { _p: [u8; 0] }
+#[repr(C)] pub struct cake_b200_pages { _p: [u8; 0] }
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -96,6 +97,18 @@ extern "C" {
     pub fn cake_b200_cache_write(c: *mut cake_b200_cache, block_idx: c_int, k_dev: *const c_void, k_tok: usize, k_batch: usize, v_dev: *const c_void, v_tok: usize, v_batch: usize, seq: c_int, index_pos: c_int, stream: *mut c_void) -> c_int;
     pub fn cake_b200_cache_unpack(c: *mut cake_b200_cache, block_idx: c_int, which: c_int, first: c_int, n: c_int, out_dev: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn cake_b200_cache_attend(c: *mut cake_b200_cache, block_idx: c_int, q_dev: *const c_void, q_tok: usize, q_batch: usize, out_dev: *mut c_void, seq: c_int, index_pos: c_int, first: c_int, scale: f32, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_pages_create(c: *mut cake_b200_ctx, n_pages: c_int, page_size: c_int, max_seqs: c_int, max_seq: c_int, cos_dev: *const f32, sin_dev: *const f32, rot: c_int, out: *mut *mut cake_b200_pages) -> c_int;
+    pub fn cake_b200_pages_free(p: *mut cake_b200_pages);
+    pub fn cake_b200_pages_add(p: *mut cake_b200_pages, seq: *mut c_int) -> c_int;
+    pub fn cake_b200_pages_drop(p: *mut cake_b200_pages, seq: c_int) -> c_int;
+    pub fn cake_b200_pages_truncate(p: *mut cake_b200_pages, seq: c_int, len: c_int) -> c_int;
+    pub fn cake_b200_pages_len(p: *const cake_b200_pages, seq: c_int) -> c_int;
+    pub fn cake_b200_pages_available(p: *const cake_b200_pages) -> c_int;
+    pub fn cake_b200_pages_step(p: *mut cake_b200_pages, seqs: *const c_int, counts: *const c_int, n: c_int, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_pages_append(p: *mut cake_b200_pages, block_idx: c_int, q_dev: *const c_void, q_tok: usize, k_dev: *const c_void, k_tok: usize, v_dev: *const c_void, v_tok: usize, q_out: *mut c_void, rotate: c_int, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_pages_attend(p: *mut cake_b200_pages, block_idx: c_int, q_dev: *const c_void, q_tok: usize, out_dev: *mut c_void, window: c_int, scale: f32, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_pages_read(p: *mut cake_b200_pages, block_idx: c_int, seq: c_int, first: c_int, n: c_int, k_dev: *mut c_void, v_dev: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn cake_b200_forward_paged(c: *mut cake_b200_ctx, blocks: *const *mut cake_b200_block, block_idx: *const c_int, n_blocks: c_int, p: *mut cake_b200_pages, x_dev: *const c_void, y_dev: *mut c_void, n_rows: c_int) -> c_int;
     pub fn cake_b200_cache_fill_synthetic(c: *mut cake_b200_cache, block_idx: *const c_int, n_blocks: c_int, len: c_int, seed: u32) -> c_int;
     pub fn cake_b200_bench_kernel(ctx: *mut cake_b200_ctx, blocks: *const *mut cake_b200_block, block_idx: *const c_int,
         n_blocks: c_int, cache: *mut cake_b200_cache, which: c_int, reps: c_int, ms_per_launch: *mut f32) -> c_int;
