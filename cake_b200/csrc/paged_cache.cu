@@ -1,6 +1,6 @@
 // paged_cache.cu — kernels of the cache in pages (format and interface: paged_cache.cuh)
 #include "paged_cache.cuh"
-#include "common.cuh"
+#include "paged_few.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -26,17 +26,6 @@ static int launch(cudaStream_t s, uint64_t *launches, void (*kern)(KArgs...), di
 }
 template <typename T> struct Tag { typedef T type; };
 template <typename F> static int by_type(int dtype, F &&f) { return dtype == 1 ? f(Tag<__half>{}) : f(Tag<__nv_bfloat16>{}); }
-
-// whether this call is the present step's; a replayed call of another one does nothing
-__device__ __forceinline__ bool same_step(const Pool &p) {
-  if (__ldg(&p.step->shape) == p.shape) return true;
-  if (threadIdx.x == 0) *p.bad = 1;
-  return false;
-}
-__device__ __forceinline__ char *rows_of(const Pool &p, int page, int kvh, int which) {
-  return p.pages + ((size_t)page * p.n_kv + kvh) * (rows_bytes(p.hd, 2) << p.page_log2) + (which ? rows_bytes(p.hd, 1) << p.page_log2 : (size_t)0);
-}
-__device__ __forceinline__ int page_of(const Pool &p, int slot, int pos) { return __ldg(p.table + (size_t)slot * p.per_seq + (pos >> p.page_log2)); }
 
 // ------------------------------------------------------------------------------------------ a step's sequences and rows
 __global__ void __launch_bounds__(256) spread_kernel(const StepHead *step, int max_seqs, int n_seqs, int *table, int2 *rows) {
@@ -179,6 +168,8 @@ __global__ void __launch_bounds__(128) attend_kernel(const Pool p, const Attend 
   const int row = (int)(item / a.n_heads), head = (int)(item % a.n_heads), kvh = head / (a.n_heads / p.n_kv);
   const int2 at = a.rows[row];
   int lo = 0;
+  for (int i = 0; i < a.n_few; i++)
+    if (a.seqs[i].slot == at.x) return;
   if (a.win.w > 0 && !a.win.by_call) lo = max(0, at.y + 1 - a.win.w);
   if (a.win.w > 0 && a.win.by_call)
     for (int i = 0; i < p.step->n_seqs; i++)
@@ -202,15 +193,44 @@ __global__ void __launch_bounds__(128) attend_kernel(const Pool p, const Attend 
   }
   for (int e = 0; e < E; e++) reinterpret_cast<T *>(a.out)[((size_t)row * a.n_heads + head) * HD + lane * E + e] = DT<T>::from_f(o[e] / l);
 }
-int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, uint64_t *launches) {
-  const dim3 grid((unsigned)(((long)a.n_rows * a.n_heads + 3) / 4));
+int few_ctas(int hd, int sms) { return (hd == 256 ? 1 : 2) * sms; }
+size_t few_floats(int hd, int sms) { return (size_t)2 * few_ctas(hd, sms) * TOKEN_COLS * (hd + 2); }
+// f(T, HD): the instances of a kind of cache
+template <typename F> static int by_kind(int dtype, int hd, F &&f) {
   return by_type(dtype, [&](auto t) {
-    typedef typename decltype(t)::type T;
-    switch (p.hd) {
-      case 64: return launch(s, launches, attend_kernel<T, 64>, grid, dim3(128), 0, p, a);
-      case 128: return launch(s, launches, attend_kernel<T, 128>, grid, dim3(128), 0, p, a);
-      default: return launch(s, launches, attend_kernel<T, 256>, grid, dim3(128), 0, p, a);
+    switch (hd) {
+      case 64: return f(t, std::integral_constant<int, 64>{});
+      case 128: return f(t, std::integral_constant<int, 128>{});
+      default: return f(t, std::integral_constant<int, 256>{});
     }
+  });
+}
+int prepare(int dtype, int hd) {
+  return by_kind(dtype, hd, [&](auto t, auto h) {
+    typedef typename decltype(t)::type T;
+    constexpr int HD = decltype(h)::value;
+    cudaError_t e = cudaFuncSetAttribute(few_kernel<T, HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 1>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_kernel<T, HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 2>::SMEM);
+    return (int)e;
+  });
+}
+int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scratch &w, uint64_t *launches) {
+  if (a.n_few) {
+    const Few f{p, a.few, a.seqs, a.q, a.q_tok, a.out, w.ws, w.tickets, a.n_heads, a.n_heads / p.n_kv, a.win, a.scale * 1.4426950408889634f, a.err};
+    const int e = by_kind(dtype, p.hd, [&](auto t, auto h) {
+      typedef typename decltype(t)::type T;
+      constexpr int HD = decltype(h)::value;
+      const dim3 grid((unsigned)few_ctas(HD, w.sms)), block(FEW_THREADS);
+      if (a.few_cols <= 8) return launch(s, launches, few_kernel<T, HD, 1>, grid, block, FewCfg<HD, 1>::SMEM, f);
+      return launch(s, launches, few_kernel<T, HD, 2>, grid, block, FewCfg<HD, 2>::SMEM, f);
+    });
+    if (e) return e;
+  }
+  if (a.n_few == a.n_seqs) return 0;
+  return by_kind(dtype, p.hd, [&](auto t, auto h) {
+    typedef typename decltype(t)::type T;
+    constexpr int HD = decltype(h)::value;
+    return launch(s, launches, attend_kernel<T, HD>, dim3((unsigned)(((long)a.n_rows * a.n_heads + 3) / 4)), dim3(128), 0, p, a);
   });
 }
 

@@ -61,6 +61,17 @@ int append(cudaStream_t, int dtype, const Pool &, const Append &, int sms, uint6
 struct Read { const int2 *rows; int slot, first, n; void *k, *v; };
 int read(cudaStream_t, int dtype, const Pool &, const Read &, uint64_t *launches);
 
+// A step's attention as it is cut for one window (paged_plan.hpp), on the device: the head and the workers of the few-row kernel; what the calls on a cache
+// share: sums of runs and tiles that are cut, and how many of their parts have come (all zero between calls)
+struct FewHead { int W, T, pad[6]; };
+struct Scratch {
+  float *ws;          // few_floats
+  unsigned *tickets;  // [sequences][key heads]
+  int sms;
+};
+int few_ctas(int hd, int sms);             // CTAs of the few-row kernel: no more workers than that
+size_t few_floats(int hd, int sms);
+int prepare(int dtype, int hd);            // once per device and kind of cache, in front of the first call
 struct Attend {
   const int2 *rows;
   const void *q;
@@ -70,8 +81,11 @@ struct Attend {
   int n_rows, n_heads;
   float scale;
   Window win;
+  const FewHead *few;            // and its workers
+  int n_few, few_cols, n_seqs;   // sequences of few rows, query rows of a key head that they have at most; all sequences
+  int *err;
 };
-int attend(cudaStream_t, int dtype, const Pool &, const Attend &, uint64_t *launches);
+int attend(cudaStream_t, int dtype, const Pool &, const Attend &, const Scratch &, uint64_t *launches);
 
 }  // namespace pg
 }  // namespace cake

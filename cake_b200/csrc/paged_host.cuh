@@ -13,6 +13,16 @@ struct cake_b200_pages {
   std::vector<void *> pool;          // of each block: the pages and, behind them, their marks
   std::vector<std::vector<int>> len; // positions written, of each block and sequence
   std::vector<char> in_graph;        // a captured call writes this block's rows: how far, only its user knows
+  // how a step's attention is cut, for each window that calls have asked for
+  struct Plan {
+    pg::Window win;
+    unsigned long long step = 0, used = 0;   // made for this step; last used in this call
+    bool kept = false;                       // captured calls read it: it is made anew with every step
+    char *dev = nullptr;
+  } plans[8];
+  unsigned long long steps = 0, calls = 0;
+  float *ws = nullptr;
+  unsigned *tickets = nullptr;
   const float *cos_t = nullptr, *sin_t = nullptr;
   int rot = 0;
   int *bad = nullptr;                // pinned: a replayed call met a step of another shape
@@ -104,16 +114,19 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
   CU(cudaMallocHost(&g->bad, 4));
   *g->bad = 0;
+  CU((cudaError_t)pg::prepare(f.dtype, f.head_dim));
   const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
-               s_rows = (size_t)n_pages * page_size * 8;
+               s_tickets = (size_t)max_seqs * f.n_kv_heads * 4, s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   void *arena = nullptr;
-  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + s_rows, c->pc_pool, c->stream));
+  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_tickets) + up(s_ws) + s_rows, c->pc_pool, c->stream));
   g->arena = (char *)arena;
   g->step = (pg::StepHead *)g->arena;
   g->table = (int *)(g->arena + up(s_step));
-  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table));
-  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table), c->stream));
+  g->tickets = (unsigned *)(g->arena + up(s_step) + up(s_table));
+  g->ws = (float *)(g->arena + up(s_step) + up(s_table) + up(s_tickets));
+  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_tickets) + up(s_ws));
+  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table) + up(s_tickets), c->stream));
   c->pc_behind = true;
   guard.g = nullptr;
   *out = g;
@@ -131,6 +144,8 @@ extern "C" void cake_b200_pages_free(cake_b200_pages *g) {
     }
     for (void *p : g->pool)
       if (p) (void)(live ? cudaFreeAsync(p, g->ctx->stream) : cudaFree(p));
+    for (auto &p : g->plans)
+      if (p.dev) (void)(live ? cudaFreeAsync(p.dev, g->ctx->stream) : cudaFree(p.dev));
     if (g->arena) (void)(live ? cudaFreeAsync(g->arena, g->ctx->stream) : cudaFree(g->arena));
     if (live && cudaStreamSynchronize(g->ctx->stream) == cudaSuccess) (void)cudaMemPoolTrimTo(g->ctx->pc_pool, PC_POOL_KEEPS);
   }
@@ -164,6 +179,50 @@ extern "C" int cake_b200_pages_drop(cake_b200_pages *g, int seq) {
 extern "C" int cake_b200_pages_len(const cake_b200_pages *g, int seq) { return !g || !g->book.has(seq) ? -1 : g->book.seqs[(size_t)seq].len; }
 extern "C" int cake_b200_pages_available(const cake_b200_pages *g) { return g ? (int)g->book.free_pages.size() : -1; }
 
+static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // on the ctx's stream of the moment
+  cake_b200_ctx *c = g->ctx;
+  const int n_kv = c->cfg.n_kv_heads, hd = c->cfg.head_dim;
+  const int most = pg::few_ctas(hd, c->sm_count);
+  std::vector<pg::Worker> few;
+  pg::FewHead h{};
+  h.T = g->book.cut_few(p->win, n_kv, most, &few);
+  h.W = (int)few.size();
+  std::vector<char> blob(sizeof h + few.size() * sizeof(pg::Worker));
+  memcpy(blob.data(), &h, sizeof h);
+  if (!few.empty()) memcpy(blob.data() + sizeof h, few.data(), few.size() * sizeof(pg::Worker));
+  RC(pages_upload(c, p->dev, blob.data(), blob.size()));
+  p->step = g->steps;
+  return CAKE_B200_OK;
+}
+static int pages_plan(cake_b200_pages *g, const pg::Window &win, const cake_b200_pages::Plan **out) {
+  cake_b200_ctx *c = g->ctx;
+  const bool capturing = is_capturing(c->stream);
+  cake_b200_pages::Plan *p = nullptr;
+  for (auto &x : g->plans)
+    if (x.dev && x.win.w == win.w && x.win.by_call == win.by_call) p = &x;
+  if (!p) {
+    RC(no_capture(c->stream, "the plan of attention with this window"));
+    for (auto &x : g->plans)
+      if (!x.kept && (!p || x.used < p->used)) p = &x;
+    if (!p) return fail(CAKE_B200_EINVAL, "captured calls have used %d windows: there is room for no other", (int)(sizeof g->plans / sizeof g->plans[0]));
+    if (!p->dev) {
+      void *m = nullptr;
+      CU(cudaMallocFromPoolAsync(&m, sizeof(pg::FewHead) + (size_t)pg::few_ctas(c->cfg.head_dim, c->sm_count) * sizeof(pg::Worker), c->pc_pool, c->stream));
+      p->dev = (char *)m;
+    }
+    p->win = win;
+    p->step = 0;
+  }
+  p->used = ++g->calls;
+  if (p->step != g->steps) {
+    RC(no_capture(c->stream, "this step's plan of attention"));
+    RC(pages_plan_make(g, p));
+  }
+  p->kept = p->kept || capturing;
+  *out = p;
+  return CAKE_B200_OK;
+}
+
 extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const int *counts, int n, void *stream) {
   RC(pages_call(g, "pages_step"));
   if (!seqs || !counts || n < 1) return fail(CAKE_B200_EINVAL, "null/empty argument");
@@ -193,6 +252,9 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
     int most = 1;
     for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
     CU((cudaError_t)pg::spread(c->stream, g->step, k.max_seqs, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
+    g->steps++;
+    for (auto &p : g->plans)
+      if (p.kept) RC(pages_plan_make(g, &p));
     return CAKE_B200_OK;
   });
 }
@@ -240,8 +302,13 @@ static int pages_append_on(cake_b200_pages *g, int l, const pg::Append &a) {   /
 }
 static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_tok, void *out, const pg::Window &win, float scale) {
   cake_b200_ctx *c = g->ctx;
-  const pg::Attend a{g->rows, q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), g->book.n_rows, c->cfg.n_heads, scale, win};
-  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, launch_counter(c)));
+  const cake_b200_pages::Plan *plan = nullptr;
+  RC(pages_plan(g, win, &plan));
+  int cols = 0;
+  for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
+  const pg::Attend a{g->rows, q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), g->book.n_rows, c->cfg.n_heads, scale, win,
+                     (const pg::FewHead *)plan->dev, g->book.n_few, cols, (int)g->book.step.size(), c->wait_err};
+  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->ws, g->tickets, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,
