@@ -48,7 +48,7 @@ UNITS = {
     "mixers_window.o": ("mixers_window.cu", ("mixers.cuh", "common.cuh")),
     "mixers_streams.o": ("mixers_streams.cu", ("mixers.cuh", "common.cuh")),
     "packed_cache.o": ("packed_cache.cu", ("packed_cache.cuh", "common.cuh")),
-    "paged_cache.o": ("paged_cache.cu", ("paged_cache.cuh", "paged_plan.hpp", "paged_few.cuh", "gemm_tc.cuh", "attn_prefill_tc.cuh", "common.cuh")),
+    "paged_cache.o": ("paged_cache.cu", ("paged_cache.cuh", "paged_plan.hpp", "paged_few.cuh", "paged_tiles.cuh", "gemm_tc.cuh", "attn_prefill_tc.cuh", "common.cuh")),
 }
 
 

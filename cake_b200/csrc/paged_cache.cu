@@ -1,6 +1,7 @@
 // paged_cache.cu — kernels of the cache in pages (format and interface: paged_cache.cuh)
 #include "paged_cache.cuh"
 #include "paged_few.cuh"
+#include "paged_tiles.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -156,44 +157,9 @@ int read(cudaStream_t s, int, const Pool &p, const Read &a, uint64_t *launches) 
 }
 
 // ------------------------------------------------------------------------------------------ attention
-// A warp per row and head, a key after the other.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) attend_kernel(const Pool p, const Attend a) {
-  pdl_launch_dependents();
-  constexpr int E = HD / 32;   // entries of a lane: E lane .. E lane + E - 1
-  const int lane = threadIdx.x & 31;
-  const long item = blockIdx.x * 4l + (threadIdx.x >> 5);
-  pdl_wait();
-  if (!same_step(p) || item >= (long)a.n_rows * a.n_heads) return;
-  const int row = (int)(item / a.n_heads), head = (int)(item % a.n_heads), kvh = head / (a.n_heads / p.n_kv);
-  const int2 at = a.rows[row];
-  int lo = 0;
-  for (int i = 0; i < a.n_few; i++)
-    if (a.seqs[i].slot == at.x) return;
-  if (a.win.w > 0 && !a.win.by_call) lo = max(0, at.y + 1 - a.win.w);
-  if (a.win.w > 0 && a.win.by_call)
-    for (int i = 0; i < p.step->n_seqs; i++)
-      if (a.seqs[i].slot == at.x) lo = a.seqs[i].pos0 > 0 ? max(0, a.seqs[i].pos0 + a.seqs[i].count - a.win.w) : 0;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; e++) {
-    q[e] = DT<T>::to_f(reinterpret_cast<const T *>(a.q)[(size_t)row * a.q_tok + head * HD + lane * E + e]) * a.scale * 1.4426950408889634f;
-    o[e] = 0.f;
-  }
-  const int c = lane * E / 8, e0 = lane * E % 8;
-  for (int j = lo; j <= at.y; j++) {
-    const int page = page_of(p, at.x, j), r = j & ((1 << p.page_log2) - 1);
-    const T *k = reinterpret_cast<const T *>(rows_of(p, page, kvh, 0) + chunk_at(HD, r, c)) + e0, *v = reinterpret_cast<const T *>(rows_of(p, page, kvh, 1) + chunk_at(HD, r, c)) + e0;
-    float s = 0.f;
-    for (int e = 0; e < E; e++) s += q[e] * DT<T>::to_f(k[e]);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), f = m == mn ? 1.f : exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = l * f + w;
-    for (int e = 0; e < E; e++) o[e] = o[e] * f + w * DT<T>::to_f(v[e]);
-  }
-  for (int e = 0; e < E; e++) reinterpret_cast<T *>(a.out)[((size_t)row * a.n_heads + head) * HD + lane * E + e] = DT<T>::from_f(o[e] / l);
-}
 int few_ctas(int hd, int sms) { return (hd == 256 ? 1 : 2) * sms; }
+int room(int hd, int sms, int n_kv) { return std::max(1, (hd == 256 ? 1 : 2) * sms / n_kv); }
+size_t tiles_floats(int hd, int sms, int n_kv) { return (size_t)room(hd, sms, n_kv) * n_kv * TILE_ROWS * (hd + 2); }
 size_t few_floats(int hd, int sms) { return (size_t)2 * few_ctas(hd, sms) * TOKEN_COLS * (hd + 2); }
 // f(T, HD): the instances of a kind of cache
 template <typename F> static int by_kind(int dtype, int hd, F &&f) {
@@ -211,12 +177,15 @@ int prepare(int dtype, int hd) {
     constexpr int HD = decltype(h)::value;
     cudaError_t e = cudaFuncSetAttribute(few_kernel<T, HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 1>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(few_kernel<T, HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 2>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tiles_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<HD>::SMEM);
     return (int)e;
   });
 }
 int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scratch &w, uint64_t *launches) {
+  const int G = a.n_heads / p.n_kv;
+  const float scale_log2 = a.scale * 1.4426950408889634f;
   if (a.n_few) {
-    const Few f{p, a.few, a.seqs, a.q, a.q_tok, a.out, w.ws, w.tickets, a.n_heads, a.n_heads / p.n_kv, a.win, a.scale * 1.4426950408889634f, a.err};
+    const Few f{p, a.plan, a.seqs, a.q, a.q_tok, a.out, w.few_ws, w.tickets, a.n_heads, G, a.win, scale_log2, a.err, a.n_items ? 1 : 0};
     const int e = by_kind(dtype, p.hd, [&](auto t, auto h) {
       typedef typename decltype(t)::type T;
       constexpr int HD = decltype(h)::value;
@@ -226,11 +195,14 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
     });
     if (e) return e;
   }
-  if (a.n_few == a.n_seqs) return 0;
+  if (!a.n_items) return 0;
+  const Item *items = reinterpret_cast<const Item *>(reinterpret_cast<const Worker *>(a.plan + 1) + few_ctas(p.hd, w.sms));
+  const Tiles t8{p, a.plan, items, a.q, a.q_tok, a.out, w.tiles_ws, w.tickets + (size_t)w.max_seqs * p.n_kv, a.n_heads, G, TILE_ROWS / G, a.win, scale_log2, 8.f, a.err,
+                 a.n_few ? 1 : 0};
   return by_kind(dtype, p.hd, [&](auto t, auto h) {
     typedef typename decltype(t)::type T;
     constexpr int HD = decltype(h)::value;
-    return launch(s, launches, attend_kernel<T, HD>, dim3((unsigned)(((long)a.n_rows * a.n_heads + 3) / 4)), dim3(128), 0, p, a);
+    return launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, t8);
   });
 }
 

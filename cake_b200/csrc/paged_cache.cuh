@@ -61,28 +61,30 @@ int append(cudaStream_t, int dtype, const Pool &, const Append &, int sms, uint6
 struct Read { const int2 *rows; int slot, first, n; void *k, *v; };
 int read(cudaStream_t, int dtype, const Pool &, const Read &, uint64_t *launches);
 
-// A step's attention as it is cut for one window (paged_plan.hpp), on the device: the head and the workers of the few-row kernel; what the calls on a cache
-// share: sums of runs and tiles that are cut, and how many of their parts have come (all zero between calls)
-struct FewHead { int W, T, pad[6]; };
+// A step's attention as it is cut for one window (paged_plan.hpp), on the device: this head, few_ctas workers of the few-row kernel, the items of the many-row
+// kernel.  What the calls on a cache share: sums of runs and tiles that are cut, and how many of their parts have come (all zero between calls)
+struct PlanHead { int W, T, n_items, parts, pad[4]; };   // workers, tiles of their line; items, parts of those that are cut
 struct Scratch {
-  float *ws;          // few_floats
-  unsigned *tickets;  // [sequences][key heads]
-  int sms;
+  float *few_ws, *tiles_ws;      // few_floats; tiles_floats (nullptr: the step has no sequence of many rows)
+  unsigned *tickets;             // [sequences][key heads], then [room][key heads]
+  int max_seqs, sms;
 };
 int few_ctas(int hd, int sms);             // CTAs of the few-row kernel: no more workers than that
+int room(int hd, int sms, int n_kv);       // items of the many-row kernel that fill the chip, and parts of cut ones at most
 size_t few_floats(int hd, int sms);
+size_t tiles_floats(int hd, int sms, int n_kv);
 int prepare(int dtype, int hd);            // once per device and kind of cache, in front of the first call
 struct Attend {
-  const int2 *rows;
   const void *q;
-  long long q_tok;
-  void *out;                     // [n_rows, n_heads, hd]
+  long long q_tok;               // multiple of 8
+  void *out;                     // [rows, n_heads, hd]
   const SeqRow *seqs;
-  int n_rows, n_heads;
+  int n_heads;
   float scale;
   Window win;
-  const FewHead *few;            // and its workers
-  int n_few, few_cols, n_seqs;   // sequences of few rows, query rows of a key head that they have at most; all sequences
+  const PlanHead *plan;
+  int n_few, few_cols;           // sequences of few rows, query rows of a key head that they have at most
+  int n_items;                   // of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
   int *err;
 };
 int attend(cudaStream_t, int dtype, const Pool &, const Attend &, const Scratch &, uint64_t *launches);

@@ -40,7 +40,7 @@ __device__ __forceinline__ int page_of(const Pool &p, int slot, int pos) { retur
 
 struct Few {
   Pool pool;
-  const FewHead *plan;
+  const PlanHead *plan;
   const SeqRow *seqs;
   const void *q;
   long long q_tok;
@@ -51,6 +51,7 @@ struct Few {
   Window win;
   float scale_log2;
   int *err;
+  int beside;           // the many-row kernel runs beside this one: it may start when this one has waited for what both read
 };
 
 __device__ __forceinline__ void ldm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -137,6 +138,10 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
     mbar_fence_init();
   }
   __syncthreads();
+  if (a.beside) {
+    pdl_wait();
+    __syncthreads();
+  }
   pdl_launch_dependents();
   if (!same_step(a.pool) || (int)blockIdx.x >= a.plan->W) {   // (nothing in flight, no barrier ahead of anybody)
     pdl_wait();

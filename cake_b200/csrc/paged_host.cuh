@@ -18,10 +18,11 @@ struct cake_b200_pages {
     pg::Window win;
     unsigned long long step = 0, used = 0;   // made for this step; last used in this call
     bool kept = false;                       // captured calls read it: it is made anew with every step
+    int n_items = 0, most_items = 0;         // of the many-row kernel, now and for any lengths of this shape
     char *dev = nullptr;
   } plans[8];
   unsigned long long steps = 0, calls = 0;
-  float *ws = nullptr;
+  float *few_ws = nullptr, *tiles_ws = nullptr;
   unsigned *tickets = nullptr;
   const float *cos_t = nullptr, *sin_t = nullptr;
   int rot = 0;
@@ -116,7 +117,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   *g->bad = 0;
   CU((cudaError_t)pg::prepare(f.dtype, f.head_dim));
   const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
-               s_tickets = (size_t)max_seqs * f.n_kv_heads * 4, s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
+               s_tickets = ((size_t)max_seqs + pg::room(f.head_dim, c->sm_count, f.n_kv_heads)) * f.n_kv_heads * 4, s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   void *arena = nullptr;
   CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_tickets) + up(s_ws) + s_rows, c->pc_pool, c->stream));
@@ -124,7 +125,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   g->step = (pg::StepHead *)g->arena;
   g->table = (int *)(g->arena + up(s_step));
   g->tickets = (unsigned *)(g->arena + up(s_step) + up(s_table));
-  g->ws = (float *)(g->arena + up(s_step) + up(s_table) + up(s_tickets));
+  g->few_ws = (float *)(g->arena + up(s_step) + up(s_table) + up(s_tickets));
   g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_tickets) + up(s_ws));
   CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table) + up(s_tickets), c->stream));
   c->pc_behind = true;
@@ -146,6 +147,7 @@ extern "C" void cake_b200_pages_free(cake_b200_pages *g) {
       if (p) (void)(live ? cudaFreeAsync(p, g->ctx->stream) : cudaFree(p));
     for (auto &p : g->plans)
       if (p.dev) (void)(live ? cudaFreeAsync(p.dev, g->ctx->stream) : cudaFree(p.dev));
+    if (g->tiles_ws) (void)(live ? cudaFreeAsync(g->tiles_ws, g->ctx->stream) : cudaFree(g->tiles_ws));
     if (g->arena) (void)(live ? cudaFreeAsync(g->arena, g->ctx->stream) : cudaFree(g->arena));
     if (live && cudaStreamSynchronize(g->ctx->stream) == cudaSuccess) (void)cudaMemPoolTrimTo(g->ctx->pc_pool, PC_POOL_KEEPS);
   }
@@ -179,18 +181,37 @@ extern "C" int cake_b200_pages_drop(cake_b200_pages *g, int seq) {
 extern "C" int cake_b200_pages_len(const cake_b200_pages *g, int seq) { return !g || !g->book.has(seq) ? -1 : g->book.seqs[(size_t)seq].len; }
 extern "C" int cake_b200_pages_available(const cake_b200_pages *g) { return g ? (int)g->book.free_pages.size() : -1; }
 
+static size_t pages_plan_bytes(const cake_b200_pages *g) {
+  const cake_b200_config &f = g->ctx->cfg;
+  const int sms = g->ctx->sm_count;
+  return sizeof(pg::PlanHead) + (size_t)pg::few_ctas(f.head_dim, sms) * sizeof(pg::Worker) +
+         pg::Book::most_items((long long)g->book.n_pages * g->book.page, g->book.max_seqs, f.n_heads / f.n_kv_heads, pg::room(f.head_dim, sms, f.n_kv_heads)) * sizeof(pg::Item);
+}
 static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // on the ctx's stream of the moment
   cake_b200_ctx *c = g->ctx;
-  const int n_kv = c->cfg.n_kv_heads, hd = c->cfg.head_dim;
-  const int most = pg::few_ctas(hd, c->sm_count);
+  const int n_kv = c->cfg.n_kv_heads, hd = c->cfg.head_dim, G = c->cfg.n_heads / n_kv, room = pg::room(hd, c->sm_count, n_kv);
+  const size_t most = (size_t)pg::few_ctas(hd, c->sm_count);
   std::vector<pg::Worker> few;
-  pg::FewHead h{};
-  h.T = g->book.cut_few(p->win, n_kv, most, &few);
+  std::vector<pg::Item> many;
+  pg::PlanHead h{};
+  h.T = g->book.cut_few(p->win, n_kv, (int)most, &few);
   h.W = (int)few.size();
-  std::vector<char> blob(sizeof h + few.size() * sizeof(pg::Worker));
+  h.parts = g->book.cut_many(p->win, G, room, &many);
+  h.n_items = (int)many.size();
+  if (h.n_items && !g->tiles_ws) {
+    void *m = nullptr;
+    CU(cudaMallocFromPoolAsync(&m, pg::tiles_floats(hd, c->sm_count, n_kv) * 4, c->pc_pool, c->stream));
+    g->tiles_ws = (float *)m;
+  }
+  std::vector<char> blob(sizeof h + (many.empty() ? few.size() : most) * sizeof(pg::Worker) + many.size() * sizeof(pg::Item));
   memcpy(blob.data(), &h, sizeof h);
   if (!few.empty()) memcpy(blob.data() + sizeof h, few.data(), few.size() * sizeof(pg::Worker));
+  if (!many.empty()) memcpy(blob.data() + sizeof h + most * sizeof(pg::Worker), many.data(), many.size() * sizeof(pg::Item));
   RC(pages_upload(c, p->dev, blob.data(), blob.size()));
+  int tiles = 0;
+  for (size_t i = 0; i < many.size(); i++) tiles += many[i].part == 0;
+  p->n_items = h.n_items;
+  p->most_items = tiles ? std::max(tiles, room) : 0;
   p->step = g->steps;
   return CAKE_B200_OK;
 }
@@ -207,7 +228,7 @@ static int pages_plan(cake_b200_pages *g, const pg::Window &win, const cake_b200
     if (!p) return fail(CAKE_B200_EINVAL, "captured calls have used %d windows: there is room for no other", (int)(sizeof g->plans / sizeof g->plans[0]));
     if (!p->dev) {
       void *m = nullptr;
-      CU(cudaMallocFromPoolAsync(&m, sizeof(pg::FewHead) + (size_t)pg::few_ctas(c->cfg.head_dim, c->sm_count) * sizeof(pg::Worker), c->pc_pool, c->stream));
+      CU(cudaMallocFromPoolAsync(&m, pages_plan_bytes(g), c->pc_pool, c->stream));
       p->dev = (char *)m;
     }
     p->win = win;
@@ -306,9 +327,9 @@ static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_to
   RC(pages_plan(g, win, &plan));
   int cols = 0;
   for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
-  const pg::Attend a{g->rows, q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), g->book.n_rows, c->cfg.n_heads, scale, win,
-                     (const pg::FewHead *)plan->dev, g->book.n_few, cols, (int)g->book.step.size(), c->wait_err};
-  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->ws, g->tickets, c->sm_count}, launch_counter(c)));
+  const pg::Attend a{q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), c->cfg.n_heads, scale, win, (const pg::PlanHead *)plan->dev, g->book.n_few, cols,
+                     is_capturing(c->stream) ? plan->most_items : plan->n_items, c->wait_err};
+  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, g->tickets, g->book.max_seqs, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,

@@ -1,0 +1,419 @@
+// paged_tiles.cuh — attention of many rows a sequence over a cache in pages (portions of prompts, prompts), on tcgen05
+//
+// The same division of work as attn_prefill_tc.cuh: 128 query rows (the G heads of a key head x 128 / G tokens) a CTA, softmax in warps 0-3 with a thread a
+// row, warp 4 copies, warp 5 multiplies; S in fp32 in TMEM, P as two operands of D (16 bits and more) over the S that it came from, O in TMEM, rescaled where a
+// maximum grew by more than tau.  Bound by the softmax's exponentials and conversions, then the products (6 hd operations a pair instead of 4: P V twice).
+// What is different:
+//   - keys and values come page by page as they lie: a page's groups of eight rows are the operands' own layout, so that bulk copies without a tensor map fill
+//     a tile from pages of any size, and Q is laid out by the softmax warps (no map to encode, any stride)
+//   - a CTA's sequence, tokens and keys stand in a list (paged_plan.hpp, cut_many): sequences of any lengths side by side, the tiles with the most keys first, and
+//     keys cut into parts where the tiles do not fill the chip; the parts are joined by whichever CTA comes last, in their order
+//   - only whole sixteens of positions that hold a visible one are multiplied; where a page is marked (an infinity or a NaN in its values) a row sums what it sees by itself
+#pragma once
+#include "attn_prefill_tc.cuh"
+#include "paged_few.cuh"
+
+namespace cake {
+namespace pg {
+
+template <int HD> struct TileCfg {
+  static constexpr int Q_BYTES = TILE_ROWS * HD * 2, KV_BYTES = TILE * HD * 2;
+  static constexpr int BARS = 14, SMEM = Q_BYTES + 4 * KV_BYTES + 1024 + BARS * 8 + 32;
+  static constexpr int TMEM = HD == 256 ? 512 : 256;   // S and P: columns 0 .. 63 and 64 .. 127; O from 128
+  static constexpr int CTAS = HD == 256 ? 1 : 2;
+  static constexpr size_t PART = (size_t)TILE_ROWS * (HD + 2);   // floats of a part: O as [HD / 4][row][4], then (m, l) of the rows
+};
+struct Tiles {
+  Pool pool;
+  const PlanHead *plan;
+  const Item *items;
+  const void *q;
+  long long q_tok;
+  void *out;
+  float *ws;             // [key head][parts][PART]
+  unsigned *tickets;     // [parts][key head], zero between calls
+  int n_heads, G, tpt;
+  Window win;
+  float scale_log2, tau_log2;
+  int *err;
+  int beside;            // the few-row kernel in front of this one waited for what both read: this one waits for it at its end
+};
+
+__device__ __forceinline__ float tc_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  return __uint_as_float(r);
+}
+// an operand whose groups of eight rows lie `group` bytes apart and whose 64-entry ranges 1 KB: K-major (keys), and MN-major (values)
+__device__ __forceinline__ uint64_t desc_keys(const void *tile, uint32_t group) {
+  return (uint64_t)((smem_u32(tile) & 0x3ffff) >> 4) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_values(const void *tile, uint32_t group) {
+  return (uint64_t)((smem_u32(tile) & 0x3ffff) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(const Tiles a) {
+  typedef TileCfg<HD> C;
+  constexpr uint32_t GROUP = HD / 64 * 1024;
+  extern __shared__ unsigned char tiles_smem[];
+  unsigned char *q_s = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(tiles_smem) + 1023) & ~(uintptr_t)1023);
+  unsigned char *k_s = q_s + C::Q_BYTES, *v_s = k_s + 2 * C::KV_BYTES;   // two stages each
+  uint64_t *bars = reinterpret_cast<uint64_t *>(v_s + 2 * C::KV_BYTES);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 12;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + C::BARS);
+  int *gave_up = reinterpret_cast<int *>(tmem_ptr + 1), *last_come = gave_up + 1;
+  volatile uint32_t *marked = tmem_ptr + 4;   // of tiles j, j + 1 .. j + 3: a slot is written again when the tile two in front of it has been multiplied
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = (int)blockIdx.x % a.pool.n_kv, nth = (int)blockIdx.x / a.pool.n_kv;
+  if (!same_step(a.pool) || nth >= a.plan->n_items) {
+    pdl_wait();
+    return;
+  }
+  Item it;
+  {
+    const int4 *x = reinterpret_cast<const int4 *>(a.items + nth);
+    const int4 u = __ldg(x), v = __ldg(x + 1), w = __ldg(x + 2);
+    it = Item{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w, SeqRow{w.x, w.y, w.z, w.w}};
+  }
+  const int G = a.G, n_tok = min(a.tpt, it.s.count - it.tok0), rows = G * n_tok, n_tiles = it.t1 - it.t0;
+  const int p0 = it.s.pos0 + it.tok0, kv_end = p0 + n_tok;   // the first token's position; keys that the last one sees
+  const int row = (warp & 3) * 32 + lane, tok = row / G;
+  const int by_call = a.win.w > 0 && a.win.by_call ? dev_first(it.s, a.win) : 0;
+  const int late = a.win.w <= 0 ? 0 : a.win.by_call ? by_call : max(0, kv_end - a.win.w);   // what the last token begins at
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::BARS; i++) mbar_init(&bars[i], i == 11 || i == 0 ? 128u : 1u);
+    *gave_up = 0;
+    mbar_fence_init();
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_ptr)), "n"(C::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem_base = *tmem_ptr, tmem_o = tmem_base + 128u, lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+  const bool busy = warp < 4 && warp * 32 < rows;
+  float m_run = -INFINITY, l_run = 0.f;
+  int left = MBAR_TRIES, k_loads = 0, v_loads = 0;
+
+  if (warp == 4) {
+    // ---- copies.  A lane has one piece (a page, or 64 rows of one) of a batch of tiles
+    const int P = 1 << a.pool.page_log2, pr = min(P, TILE), ppt = TILE / pr, most = 32 / ppt, piece = lane % ppt;
+    const size_t head_bytes = rows_bytes(HD, 2 * P);
+    auto look = [&](int j, int n) -> int { return lane < n * ppt ? page_of(a.pool, it.s.slot, min((it.t0 + j + lane / ppt) * TILE + piece * pr, kv_end - 1)) : 0; };
+    int n = min(n_tiles, most), page = look(0, n);
+    if (!a.beside) pdl_wait();
+    for (int j0 = 0; j0 < n_tiles; j0 += most) {
+      const uint32_t mark = lane < n * ppt ? __ldcg(a.pool.marks + (size_t)page * a.pool.n_kv + kvh) : 0u;
+      const int nn = min(max(0, n_tiles - j0 - most), most), npage = look(j0 + most, nn);
+      const char *src = a.pool.pages + ((size_t)page * a.pool.n_kv + kvh) * head_bytes;
+      auto copy = [&](int t, bool values) {
+        const int j = j0 + t, st = j & 1, at = (it.t0 + j) * TILE, mine = at + piece * pr;
+        uint64_t *full = values ? &v_full[st] : &k_full[st];
+        if (j >= 2) {
+          mbar_wait_lim(values ? &v_empty[st] : &k_empty[st], (uint32_t)((j >> 1) - 1) & 1u, a.err, left);
+          if (__any_sync(0xffffffffu, left == 0)) left = 0;
+        }
+        const int of_tile = min(TILE, (kv_end - at + 15) & ~15), of_piece = min(pr, max(0, (kv_end - mine + 15) & ~15));
+        if (left && lane == 0) mbar_expect_tx(full, (uint32_t)rows_bytes(HD, of_tile));
+        __syncwarp();
+        if (left && of_piece > 0 && lane / ppt == t)
+          bulk_copy((values ? v_s : k_s) + st * C::KV_BYTES + rows_bytes(HD, piece * pr), src + rows_bytes(HD, (mine & (P - 1)) + (values ? P : 0)), (uint32_t)rows_bytes(HD, of_piece), full);
+        (values ? v_loads : k_loads)++;
+      };
+      auto arrive = [&](int t) {
+        const uint32_t any = __ballot_sync(0xffffffffu, mark != 0u && lane / ppt == t);
+        if (lane == 0) {
+          marked[(j0 + t) & 3] = any;
+          mbar_arrive(&k_full[(j0 + t) & 1]);
+        }
+      };
+      int t = 0;
+      if (j0 == 0) {   // nothing in the stages yet: the copies first
+        for (; t < min(n, 2); t++) {
+          copy(t, false);
+          copy(t, true);
+        }
+        for (int i = 0; i < t; i++) {
+          arrive(i);
+          if (lane == 0) mbar_arrive(&v_full[i]);
+        }
+      }
+      for (; t < n; t++) {
+        copy(t, false);
+        arrive(t);
+        copy(t, true);
+        if (lane == 0) mbar_arrive(&v_full[(j0 + t) & 1]);
+      }
+      n = nn; page = npage;
+    }
+  } else if (warp == 5) {
+    // ---- products (one thread issues them; the warp runs the loop with it)
+    const uint32_t one = elect_one();
+    const uint32_t idesc_s = tc_idesc<T>(TILE), idesc_o = tc_idesc<T>(HD) | (1u << 16);   // M128 N64, both K-major; M128 N hd, A from TMEM, B (V) MN-major
+    auto issue_s = [&](int j) {   // S_j = Q K_j^T into S buffer j & 1
+      const int st = j & 1;
+      mbar_wait_lim(&k_full[st], (uint32_t)(j >> 1) & 1u, a.err, left);
+      __syncwarp();
+      tc_fence_after();
+      const uint64_t q0 = tc_smem_desc(q_s), kt = desc_keys(k_s, GROUP) + (uint64_t)(st * (C::KV_BYTES >> 4));
+      if (one) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; k++)
+          tc_mma_f16(tmem_base + (uint32_t)(st * 64), q0 + (uint64_t)((k >> 2) * (TILE_ROWS * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((k >> 2) * (1024 >> 4) + (k & 3) * 2), idesc_s,
+                     k ? 1u : 0u);
+        tc_commit(&k_empty[st], left);
+        tc_commit(&s_full[st], left);
+      }
+      __syncwarp();
+    };
+    mbar_wait_lim(q_full, 0, a.err, left);
+    __syncwarp();
+    issue_s(0);
+    for (int j = 0; j < n_tiles; j++) {
+      const int st = j & 1;
+      if (j + 1 < n_tiles) issue_s(j + 1);   // (its buffer held P of tile j - 1, whose P V is in front of it in the pipe)
+      mbar_wait_lim(p_full, (uint32_t)j & 1u, a.err, left);
+      mbar_wait_lim(&v_full[st], (uint32_t)(j >> 1) & 1u, a.err, left);
+      __syncwarp();
+      tc_fence_after();
+      const uint64_t vt = desc_values(v_s, GROUP) + (uint64_t)(st * (C::KV_BYTES >> 4));
+      const int steps = marked[j & 3] ? 0 : min(TILE, (kv_end - (it.t0 + j) * TILE + 15) & ~15) / 16;   // sixteens of positions; marked: the rows have summed by themselves
+      if (one) {
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+          for (int ks = 0; ks < TILE / 16; ks++)
+            if (ks < steps)
+              tc_mma_f16_ts(tmem_o, tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8), vt + (uint64_t)(ks * (2 * GROUP >> 4)), idesc_o, (j | half | ks) ? 1u : 0u);
+        tc_commit(&v_empty[st], left);
+        tc_commit(o_full, left);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- queries into shared memory, in the operand's layout; rows that are not there are zero
+    if (!a.beside) pdl_wait();
+    const T *q = reinterpret_cast<const T *>(a.q) + (size_t)(it.s.row0 + it.tok0) * a.q_tok + (size_t)kvh * G * HD;
+#pragma unroll 8
+    for (int i = 0; i < HD / 8; i++) {
+      const int x = i * 128 + (int)threadIdx.x, r = x / (HD / 8), c = x % (HD / 8), tk = r / G;
+      const uint4 v = r < rows ? __ldcg(reinterpret_cast<const uint4 *>(q + (size_t)tk * a.q_tok + (size_t)(r - tk * G) * HD + 8 * c)) : make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4 *>(q_s + (c >> 3) * (TILE_ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mbar_arrive(q_full);
+    if (!busy) {
+      for (int j = 0; j < n_tiles; j++) {   // (P V of tile j - 1 first: an arrival for tile j must not join the barrier's previous phase)
+        if (j > 0) mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, a.err, left);
+        mbar_arrive(p_full);
+      }
+      mbar_wait_lim(o_full, (uint32_t)(n_tiles - 1) & 1u, a.err, left);
+    } else {
+      // ---- softmax (a thread a query row)
+      const int qp = p0 + tok, lo = a.win.w <= 0 ? 0 : a.win.by_call ? by_call : max(0, qp + 1 - a.win.w);
+      for (int j = 0; j < n_tiles; j++) {
+        const uint32_t tmem_sp = tmem_base + lane_addr + (uint32_t)((j & 1) * 64);
+        mbar_wait_lim(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, left);
+        tc_fence_after();
+        float sv[TILE];
+        {
+          uint32_t r[32];
+          tc_ld32(tmem_sp, r);
+#pragma unroll
+          for (int i = 0; i < 32; i++) sv[i] = __uint_as_float(r[i]);
+          tc_ld32(tmem_sp + 32u, r);
+#pragma unroll
+          for (int i = 0; i < 32; i++) sv[32 + i] = __uint_as_float(r[i]);
+        }
+        const int k0 = (it.t0 + j) * TILE;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (k0 + TILE - 1 > p0 || k0 < late) {   // a row of the tile does not see all of these
+#pragma unroll
+          for (int i = 0; i < TILE; i++) {
+            if (k0 + i > qp || k0 + i < lo) sv[i] = -INFINITY;
+            mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < TILE; i++) mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        float fac = 1.f;
+        bool resc = false;
+        if (j == 0) {
+          m_run = mx;
+        } else if ((mx - m_run) * a.scale_log2 > a.tau_log2) {   // (from -inf: factor 0)
+          fac = ft_ex2((m_run - mx) * a.scale_log2);
+          m_run = mx;
+          resc = true;
+        }
+        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;   // a row that has seen nothing yet counts from 0
+        float rs = 0.f;
+#pragma unroll
+        for (int i = 0; i < TILE; i++) {
+          const float e = ft_ex2(fmaf(sv[i], a.scale_log2, -mc));
+          sv[i] = e;
+          rs += e;
+        }
+        l_run = l_run * fac + rs;
+        if (j > 0) {
+          mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, a.err, left);   // P V of the previous tile is there: O is at rest
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, resc)) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+              uint32_t r[32];
+              tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+#pragma unroll
+              for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * fac);
+              tc_st32(tmem_o + lane_addr + (uint32_t)c0, r);
+            }
+          }
+        }
+        if (marked[j & 3] == 0u) {
+          uint32_t hi[32], lw[32];
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            const float x0 = sv[2 * i], x1 = sv[2 * i + 1];
+            hi[i] = pack2x<T>(x0, x1);
+            const float2 hf = DT<T>::unpack2(hi[i]);
+            lw[i] = pack2x<T>(x0 - hf.x, x1 - hf.y);
+          }
+          tc_st32(tmem_sp, hi);
+          tc_st32(tmem_sp + 32u, lw);
+        } else {
+          // the tile's values hold an infinity or a NaN: the row sums those that it sees, weights by way of TMEM
+          {
+            uint32_t r[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sv[i]);
+            tc_st32(tmem_sp, r);
+#pragma unroll
+            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sv[32 + i]);
+            tc_st32(tmem_sp + 32u, r);
+          }
+          tc_wait_st();
+          mbar_wait_lim(&v_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, left);
+          __syncwarp();
+          const unsigned char *vt = v_s + (j & 1) * C::KV_BYTES;
+          const int n = min(TILE, kv_end - k0);
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 32) {
+            uint32_t r[32];
+            tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+            float o[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = j > 0 ? __uint_as_float(r[i]) : 0.f;
+#pragma unroll 1
+            for (int k = 0; k < n; k++) {
+              const float p = tc_ld1(tmem_sp + (uint32_t)k);
+              if (k0 + k <= qp && k0 + k >= lo) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  const int c = (c0 >> 3) + i;
+                  float v[8];
+                  unpack8<T>(*reinterpret_cast<const uint4 *>(vt + (k >> 3) * GROUP + (c >> 3) * 1024 + (k & 7) * 128 + (((c & 7) ^ (k & 7)) << 4)), v);
+#pragma unroll
+                  for (int e = 0; e < 8; e++) o[8 * i + e] = fmaf(p, v[e], o[8 * i + e]);
+                }
+              }
+              __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(o[i]);
+            tc_st32(tmem_o + lane_addr + (uint32_t)c0, r);
+          }
+        }
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full);
+      }
+      mbar_wait_lim(o_full, (uint32_t)(n_tiles - 1) & 1u, a.err, left);   // every product of this CTA is there
+      tc_fence_after();
+    }
+  }
+  // ---- O / l, one rounding to D; or a part's sums for the one that joins them
+  auto store = [&](int c0, const float (&v)[32], float inv) {
+    T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(it.s.row0 + it.tok0 + tok) * a.n_heads + kvh * G + row - tok * G) * HD + c0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      reinterpret_cast<uint4 *>(dst)[i] = make_uint4(pack2x<T>(v[8 * i] * inv, v[8 * i + 1] * inv), pack2x<T>(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
+                                                     pack2x<T>(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack2x<T>(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
+  };
+  auto place = [&](int part) { return a.ws + ((size_t)kvh * a.plan->parts + it.part0 + part) * C::PART; };
+  if (busy) {
+    const float inv_l = 1.0f / l_run;
+    float4 *to = reinterpret_cast<float4 *>(place(it.part));
+#pragma unroll 1
+    for (int c0 = 0; c0 < HD; c0 += 32) {
+      uint32_t r[32];
+      tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+      if (row < rows) {
+        if (it.parts == 1) store(c0, v, inv_l);
+        else
+#pragma unroll
+          for (int i = 0; i < 8; i++) __stcg(to + (c0 / 4 + i) * TILE_ROWS + row, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+      }
+    }
+    if (it.parts > 1 && row < rows) __stcg(reinterpret_cast<float2 *>(place(it.part) + TILE_ROWS * HD) + row, make_float2(m_run, l_run));
+  }
+  if (!left) *gave_up = 1;
+  if (it.parts > 1) __threadfence();
+  tc_fence_before();
+  __syncthreads();
+  if (it.parts > 1) {
+    if (threadIdx.x == 0) {
+      unsigned *tk = a.tickets + (size_t)it.part0 * a.pool.n_kv + kvh;
+      const bool last = atomicAdd(tk, 1u) == (unsigned)it.parts - 1;
+      if (last) *tk = 0u;
+      *last_come = last;
+      __threadfence();
+    }
+    __syncthreads();
+    if (*last_come && busy && row < rows) {
+      float M = -INFINITY, L = 0.f;
+      for (int k = 0; k < it.parts; k++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row).x);
+      for (int k = 0; k < it.parts; k++) {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row);
+        L += x.x == -INFINITY ? x.y : x.y * ft_ex2((x.x - M) * a.scale_log2);
+      }
+      const float inv = 1.0f / L;
+#pragma unroll 1
+      for (int c0 = 0; c0 < HD; c0 += 32) {
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < it.parts; k++) {
+          const float m = __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row).x, f = m == -INFINITY ? 0.f : ft_ex2((m - M) * a.scale_log2);
+          const float4 *from = reinterpret_cast<const float4 *>(place(k)) + (c0 / 4) * TILE_ROWS + row;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float4 x = __ldcg(from + i * TILE_ROWS);
+            v[4 * i] = fmaf(x.x, f, v[4 * i]); v[4 * i + 1] = fmaf(x.y, f, v[4 * i + 1]); v[4 * i + 2] = fmaf(x.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(x.w, f, v[4 * i + 3]);
+          }
+        }
+        store(c0, v, inv);
+      }
+    }
+  }
+  if (*gave_up) ft_drain(bars, warp, lane, k_loads, v_loads);
+  if (a.beside) pdl_wait();
+  if (warp == 5) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(C::TMEM) : "memory");
+  }
+}
+
+}  // namespace pg
+}  // namespace cake
