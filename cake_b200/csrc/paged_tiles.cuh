@@ -45,6 +45,14 @@ __device__ __forceinline__ float tc_ld1(uint32_t taddr) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   return __uint_as_float(r);
 }
+// the product with P from TMEM, or nothing: a predicate and not a branch (behind one every product's operands make their own way to the uniform registers)
+__device__ __forceinline__ void mma_ts_if(uint32_t yes, uint32_t tmem_c, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_c),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(yes)
+      : "memory");
+}
 // an operand whose groups of eight rows lie `group` bytes apart and whose 64-entry ranges 1 KB: K-major (keys), and MN-major (values)
 __device__ __forceinline__ uint64_t desc_keys(const void *tile, uint32_t group) {
   return (uint64_t)((smem_u32(tile) & 0x3ffff) >> 4) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -157,11 +165,14 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     // ---- products (one thread issues them; the warp runs the loop with it)
     const uint32_t one = elect_one();
     const uint32_t idesc_s = tc_idesc<T>(TILE), idesc_o = tc_idesc<T>(HD) | (1u << 16);   // M128 N64, both K-major; M128 N hd, A from TMEM, B (V) MN-major
+    uint32_t mark = 0u, next_mark = 0u;   // of tiles j and j + 1
     auto issue_s = [&](int j) {   // S_j = Q K_j^T into S buffer j & 1
       const int st = j & 1;
       mbar_wait_lim(&k_full[st], (uint32_t)(j >> 1) & 1u, a.err, left);
       __syncwarp();
       tc_fence_after();
+      mark = next_mark;
+      next_mark = marked[j & 3];
       const uint64_t q0 = tc_smem_desc(q_s), kt = desc_keys(k_s, GROUP) + (uint64_t)(st * (C::KV_BYTES >> 4));
       if (one) {
 #pragma unroll
@@ -184,14 +195,13 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
       __syncwarp();
       tc_fence_after();
       const uint64_t vt = desc_values(v_s, GROUP) + (uint64_t)(st * (C::KV_BYTES >> 4));
-      const int steps = marked[j & 3] ? 0 : min(TILE, (kv_end - (it.t0 + j) * TILE + 15) & ~15) / 16;   // sixteens of positions; marked: the rows have summed by themselves
+      const int steps = (j + 1 < n_tiles ? mark : next_mark) ? 0 : min(TILE, (kv_end - (it.t0 + j) * TILE + 15) & ~15) / 16;   // sixteens of positions; marked: the rows have summed by themselves
       if (one) {
 #pragma unroll
         for (int half = 0; half < 2; half++)
 #pragma unroll
           for (int ks = 0; ks < TILE / 16; ks++)
-            if (ks < steps)
-              tc_mma_f16_ts(tmem_o, tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8), vt + (uint64_t)(ks * (2 * GROUP >> 4)), idesc_o, (j | half | ks) ? 1u : 0u);
+            mma_ts_if(ks < steps ? 1u : 0u, tmem_o, tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8), vt + (uint64_t)(ks * (2 * GROUP >> 4)), idesc_o, (j | half | ks) ? 1u : 0u);
         tc_commit(&v_empty[st], left);
         tc_commit(o_full, left);
       }
@@ -222,6 +232,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
         const uint32_t tmem_sp = tmem_base + lane_addr + (uint32_t)((j & 1) * 64);
         mbar_wait_lim(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, left);
         tc_fence_after();
+        const uint32_t mark = marked[j & 3];
         float sv[TILE];
         {
           uint32_t r[32];
@@ -277,7 +288,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
             }
           }
         }
-        if (marked[j & 3] == 0u) {
+        if (mark == 0u) {
           uint32_t hi[32], lw[32];
 #pragma unroll
           for (int i = 0; i < 32; i++) {
