@@ -81,48 +81,59 @@ __global__ void __launch_bounds__(128) append_kernel(const Pool p, const Append 
       sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
     }
   }
-#pragma unroll 2
-  for (int g = blockIdx.y; g * at_once < heads; g += parts) {
-    const int head = g * at_once + sub;
-    const bool in = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + p.n_kv;
-    const int h = is_q ? head : is_v ? head - a.n_q - p.n_kv : head - a.n_q;
-    const T *src = is_q ? reinterpret_cast<const T *>(a.q) + (size_t)row * a.q_tok
-                   : is_v ? reinterpret_cast<const T *>(a.v) + (size_t)row * a.v_tok : reinterpret_cast<const T *>(a.k) + (size_t)row * a.k_tok;
-    uint4 w = in ? *reinterpret_cast<const uint4 *>(src + (size_t)h * p.hd + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-    const bool dirty = in && is_v && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w));
-    const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
-    if (a.cos_t || a.q_norm || a.k_norm) {   // (the same for all lanes, as the exchanges have to be)
-      float x[8], y[8];
-      unpack8<T>(w, x);
-      if (a.q_norm || a.k_norm) {
-        float ss = 0.f;
+  constexpr int U = 4;   // loads of a warp in flight (12314 rows of 48 heads: 73 us with two)
+  for (int g0 = blockIdx.y; g0 * at_once < heads; g0 += U * parts) {
+    uint4 in4[U];
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-        for (int o = 1; o < cph; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (nw && !is_v) {
-          const float inv = 1.0f / sqrtf(ss / (float)p.hd + a.eps);
-          float g8[8];
-          unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c), g8);
-#pragma unroll
-          for (int i = 0; i < 8; i++) x[i] = a.as_blocks ? rnd<T>(x[i] * inv * g8[i]) : x[i] * inv * g8[i];
-        }
-      }
-      if (a.cos_t) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other);
-        if (turns && !is_v)
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float f = x[i] * cs[i], s = low ? -y[i] * sn[i] : y[i] * sn[i];
-            x[i] = a.as_blocks ? rnd<T>(f) + rnd<T>(s) : f + s;
-          }
-      }
-      if (!is_v) w = make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+    for (int u = 0; u < U; u++) {
+      const int head = (g0 + u * parts) * at_once + sub;
+      const T *src = head < a.n_q ? reinterpret_cast<const T *>(a.q) + (size_t)row * a.q_tok + (size_t)head * p.hd
+                     : head < a.n_q + p.n_kv ? reinterpret_cast<const T *>(a.k) + (size_t)row * a.k_tok + (size_t)(head - a.n_q) * p.hd
+                                             : reinterpret_cast<const T *>(a.v) + (size_t)row * a.v_tok + (size_t)(head - a.n_q - p.n_kv) * p.hd;
+      in4[u] = head < heads ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
     }
-    if (in) {
-      void *to = is_q ? (void *)(reinterpret_cast<T *>(a.q_out) + (size_t)row * a.out_tok + (size_t)h * p.hd + 8 * c) : (void *)(rows_of(p, page, h, is_v) + chunk_at(p.hd, r, c));
-      *reinterpret_cast<uint4 *>(to) = w;
-      if (dirty) p.marks[(size_t)page * p.n_kv + h] = 1u;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if ((g0 + u * parts) * at_once >= heads) break;   // (the same for all lanes)
+      const int head = (g0 + u * parts) * at_once + sub;
+      const bool in = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + p.n_kv;
+      const int h = is_q ? head : is_v ? head - a.n_q - p.n_kv : head - a.n_q;
+      uint4 w = in4[u];
+      const bool dirty = in && is_v && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w));
+      const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
+      if (a.cos_t || a.q_norm || a.k_norm) {   // (the same for all lanes, as the exchanges have to be)
+        float x[8], y[8];
+        unpack8<T>(w, x);
+        if (a.q_norm || a.k_norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+          for (int o = 1; o < cph; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (nw && !is_v) {
+            const float inv = 1.0f / sqrtf(ss / (float)p.hd + a.eps);
+            float g8[8];
+            unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c), g8);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = a.as_blocks ? rnd<T>(x[i] * inv * g8[i]) : x[i] * inv * g8[i];
+          }
+        }
+        if (a.cos_t) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other);
+          if (turns && !is_v)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const float f = x[i] * cs[i], s = low ? -y[i] * sn[i] : y[i] * sn[i];
+              x[i] = a.as_blocks ? rnd<T>(f) + rnd<T>(s) : f + s;
+            }
+        }
+        if (!is_v) w = make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+      }
+      if (in) {
+        void *to = is_q ? (void *)(reinterpret_cast<T *>(a.q_out) + (size_t)row * a.out_tok + (size_t)h * p.hd + 8 * c) : (void *)(rows_of(p, page, h, is_v) + chunk_at(p.hd, r, c));
+        *reinterpret_cast<uint4 *>(to) = w;
+        if (dirty) p.marks[(size_t)page * p.n_kv + h] = 1u;
+      }
     }
   }
 }
@@ -159,7 +170,7 @@ int read(cudaStream_t s, int, const Pool &p, const Read &a, uint64_t *launches) 
 // ------------------------------------------------------------------------------------------ attention
 int few_ctas(int hd, int sms) { return (hd == 256 ? 1 : 2) * sms; }
 int room(int hd, int sms, int n_kv) { return std::max(1, (hd == 256 ? 1 : 2) * sms / n_kv); }
-size_t tiles_floats(int hd, int sms, int n_kv) { return (size_t)room(hd, sms, n_kv) * n_kv * TILE_ROWS * (hd + 2); }
+size_t tiles_floats(int hd, int sms, int n_kv) { return (size_t)2 * room(hd, sms, n_kv) * n_kv * TILE_ROWS * (hd + 2); }
 size_t few_floats(int hd, int sms) { return (size_t)2 * few_ctas(hd, sms) * TOKEN_COLS * (hd + 2); }
 // f(T, HD): the instances of a kind of cache
 template <typename F> static int by_kind(int dtype, int hd, F &&f) {
@@ -185,24 +196,30 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
   const int G = a.n_heads / p.n_kv;
   const float scale_log2 = a.scale * 1.4426950408889634f;
   if (a.n_few) {
-    const Few f{p, a.plan, a.seqs, a.q, a.q_tok, a.out, w.few_ws, w.tickets, a.n_heads, G, a.win, scale_log2, a.err, a.n_items ? 1 : 0};
+    const Few f{p, a.plan, a.seqs, a.q, a.q_tok, a.out, w.few_ws, a.n_heads, G, a.win, scale_log2, a.err, a.n_items ? 1 : 0};
+    const Cut *cuts = reinterpret_cast<const Cut *>(reinterpret_cast<const Worker *>(a.plan + 1) + few_ctas(p.hd, w.sms));
     const int e = by_kind(dtype, p.hd, [&](auto t, auto h) {
       typedef typename decltype(t)::type T;
       constexpr int HD = decltype(h)::value;
-      const dim3 grid((unsigned)few_ctas(HD, w.sms)), block(FEW_THREADS);
-      if (a.few_cols <= 8) return launch(s, launches, few_kernel<T, HD, 1>, grid, block, FewCfg<HD, 1>::SMEM, f);
-      return launch(s, launches, few_kernel<T, HD, 2>, grid, block, FewCfg<HD, 2>::SMEM, f);
+      auto both = [&](auto n) {
+        constexpr int NT = decltype(n)::value;
+        const int rc = launch(s, launches, few_kernel<T, HD, NT>, dim3((unsigned)few_ctas(HD, w.sms)), dim3(FEW_THREADS), FewCfg<HD, NT>::SMEM, f);
+        if (rc || !a.n_cuts) return rc;
+        return launch(s, launches, few_join_kernel<T, HD, NT>, dim3((unsigned)a.n_cuts, (unsigned)a.few_cols), dim3(128), 0, f, cuts);
+      };
+      return a.few_cols <= 8 ? both(std::integral_constant<int, 1>{}) : both(std::integral_constant<int, 2>{});
     });
     if (e) return e;
   }
   if (!a.n_items) return 0;
-  const Item *items = reinterpret_cast<const Item *>(reinterpret_cast<const Worker *>(a.plan + 1) + few_ctas(p.hd, w.sms));
-  const Tiles t8{p, a.plan, items, a.q, a.q_tok, a.out, w.tiles_ws, w.tickets + (size_t)w.max_seqs * p.n_kv, a.n_heads, G, TILE_ROWS / G, a.win, scale_log2, 8.f, a.err,
-                 a.n_few ? 1 : 0};
+  const Item *items = reinterpret_cast<const Item *>(reinterpret_cast<const char *>(a.plan + 1) + (size_t)few_ctas(p.hd, w.sms) * (sizeof(Worker) + sizeof(Cut)));
+  const Tiles t8{p, a.plan, items, a.q, a.q_tok, a.out, w.tiles_ws, a.n_heads, G, TILE_ROWS / G, a.win, scale_log2, 8.f, a.err, a.n_few ? 1 : 0};
   return by_kind(dtype, p.hd, [&](auto t, auto h) {
     typedef typename decltype(t)::type T;
     constexpr int HD = decltype(h)::value;
-    return launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, t8);
+    const int e = launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, t8);
+    if (e || !a.cut) return e;
+    return launch(s, launches, join_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv * (HD / 32))), dim3(128), 0, t8);
   });
 }
 

@@ -61,16 +61,15 @@ int append(cudaStream_t, int dtype, const Pool &, const Append &, int sms, uint6
 struct Read { const int2 *rows; int slot, first, n; void *k, *v; };
 int read(cudaStream_t, int dtype, const Pool &, const Read &, uint64_t *launches);
 
-// A step's attention as it is cut for one window (paged_plan.hpp), on the device: this head, few_ctas workers of the few-row kernel, the items of the many-row
-// kernel.  What the calls on a cache share: sums of runs and tiles that are cut, and how many of their parts have come (all zero between calls)
-struct PlanHead { int W, T, n_items, parts, pad[4]; };   // workers, tiles of their line; items, parts of those that are cut
+// A step's attention as it is cut for one window (paged_plan.hpp), on the device: this head, few_ctas workers and as many cuts of the few-row kernel, the items of
+// the many-row kernel.  What the calls on a cache share: sums of runs and tiles that are cut
+struct PlanHead { int W, n_cuts, n_items, parts, pad[4]; };   // workers, cut runs; items, parts of those that are cut
 struct Scratch {
   float *few_ws, *tiles_ws;      // few_floats; tiles_floats (nullptr: the step has no sequence of many rows)
-  unsigned *tickets;             // [sequences][key heads], then [room][key heads]
-  int max_seqs, sms;
+  int sms;
 };
 int few_ctas(int hd, int sms);             // CTAs of the few-row kernel: no more workers than that
-int room(int hd, int sms, int n_kv);       // items of the many-row kernel that fill the chip, and parts of cut ones at most
+int room(int hd, int sms, int n_kv);       // items of the many-row kernel that fill the chip (parts of cut ones: twice as many at most)
 size_t few_floats(int hd, int sms);
 size_t tiles_floats(int hd, int sms, int n_kv);
 int prepare(int dtype, int hd);            // once per device and kind of cache, in front of the first call
@@ -84,7 +83,8 @@ struct Attend {
   Window win;
   const PlanHead *plan;
   int n_few, few_cols;           // sequences of few rows, query rows of a key head that they have at most
-  int n_items;                   // of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
+  int n_cuts, n_items;           // runs that are cut, items of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
+  bool cut;                      // some of the items are parts (of a captured call: may be)
   int *err;
 };
 int attend(cudaStream_t, int dtype, const Pool &, const Attend &, const Scratch &, uint64_t *launches);

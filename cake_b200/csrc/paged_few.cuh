@@ -2,7 +2,8 @@
 //
 // Bound by memory: every key and value is read once, 4 hd bytes a position and key head, for 4 operations an entry and query head.  The line of all
 // (sequence, key head, tile of 64 positions) is cut into equal shares, one a CTA (paged_plan.hpp, cut_few), so that sequences of any lengths fill the chip
-// evenly; a (sequence, key head) that is cut has its parts joined by whichever CTA comes last, in the order of the parts.  In a CTA a warp copies tiles into a
+// evenly; the parts of a (sequence, key head) that is cut are joined by a kernel of its own (the CTA that comes last, behind a fence, a ticket and a loop over the
+// parts, took 4 to 9 us, others waiting for it).  In a CTA a warp copies tiles into a
 // ring of shared memory by bulk copies of whole pages (or halves of tiles), looking up the pages of up to 32 copies at once and ahead; four warps take 16
 // positions of a tile each and never wait for one another before the share's end.
 //
@@ -20,12 +21,13 @@ namespace pg {
 
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int HD, int NT> struct FewCfg {
-  static constexpr int STAGES = HD == 64 ? 6 : 3;
+  static constexpr int STAGES = HD == 64 ? 6 : NT == 1 ? 3 : 2;
   static constexpr int ROWS_BYTES = TILE * HD * 2;          // keys, or values, of a tile
   static constexpr int COLS = 8 * NT;
-  static constexpr int RED_BYTES = 2 * COLS * HD * 4, ML_BYTES = FEW_WARPS * COLS * 8;
+  static constexpr int RED_BYTES = FEW_WARPS * COLS * HD * 4, ML_BYTES = FEW_WARPS * COLS * 8;
   static constexpr int SMEM = STAGES * 2 * ROWS_BYTES + RED_BYTES + ML_BYTES + STAGES * (16 + 4) + 16;
   static constexpr int CTAS = HD == 256 ? 1 : 2;
+  static_assert(SMEM <= 227 * 1024 && CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 // whether this call is the present step's; a replayed call of another one does nothing
 __device__ __forceinline__ bool same_step(const Pool &p) {
@@ -45,8 +47,7 @@ struct Few {
   const void *q;
   long long q_tok;
   void *out;
-  float *ws;            // [2 W][COLS][HD + 2]
-  unsigned *tickets;    // [sequences][key heads], zero between calls
+  float *ws;            // [2 CTAs][COLS][HD + 2]
   int n_heads, G;
   Window win;
   float scale_log2;
@@ -124,17 +125,17 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
   extern __shared__ __align__(128) unsigned char few_smem[];
   unsigned char *ring = few_smem;
   float *red = reinterpret_cast<float *>(ring + C::STAGES * 2 * C::ROWS_BYTES);
-  float2 *ml = reinterpret_cast<float2 *>(red + 2 * C::COLS * HD);
+  float2 *ml = reinterpret_cast<float2 *>(red + FEW_WARPS * C::COLS * HD);
   uint64_t *full = reinterpret_cast<uint64_t *>(ml + FEW_WARPS * C::COLS), *empty = full + C::STAGES;
   uint32_t *marked = reinterpret_cast<uint32_t *>(empty + C::STAGES);
-  int *flags = reinterpret_cast<int *>(marked + C::STAGES);   // [0] a wait was given up; [1] the last to come
+  int *gave_up = reinterpret_cast<int *>(marked + C::STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; i++) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], FEW_WARPS);
     }
-    flags[0] = 0;
+    *gave_up = 0;
     mbar_fence_init();
   }
   __syncthreads();
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
       }
       b = nb; n = nn; page = npage;
     }
-    if (left == 0) flags[0] = 1;
+    if (left == 0) *gave_up = 1;
     in_ring = issued;
   } else {
     // ---- products
@@ -376,42 +377,13 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
           v += __shfl_xor_sync(0xffffffffu, v, 16);
           if (g == 0) ml[warp * C::COLS + 8 * x + 2 * t + e] = make_float2(m[x][e], v);
         }
-      named_bar_sync(1, 32 * FEW_WARPS);
+      auto in_red = [](int k, int c, int d) { return (k * C::COLS + c) * HD + (d ^ ((c >> 1 & 3) << 3)); };   // (a warp's 8 entries of 4 pairs of columns: 32 banks)
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int c = 8 * x + 2 * t + e;
-          float M = -INFINITY;
-          for (int k = 0; k < FEW_WARPS; k++) M = fmaxf(M, ml[k * C::COLS + c].x);
-          const float f = m[x][e] == -INFINITY ? 0.f : ex2((m[x][e] - M) * a.scale_log2);
-          // (a warp that has seen nothing has sums of 0)
+        for (int i = 0; i < HD / 16; i++)
 #pragma unroll
-          for (int i = 0; i < HD / 16; i++) {
-            o[x][i][e] *= f;
-            o[x][i][e + 2] *= f;
-          }
-        }
-      auto in_red = [](int c, int d) { return c * HD + (d ^ ((c >> 1 & 3) << 3)); };   // (a warp's 8 entries of 4 pairs of columns: 32 banks)
-      auto put = [&](int slot) {
-#pragma unroll
-        for (int x = 0; x < NT; x++)
-#pragma unroll
-          for (int i = 0; i < HD / 16; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) red[in_red(slot * C::COLS + 8 * x + 2 * t + (e & 1), 16 * i + g + (e >> 1) * 8)] = o[x][i][e];
-      };
-      if (warp >= 2) put(warp - 2);
-      named_bar_sync(1, 32 * FEW_WARPS);
-      if (warp < 2) {
-#pragma unroll
-        for (int x = 0; x < NT; x++)
-#pragma unroll
-          for (int i = 0; i < HD / 16; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[x][i][e] += red[in_red(warp * C::COLS + 8 * x + 2 * t + (e & 1), 16 * i + g + (e >> 1) * 8)];
-        put(warp);
-      }
+          for (int e = 0; e < 4; e++) red[in_red(warp, 8 * x + 2 * t + (e & 1), 16 * i + g + (e >> 1) * 8)] = o[x][i][e];
       named_bar_sync(1, 32 * FEW_WARPS);
       const bool whole = w.tile == 0 && n == w.n;
       const int per = HD / 4;   // pieces of four entries of a column
@@ -425,60 +397,99 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
       for (int u = threadIdx.x; u < cols * per; u += 32 * FEW_WARPS) {
         const int c = u / per, d = 4 * (u - c * per);
         float M = -INFINITY, L = 0.f;
-        for (int k = 0; k < FEW_WARPS; k++) M = fmaxf(M, ml[k * C::COLS + c].x);
+        float2 of[FEW_WARPS];
+#pragma unroll
         for (int k = 0; k < FEW_WARPS; k++) {
-          const float2 v = ml[k * C::COLS + c];
-          L += v.x == -INFINITY ? v.y : v.y * ex2((v.x - M) * a.scale_log2);   // (0, or NaN where a score was none)
+          of[k] = ml[k * C::COLS + c];
+          M = fmaxf(M, of[k].x);
         }
-        const float4 x = *reinterpret_cast<const float4 *>(&red[in_red(c, d)]), y = *reinterpret_cast<const float4 *>(&red[in_red(C::COLS + c, d)]);
-        const float4 v = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; k++) {   // (a warp that has seen nothing, or no number, has sums of 0 or NaN)
+          const float f = of[k].x == -INFINITY ? 1.f : ex2((of[k].x - M) * a.scale_log2);
+          const float4 y = *reinterpret_cast<const float4 *>(&red[in_red(k, c, d)]);
+          L = fmaf(of[k].y, f, L);
+          v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+        }
         if (whole) store(c, d, v, 1.0f / L);
         else {
           __stcg(reinterpret_cast<float4 *>(place(mine) + c * HD + d), v);
           if (d == 0) __stcg(reinterpret_cast<float2 *>(place(mine) + C::COLS * HD) + c, make_float2(M, L));
         }
       }
-      if (!whole) {
-        const long long T_ = a.plan->T, W = a.plan->W, begin = T_ * (long long)blockIdx.x / W + (T_ * ((long long)blockIdx.x + 1) / W - T_ * (long long)blockIdx.x / W - w.left) - w.tile;
-        const int first = (int)(((begin + 1) * W - 1) / T_), parts = (int)(((begin + w.n) * W - 1) / T_) - first + 1;
-        __threadfence();
-        named_bar_sync(1, 32 * FEW_WARPS);
-        if (threadIdx.x == 0) {
-          unsigned *tk = a.tickets + (size_t)w.i * a.pool.n_kv + w.kvh;
-          const bool last = atomicAdd(tk, 1u) == (unsigned)parts - 1;
-          if (last) *tk = 0u;
-          flags[1] = last;
-          __threadfence();
-        }
-        named_bar_sync(1, 32 * FEW_WARPS);
-        if (flags[1]) {
-          for (int u = threadIdx.x; u < cols * per; u += 32 * FEW_WARPS) {
-            const int c = u / per, d = 4 * (u - c * per);
-            auto at = [&](int k) { return place(k ? 2 * (first + k) : 2 * first + 1); };
-            float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-            for (int k = 0; k < parts; k++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(at(k) + C::COLS * HD) + c).x);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int k = 0; k < parts; k++) {
-              const float2 x = __ldcg(reinterpret_cast<const float2 *>(at(k) + C::COLS * HD) + c);
-              const float4 y = __ldcg(reinterpret_cast<const float4 *>(at(k) + c * HD + d));
-              const float f = x.x == -INFINITY ? 0.f : ex2((x.x - M) * a.scale_log2);
-              L += x.x == -INFINITY ? x.y : x.y * f;
-              v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
-            }
-            store(c, d, v, 1.0f / L);
-          }
-        }
-      }
-      named_bar_sync(1, 32 * FEW_WARPS);   // (red, ml and flags are free again)
+      named_bar_sync(1, 32 * FEW_WARPS);   // (red and ml are free again)
       w.next(a, n);
     }
-    if (left == 0) flags[0] = 1;
+    if (left == 0) *gave_up = 1;
   }
   __syncthreads();
-  if (flags[0] && threadIdx.x == 32 * FEW_WARPS)   // a wait was given up: copies in flight end before the CTA does
+  if (*gave_up && threadIdx.x == 32 * FEW_WARPS)   // a wait was given up: copies in flight end before the CTA does
     for (int j = max(0, in_ring - C::STAGES); j < in_ring; j++) mbar_drain(&full[j % C::STAGES], (uint32_t)(j / C::STAGES) & 1u);
+}
+
+// The parts of a run: a CTA a query row, a thread four entries of every PG-th part, up to eight of them asked for at once
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(128) few_join_kernel(const Few a, const Cut *cuts) {
+  pdl_launch_dependents();
+  constexpr int PER = HD / 4, PG = 128 / PER, AT_ONCE = 8, COLS = 8 * NT;
+  __shared__ float4 sums[128];
+  __shared__ float2 tops[128];
+  const int col = (int)blockIdx.y, d = 4 * (threadIdx.x % PER), pg = threadIdx.x / PER;
+  const bool any = same_step(a.pool) && (int)blockIdx.x < a.plan->n_cuts;
+  Cut cut{};
+  if (any) {
+    const int4 *x = reinterpret_cast<const int4 *>(cuts + blockIdx.x);
+    const int4 u = __ldg(x), v = __ldg(x + 1);
+    cut = Cut{SeqRow{u.x, u.y, u.z, u.w}, v.x, v.y, v.z, 0};
+  }
+  pdl_wait();
+  if (!any || col >= cut.s.count * a.G) return;
+  float M = -INFINITY, L = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = pg; k < cut.parts; k += PG * AT_ONCE) {
+    float4 y[AT_ONCE];
+    float2 m[AT_ONCE];
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) {
+      const int j = k + PG * i;
+      const float *place = a.ws + (size_t)(j ? 2 * (cut.first + j) : 2 * cut.first + 1) * COLS * (HD + 2);
+      m[i] = j < cut.parts ? __ldcg(reinterpret_cast<const float2 *>(place + COLS * HD) + col) : make_float2(-INFINITY, 0.f);
+      y[i] = j < cut.parts ? __ldcg(reinterpret_cast<const float4 *>(place + col * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) top = fmaxf(top, m[i].x);
+    const float old = M == -INFINITY ? 1.f : ex2((M - top) * a.scale_log2);   // (nothing, or no number, so far: sums of 0 or NaN)
+    M = top;
+    L *= old; v.x *= old; v.y *= old; v.z *= old; v.w *= old;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) {
+      const float f = m[i].x == -INFINITY ? 1.f : ex2((m[i].x - M) * a.scale_log2);
+      L = fmaf(m[i].y, f, L);
+      v.x = fmaf(y[i].x, f, v.x); v.y = fmaf(y[i].y, f, v.y); v.z = fmaf(y[i].z, f, v.z); v.w = fmaf(y[i].w, f, v.w);
+    }
+  }
+  sums[threadIdx.x] = v;
+  tops[threadIdx.x] = make_float2(M, L);
+  __syncthreads();
+  if (pg) return;
+  float top = M;
+#pragma unroll
+  for (int k = 1; k < PG; k++) top = fmaxf(top, tops[k * PER + threadIdx.x].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  L = 0.f;
+#pragma unroll
+  for (int k = 0; k < PG; k++) {
+    const float2 m = tops[k * PER + threadIdx.x];
+    const float4 y = sums[k * PER + threadIdx.x];
+    const float f = m.x == -INFINITY ? 1.f : ex2((m.x - top) * a.scale_log2);
+    L = fmaf(m.y, f, L);
+    o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+  }
+  const float inv = 1.0f / L;
+  const int tok = col / a.G;
+  *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + ((size_t)(cut.s.row0 + tok) * a.n_heads + cut.kvh * a.G + col - tok * a.G) * HD + d) =
+      make_uint2(pack2x<T>(o.x * inv, o.y * inv), pack2x<T>(o.z * inv, o.w * inv));
 }
 
 }  // namespace pg

@@ -18,12 +18,12 @@ struct cake_b200_pages {
     pg::Window win;
     unsigned long long step = 0, used = 0;   // made for this step; last used in this call
     bool kept = false;                       // captured calls read it: it is made anew with every step
-    int n_items = 0, most_items = 0;         // of the many-row kernel, now and for any lengths of this shape
+    int n_cuts = 0, n_items = 0, most_items = 0;   // cut runs; items of the many-row kernel, now and for any lengths of this shape
+    bool cut = false;                        // some are parts of tiles
     char *dev = nullptr;
   } plans[8];
   unsigned long long steps = 0, calls = 0;
   float *few_ws = nullptr, *tiles_ws = nullptr;
-  unsigned *tickets = nullptr;
   const float *cos_t = nullptr, *sin_t = nullptr;
   int rot = 0;
   int *bad = nullptr;                // pinned: a replayed call met a step of another shape
@@ -117,17 +117,16 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   *g->bad = 0;
   CU((cudaError_t)pg::prepare(f.dtype, f.head_dim));
   const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
-               s_tickets = ((size_t)max_seqs + pg::room(f.head_dim, c->sm_count, f.n_kv_heads)) * f.n_kv_heads * 4, s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
+               s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   void *arena = nullptr;
-  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_tickets) + up(s_ws) + s_rows, c->pc_pool, c->stream));
+  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_ws) + s_rows, c->pc_pool, c->stream));
   g->arena = (char *)arena;
   g->step = (pg::StepHead *)g->arena;
   g->table = (int *)(g->arena + up(s_step));
-  g->tickets = (unsigned *)(g->arena + up(s_step) + up(s_table));
-  g->few_ws = (float *)(g->arena + up(s_step) + up(s_table) + up(s_tickets));
-  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_tickets) + up(s_ws));
-  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table) + up(s_tickets), c->stream));
+  g->few_ws = (float *)(g->arena + up(s_step) + up(s_table));
+  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_ws));
+  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table), c->stream));
   c->pc_behind = true;
   guard.g = nullptr;
   *out = g;
@@ -184,7 +183,7 @@ extern "C" int cake_b200_pages_available(const cake_b200_pages *g) { return g ? 
 static size_t pages_plan_bytes(const cake_b200_pages *g) {
   const cake_b200_config &f = g->ctx->cfg;
   const int sms = g->ctx->sm_count;
-  return sizeof(pg::PlanHead) + (size_t)pg::few_ctas(f.head_dim, sms) * sizeof(pg::Worker) +
+  return sizeof(pg::PlanHead) + (size_t)pg::few_ctas(f.head_dim, sms) * (sizeof(pg::Worker) + sizeof(pg::Cut)) +
          pg::Book::most_items((long long)g->book.n_pages * g->book.page, g->book.max_seqs, f.n_heads / f.n_kv_heads, pg::room(f.head_dim, sms, f.n_kv_heads)) * sizeof(pg::Item);
 }
 static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // on the ctx's stream of the moment
@@ -192,10 +191,12 @@ static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // 
   const int n_kv = c->cfg.n_kv_heads, hd = c->cfg.head_dim, G = c->cfg.n_heads / n_kv, room = pg::room(hd, c->sm_count, n_kv);
   const size_t most = (size_t)pg::few_ctas(hd, c->sm_count);
   std::vector<pg::Worker> few;
+  std::vector<pg::Cut> cuts;
   std::vector<pg::Item> many;
   pg::PlanHead h{};
-  h.T = g->book.cut_few(p->win, n_kv, (int)most, &few);
+  g->book.cut_few(p->win, n_kv, (int)most, &few, &cuts);
   h.W = (int)few.size();
+  h.n_cuts = (int)cuts.size();
   h.parts = g->book.cut_many(p->win, G, room, &many);
   h.n_items = (int)many.size();
   if (h.n_items && !g->tiles_ws) {
@@ -203,21 +204,24 @@ static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // 
     CU(cudaMallocFromPoolAsync(&m, pg::tiles_floats(hd, c->sm_count, n_kv) * 4, c->pc_pool, c->stream));
     g->tiles_ws = (float *)m;
   }
-  std::vector<char> blob(sizeof h + (many.empty() ? few.size() : most) * sizeof(pg::Worker) + many.size() * sizeof(pg::Item));
+  const size_t at_cuts = sizeof h + most * sizeof(pg::Worker), at_many = at_cuts + most * sizeof(pg::Cut);
+  std::vector<char> blob(!many.empty() ? at_many + many.size() * sizeof(pg::Item) : at_cuts + cuts.size() * sizeof(pg::Cut));
   memcpy(blob.data(), &h, sizeof h);
   if (!few.empty()) memcpy(blob.data() + sizeof h, few.data(), few.size() * sizeof(pg::Worker));
-  if (!many.empty()) memcpy(blob.data() + sizeof h + most * sizeof(pg::Worker), many.data(), many.size() * sizeof(pg::Item));
+  if (!cuts.empty()) memcpy(blob.data() + at_cuts, cuts.data(), cuts.size() * sizeof(pg::Cut));
+  if (!many.empty()) memcpy(blob.data() + at_many, many.data(), many.size() * sizeof(pg::Item));
   RC(pages_upload(c, p->dev, blob.data(), blob.size()));
   int tiles = 0;
   for (size_t i = 0; i < many.size(); i++) tiles += many[i].part == 0;
+  p->n_cuts = h.n_cuts;
   p->n_items = h.n_items;
-  p->most_items = tiles ? std::max(tiles, room) : 0;
+  p->most_items = tiles ? tiles + 2 * room : 0;
+  p->cut = h.parts > 0;
   p->step = g->steps;
   return CAKE_B200_OK;
 }
-static int pages_plan(cake_b200_pages *g, const pg::Window &win, const cake_b200_pages::Plan **out) {
+static int pages_plan(cake_b200_pages *g, const pg::Window &win, bool capturing, const cake_b200_pages::Plan **out) {
   cake_b200_ctx *c = g->ctx;
-  const bool capturing = is_capturing(c->stream);
   cake_b200_pages::Plan *p = nullptr;
   for (auto &x : g->plans)
     if (x.dev && x.win.w == win.w && x.win.by_call == win.by_call) p = &x;
@@ -324,12 +328,14 @@ static int pages_append_on(cake_b200_pages *g, int l, const pg::Append &a) {   /
 static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_tok, void *out, const pg::Window &win, float scale) {
   cake_b200_ctx *c = g->ctx;
   const cake_b200_pages::Plan *plan = nullptr;
-  RC(pages_plan(g, win, &plan));
+  const bool capturing = is_capturing(c->stream);
+  RC(pages_plan(g, win, capturing, &plan));
   int cols = 0;
+  const int most_cuts = std::min(g->book.n_few * c->cfg.n_kv_heads, pg::few_ctas(c->cfg.head_dim, c->sm_count));
   for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
   const pg::Attend a{q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), c->cfg.n_heads, scale, win, (const pg::PlanHead *)plan->dev, g->book.n_few, cols,
-                     is_capturing(c->stream) ? plan->most_items : plan->n_items, c->wait_err};
-  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, g->tickets, g->book.max_seqs, c->sm_count}, launch_counter(c)));
+                     capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, capturing || plan->cut, c->wait_err};
+  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,

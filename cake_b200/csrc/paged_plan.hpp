@@ -19,6 +19,8 @@ struct SeqRow { int slot, pos0, count, row0; };   // a sequence of a step: its r
 
 // One CTA's share of the few-row kernel's work: `left` tiles from tile `tile` of (sequence i, key head kvh) on, in the order of sequences, key heads, tiles
 struct Worker { int i, kvh, tile, left; SeqRow s; };
+// A run (sequence, key head) that is cut: in `parts` neighbouring shares from `first` on
+struct Cut { SeqRow s; int kvh, first, parts, pad; };
 // One CTA row of the many-row kernel (for every key head): tokens tok0 .. of sequence i against key tiles [t0, t1); part of parts, whose sums are in the
 // places part0 .. of the workspace (for key head 0; the parts of all tiles follow one another)
 struct Item { int i, tok0, t0, t1, part, parts, part0, tile; SeqRow s; };
@@ -122,25 +124,45 @@ struct Book {
     return OK;
   }
 
-  // Few rows: all (sequence, key head)s' tiles in one line, cut into equal shares.  Returns the number of tiles
-  int cut_few(const Window &win, int n_kv, int most, std::vector<Worker> *out) const {
+  // Few rows: all (sequence, key head)s' tiles in one line, cut into shares of the same cost: a tile 1, a piece of a run RUN_COST more (its sums have to be
+  // brought together).  A piece that would leave a single tile to the next share takes it.
+  void cut_few(const Window &win, int n_kv, int most, std::vector<Worker> *out, std::vector<Cut> *cuts) const {
+    constexpr double RUN_COST = 1;
     out->clear();
+    cuts->clear();
     long long total = 0;
     for (int i = 0; i < n_few; i++) total += (long long)tiles_of(step[(size_t)i], win) * n_kv;
-    if (!total) return 0;
     const int W = (int)std::min<long long>(most, total);
-    int i = 0;
-    long long at = 0;   // the line's place where sequence i begins
-    for (int w = 0; w < W; w++) {
-      const long long b = total * w / W, e = total * (w + 1) / W;
-      while (b >= at + (long long)tiles_of(step[(size_t)i], win) * n_kv) at += (long long)tiles_of(step[(size_t)i++], win) * n_kv;
-      const int t = tiles_of(step[(size_t)i], win);
-      out->push_back(Worker{i, (int)((b - at) / t), (int)((b - at) % t), (int)(e - b), step[(size_t)i]});
+    double rest = (double)total + RUN_COST * n_few * n_kv;
+    int i = 0, h = 0, k = 0, t = W ? tiles_of(step[0], win) : 0, first = 0;   // the next tile; the share where its run began
+    for (int w = 0; w < W && i < n_few; w++) {
+      const double goal = rest / (W - w);
+      Worker x{i, h, k, 0, step[(size_t)i]};
+      double load = 0;
+      while (i < n_few) {
+        const double room = goal - load - RUN_COST;
+        if (x.left && room < 0.5) break;
+        int n = std::max(1, std::min(t - k, (int)(room + 0.5)));
+        if (t - k - n <= 1 || w == W - 1) n = t - k;
+        if (!k) first = w;
+        x.left += n;
+        k += n;
+        load += RUN_COST + n;
+        rest -= n;
+        if (k < t) break;
+        if (first < w) cuts->push_back(Cut{step[(size_t)i], h, first, w - first + 1, 0});
+        rest -= RUN_COST;
+        k = 0;
+        if (++h == n_kv) {
+          h = 0;
+          if (++i < n_few) t = tiles_of(step[(size_t)i], win);
+        }
+      }
+      out->push_back(x);
     }
-    return (int)total;
   }
-  // Many rows: a CTA row per tile of 128 query rows, the one with the most keys first; where these do not fill `room` CTA rows, their keys are cut into
-  // parts of a like size, of LEAST tiles or more.  Returns the parts of all tiles that are cut
+  // Many rows: a CTA row per tile of 128 query rows, the one with the most keys first.  `room` CTA rows run at once; a tile with more keys than an equal share
+  // of them is cut into parts of a like size, of LEAST key tiles or more.  Returns the parts of all tiles that are cut, at most 2 room
   int cut_many(const Window &win, int G, int room, std::vector<Item> *out) const {
     constexpr int LEAST = 4;
     out->clear();
@@ -159,14 +181,20 @@ struct Book {
       }
     }
     std::stable_sort(whole.begin(), whole.end(), [](const Item &a, const Item &b) { return a.t1 - a.t0 > b.t1 - b.t0; });
-    int parts = 0, spare = std::max(0, room - (int)whole.size());
-    const long long share = std::max<long long>(LEAST, (total + room - 1) / room);   // key tiles of a part
+    // key tiles of a part: an equal share of the chip, and more where the parts would not fit it side by side
+    long long share = std::max<long long>(LEAST, (total + room - 1) / room);
+    auto cut = [&](int n) { return n > share ? (int)((n + share - 1) / share) : 1; };
+    auto all = [&]() {
+      long long p = 0;
+      for (const Item &x : whole) p += cut(x.t1 - x.t0);
+      return p;
+    };
+    if ((int)whole.size() <= room)
+      while (all() > room) share++;
+    int parts = 0;
     for (size_t k = 0; k < whole.size(); k++) {
       Item it = whole[k];
-      const int n = it.t1 - it.t0;
-      int p = spare > 0 ? (int)std::min<long long>((n + share - 1) / share, 1 + spare) : 1;
-      if (p < 1) p = 1;
-      spare -= p - 1;
+      const int n = it.t1 - it.t0, p = cut(n);
       it.tile = (int)k;
       it.parts = p;
       it.part0 = p > 1 ? parts : 0;
@@ -184,7 +212,7 @@ struct Book {
   // what a step of at most `rows` rows can need at most
   static size_t most_items(long long rows, int max_seqs, int G, int room) {
     const int tpt = TILE_ROWS / G;
-    return (size_t)(rows / tpt + max_seqs + room);
+    return (size_t)(rows / tpt + max_seqs + 2 * room);
   }
 };
 

@@ -7,7 +7,8 @@
 //   - keys and values come page by page as they lie: a page's groups of eight rows are the operands' own layout, so that bulk copies without a tensor map fill
 //     a tile from pages of any size, and Q is laid out by the softmax warps (no map to encode, any stride)
 //   - a CTA's sequence, tokens and keys stand in a list (paged_plan.hpp, cut_many): sequences of any lengths side by side, the tiles with the most keys first, and
-//     keys cut into parts where the tiles do not fill the chip; the parts are joined by whichever CTA comes last, in their order
+//     keys cut into parts where the tiles do not fill the chip; a kernel of its own joins them, in their order (one CTA's loads do not suffice: 512 rows of 8 / 4
+//     heads of 256 on 4000 positions, 5 parts of 132 KB a tile: JOINED)
 //   - only whole sixteens of positions that hold a visible one are multiplied; where a page is marked (an infinity or a NaN in its values) a row sums what it sees by itself
 #pragma once
 #include "attn_prefill_tc.cuh"
@@ -31,7 +32,6 @@ struct Tiles {
   long long q_tok;
   void *out;
   float *ws;             // [key head][parts][PART]
-  unsigned *tickets;     // [parts][key head], zero between calls
   int n_heads, G, tpt;
   Window win;
   float scale_log2, tau_log2;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
   uint64_t *bars = reinterpret_cast<uint64_t *>(v_s + 2 * C::KV_BYTES);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 12;
   uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(bars + C::BARS);
-  int *gave_up = reinterpret_cast<int *>(tmem_ptr + 1), *last_come = gave_up + 1;
+  int *gave_up = reinterpret_cast<int *>(tmem_ptr + 1);
   volatile uint32_t *marked = tmem_ptr + 4;   // of tiles j, j + 1 .. j + 3: a slot is written again when the tile two in front of it has been multiplied
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -379,51 +379,51 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     if (it.parts > 1 && row < rows) __stcg(reinterpret_cast<float2 *>(place(it.part) + TILE_ROWS * HD) + row, make_float2(m_run, l_run));
   }
   if (!left) *gave_up = 1;
-  if (it.parts > 1) __threadfence();
   tc_fence_before();
   __syncthreads();
-  if (it.parts > 1) {
-    if (threadIdx.x == 0) {
-      unsigned *tk = a.tickets + (size_t)it.part0 * a.pool.n_kv + kvh;
-      const bool last = atomicAdd(tk, 1u) == (unsigned)it.parts - 1;
-      if (last) *tk = 0u;
-      *last_come = last;
-      __threadfence();
-    }
-    __syncthreads();
-    if (*last_come && busy && row < rows) {
-      float M = -INFINITY, L = 0.f;
-      for (int k = 0; k < it.parts; k++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row).x);
-      for (int k = 0; k < it.parts; k++) {
-        const float2 x = __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row);
-        L += x.x == -INFINITY ? x.y : x.y * ft_ex2((x.x - M) * a.scale_log2);
-      }
-      const float inv = 1.0f / L;
-#pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += 32) {
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; i++) v[i] = 0.f;
-#pragma unroll 1
-        for (int k = 0; k < it.parts; k++) {
-          const float m = __ldcg(reinterpret_cast<const float2 *>(place(k) + TILE_ROWS * HD) + row).x, f = m == -INFINITY ? 0.f : ft_ex2((m - M) * a.scale_log2);
-          const float4 *from = reinterpret_cast<const float4 *>(place(k)) + (c0 / 4) * TILE_ROWS + row;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float4 x = __ldcg(from + i * TILE_ROWS);
-            v[4 * i] = fmaf(x.x, f, v[4 * i]); v[4 * i + 1] = fmaf(x.y, f, v[4 * i + 1]); v[4 * i + 2] = fmaf(x.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(x.w, f, v[4 * i + 3]);
-          }
-        }
-        store(c0, v, inv);
-      }
-    }
-  }
   if (*gave_up) ft_drain(bars, warp, lane, k_loads, v_loads);
   if (a.beside) pdl_wait();
   if (warp == 5) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(C::TMEM) : "memory");
   }
+}
+
+// A CTA for 32 entries of a tile's rows, a thread a row
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) join_kernel(const Tiles a) {
+  pdl_launch_dependents();
+  const int row = threadIdx.x, c0 = 32 * (int)(blockIdx.x % (HD / 32)), kvh = (int)blockIdx.x / (HD / 32) % a.pool.n_kv, nth = (int)blockIdx.x / (HD / 32) / a.pool.n_kv;
+  pdl_wait();
+  if (!same_step(a.pool) || nth >= a.plan->n_items) return;
+  const Item it = a.items[nth];
+  const int rows = a.G * min(a.tpt, it.s.count - it.tok0);
+  if (it.part || it.parts == 1 || row >= rows) return;
+  const float *place = a.ws + ((size_t)kvh * a.plan->parts + it.part0) * TileCfg<HD>::PART;
+  float M = -INFINITY, L = 0.f, v[32];
+#pragma unroll 8
+  for (int k = 0; k < it.parts; k++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(place + k * TileCfg<HD>::PART + TILE_ROWS * HD) + row).x);
+#pragma unroll
+  for (int i = 0; i < 32; i++) v[i] = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < it.parts; k++) {
+    const float2 x = __ldcg(reinterpret_cast<const float2 *>(place + k * TileCfg<HD>::PART + TILE_ROWS * HD) + row);
+    const float f = x.x == -INFINITY ? 0.f : ft_ex2((x.x - M) * a.scale_log2);
+    L += x.x == -INFINITY ? x.y : x.y * f;
+    const float4 *from = reinterpret_cast<const float4 *>(place + k * TileCfg<HD>::PART) + (c0 / 4) * TILE_ROWS + row;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float4 y = __ldcg(from + i * TILE_ROWS);
+      v[4 * i] = fmaf(y.x, f, v[4 * i]); v[4 * i + 1] = fmaf(y.y, f, v[4 * i + 1]); v[4 * i + 2] = fmaf(y.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(y.w, f, v[4 * i + 3]);
+    }
+  }
+  const float inv = 1.0f / L;
+  const int tok = row / a.G;
+  T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(it.s.row0 + it.tok0 + tok) * a.n_heads + kvh * a.G + row - tok * a.G) * HD + c0;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    reinterpret_cast<uint4 *>(dst)[i] = make_uint4(pack2x<T>(v[8 * i] * inv, v[8 * i + 1] * inv), pack2x<T>(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
+                                                   pack2x<T>(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack2x<T>(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
 }
 
 }  // namespace pg

@@ -178,17 +178,36 @@ int main() {
           for (const SeqRow &s : b.step) none = none || (win.by_call && s.pos0 > 0 && s.count > win.w);
           if (none) continue;
           std::vector<Worker> ws;
-          const int most = 1 + rnd(300), total = b.cut_few(win, n_kv, most, &ws);
+          std::vector<Cut> cuts;
+          const int most = 1 + rnd(300);
+          int total = 0;
+          for (int s = 0; s < b.n_few; s++) total += tiles_of(b.step[s], win) * n_kv;
+          b.cut_few(win, n_kv, most, &ws, &cuts);
           IS((int)ws.size() <= most && (ws.empty() == (b.n_few == 0)));
           int i = 0, h = 0, t = 0, sum = 0;   // the workers follow one another through (sequence, key head, tile)
+          std::vector<std::vector<int>> pieces;   // of the runs, in whose shares
           for (size_t j = 0; j < ws.size(); j++) {
-            IS(ws[j].i == i && ws[j].kvh == h && ws[j].tile == t && ws[j].left >= 1 && ws[j].s.slot == b.step[i].slot && ws[j].s.pos0 == b.step[i].pos0);
-            IS((long long)total * (long long)j / (long long)ws.size() == sum);
-            for (int x = 0; x < ws[j].left; x++) {
+            const Worker &x = ws[j];
+            IS(x.i == i && x.kvh == h && x.tile == t && x.left >= 1 && x.s.slot == b.step[i].slot && x.s.pos0 == b.step[i].pos0);
+            bool fresh = true;
+            for (int y = 0; y < x.left; y++) {
+              if (t == 0) pieces.push_back({});
+              if (t == 0 || fresh) pieces.back().push_back((int)j);
+              fresh = false;
               sum++;
-              if (++t == tiles_of(b.step[i], win)) { t = 0; if (++h == n_kv) { h = 0; i++; } }
+              if (++t == tiles_of(b.step[i], win)) { t = 0; fresh = true; if (++h == n_kv) { h = 0; i++; } }
             }
           }
+          size_t cut = 0;
+          for (size_t y = 0; y < pieces.size(); y++) {
+            const std::vector<int> &p = pieces[y];
+            for (size_t z = 0; z < p.size(); z++) IS(p[z] == p[0] + (int)z);
+            if (p.size() == 1) continue;
+            IS(cut < cuts.size());
+            const Cut &x = cuts[cut++];
+            IS(x.kvh == (int)y % n_kv && x.s.slot == b.step[y / n_kv].slot && x.first == p[0] && x.parts == (int)p.size());
+          }
+          IS(cut == cuts.size() && (int)cut <= most);
           IS(sum == total && i == b.n_few && h == 0 && t == 0);
           for (int s = 0; s < b.n_few; s++) {
             IS(tile_first(b.step[s], win) * TILE <= first_of(b.step[s], win, 0) && tiles_of(b.step[s], win) >= 1);
@@ -212,8 +231,8 @@ int main() {
               }
             }
           IS(of.size() == whole && (int)places.size() == parts);
-          IS(it.size() <= std::max<size_t>(whole, (size_t)room) && it.size() <= Book::most_items(b.n_rows, seqs, G, room));
-          IS(parts <= room);
+          IS(it.size() <= whole + 2 * (size_t)room && it.size() <= Book::most_items(b.n_rows, seqs, G, room));
+          IS(parts <= 2 * room && (whole > (size_t)room || it.size() <= (size_t)room));
         }
       }
       if (!rnd(3)) {
