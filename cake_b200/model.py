@@ -159,7 +159,9 @@ class PagedCache:
         self.max_seq = max_seq or ctx.max_seq
         c = ctx.config
         self._heads, self._kv, self._hd, self._dtype = c.num_attention_heads, c.num_key_value_heads, c.hd, ctx.torch_dtype
+        self._dev, self._device = ctx.device, ctx.torch_device
         self._rows = 0   # of the present step
+        self._q_size, self._kv_size = (torch.Size((0, heads, self._hd)) for heads in (self._heads, self._kv))
         self.h = c_void_p()
         self._lib = lib()
         cos = sin = None
@@ -205,7 +207,7 @@ class PagedCache:
         return self._lib.cake_b200_pages_available(self.h)
 
     def _stream(self) -> int:
-        return torch._C._cuda_getCurrentRawStream(self.ctx.device) or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's
+        return torch._C._cuda_getCurrentRawStream(self._dev) or 1   # the default stream by its other name (cudaStreamLegacy): NULL is the context's
 
     def step(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
         """The next step: counts[i] new rows of sequence seqs[i], packed in this order."""
@@ -213,49 +215,57 @@ class PagedCache:
             raise ValueError(f"{len(seqs)} sequences and {len(counts)} counts")
         check(self._lib.cake_b200_pages_step(self.h, int_array(seqs), int_array(counts), len(seqs), self._stream()))
         self._rows = sum(counts)
+        self._q_size, self._kv_size = (torch.Size((self._rows, heads, self._hd)) for heads in (self._heads, self._kv))
 
-    def _in(self, t: torch.Tensor, name: str, heads: int) -> torch.Tensor:
-        """(rows, heads, hd) as the library takes them: heads side by side on 16-byte boundaries (copied where they are not)."""
-        shape = t.shape
-        if len(shape) != 3 or shape[0] != self._rows or shape[1] != heads or shape[2] != self._hd:
-            raise ValueError(f"{name} has shape {list(shape)}, expected (the step's rows, heads, head_dim) = {[self._rows, heads, self._hd]}")
-        if t.dtype != self._dtype or t.get_device() != self.ctx.device:   # (-1: not on a GPU)
-            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self._dtype} on cuda:{self.ctx.device}")
+    def _in(self, t: torch.Tensor, name: str, size: torch.Size) -> Tuple[torch.Tensor, int, int]:
+        """(rows, heads, hd) as the library takes them, heads side by side on 16-byte boundaries (copied where they are not), their address and their rows' stride."""
+        if t.shape != size:
+            raise ValueError(f"{name} has shape {list(t.shape)}, expected (the step's rows, heads, head_dim) = {list(size)}")
+        if t.dtype is not self._dtype or t.get_device() != self._dev:   # (-1: not on a GPU)
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self._dtype} on cuda:{self._dev}")
         st, sh, sd = t.stride()
-        if sd != 1 or (sh != self._hd and heads > 1) or st % 8 or t.data_ptr() % 16:
+        at = t.data_ptr()
+        if sd != 1 or (sh != self._hd and size[1] > 1) or st & 7 or at & 15:
             t = t.clone() if t.is_contiguous() else t.contiguous()
-        return t
+            st, at = t.stride(0), t.data_ptr()
+        return t, at, st
 
     def append(self, block_idx: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rotate: bool = True) -> Optional[torch.Tensor]:
         """The step's rows k, v (rows, n_kv, head_dim) in D join the block's pages, k rotated by its position; the result is q (rows, n_heads, head_dim), rotated
         likewise (None without q)."""
-        k, v = self._in(k, "k", self._kv), self._in(v, "v", self._kv)
-        out, at, tok = None, 0, 0
+        k, k_at, k_tok = self._in(k, "k", self._kv_size)
+        v, v_at, v_tok = self._in(v, "v", self._kv_size)
+        out, q_at, q_tok, out_at = None, 0, 0, 0
         if q is not None:
-            q = self._in(q, "q", self._heads)
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            at, tok = q.data_ptr(), q.stride(0)
-        check(self._lib.cake_b200_pages_append(self.h, block_idx, at, tok, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-                                               out.data_ptr() if at else 0, 1 if rotate else 0, self._stream()))
+            q, q_at, q_tok = self._in(q, "q", self._q_size)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out_at = out.data_ptr()
+        rc = self._lib.cake_b200_pages_append(self.h, block_idx, q_at, q_tok, k_at, k_tok, v_at, v_tok, out_at, 1 if rotate else 0, self._stream())
+        if rc:
+            check(rc)
         return out
 
     def attend(self, block_idx: int, q: torch.Tensor, window: int = 0, scale: float = 0.0) -> torch.Tensor:
         """Attention of the step's rows q (rows, n_heads, head_dim) in D over their sequences: a row at position p sees the positions up to p, with a window
         only the last ``window`` of them.  scale 0: head_dim^-1/2.  (rows, n_heads, head_dim) in D."""
-        q = self._in(q, "q", self._heads)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        check(self._lib.cake_b200_pages_attend(self.h, block_idx, q.data_ptr(), q.stride(0), out.data_ptr(), window, scale, self._stream()))
+        q, q_at, q_tok = self._in(q, "q", self._q_size)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        rc = self._lib.cake_b200_pages_attend(self.h, block_idx, q_at, q_tok, out.data_ptr(), window, scale, self._stream())
+        if rc:
+            check(rc)
         return out
 
     def read(self, block_idx: int, seq: Optional[int] = None, first: int = 0, n: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """(K, V), each (rows, n_kv, head_dim) in D, as the block's pages hold them: the step's rows, or positions [first, first + n) (to the end without n)
         of one sequence."""
         if seq is None:
-            n = self._rows
+            seq, n = -1, self._rows
         elif n is None:
             n = self.len(seq) - first
-        k, v = (torch.empty(max(n, 0), self._kv, self._hd, dtype=self._dtype, device=self.ctx.torch_device) for _ in range(2))
-        check(self._lib.cake_b200_pages_read(self.h, block_idx, -1 if seq is None else seq, first, n, k.data_ptr(), v.data_ptr(), self._stream()))
+        k, v = torch.empty((2, n if n > 0 else 0, self._kv, self._hd), dtype=self._dtype, device=self._device).unbind()
+        rc = self._lib.cake_b200_pages_read(self.h, block_idx, seq, first, n, k.data_ptr(), v.data_ptr(), self._stream())
+        if rc:
+            check(rc)
         return k, v
 
     def __del__(self):
