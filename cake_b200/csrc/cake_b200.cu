@@ -166,6 +166,7 @@ struct cake_b200_ctx {
   struct Staging { void *p = nullptr; size_t cap = 0; cudaEvent_t done = nullptr; bool busy = false; } pg_stage[4];
   unsigned pg_next = 0;
   float *pg_cos = nullptr, *pg_sin = nullptr;   // (one piece)
+  pg::Clusters pg_clusters{};
   unsigned long long pc_on = 0;   // the id of the stream that pc_out was recorded on last and nobody has waited for yet; 0: none
   bool pc_behind = true;
   // head of a batch: its logits where the caller keeps none, its tokens

@@ -10,17 +10,20 @@ namespace cake {
 namespace pg {
 
 template <typename... KArgs, typename... Args>
-static int launch(cudaStream_t s, uint64_t *launches, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+static int launch(cudaStream_t s, uint64_t *launches, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
   if (e == cudaSuccess) ++*launches;
   return (int)e;
@@ -143,7 +146,7 @@ int append(cudaStream_t s, int dtype, const Pool &p, const Append &a, int sms, u
   while (parts < groups && (long)a.n_rows * parts < 16l * sms) parts++;
   return by_type(dtype, [&](auto t) {
     typedef typename decltype(t)::type T;
-    return launch(s, launches, append_kernel<T>, dim3((unsigned)((a.n_rows + 3) / 4), (unsigned)parts), dim3(128), 0, p, a, parts);
+    return launch(s, launches, append_kernel<T>, dim3((unsigned)((a.n_rows + 3) / 4), (unsigned)parts), dim3(128), 0, 1, p, a, parts);
   });
 }
 
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Pool p, const Read a) {
 }
 int read(cudaStream_t s, int, const Pool &p, const Read &a, uint64_t *launches) {
   const size_t n = (size_t)a.n * p.n_kv * (p.hd >> 3);
-  return launch(s, launches, read_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 148 * 32)), dim3(256), 0, p, a);
+  return launch(s, launches, read_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 148 * 32)), dim3(256), 0, 1, p, a);
 }
 
 // ------------------------------------------------------------------------------------------ attention
@@ -182,15 +185,48 @@ template <typename F> static int by_kind(int dtype, int hd, F &&f) {
     }
   });
 }
-int prepare(int dtype, int hd) {
+int prepare(int dtype, int hd, Clusters *out) {
   return by_kind(dtype, hd, [&](auto t, auto h) {
     typedef typename decltype(t)::type T;
     constexpr int HD = decltype(h)::value;
-    cudaError_t e = cudaFuncSetAttribute(few_kernel<T, HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 1>::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_kernel<T, HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<HD, 2>::SMEM);
+    cudaError_t e = cudaSuccess;
+    auto few = [&](auto n) {
+      constexpr int NT = decltype(n)::value, SMEM = FewCfg<HD, NT>::SMEM;
+      for (auto k : {few_kernel<T, HD, NT, false>, few_kernel<T, HD, NT, true>})
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+      for (int i = 0; i < 4 && e == cudaSuccess; i++) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 1u << i;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(1u << i);
+        cfg.blockDim = dim3(FEW_THREADS);
+        cfg.dynamicSmemBytes = SMEM;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&out->most[NT - 1][i], few_kernel<T, HD, NT, true>, &cfg);
+      }
+    };
+    few(std::integral_constant<int, 1>{});
+    few(std::integral_constant<int, 2>{});
     if (e == cudaSuccess) e = cudaFuncSetAttribute(tiles_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileCfg<HD>::SMEM);
     return (int)e;
   });
+}
+// A cluster's CTAs for each run, or 0: shares.  One launch without a list, whose sums meet in shared memory, is the faster way where all clusters are on the chip
+// at once and no CTA has many more tiles than an equal share.  Clusters / shares in us (shares in a graph; alone their second launch costs 2 more of the
+// host's), sequences x positions:  8 key heads of 128, 1 x 500 7.1 (the host's) / 5.7, 1 x 4000 9.7 / 12.1, 4 x 1000 7.1 / 9.8, 9 x 500 7.4 / 8.8, 9 x 2000 (16 tiles a CTA,
+// an equal share 8) 15.0 / 13.9, 16 x 1000 10.7 / 11.7, 32 x 1000 23.5 / 27.3, 32 x 4000 81 / 84;  2 of 64, 1 x 4000 8.4 / 7.1, 32 x 1000 7.1 / 8.2, 64 x 4000 25 / 28;  4 of 256,
+// 2 x 2000 8.0 / 12.4, 4 x 4000 (16 tiles, 7) 15.9 / 14.8, 16 x 1000 11.1 / 12.6.
+constexpr int CLUSTER_TILES = 8;
+static int cluster_of(int runs, int longest, int tiles, int ctas, const int (&most)[4]) {
+  int best = 0;
+  for (int k = 0; k < 4 && 1 << k < 2 * longest; k++) {
+    const int mine = (longest + (1 << k) - 1) >> k;
+    if (runs <= most[k] && (mine <= CLUSTER_TILES || mine <= 1.5 * tiles / ctas)) best = 1 << k;
+  }
+  return best;
 }
 int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scratch &w, uint64_t *launches) {
   const int G = a.n_heads / p.n_kv;
@@ -198,14 +234,17 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
   if (a.n_few) {
     const Few f{p, a.plan, a.seqs, a.q, a.q_tok, a.out, w.few_ws, a.n_heads, G, a.win, scale_log2, a.err, a.n_items ? 1 : 0};
     const Cut *cuts = reinterpret_cast<const Cut *>(reinterpret_cast<const Worker *>(a.plan + 1) + few_ctas(p.hd, w.sms));
+    const int cluster = a.longest ? cluster_of(a.n_few * p.n_kv, a.longest, a.tiles, few_ctas(p.hd, w.sms), w.clusters->most[a.few_cols <= 8 ? 0 : 1]) : 0;
     const int e = by_kind(dtype, p.hd, [&](auto t, auto h) {
       typedef typename decltype(t)::type T;
       constexpr int HD = decltype(h)::value;
       auto both = [&](auto n) {
         constexpr int NT = decltype(n)::value;
-        const int rc = launch(s, launches, few_kernel<T, HD, NT>, dim3((unsigned)few_ctas(HD, w.sms)), dim3(FEW_THREADS), FewCfg<HD, NT>::SMEM, f);
+        if (cluster)
+          return launch(s, launches, few_kernel<T, HD, NT, true>, dim3((unsigned)(a.n_few * p.n_kv * cluster)), dim3(FEW_THREADS), FewCfg<HD, NT>::SMEM, cluster, f);
+        const int rc = launch(s, launches, few_kernel<T, HD, NT, false>, dim3((unsigned)few_ctas(HD, w.sms)), dim3(FEW_THREADS), FewCfg<HD, NT>::SMEM, 1, f);
         if (rc || !a.n_cuts) return rc;
-        return launch(s, launches, few_join_kernel<T, HD, NT>, dim3((unsigned)a.n_cuts, (unsigned)a.few_cols), dim3(128), 0, f, cuts);
+        return launch(s, launches, few_join_kernel<T, HD, NT>, dim3((unsigned)a.n_cuts, (unsigned)a.few_cols), dim3(128), 0, 1, f, cuts);
       };
       return a.few_cols <= 8 ? both(std::integral_constant<int, 1>{}) : both(std::integral_constant<int, 2>{});
     });
@@ -217,9 +256,9 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
   return by_kind(dtype, p.hd, [&](auto t, auto h) {
     typedef typename decltype(t)::type T;
     constexpr int HD = decltype(h)::value;
-    const int e = launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, t8);
+    const int e = launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, 1, t8);
     if (e || !a.cut) return e;
-    return launch(s, launches, join_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv * (HD / 32))), dim3(128), 0, t8);
+    return launch(s, launches, join_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv * (HD / 32))), dim3(128), 0, 1, t8);
   });
 }
 

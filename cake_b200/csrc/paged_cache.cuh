@@ -67,12 +67,15 @@ struct PlanHead { int W, n_cuts, n_items, parts, pad[4]; };   // workers, cut ru
 struct Scratch {
   float *few_ws, *tiles_ws;      // few_floats; tiles_floats (nullptr: the step has no sequence of many rows)
   int sms;
+  const struct Clusters *clusters;
 };
+// clusters of 1, 2, 4 and 8 CTAs of the few-row kernel (up to 8 query rows, up to 16) that are on the chip at once
+struct Clusters { int most[2][4]; };
 int few_ctas(int hd, int sms);             // CTAs of the few-row kernel: no more workers than that
 int room(int hd, int sms, int n_kv);       // items of the many-row kernel that fill the chip (parts of cut ones: twice as many at most)
 size_t few_floats(int hd, int sms);
 size_t tiles_floats(int hd, int sms, int n_kv);
-int prepare(int dtype, int hd);            // once per device and kind of cache, in front of the first call
+int prepare(int dtype, int hd, Clusters *);   // once per device and kind of cache, in front of the first call
 struct Attend {
   const void *q;
   long long q_tok;               // multiple of 8
@@ -83,6 +86,7 @@ struct Attend {
   Window win;
   const PlanHead *plan;
   int n_few, few_cols;           // sequences of few rows, query rows of a key head that they have at most
+  int longest, tiles;            // tiles of their longest run, of all; 0: a captured call, whose lengths may become any
   int n_cuts, n_items;           // runs that are cut, items of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
   bool cut;                      // some of the items are parts (of a captured call: may be)
   int *err;

@@ -87,6 +87,16 @@ __device__ __forceinline__ void bulk_copy(void *dst, const void *src, uint32_t b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
                "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ int dev_first(const SeqRow &s, const Window &w) {   // first_seen
   if (w.w <= 0) return 0;
   if (w.by_call) return s.pos0 > 0 ? max(0, s.pos0 + s.count - w.w) : 0;
@@ -119,7 +129,8 @@ struct Walk {
   }
 };
 
-template <typename T, int HD, int NT>
+// CLUSTER: no list of shares; a cluster of CTAs has a run, whose tiles they cut between them, and joins their sums over its shared memory
+template <typename T, int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(const Few a) {
   typedef FewCfg<HD, NT> C;
   extern __shared__ __align__(128) unsigned char few_smem[];
@@ -144,16 +155,30 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
     __syncthreads();
   }
   pdl_launch_dependents();
-  if (!same_step(a.pool) || (int)blockIdx.x >= a.plan->W) {   // (nothing in flight, no barrier ahead of anybody)
+  if (!same_step(a.pool) || (!CLUSTER && (int)blockIdx.x >= a.plan->W)) {   // (nothing in flight, no barrier ahead of anybody)
     pdl_wait();
     return;
   }
   Walk w;
-  {
+  const int size = CLUSTER ? (int)cluster_size() : 1, rank = CLUSTER ? (int)cluster_rank() : 0;
+  if (CLUSTER) {
+    const int run = (int)blockIdx.x / size;
+    w.i = run / a.pool.n_kv;
+    w.kvh = run - w.i * a.pool.n_kv;
+    const int4 v = __ldg(reinterpret_cast<const int4 *>(a.seqs + w.i));
+    w.s = SeqRow{v.x, v.y, v.z, v.w};
+    w.run(a.win);
+    w.tile = w.n * rank / size;
+    w.left = w.n * (rank + 1) / size - w.tile;
+  } else {
     const int4 *x = reinterpret_cast<const int4 *>(reinterpret_cast<const Worker *>(a.plan + 1) + blockIdx.x);
     const int4 u = __ldg(x), v = __ldg(x + 1);
     w.start(Worker{u.x, u.y, u.z, u.w, SeqRow{v.x, v.y, v.z, v.w}}, a.win);
   }
+  // (a cluster's sums of this CTA, where its tiles were)
+  float *sums = reinterpret_cast<float *>(ring);
+  float2 *tops = reinterpret_cast<float2 *>(ring + C::COLS * HD * 4);
+  const int all_cols = w.s.count * a.G;
   int left = MBAR_TRIES, in_ring = 0;
   if (warp == FEW_WARPS) {
     // ---- copies.  A lane has one piece (a page, or 64 rows of one) of a batch of tiles; the next batch's pages are looked up ahead
@@ -385,7 +410,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
 #pragma unroll
           for (int e = 0; e < 4; e++) red[in_red(warp, 8 * x + 2 * t + (e & 1), 16 * i + g + (e >> 1) * 8)] = o[x][i][e];
       named_bar_sync(1, 32 * FEW_WARPS);
-      const bool whole = w.tile == 0 && n == w.n;
+      const bool whole = CLUSTER ? size == 1 : w.tile == 0 && n == w.n;
       const int per = HD / 4;   // pieces of four entries of a column
       auto store = [&](int c, int d, float4 v, float inv) {
         const int tok = c / a.G;
@@ -412,15 +437,57 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
           v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
         }
         if (whole) store(c, d, v, 1.0f / L);
-        else {
+        else if (CLUSTER) {
+          *reinterpret_cast<float4 *>(sums + c * HD + d) = v;
+          if (d == 0) tops[c] = make_float2(M, L);
+        } else {
           __stcg(reinterpret_cast<float4 *>(place(mine) + c * HD + d), v);
           if (d == 0) __stcg(reinterpret_cast<float2 *>(place(mine) + C::COLS * HD) + c, make_float2(M, L));
         }
       }
+      if (CLUSTER) break;
       named_bar_sync(1, 32 * FEW_WARPS);   // (red and ml are free again)
       w.next(a, n);
     }
     if (left == 0) *gave_up = 1;
+  }
+  if (CLUSTER && size > 1) {
+    if (w.left == 0)   // fewer tiles than CTAs
+      for (int c = threadIdx.x; c < all_cols; c += FEW_THREADS) tops[c] = make_float2(-INFINITY, 0.f);
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    for (int u = rank * FEW_THREADS + (int)threadIdx.x; u < all_cols * (HD / 4); u += size * FEW_THREADS) {
+      const int c = u / (HD / 4), d = 4 * (u - c * (HD / 4)), tok = c / a.G;
+      const uint32_t of_sums = smem_u32(sums + c * HD + d), of_tops = smem_u32(tops + c);
+      float M = -INFINITY, L = 0.f;
+      float2 m[8];
+      float4 y[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        m[k] = make_float2(-INFINITY, 0.f);
+        y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < size) {
+          m[k] = ld_cluster_f2(cluster_map(of_tops, (uint32_t)k));
+          y[k] = ld_cluster_f4(cluster_map(of_sums, (uint32_t)k));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) M = fmaxf(M, m[k].x);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const bool none = m[k].x == -INFINITY && m[k].y == 0.f;   // (a CTA without tiles, or one of rows that see none of them: its sums are not there, or 0)
+        const float f = none ? 0.f : m[k].x == -INFINITY ? 1.f : ex2((m[k].x - M) * a.scale_log2);
+        L = fmaf(m[k].y, f, L);
+        if (!none) { v.x = fmaf(y[k].x, f, v.x); v.y = fmaf(y[k].y, f, v.y); v.z = fmaf(y[k].z, f, v.z); v.w = fmaf(y[k].w, f, v.w); }
+      }
+      const float inv = 1.0f / L;
+      *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + ((size_t)(w.s.row0 + tok) * a.n_heads + w.kvh * a.G + c - tok * a.G) * HD + d) =
+          make_uint2(pack2x<T>(v.x * inv, v.y * inv), pack2x<T>(v.z * inv, v.w * inv));
+    }
+    __syncwarp();
+    cluster_arrive();   // (nobody leaves while another reads its sums)
+    cluster_wait();
   }
   __syncthreads();
   if (*gave_up && threadIdx.x == 32 * FEW_WARPS)   // a wait was given up: copies in flight end before the CTA does

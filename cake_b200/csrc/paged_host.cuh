@@ -18,7 +18,7 @@ struct cake_b200_pages {
     pg::Window win;
     unsigned long long step = 0, used = 0;   // made for this step; last used in this call
     bool kept = false;                       // captured calls read it: it is made anew with every step
-    int n_cuts = 0, n_items = 0, most_items = 0;   // cut runs; items of the many-row kernel, now and for any lengths of this shape
+    int longest = 0, tiles = 0, n_cuts = 0, n_items = 0, most_items = 0;   // tiles of the longest run of few rows, of all; cut runs; items of the many-row kernel, now and for any lengths of this shape
     bool cut = false;                        // some are parts of tiles
     char *dev = nullptr;
   } plans[8];
@@ -115,7 +115,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
   CU(cudaMallocHost(&g->bad, 4));
   *g->bad = 0;
-  CU((cudaError_t)pg::prepare(f.dtype, f.head_dim));
+  if (!c->pg_clusters.most[0][0]) CU((cudaError_t)pg::prepare(f.dtype, f.head_dim, &c->pg_clusters));
   const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
                s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -213,6 +213,12 @@ static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // 
   RC(pages_upload(c, p->dev, blob.data(), blob.size()));
   int tiles = 0;
   for (size_t i = 0; i < many.size(); i++) tiles += many[i].part == 0;
+  p->longest = p->tiles = 0;
+  for (int i = 0; i < g->book.n_few; i++) {
+    const int t = pg::tiles_of(g->book.step[(size_t)i], p->win);
+    p->longest = std::max(p->longest, t);
+    p->tiles += t * n_kv;
+  }
   p->n_cuts = h.n_cuts;
   p->n_items = h.n_items;
   p->most_items = tiles ? tiles + 2 * room : 0;
@@ -334,8 +340,8 @@ static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_to
   const int most_cuts = std::min(g->book.n_few * c->cfg.n_kv_heads, pg::few_ctas(c->cfg.head_dim, c->sm_count));
   for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
   const pg::Attend a{q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), c->cfg.n_heads, scale, win, (const pg::PlanHead *)plan->dev, g->book.n_few, cols,
-                     capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, capturing || plan->cut, c->wait_err};
-  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count}, launch_counter(c)));
+                     capturing ? 0 : plan->longest, plan->tiles, capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, capturing || plan->cut, c->wait_err};
+  CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count, &c->pg_clusters}, launch_counter(c)));
   return CAKE_B200_OK;
 }
 extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,
