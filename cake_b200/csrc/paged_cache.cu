@@ -53,101 +53,114 @@ int spread(cudaStream_t s, const StepHead *step, int max_seqs, int n_seqs, int n
 }
 
 // ------------------------------------------------------------------------------------------ rows into the pages
-// Bound by memory: what comes in goes out.  A lane has 16 bytes of a row, hd / 8 lanes a head, a warp 32 / (hd / 8) heads of a token at once and, where the
-// tokens alone do not fill the chip, a part of its heads; the row of the tables is read once a warp.  A pair's other entry comes from the lane that has it.
-// Norm and rotation in fp32 and one rounding; in a block's step they are rounded where the blocks' other paths round them (the normed entries, the products),
-// so that its rows are those that any other cache would hold: logits of three layers within 4 units in the last place of the oracle, else up to 6.
+// Bound by memory: what comes in goes out.  A lane has two 16-byte chunks of a head, those of a rotation's pairs (entries e .. e + 7 and e + rot / 2 ..) or, behind the
+// rotated entries, two neighbours: no exchange between lanes.  hd / 16 lanes a head, 512 / hd heads of a token a warp at once, several times that asked for
+// before the first is worked on; where the tokens alone do not fill the chip, a warp has a part of a token's heads.  The row of the tables is read once a warp.
+// 12314 rows of 48 heads of 128: a chunk a lane, its pair's other one by 8 exchanges, 73 us with 2 loads in flight and 66 with 4; so 50.
+// Norm and rotation in fp32 and one rounding; in a block's step (BLOCKS) they are rounded where the blocks' other paths round them (the normed entries, the
+// products), so that its rows are those that any other cache would hold: logits of three layers within 4 units in the last place of the oracle, else up to 6.
 template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {
   const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return (w & e) == e || (w >> 16 & e) == e;
 }
-template <typename T>
+template <typename T> __device__ __forceinline__ bool not_finite(const uint4 &w) { return not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w); }
+template <typename T> __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+}
+template <typename T, int HD, bool BLOCKS>
 __global__ void __launch_bounds__(128) append_kernel(const Pool p, const Append a, int parts) {
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cph = p.hd >> 3, at_once = 32 / cph, c = lane & (cph - 1), sub = lane / cph;
+  constexpr int LPH = HD / 16, AT_ONCE = 32 / LPH, U = 4;   // lanes of a head; heads of a warp at once; such groups asked for at once
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pair = lane % LPH, sub = lane / LPH;
   const int row = blockIdx.x * 4 + warp, heads = a.n_q + 2 * p.n_kv;
+  const int h8 = a.cos_t ? a.rot >> 4 : 0;   // chunks of the pairs' first entries
+  const bool turns = pair < h8;
+  const int c0 = turns ? pair : 2 * h8 + 2 * (pair - h8), c1 = turns ? pair + h8 : c0 + 1;
   pdl_wait();
   if (!same_step(p) || row >= a.n_rows) return;
   const int2 at = __ldg(a.rows + row);
   const int page = page_of(p, at.x, at.y), r = at.y & ((1 << p.page_log2) - 1);
-  const int h8 = a.rot >> 4;   // chunks of the pairs' first entries
-  const bool turns = a.cos_t && c < 2 * h8, low = c < h8;
-  const int other = lane - c + (turns ? (low ? c + h8 : c - h8) : c);
   float cs[8], sn[8];
-  if (turns) {
-    const size_t o = (size_t)at.y * (8 * h8) + 8 * (low ? c : c - h8);
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4 *>(a.cos_t + o + i)), y = __ldg(reinterpret_cast<const float4 *>(a.sin_t + o + i));
-      cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
-      sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
-    }
+  for (int i = 0; i < 8; i += 4) {
+    const size_t o = (size_t)at.y * (8 * h8) + 8 * pair + i;
+    const float4 x = turns ? __ldg(reinterpret_cast<const float4 *>(a.cos_t + o)) : make_float4(1.f, 1.f, 1.f, 1.f);
+    const float4 y = turns ? __ldg(reinterpret_cast<const float4 *>(a.sin_t + o)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
+    sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
   }
-  constexpr int U = 4;   // loads of a warp in flight (12314 rows of 48 heads: 73 us with two)
-  for (int g0 = blockIdx.y; g0 * at_once < heads; g0 += U * parts) {
-    uint4 in4[U];
+  const T *q = reinterpret_cast<const T *>(a.q) + (size_t)row * a.q_tok, *k = reinterpret_cast<const T *>(a.k) + (size_t)row * a.k_tok,
+          *v = reinterpret_cast<const T *>(a.v) + (size_t)row * a.v_tok;
+  for (int g0 = blockIdx.y; g0 * AT_ONCE < heads; g0 += U * parts) {
+    uint4 in[U][2];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int head = (g0 + u * parts) * at_once + sub;
-      const T *src = head < a.n_q ? reinterpret_cast<const T *>(a.q) + (size_t)row * a.q_tok + (size_t)head * p.hd
-                     : head < a.n_q + p.n_kv ? reinterpret_cast<const T *>(a.k) + (size_t)row * a.k_tok + (size_t)(head - a.n_q) * p.hd
-                                             : reinterpret_cast<const T *>(a.v) + (size_t)row * a.v_tok + (size_t)(head - a.n_q - p.n_kv) * p.hd;
-      in4[u] = head < heads ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+      const int head = (g0 + u * parts) * AT_ONCE + sub;
+      if (head < heads) {
+        const T *src = head < a.n_q ? q + (size_t)head * HD : head < a.n_q + p.n_kv ? k + (size_t)(head - a.n_q) * HD : v + (size_t)(head - a.n_q - p.n_kv) * HD;
+        in[u][0] = *reinterpret_cast<const uint4 *>(src + 8 * c0);
+        in[u][1] = *reinterpret_cast<const uint4 *>(src + 8 * c1);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if ((g0 + u * parts) * at_once >= heads) break;   // (the same for all lanes)
-      const int head = (g0 + u * parts) * at_once + sub;
-      const bool in = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + p.n_kv;
-      const int h = is_q ? head : is_v ? head - a.n_q - p.n_kv : head - a.n_q;
-      uint4 w = in4[u];
-      const bool dirty = in && is_v && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w));
+      const int head = (g0 + u * parts) * AT_ONCE + sub;
+      const bool there = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + p.n_kv;
       const T *nw = reinterpret_cast<const T *>(is_q ? a.q_norm : a.k_norm);
-      if (a.cos_t || a.q_norm || a.k_norm) {   // (the same for all lanes, as the exchanges have to be)
-        float x[8], y[8];
-        unpack8<T>(w, x);
-        if (a.q_norm || a.k_norm) {
-          float ss = 0.f;
+      float inv = 0.f;
+      if (BLOCKS && (a.q_norm || a.k_norm)) {   // (the same for all lanes, as the exchanges have to be)
+        float x[8], y[8], ss = 0.f;
+        unpack8<T>(in[u][0], x);
+        unpack8<T>(in[u][1], y);
 #pragma unroll
-          for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-          for (int o = 1; o < cph; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (nw && !is_v) {
-            const float inv = 1.0f / sqrtf(ss / (float)p.hd + a.eps);
-            float g8[8];
-            unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c), g8);
+        for (int i = 0; i < 8; i++) ss += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = a.as_blocks ? rnd<T>(x[i] * inv * g8[i]) : x[i] * inv * g8[i];
-          }
-        }
-        if (a.cos_t) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other);
-          if (turns && !is_v)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const float f = x[i] * cs[i], s = low ? -y[i] * sn[i] : y[i] * sn[i];
-              x[i] = a.as_blocks ? rnd<T>(f) + rnd<T>(s) : f + s;
-            }
-        }
-        if (!is_v) w = make_uint4(pack2x<T>(x[0], x[1]), pack2x<T>(x[2], x[3]), pack2x<T>(x[4], x[5]), pack2x<T>(x[6], x[7]));
+        for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
       }
-      if (in) {
-        void *to = is_q ? (void *)(reinterpret_cast<T *>(a.q_out) + (size_t)row * a.out_tok + (size_t)h * p.hd + 8 * c) : (void *)(rows_of(p, page, h, is_v) + chunk_at(p.hd, r, c));
-        *reinterpret_cast<uint4 *>(to) = w;
-        if (dirty) p.marks[(size_t)page * p.n_kv + h] = 1u;
+      if (!there) continue;
+      if (is_v) {
+        const int h = head - a.n_q - p.n_kv;
+        char *to = rows_of(p, page, h, 1);
+        *reinterpret_cast<uint4 *>(to + chunk_at(HD, r, c0)) = in[u][0];
+        *reinterpret_cast<uint4 *>(to + chunk_at(HD, r, c1)) = in[u][1];
+        if (not_finite<T>(in[u][0]) || not_finite<T>(in[u][1])) p.marks[(size_t)page * p.n_kv + h] = 1u;
+        continue;
+      }
+      if (turns || (BLOCKS && nw)) {
+        float x[8], y[8];
+        unpack8<T>(in[u][0], x);
+        unpack8<T>(in[u][1], y);
+        if (BLOCKS && nw) {
+          float g[8];
+          unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c0), g);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = rnd<T>(x[i] * inv * g[i]);
+          unpack8<T>(*reinterpret_cast<const uint4 *>(nw + 8 * c1), g);
+#pragma unroll
+          for (int i = 0; i < 8; i++) y[i] = rnd<T>(y[i] * inv * g[i]);
+        }
+        if (turns)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float s = x[i], t = y[i];
+            x[i] = BLOCKS ? rnd<T>(s * cs[i]) - rnd<T>(t * sn[i]) : s * cs[i] - t * sn[i];
+            y[i] = BLOCKS ? rnd<T>(t * cs[i]) + rnd<T>(s * sn[i]) : t * cs[i] + s * sn[i];
+          }
+        in[u][0] = pack8<T>(x);
+        in[u][1] = pack8<T>(y);
+      }
+      if (is_q) {
+        T *to = reinterpret_cast<T *>(a.q_out) + (size_t)row * a.out_tok + (size_t)head * HD;
+        *reinterpret_cast<uint4 *>(to + 8 * c0) = in[u][0];
+        *reinterpret_cast<uint4 *>(to + 8 * c1) = in[u][1];
+      } else {
+        char *to = rows_of(p, page, head - a.n_q, 0);
+        *reinterpret_cast<uint4 *>(to + chunk_at(HD, r, c0)) = in[u][0];
+        *reinterpret_cast<uint4 *>(to + chunk_at(HD, r, c1)) = in[u][1];
       }
     }
   }
-}
-int append(cudaStream_t s, int dtype, const Pool &p, const Append &a, int sms, uint64_t *launches) {
-  const int at_once = 256 / p.hd, groups = (a.n_q + 2 * p.n_kv + at_once - 1) / at_once;
-  int parts = 1;
-  while (parts < groups && (long)a.n_rows * parts < 16l * sms) parts++;
-  return by_type(dtype, [&](auto t) {
-    typedef typename decltype(t)::type T;
-    return launch(s, launches, append_kernel<T>, dim3((unsigned)((a.n_rows + 3) / 4), (unsigned)parts), dim3(128), 0, 1, p, a, parts);
-  });
 }
 
 // ------------------------------------------------------------------------------------------ rows out of the pages
@@ -183,6 +196,16 @@ template <typename F> static int by_kind(int dtype, int hd, F &&f) {
       case 128: return f(t, std::integral_constant<int, 128>{});
       default: return f(t, std::integral_constant<int, 256>{});
     }
+  });
+}
+int append(cudaStream_t s, int dtype, const Pool &p, const Append &a, int sms, uint64_t *launches) {
+  const int at_once = 512 / p.hd, groups = (a.n_q + 2 * p.n_kv + at_once - 1) / at_once;
+  int parts = 1;
+  while (parts < groups && (long)a.n_rows * parts < 16l * sms) parts++;
+  return by_kind(dtype, p.hd, [&](auto t, auto h) {
+    typedef typename decltype(t)::type T;
+    constexpr int HD = decltype(h)::value;
+    return launch(s, launches, a.as_blocks ? append_kernel<T, HD, true> : append_kernel<T, HD, false>, dim3((unsigned)((a.n_rows + 3) / 4), (unsigned)parts), dim3(128), 0, 1, p, a, parts);
   });
 }
 int prepare(int dtype, int hd, Clusters *out) {

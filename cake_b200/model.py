@@ -159,9 +159,11 @@ class PagedCache:
         self.max_seq = max_seq or ctx.max_seq
         c = ctx.config
         self._heads, self._kv, self._hd, self._dtype = c.num_attention_heads, c.num_key_value_heads, c.hd, ctx.torch_dtype
-        self._dev, self._device = ctx.device, ctx.torch_device
+        self._dev = ctx.device
         self._rows = 0   # of the present step
         self._q_size, self._kv_size = (torch.Size((0, heads, self._hd)) for heads in (self._heads, self._kv))
+        self._one = torch.empty(1, dtype=self._dtype, device=ctx.torch_device)   # (a new tensor like one that is there takes half the time of one by its size)
+        self._kv_like = self._one.expand(self._kv_size)
         self.h = c_void_p()
         self._lib = lib()
         cos = sin = None
@@ -216,6 +218,7 @@ class PagedCache:
         check(self._lib.cake_b200_pages_step(self.h, int_array(seqs), int_array(counts), len(seqs), self._stream()))
         self._rows = sum(counts)
         self._q_size, self._kv_size = (torch.Size((self._rows, heads, self._hd)) for heads in (self._heads, self._kv))
+        self._kv_like = self._one.expand(self._kv_size)
 
     def _in(self, t: torch.Tensor, name: str, size: torch.Size) -> Tuple[torch.Tensor, int, int]:
         """(rows, heads, hd) as the library takes them, heads side by side on 16-byte boundaries (copied where they are not), their address and their rows' stride."""
@@ -259,10 +262,11 @@ class PagedCache:
         """(K, V), each (rows, n_kv, head_dim) in D, as the block's pages hold them: the step's rows, or positions [first, first + n) (to the end without n)
         of one sequence."""
         if seq is None:
-            seq, n = -1, self._rows
-        elif n is None:
-            n = self.len(seq) - first
-        k, v = torch.empty((2, n if n > 0 else 0, self._kv, self._hd), dtype=self._dtype, device=self._device).unbind()
+            seq, n, like = -1, self._rows, self._kv_like
+        else:
+            n = self.len(seq) - first if n is None else n
+            like = self._one.expand(max(n, 0), self._kv, self._hd)
+        k, v = (torch.empty_like(like, memory_format=torch.contiguous_format), torch.empty_like(like, memory_format=torch.contiguous_format))
         rc = self._lib.cake_b200_pages_read(self.h, block_idx, seq, first, n, k.data_ptr(), v.data_ptr(), self._stream())
         if rc:
             check(rc)
