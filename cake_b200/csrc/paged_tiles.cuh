@@ -23,6 +23,7 @@ template <int HD> struct TileCfg {
   static constexpr int TMEM = HD == 256 ? 512 : 256;   // S and P: columns 0 .. 63 and 64 .. 127; O from 128
   static constexpr int CTAS = HD == 256 ? 1 : 2;
   static constexpr size_t PART = (size_t)TILE_ROWS * (HD + 2);   // floats of a part: O as [HD / 4][row][4], then (m, l) of the rows
+  static_assert(128 + HD <= TMEM && CTAS * TMEM <= 512 && CTAS * (SMEM + 1024) <= 228 * 1024, "TMEM columns, shared memory");
 };
 struct Tiles {
   Pool pool;
@@ -39,6 +40,58 @@ struct Tiles {
   int beside;            // the few-row kernel in front of this one waited for what both read: this one waits for it at its end
 };
 
+// two fp32 numbers in one operation
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 of_two(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 32 columns on their way; tc_wait_ld in front of their use
+__device__ __forceinline__ void tc_ld32_go(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// (the registers pass through it, so that nothing that uses them is moved in front; an asm takes no more than 30 operands)
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                 "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ float tc_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
@@ -88,7 +141,8 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
   }
   const int G = a.G, n_tok = min(a.tpt, it.s.count - it.tok0), rows = G * n_tok, n_tiles = it.t1 - it.t0;
   const int p0 = it.s.pos0 + it.tok0, kv_end = p0 + n_tok;   // the first token's position; keys that the last one sees
-  const int row = (warp & 3) * 32 + lane, tok = row / G;
+  const uint32_t by_G = (65536u + (uint32_t)G - 1u) / (uint32_t)G;   // r / G = r by_G >> 16 for r < 128, G <= 128
+  const int row = (warp & 3) * 32 + lane, tok = (int)((uint32_t)row * by_G >> 16);
   const int by_call = a.win.w > 0 && a.win.by_call ? dev_first(it.s, a.win) : 0;
   const int late = a.win.w <= 0 ? 0 : a.win.by_call ? by_call : max(0, kv_end - a.win.w);   // what the last token begins at
 
@@ -101,7 +155,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     Chunks x;
 #pragma unroll
     for (int i = 0; i < FEW; i++) {
-      const int r = qr + (i0 + i) * BY, tk = r / G;
+      const int r = qr + (i0 + i) * BY, tk = (int)((uint32_t)r * by_G >> 16);
       x.v[i] = r < rows ? __ldcg(reinterpret_cast<const uint4 *>(q + (size_t)tk * a.q_tok + (size_t)(r - tk * G) * HD)) : make_uint4(0u, 0u, 0u, 0u);
     }
     return x;
@@ -150,7 +204,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
         const int j = j0 + t, st = j & 1, at = (it.t0 + j) * TILE, mine = at + piece * pr;
         uint64_t *full = values ? &v_full[st] : &k_full[st];
         if (j >= 2) {
-          mbar_wait_lim(values ? &v_empty[st] : &k_empty[st], (uint32_t)((j >> 1) - 1) & 1u, a.err, left);
+          mbar_wait_lim(values ? &v_empty[st] : &k_empty[st], (uint32_t)(j / 2 - 1) & 1u, a.err, left);
           if (__any_sync(0xffffffffu, left == 0)) left = 0;
         }
         const int of_tile = min(TILE, (kv_end - at + 15) & ~15), of_piece = min(pr, max(0, (kv_end - mine + 15) & ~15));
@@ -189,11 +243,11 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
   } else if (warp == 5) {
     // ---- products (one thread issues them; the warp runs the loop with it)
     const uint32_t one = elect_one();
-    const uint32_t idesc_s = tc_idesc<T>(TILE), idesc_o = tc_idesc<T>(HD) | (1u << 16);   // M128 N64, both K-major; M128 N hd, A from TMEM, B (V) MN-major
+    const uint32_t idesc_s = tc_idesc<T>(TILE), idesc_o = tc_idesc<T>(HD) | (1u << 16);   // M128 N TILE, both K-major; M128 N hd, A from TMEM, B (V) MN-major
     uint32_t mark = 0u, next_mark = 0u;   // of tiles j and j + 1
     auto issue_s = [&](int j) {   // S_j = Q K_j^T into S buffer j & 1
       const int st = j & 1;
-      mbar_wait_lim(&k_full[st], (uint32_t)(j >> 1) & 1u, a.err, left);
+      mbar_wait_lim(&k_full[st], (uint32_t)(j / 2) & 1u, a.err, left);
       __syncwarp();
       tc_fence_after();
       mark = next_mark;
@@ -202,7 +256,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
       if (one) {
 #pragma unroll
         for (int k = 0; k < HD / 16; k++)
-          tc_mma_f16(tmem_base + (uint32_t)(st * 64), q0 + (uint64_t)((k >> 2) * (TILE_ROWS * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((k >> 2) * (1024 >> 4) + (k & 3) * 2), idesc_s,
+          tc_mma_f16(tmem_base + (uint32_t)(st * TILE), q0 + (uint64_t)((k >> 2) * (TILE_ROWS * 128 >> 4) + (k & 3) * 2), kt + (uint64_t)((k >> 2) * (1024 >> 4) + (k & 3) * 2), idesc_s,
                      k ? 1u : 0u);
         tc_commit(&k_empty[st], left);
         tc_commit(&s_full[st], left);
@@ -215,18 +269,20 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     for (int j = 0; j < n_tiles; j++) {
       const int st = j & 1;
       if (j + 1 < n_tiles) issue_s(j + 1);   // (its buffer held P of tile j - 1, whose P V is in front of it in the pipe)
+      else mark = next_mark;
       mbar_wait_lim(p_full, (uint32_t)j & 1u, a.err, left);
-      mbar_wait_lim(&v_full[st], (uint32_t)(j >> 1) & 1u, a.err, left);
+      mbar_wait_lim(&v_full[st], (uint32_t)(j / 2) & 1u, a.err, left);
       __syncwarp();
       tc_fence_after();
       const uint64_t vt = desc_values(v_s, GROUP) + (uint64_t)(st * (C::KV_BYTES >> 4));
-      const int steps = (j + 1 < n_tiles ? mark : next_mark) ? 0 : min(TILE, (kv_end - (it.t0 + j) * TILE + 15) & ~15) / 16;   // sixteens of positions; marked: the rows have summed by themselves
+      const int steps = mark ? 0 : min(TILE, (kv_end - (it.t0 + j) * TILE + 15) & ~15) / 16;   // sixteens of positions; marked: the rows have summed by themselves
       if (one) {
 #pragma unroll
-        for (int half = 0; half < 2; half++)
+        for (int ks = 0; ks < TILE / 16; ks++)   // P of 32 keys: 16 columns of hi, 16 of lo
 #pragma unroll
-          for (int ks = 0; ks < TILE / 16; ks++)
-            mma_ts_if(ks < steps ? 1u : 0u, tmem_o, tmem_base + (uint32_t)(st * 64 + half * 32 + ks * 8), vt + (uint64_t)(ks * (2 * GROUP >> 4)), idesc_o, (j | half | ks) ? 1u : 0u);
+          for (int half = 0; half < 2; half++)
+            mma_ts_if(ks < steps ? 1u : 0u, tmem_o, tmem_base + (uint32_t)(st * TILE + (ks >> 1) * 32 + half * 16 + (ks & 1) * 8), vt + (uint64_t)(ks * (2 * GROUP >> 4)), idesc_o,
+                      (j | half | ks) ? 1u : 0u);
         tc_commit(&v_empty[st], left);
         tc_commit(o_full, left);
       }
@@ -239,108 +295,119 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mbar_arrive(q_full);
     if (!busy) {
-      for (int j = 0; j < n_tiles; j++) {   // (P V of tile j - 1 first: an arrival for tile j must not join the barrier's previous phase)
+      for (int j = 0; j < n_tiles; j++) {   // (an arrival for tile j must not join the barrier's previous phase)
         if (j > 0) mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, a.err, left);
         mbar_arrive(p_full);
       }
       mbar_wait_lim(o_full, (uint32_t)(n_tiles - 1) & 1u, a.err, left);
     } else {
-      // ---- softmax (a thread a query row)
+      // ---- softmax (a thread a query row), 32 keys at a time: their maximum first, then weights over the scores that they come from
       const int qp = p0 + tok, lo = a.win.w <= 0 ? 0 : a.win.by_call ? by_call : max(0, qp + 1 - a.win.w);
+      const uint64_t scale2 = two(a.scale_log2, a.scale_log2), minus1 = two(-1.f, -1.f);
       for (int j = 0; j < n_tiles; j++) {
         const uint32_t tmem_sp = tmem_base + lane_addr + (uint32_t)((j & 1) * 64);
-        mbar_wait_lim(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, left);
+        mbar_wait_lim(&s_full[j & 1], (uint32_t)(j / 2) & 1u, a.err, left);
         tc_fence_after();
         const uint32_t mark = marked[j & 3];
-        float sv[TILE];
-        {
-          uint32_t r[32];
-          tc_ld32(tmem_sp, r);
-#pragma unroll
-          for (int i = 0; i < 32; i++) sv[i] = __uint_as_float(r[i]);
-          tc_ld32(tmem_sp + 32u, r);
-#pragma unroll
-          for (int i = 0; i < 32; i++) sv[32 + i] = __uint_as_float(r[i]);
-        }
         const int k0 = (it.t0 + j) * TILE;
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (k0 + TILE - 1 > p0 || k0 < late) {   // a row of the tile does not see all of these
+        const bool edge = k0 + TILE - 1 > p0 || k0 < late;   // a row of the tile does not see all of these
+        auto hide = [&](uint32_t (&r)[32], int c) {
+          if (edge)
 #pragma unroll
-          for (int i = 0; i < TILE; i++) {
-            if (k0 + i > qp || k0 + i < lo) sv[i] = -INFINITY;
-            mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
+            for (int i = 0; i < 32; i++)
+              if (k0 + 32 * c + i > qp || k0 + 32 * c + i < lo) r[i] = 0xff800000u;
+        };
+        uint32_t r[2][32];
+        float mx[2] = {-INFINITY, -INFINITY};
+        tc_ld32_go(tmem_sp, r[0]);
+#pragma unroll
+        for (int c = 0; c < TILE / 32; c++) {
+          tc_wait_ld(r[c & 1]);
+          tc_ld32_go(tmem_sp + (c + 1 < TILE / 32 ? 32u * (c + 1) : 0u), r[(c + 1) & 1]);   // (behind the last the first again, for its weights)
+          hide(r[c & 1], c);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            mx[0] = max3(mx[0], __uint_as_float(r[c & 1][i]), __uint_as_float(r[c & 1][i + 1]));
+            mx[1] = max3(mx[1], __uint_as_float(r[c & 1][i + 2]), __uint_as_float(r[c & 1][i + 3]));
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < TILE; i++) mx4[i & 3] = fmaxf(mx4[i & 3], sv[i]);
         }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        const float top = fmaxf(mx[0], mx[1]);
         float fac = 1.f;
         bool resc = false;
         if (j == 0) {
-          m_run = mx;
-        } else if ((mx - m_run) * a.scale_log2 > a.tau_log2) {   // (from -inf: factor 0)
-          fac = ft_ex2((m_run - mx) * a.scale_log2);
-          m_run = mx;
+          m_run = top;
+        } else if ((top - m_run) * a.scale_log2 > a.tau_log2) {   // (from -inf: factor 0)
+          fac = ft_ex2((m_run - top) * a.scale_log2);
+          m_run = top;
           resc = true;
         }
         const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;   // a row that has seen nothing yet counts from 0
-        float rs[4] = {0.f, 0.f, 0.f, 0.f};   // (one sum behind the other is 64 times an operation's latency)
+        const uint64_t mc2 = two(-mc, -mc);
+        uint64_t rs[2] = {0ull, 0ull};
+        auto weights = [&](auto clean) {   // two operands of D, or as they are
 #pragma unroll
-        for (int i = 0; i < TILE; i++) {
-          const float e = ft_ex2(fmaf(sv[i], a.scale_log2, -mc));
-          sv[i] = e;
-          rs[i & 3] += e;
-        }
-        l_run = l_run * fac + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-        if (j > 0) {
-          mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, a.err, left);   // P V of the previous tile is there: O is at rest
+          for (int c = 0; c < TILE / 32; c++) {
+            constexpr int B = TILE / 32 & 1;   // the buffer that the first chunk came into again
+            uint32_t (&x)[32] = r[(c + B) & 1];
+            tc_wait_ld(x);
+            if (c + 1 < TILE / 32) tc_ld32_go(tmem_sp + 32u * (c + 1), r[(c + 1 + B) & 1]);
+            hide(x, c);
+            uint32_t lw[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float2 z = of_two(fma_two(two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, mc2));
+              const float e0 = ft_ex2(z.x), e1 = ft_ex2(z.y);
+              const uint64_t e = two(e0, e1);
+              rs[i & 1] = add_two(rs[i & 1], e);
+              if (decltype(clean)::value) {
+                x[i] = pack2x<T>(e0, e1);
+                const float2 h = DT<T>::unpack2(x[i]);
+                const float2 d = of_two(fma_two(two(h.x, h.y), minus1, e));
+                lw[i] = pack2x<T>(d.x, d.y);
+              } else {
+                x[2 * i] = __float_as_uint(e0);
+                x[2 * i + 1] = __float_as_uint(e1);
+              }
+            }
+            if (decltype(clean)::value) {
+#pragma unroll
+              for (int i = 0; i < 16; i++) x[16 + i] = lw[i];
+            }
+            tc_st32(tmem_sp + 32u * c, x);
+          }
+        };
+        if (mark == 0u) weights(std::true_type{});
+        else weights(std::false_type{});
+        const float2 s0 = of_two(add_two(rs[0], rs[1]));
+        l_run = l_run * fac + (s0.x + s0.y);
+        if (j > 0) {   // P V of the previous tile is there, O at rest (waited for in front of the weights: 300 to 600 of 2200 cycles a tile)
+          mbar_wait_lim(o_full, (uint32_t)(j - 1) & 1u, a.err, left);
           tc_fence_after();
           if (__any_sync(0xffffffffu, resc)) {
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 32) {
-              uint32_t r[32];
-              tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+              uint32_t x[32];
+              tc_ld32(tmem_o + lane_addr + (uint32_t)c0, x);
 #pragma unroll
-              for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * fac);
-              tc_st32(tmem_o + lane_addr + (uint32_t)c0, r);
+              for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * fac);
+              tc_st32(tmem_o + lane_addr + (uint32_t)c0, x);
             }
           }
         }
-        if (mark == 0u) {
-          uint32_t hi[32], lw[32];
-#pragma unroll
-          for (int i = 0; i < 32; i++) {
-            const float x0 = sv[2 * i], x1 = sv[2 * i + 1];
-            hi[i] = pack2x<T>(x0, x1);
-            const float2 hf = DT<T>::unpack2(hi[i]);
-            lw[i] = pack2x<T>(x0 - hf.x, x1 - hf.y);
-          }
-          tc_st32(tmem_sp, hi);
-          tc_st32(tmem_sp + 32u, lw);
-        } else {
+        if (mark) {
           // the tile's values hold an infinity or a NaN: the row sums those that it sees, weights by way of TMEM
-          {
-            uint32_t r[32];
-#pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sv[i]);
-            tc_st32(tmem_sp, r);
-#pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sv[32 + i]);
-            tc_st32(tmem_sp + 32u, r);
-          }
           tc_wait_st();
-          mbar_wait_lim(&v_full[j & 1], (uint32_t)(j >> 1) & 1u, a.err, left);
+          mbar_wait_lim(&v_full[j & 1], (uint32_t)(j / 2) & 1u, a.err, left);
           __syncwarp();
           const unsigned char *vt = v_s + (j & 1) * C::KV_BYTES;
           const int n = min(TILE, kv_end - k0);
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 32) {
-            uint32_t r[32];
-            tc_ld32(tmem_o + lane_addr + (uint32_t)c0, r);
+            uint32_t x[32];
+            tc_ld32(tmem_o + lane_addr + (uint32_t)c0, x);
             float o[32];
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[i] = j > 0 ? __uint_as_float(r[i]) : 0.f;
+            for (int i = 0; i < 32; i++) o[i] = j > 0 ? __uint_as_float(x[i]) : 0.f;
 #pragma unroll 1
             for (int k = 0; k < n; k++) {
               const float p = tc_ld1(tmem_sp + (uint32_t)k);
@@ -357,8 +424,8 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
               __syncwarp();
             }
 #pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(o[i]);
-            tc_st32(tmem_o + lane_addr + (uint32_t)c0, r);
+            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(o[i]);
+            tc_st32(tmem_o + lane_addr + (uint32_t)c0, x);
           }
         }
         tc_wait_st();
