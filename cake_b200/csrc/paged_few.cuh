@@ -40,6 +40,8 @@ __device__ __forceinline__ char *rows_of(const Pool &p, int page, int kvh, int w
 }
 __device__ __forceinline__ int page_of(const Pool &p, int slot, int pos) { return __ldg(p.table + (size_t)slot * p.per_seq + (pos >> p.page_log2)); }
 
+// Weights of D = f16 are lifted by a power of two, so that those 2^-24 of the largest and below still count: 100000 of them may be a hundredth of the sum
+template <typename T> constexpr float lift(int log2) { return std::is_same<T, __half>::value ? (float)log2 : 0.f; }
 struct Few {
   Pool pool;
   const PlanHead *plan;
@@ -335,7 +337,8 @@ __global__ void __launch_bounds__(FEW_THREADS, FewCfg<HD, NT>::CTAS) few_kernel(
           uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
           for (int x = 0; x < NT; x++) {
-            const float c0 = m[x][0] == -INFINITY ? 0.f : m[x][0] * a.scale_log2, c1 = m[x][1] == -INFINITY ? 0.f : m[x][1] * a.scale_log2;
+            constexpr float UP = lift<T>(15);   // (the largest is 1)
+            const float c0 = m[x][0] == -INFINITY ? 0.f : m[x][0] * a.scale_log2 - UP, c1 = m[x][1] == -INFINITY ? 0.f : m[x][1] * a.scale_log2 - UP;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               s[x][e] = ex2(fmaf(s[x][e], a.scale_log2, -(e & 1 ? c1 : c0)));

@@ -27,12 +27,15 @@ struct cake_b200_pages {
   const float *cos_t = nullptr, *sin_t = nullptr;
   int rot = 0;
   int *bad = nullptr;                // pinned: a replayed call met a step of another shape
+  unsigned wait_failures = 0;        // the context's count when there was no sequence last: another one, and the rows may be no results
   size_t page_bytes() const { return (size_t)2 * book.page * ctx->cfg.n_kv_heads * ctx->cfg.head_dim * 2; }
 };
 
 static int pages_call(const cake_b200_pages *g, const char *what) {
   if (!g) return fail(CAKE_B200_EINVAL, "null argument");
   RC(check_waits(g->ctx));
+  if (g->wait_failures != g->ctx->wait_failures)
+    return fail(CAKE_B200_ESTATE, "%s: a kernel gave up a wait while these sequences were there and their rows may be no results: drop them all", what);
   if (*(volatile int *)g->bad) {
     *(volatile int *)g->bad = 0;
     return fail(CAKE_B200_ESTATE, "%s: a replayed graph's calls were made for steps of other counts than the present one and did nothing", what);
@@ -112,6 +115,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   g->len.assign((size_t)f.n_layers, std::vector<int>((size_t)max_seqs, 0));
   g->in_graph.assign((size_t)f.n_layers, 0);
   g->rot = rot;
+  g->wait_failures = c->wait_failures;
   if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
   CU(cudaMallocHost(&g->bad, 4));
   *g->bad = 0;
@@ -157,6 +161,7 @@ extern "C" void cake_b200_pages_free(cake_b200_pages *g) {
 
 extern "C" int cake_b200_pages_add(cake_b200_pages *g, int *seq) {
   if (!g || !seq) return fail(CAKE_B200_EINVAL, "null argument");
+  if (!g->book.any()) g->wait_failures = g->ctx->wait_failures;
   const int s = g->book.add();
   if (s < 0) return fail(CAKE_B200_ESTATE, "all %d sequences are taken", g->book.max_seqs);
   for (auto &l : g->len) l[(size_t)s] = 0;
@@ -370,7 +375,7 @@ extern "C" int cake_b200_pages_attend(cake_b200_pages *g, int block_idx, const v
   const OnDevice dev(g->device);
   if (!q_dev || !out_dev) return fail(CAKE_B200_EINVAL, "null argument");
   if (unaligned(q_dev, q_tok) || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "pages_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
-  if (window < 0 || !(scale >= 0.f && scale <= 3.402823466e38f)) return fail(CAKE_B200_EINVAL, "window %d or scale %g out of range", window, (double)scale);
+  if (window < 0 || !(scale >= 0.f && scale <= 2e38f)) return fail(CAKE_B200_EINVAL, "window %d or scale %g out of range", window, (double)scale);
   if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);
   RC(pages_written(g, block_idx, true));
   return on_stream(g->ctx, stream, [&]() -> int {

@@ -63,6 +63,7 @@ struct Book {
       }
     return -1;
   }
+  bool any() const { return std::any_of(seqs.begin(), seqs.end(), [](const Seq &q) { return q.live; }); }
   bool in_step(int s) const { return std::find(ids.begin(), ids.end(), s) != ids.end(); }
   void end_step() { step.clear(); ids.clear(); updates.clear(); n_few = n_rows = 0; shape = 0; }
   void cut(int s, int len) {   // what is behind len is given back

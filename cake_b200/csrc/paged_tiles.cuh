@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
           m_run = top;
           resc = true;
         }
-        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;   // a row that has seen nothing yet counts from 0
+        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2 - lift<T>(7);   // a row that has seen nothing yet counts from 0; the largest weight is 2^8
         const uint64_t mc2 = two(-mc, -mc);
         uint64_t rs[2] = {0ull, 0ull};
         auto weights = [&](auto clean) {   // two operands of D, or as they are
@@ -468,11 +468,11 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
   tc_fence_before();
   __syncthreads();
   if (*gave_up) ft_drain(bars, warp, lane, k_loads, v_loads);
-  if (a.beside) pdl_wait();
   if (warp == 5) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(C::TMEM) : "memory");
   }
+  if (a.beside) pdl_wait();
 }
 
 // A CTA for 32 entries of a tile's rows, a thread a row

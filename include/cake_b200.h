@@ -433,7 +433,9 @@ int cake_b200_cache_attend(cake_b200_cache *, int block_idx, const void *q_dev, 
  * the same counts and the present step (CAKE_B200_ESTATE otherwise).  A graph then does the captured calls for whatever step stands when it is replayed: steps of other sequences
  * and lengths, but the same counts in the same order; the step is planned in front of the replay, outside the graph, on the stream of the replay or before it.
  * A replay for a step of other counts does nothing and makes the next call on the cache fail with CAKE_B200_ESTATE.  Whether a block that a graph appends
- * to has its rows is its user's to know.  Graphs that share a cache are replayed neither at the same time nor beside its calls. */
+ * to has its rows is its user's to know.  Graphs that share a cache are replayed neither at the same time nor beside its calls, and not once it is closed; their
+ * calls may have used up to eight different windows.  (Captured calls suit any lengths; calls outside captures may cut their sums otherwise.)
+ * After a wait that a kernel gave up (cake_b200_sync) a cache refuses further use until all its sequences have been dropped. */
 /* rot, cos_dev, sin_dev: rows [max_seq][rot / 2] fp32 in device memory, pairs (e, e + rot / 2), to rotate by instead of the ctx's tables; they stay the
  * caller's and are read while the cache lives.  Both NULL: the ctx's (rot is not read). */
 int cake_b200_pages_create(cake_b200_ctx *, int n_pages, int page_size, int max_seqs, int max_seq, const float *cos_dev, const float *sin_dev, int rot,

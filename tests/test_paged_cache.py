@@ -436,6 +436,65 @@ def test_scores_that_lie_far_apart(heads, kv, hd, rows):
     ctx.close()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_weights_far_below_the_largest(rows, dtype):
+    """One position with nearly all the weight and 60000 with 2^-25 of it each, whose values are larger: together they are a good part of the result."""
+    ctx = ctx_for(8, 2, 64, dtype)
+    n = 60000
+    cache = PagedCache(ctx, n // 64 + 2, 64, max_seqs=1, max_seq=n + rows)
+    t = Talks(cache, 2, 64, dtype)
+    s = t.add()
+    k, v = torch.zeros(n + rows, 2, 64, device="cuda", dtype=TORCH_DTYPES[dtype]), normal((n + rows, 2, 64), dtype, 1) + 4
+    k[123, :, 0], v[123] = 25 * math.log(2), 0.125
+    t.step([s], [n], k=k[:n], v=v[:n])
+    t.step([s], [rows], k=k[n:], v=v[n:])
+    q = torch.zeros(rows, 8, 64, device="cuda", dtype=TORCH_DTYPES[dtype])
+    q[:, :, 0] = 8
+    t.check(q, [s], [rows])
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_more_windows_than_plans():
+    """Windows in any order, more of them than the cache keeps plans for, one captured; other windows after eight captured ones are refused."""
+    ctx = ctx_for(8, 2, 128, "bf16")
+    cache = PagedCache(ctx, 60, 16, max_seqs=3, max_seq=400)
+    t = Talks(cache, 2, 128, "bf16")
+    ids = [t.add() for _ in range(3)]
+    counts = [1, 30, 2]
+    t.step(ids, [100, 250, 7], 1)
+    t.step(ids, counts, 2)
+    q = normal((33, 8, 128), "bf16", 3)
+    rng = random.Random(2)
+    cache.attend(0, q, window=77)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = cache.attend(0, q, window=77)
+    for turn in range(3):
+        for w in rng.sample(range(1, 300), 14):
+            t.check(q, ids, counts, window=w)
+        t.step(ids, counts, 10 + turn)
+        q.copy_(normal((33, 8, 128), "bf16", 20 + turn))
+        g.replay()
+        t.check(q, ids, counts, window=77, out=out)
+    for w in range(1, 8):
+        cache.attend(0, q, window=w)
+        torch.cuda.synchronize()
+        h = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(h):
+            cache.attend(0, q, window=w)
+        del h
+    t.check(q, ids, counts, window=5)
+    with pytest.raises(CakeB200Error) as e:
+        cache.attend(0, q, window=300)
+    assert e.value.code == EINVAL
+    del g
+    ctx.close()
+
+
 BAD = [float("nan"), float("inf"), -float("inf")]
 
 
