@@ -280,8 +280,8 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
     typedef typename decltype(t)::type T;
     constexpr int HD = decltype(h)::value;
     const int e = launch(s, launches, tiles_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv)), dim3(FT_THREADS), TileCfg<HD>::SMEM, 1, t8);
-    if (e || !a.cut) return e;
-    return launch(s, launches, join_kernel<T, HD>, dim3((unsigned)(a.n_items * p.n_kv * (HD / 32))), dim3(128), 0, 1, t8);
+    if (e || !a.n_cut_tiles) return e;
+    return launch(s, launches, join_kernel<T, HD>, dim3((unsigned)(a.n_cut_tiles * p.n_kv), HD / 8), dim3(128), 0, 1, t8, reinterpret_cast<const int *>(items + a.most_items));
   });
 }
 

@@ -63,7 +63,7 @@ int read(cudaStream_t, int dtype, const Pool &, const Read &, uint64_t *launches
 
 // A step's attention as it is cut for one window (paged_plan.hpp), on the device: this head, few_ctas workers and as many cuts of the few-row kernel, the items of
 // the many-row kernel.  What the calls on a cache share: sums of runs and tiles that are cut
-struct PlanHead { int W, n_cuts, n_items, parts, pad[4]; };   // workers, cut runs; items, parts of those that are cut
+struct PlanHead { int W, n_cuts, n_items, parts, n_cut_tiles, pad[3]; };   // workers, cut runs; items, parts of tiles that are cut, such tiles (their first items behind the items)
 struct Scratch {
   float *few_ws, *tiles_ws;      // few_floats; tiles_floats (nullptr: the step has no sequence of many rows)
   int sms;
@@ -88,7 +88,8 @@ struct Attend {
   int n_few, few_cols;           // sequences of few rows, query rows of a key head that they have at most
   int longest, tiles;            // tiles of their longest run, of all; 0: a captured call, whose lengths may become any
   int n_cuts, n_items;           // runs that are cut, items of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
-  bool cut;                      // some of the items are parts (of a captured call: may be)
+  int most_items;                // that many items: the list of cut tiles is behind them
+  int n_cut_tiles;               // tiles that are cut (of a captured call: as many as may be)
   int *err;
 };
 int attend(cudaStream_t, int dtype, const Pool &, const Attend &, const Scratch &, uint64_t *launches);

@@ -19,7 +19,7 @@ struct cake_b200_pages {
     unsigned long long step = 0, used = 0;   // made for this step; last used in this call
     bool kept = false;                       // captured calls read it: it is made anew with every step
     int longest = 0, tiles = 0, n_cuts = 0, n_items = 0, most_items = 0;   // tiles of the longest run of few rows, of all; cut runs; items of the many-row kernel, now and for any lengths of this shape
-    bool cut = false;                        // some are parts of tiles
+    int n_cut_tiles = 0, most_cut_tiles = 0;               // tiles that are cut, now and for any lengths
     char *dev = nullptr;
   } plans[8];
   unsigned long long steps = 0, calls = 0;
@@ -189,7 +189,7 @@ static size_t pages_plan_bytes(const cake_b200_pages *g) {
   const cake_b200_config &f = g->ctx->cfg;
   const int sms = g->ctx->sm_count;
   return sizeof(pg::PlanHead) + (size_t)pg::few_ctas(f.head_dim, sms) * (sizeof(pg::Worker) + sizeof(pg::Cut)) +
-         pg::Book::most_items((long long)g->book.n_pages * g->book.page, g->book.max_seqs, f.n_heads / f.n_kv_heads, pg::room(f.head_dim, sms, f.n_kv_heads)) * sizeof(pg::Item);
+         pg::Book::most_items((long long)g->book.n_pages * g->book.page, g->book.max_seqs, f.n_heads / f.n_kv_heads, pg::room(f.head_dim, sms, f.n_kv_heads)) * sizeof(pg::Item) + (size_t)pg::room(f.head_dim, sms, f.n_kv_heads) * 4;
 }
 static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // on the ctx's stream of the moment
   cake_b200_ctx *c = g->ctx;
@@ -210,14 +210,23 @@ static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // 
     g->tiles_ws = (float *)m;
   }
   const size_t at_cuts = sizeof h + most * sizeof(pg::Worker), at_many = at_cuts + most * sizeof(pg::Cut);
-  std::vector<char> blob(!many.empty() ? at_many + many.size() * sizeof(pg::Item) : at_cuts + cuts.size() * sizeof(pg::Cut));
+  std::vector<int> heads;
+  int tiles = 0;
+  for (size_t i = 0; i < many.size(); i++) {
+    tiles += many[i].part == 0;
+    if (many[i].part == 0 && many[i].parts > 1) heads.push_back((int)i);
+  }
+  h.n_cut_tiles = (int)heads.size();
+  p->most_items = tiles ? tiles + 2 * room : 0;   // (of any lengths, as cut_many has it; their heads begin behind that many)
+  p->most_cut_tiles = tiles ? std::min(tiles, room) : 0;
+  const size_t at_heads = at_many + (size_t)p->most_items * sizeof(pg::Item);
+  std::vector<char> blob(!many.empty() ? at_heads + heads.size() * 4 : at_cuts + cuts.size() * sizeof(pg::Cut));
   memcpy(blob.data(), &h, sizeof h);
   if (!few.empty()) memcpy(blob.data() + sizeof h, few.data(), few.size() * sizeof(pg::Worker));
   if (!cuts.empty()) memcpy(blob.data() + at_cuts, cuts.data(), cuts.size() * sizeof(pg::Cut));
   if (!many.empty()) memcpy(blob.data() + at_many, many.data(), many.size() * sizeof(pg::Item));
+  if (!heads.empty()) memcpy(blob.data() + at_heads, heads.data(), heads.size() * 4);
   RC(pages_upload(c, p->dev, blob.data(), blob.size()));
-  int tiles = 0;
-  for (size_t i = 0; i < many.size(); i++) tiles += many[i].part == 0;
   p->longest = p->tiles = 0;
   for (int i = 0; i < g->book.n_few; i++) {
     const int t = pg::tiles_of(g->book.step[(size_t)i], p->win);
@@ -226,8 +235,7 @@ static int pages_plan_make(cake_b200_pages *g, cake_b200_pages::Plan *p) {   // 
   }
   p->n_cuts = h.n_cuts;
   p->n_items = h.n_items;
-  p->most_items = tiles ? tiles + 2 * room : 0;
-  p->cut = h.parts > 0;
+  p->n_cut_tiles = h.n_cut_tiles;
   p->step = g->steps;
   return CAKE_B200_OK;
 }
@@ -345,7 +353,7 @@ static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_to
   const int most_cuts = std::min(g->book.n_few * c->cfg.n_kv_heads, pg::few_ctas(c->cfg.head_dim, c->sm_count));
   for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
   const pg::Attend a{q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), c->cfg.n_heads, scale, win, (const pg::PlanHead *)plan->dev, g->book.n_few, cols,
-                     capturing ? 0 : plan->longest, plan->tiles, capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, capturing || plan->cut, c->wait_err};
+                     capturing ? 0 : plan->longest, plan->tiles, capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, plan->most_items, capturing ? plan->most_cut_tiles : plan->n_cut_tiles, c->wait_err};
   CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count, &c->pg_clusters}, launch_counter(c)));
   return CAKE_B200_OK;
 }

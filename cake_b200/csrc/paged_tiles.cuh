@@ -7,8 +7,8 @@
 //   - keys and values come page by page as they lie: a page's groups of eight rows are the operands' own layout, so that bulk copies without a tensor map fill
 //     a tile from pages of any size, and Q is laid out by the softmax warps (no map to encode, any stride)
 //   - a CTA's sequence, tokens and keys stand in a list (paged_plan.hpp, cut_many): sequences of any lengths side by side, the tiles with the most keys first, and
-//     keys cut into parts where the tiles do not fill the chip; a kernel of its own joins them, in their order (one CTA's loads do not suffice: 512 rows of 8 / 4
-//     heads of 256 on 4000 positions, 5 parts of 132 KB a tile: JOINED)
+//     keys cut into parts where the tiles do not fill the chip; a kernel of its own joins them, in their order (the CTA that comes last would have 5 parts of 132 KB for a
+//     tile of 256-entry heads)
 //   - only whole sixteens of positions that hold a visible one are multiplied; where a page is marked (an infinity or a NaN in its values) a row sums what it sees by itself
 #pragma once
 #include "attn_prefill_tc.cuh"
@@ -475,41 +475,82 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
   if (a.beside) pdl_wait();
 }
 
-// A CTA for 32 entries of a tile's rows, a thread a row
+// The parts of a tile: a CTA for eight entries of its rows, a thread a row; threads that few rows leave take every second, third .. part.  Up to eight parts are
+// asked for at once (two at a time by one thread a row: 33 parts of 20 rows 45 us, so 7; 32 rows, 8 parts 22 and 8)
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) join_kernel(const Tiles a) {
+__global__ void __launch_bounds__(128) join_kernel(const Tiles a, const int *cuts) {
   pdl_launch_dependents();
-  const int row = threadIdx.x, c0 = 32 * (int)(blockIdx.x % (HD / 32)), kvh = (int)blockIdx.x / (HD / 32) % a.pool.n_kv, nth = (int)blockIdx.x / (HD / 32) / a.pool.n_kv;
+  constexpr int AT_ONCE = 8;
+  __shared__ float4 sums[2][128];
+  __shared__ float2 tops[128];
+  const int kvh = (int)blockIdx.x % a.pool.n_kv, nth = (int)blockIdx.x / a.pool.n_kv;
+  const bool any = same_step(a.pool) && nth < a.plan->n_cut_tiles;
+  Item it{};
+  if (any) it = a.items[cuts[nth]];
+  const int rows = a.G * min(a.tpt, it.s.count - it.tok0), wide = rows <= 32 ? 32 : rows <= 64 ? 64 : 128, groups = 128 / wide;
+  const int row = (int)threadIdx.x % wide, pg = (int)threadIdx.x / wide;
   pdl_wait();
-  if (!same_step(a.pool) || nth >= a.plan->n_items) return;
-  const Item it = a.items[nth];
-  const int rows = a.G * min(a.tpt, it.s.count - it.tok0);
-  if (it.part || it.parts == 1 || row >= rows) return;
+  if (!any) return;
   const float *place = a.ws + ((size_t)kvh * a.plan->parts + it.part0) * TileCfg<HD>::PART;
-  float M = -INFINITY, L = 0.f, v[32];
-#pragma unroll 8
-  for (int k = 0; k < it.parts; k++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(place + k * TileCfg<HD>::PART + TILE_ROWS * HD) + row).x);
+  float M = -INFINITY, L = 0.f;
+  float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (row < rows)
+    for (int k = pg; k < it.parts; k += groups * AT_ONCE) {
+      float4 y[AT_ONCE][2];
+      float2 m[AT_ONCE];
+      float top = M;
 #pragma unroll
-  for (int i = 0; i < 32; i++) v[i] = 0.f;
-#pragma unroll 2
-  for (int k = 0; k < it.parts; k++) {
-    const float2 x = __ldcg(reinterpret_cast<const float2 *>(place + k * TileCfg<HD>::PART + TILE_ROWS * HD) + row);
-    const float f = x.x == -INFINITY ? 0.f : ft_ex2((x.x - M) * a.scale_log2);
-    L += x.x == -INFINITY ? x.y : x.y * f;
-    const float4 *from = reinterpret_cast<const float4 *>(place + k * TileCfg<HD>::PART) + (c0 / 4) * TILE_ROWS + row;
+      for (int i = 0; i < AT_ONCE; i++) {
+        const int j = k + groups * i;
+        const float *from = place + (size_t)j * TileCfg<HD>::PART;
+        m[i] = make_float2(-INFINITY, 0.f);
+        if (j < it.parts) {
+          m[i] = __ldcg(reinterpret_cast<const float2 *>(from + TILE_ROWS * HD) + row);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float4 y = __ldcg(from + i * TILE_ROWS);
-      v[4 * i] = fmaf(y.x, f, v[4 * i]); v[4 * i + 1] = fmaf(y.y, f, v[4 * i + 1]); v[4 * i + 2] = fmaf(y.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(y.w, f, v[4 * i + 3]);
+          for (int c = 0; c < 2; c++) y[i][c] = __ldcg(reinterpret_cast<const float4 *>(from) + (2 * blockIdx.y + c) * TILE_ROWS + row);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; i++) top = fmaxf(top, m[i].x);
+      const float old = M == -INFINITY ? 1.f : ft_ex2((M - top) * a.scale_log2);   // (nothing, or no number, so far: sums of 0 or NaN)
+      M = top;
+      L *= old;
+#pragma unroll
+      for (int c = 0; c < 2; c++) { v[c].x *= old; v[c].y *= old; v[c].z *= old; v[c].w *= old; }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; i++)
+        if (k + groups * i < it.parts) {
+          const float f = m[i].x == -INFINITY ? 1.f : ft_ex2((m[i].x - M) * a.scale_log2);
+          L = fmaf(m[i].y, f, L);
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            v[c].x = fmaf(y[i][c].x, f, v[c].x); v[c].y = fmaf(y[i][c].y, f, v[c].y); v[c].z = fmaf(y[i][c].z, f, v[c].z); v[c].w = fmaf(y[i][c].w, f, v[c].w);
+          }
+        }
+    }
+  sums[0][threadIdx.x] = v[0];
+  sums[1][threadIdx.x] = v[1];
+  tops[threadIdx.x] = make_float2(M, L);
+  __syncthreads();
+  if (pg || row >= rows) return;
+  for (int k = 1; k < groups; k++) M = fmaxf(M, tops[k * wide + row].x);
+  L = 0.f;
+  v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < groups; k++) {
+    const float2 m = tops[k * wide + row];
+    const float f = m.x == -INFINITY ? 1.f : ft_ex2((m.x - M) * a.scale_log2);
+    L = fmaf(m.y, f, L);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const float4 y = sums[c][k * wide + row];
+      v[c].x = fmaf(y.x, f, v[c].x); v[c].y = fmaf(y.y, f, v[c].y); v[c].z = fmaf(y.z, f, v[c].z); v[c].w = fmaf(y.w, f, v[c].w);
     }
   }
   const float inv = 1.0f / L;
   const int tok = row / a.G;
-  T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(it.s.row0 + it.tok0 + tok) * a.n_heads + kvh * a.G + row - tok * a.G) * HD + c0;
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    reinterpret_cast<uint4 *>(dst)[i] = make_uint4(pack2x<T>(v[8 * i] * inv, v[8 * i + 1] * inv), pack2x<T>(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
-                                                   pack2x<T>(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack2x<T>(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
+  T *dst = reinterpret_cast<T *>(a.out) + ((size_t)(it.s.row0 + it.tok0 + tok) * a.n_heads + kvh * a.G + row - tok * a.G) * HD + 8 * blockIdx.y;
+  *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2x<T>(v[0].x * inv, v[0].y * inv), pack2x<T>(v[0].z * inv, v[0].w * inv), pack2x<T>(v[1].x * inv, v[1].y * inv),
+                                               pack2x<T>(v[1].z * inv, v[1].w * inv));
 }
 
 }  // namespace pg
