@@ -766,9 +766,9 @@ class TextModelBase:
         check(lib().cake_b200_logits(ctx.h, ptr(x), b, s, ptr(logits), None))
         return logits
 
-    def forward_paged(self, pages: PagedCache, requests: Sequence[Tuple[int, Sequence[int]]]) -> torch.Tensor:
+    def forward_paged(self, pages: PagedCache, requests: Sequence[Tuple[int, Sequence[int]]], greedy: Optional[List[int]] = None) -> torch.Tensor:
         """One step of many sequences: requests [(sequence of ``pages``, its next token ids)] -> logits (len(requests), vocab) of their last tokens, a device
-        tensor in D.  All blocks are local ones."""
+        tensor in D.  ``greedy``: a list that receives each one's most likely next token (the call then waits for them).  All blocks are local ones."""
         ctx, L = self.ctx, lib()
         run = self._local_run()
         if run is None:
@@ -786,7 +786,10 @@ class TextModelBase:
             if n > len(counts):   # the last row of each
                 y = y.index_select(0, torch.from_numpy(np.cumsum(counts) - 1).to(y.device))
             logits = torch.empty(len(counts), ctx.config.vocab_size, dtype=ctx.logits_dtype, device=ctx.torch_device)
-            check(L.cake_b200_logits(ctx.h, ptr(y), len(counts), 1, ptr(logits), None))
+            best = None if greedy is None else (c_uint32 * len(counts))()
+            check(L.cake_b200_logits(ctx.h, ptr(y), len(counts), 1, ptr(logits), best))
+        if greedy is not None:
+            greedy[:] = [int(t) for t in best]
         return logits
 
     def _local_run(self):
@@ -942,9 +945,11 @@ class PagedSessions:
         self.cache = PagedCache(model.ctx, pages, page_size, max_requests, max_seq)
         self.live: Dict[str, int] = {}
 
-    def step(self, tokens: Dict[str, Sequence[int]]) -> Dict[str, torch.Tensor]:
-        """{request: its next token ids} -> {request: logits (vocab) of the last of them}.  A request that is not live begins with these.  Where the pages do not
-        suffice (CakeB200Error, CAKE_B200_ENOMEM) nothing has happened: another request has to end, or fewer to go on."""
+    def step(self, tokens: Dict[str, Sequence[int]], greedy: Optional[Dict[str, int]] = None) -> Dict[str, torch.Tensor]:
+        """{request: its next token ids} -> {request: logits (vocab) of the last of them}.  A request that is not live begins with these.  ``greedy``: receives each
+        one's most likely next token.  Where the pages do not suffice (CakeB200Error, CAKE_B200_ENOMEM) nothing has happened: another request has to end, or
+        fewer to go on."""
+        best = None if greedy is None else []
         new = []
         held = {rid: self.cache.len(self.live[rid]) for rid in tokens if rid in self.live}
         try:
@@ -952,14 +957,38 @@ class PagedSessions:
                 if rid not in self.live:
                     self.live[rid] = self.cache.add()
                     new.append(rid)
-            logits = self.model.forward_paged(self.cache, [(self.live[rid], ids) for rid, ids in tokens.items()])
+            logits = self.model.forward_paged(self.cache, [(self.live[rid], ids) for rid, ids in tokens.items()], best)
         except BaseException:
             for rid, n in held.items():
                 self.cache.truncate(self.live[rid], n)
             for rid in new:
                 self.end(rid)
             raise
+        if greedy is not None:
+            greedy.update(zip(tokens, best))
         return dict(zip(tokens, logits))
+
+    def generate(self, prompts: Dict[str, Sequence[int]], sample_len: int) -> Dict[str, List[int]]:
+        """Greedy generation of up to ``sample_len`` tokens for each of some new requests, all of them together; a request ends with its end of stream."""
+        out: Dict[str, List[int]] = {rid: [] for rid in prompts}
+        feed, best = dict(prompts), {}
+        try:
+            for _ in range(sample_len):
+                if not feed:
+                    break
+                best.clear()
+                self.step(feed, best)
+                feed = {}
+                for rid, token in best.items():
+                    if self.model.ctx.config.is_eos(token):
+                        self.end(rid)
+                    else:
+                        out[rid].append(token)
+                        feed[rid] = [token]
+        finally:
+            for rid in prompts:
+                self.end(rid)
+        return out
 
     def len(self, rid: str) -> int:
         return self.cache.len(self.live[rid]) if rid in self.live else 0

@@ -5,6 +5,7 @@ the caller):
 
     python -m cake_b200.run <model_dir> --prompt-ids 1,2,3 [-n 32] [--dtype bf16|f16|f32] [--max-seq S]
                             [--temperature T] [--top-k K] [--top-p P] [--seed N] [--repeat-penalty R] [--cache-bits 4]
+    python -m cake_b200.run <model_dir> --prompt-ids "1,2,3;4,5;6" [-n 32]     # several prompts, generated together (greedy, Llama-family models)
     python -m cake_b200.run <model_dir> --show-config          # resolve config.json only (needs no GPU)
 
 <model_dir> holds config.json + model.safetensors (or an index + shards).  The model class follows config.json.
@@ -13,6 +14,7 @@ from __future__ import annotations
 
 import argparse
 import sys
+import time
 from typing import List, Optional
 
 
@@ -43,17 +45,31 @@ def main(argv: Optional[List[str]] = None) -> int:
     if a.cache_bits and cfg.layer_list:
         print("error: --cache-bits is served for Llama-family models only", file=sys.stderr)
         return 2
-    prompt = [int(t) for t in a.prompt_ids.split(",") if t.strip()]
-    if not prompt:
+    prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt_ids.split(";")]
+    prompt = prompts[0]
+    if not all(prompts):
         print("error: --prompt-ids is empty", file=sys.stderr)
+        return 2
+    if len(prompts) > 1 and (cfg.layer_list or a.cache_bits or a.temperature > 0 or a.repeat_penalty != 1.0):
+        print("error: several prompts are served for Llama-family models, greedily and with rows in the model's type", file=sys.stderr)
         return 2
     from .build import build
     build(host=False, quiet=True)
-    from .model import Context, Master, TextModelBase
-    max_seq = a.max_seq or min(cfg.max_seq_len, len(prompt) + a.n + 1)
+    from .model import Context, Master, PagedSessions, TextModelBase
+    max_seq = a.max_seq or min(cfg.max_seq_len, max(map(len, prompts)) + a.n + 1)
     ctx = Context(cfg, vb, a.dtype, device=a.device, max_seq=max_seq, cache_bits=a.cache_bits)
     try:
         model = TextModelBase.load(ctx, repeat_penalty=a.repeat_penalty, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed)
+        if len(prompts) > 1:
+            page = 64
+            requests = PagedSessions(model, sum((min(len(p) + a.n, max_seq) + page - 1) // page for p in prompts), page, len(prompts), max_seq)
+            began = time.perf_counter()
+            out = requests.generate({str(i): p for i, p in enumerate(prompts)}, a.n)
+            took = time.perf_counter() - began
+            for tokens in out.values():
+                print("tokens: " + " ".join(str(t) for t in tokens))
+            print(f"tok/s: {sum(map(len, out.values())) / took:.2f}")
+            return 0
         out = Master(model).generate_text(prompt, a.n)
         print("tokens: " + " ".join(str(t) for t in out["tokens"]))
         print(f"tok/s: {out['tok_s']:.2f}")

@@ -141,3 +141,68 @@ def test_sibling_blocks_in_pages(kind):
             at[r] += len(x)
             assert max_ulp_err(to_np(got[r]), want, "bf16") <= LOGIT_TOL_ULP
     ctx.close()
+
+
+def test_several_prompts_of_the_command_line(tmp_path):
+    """``python -m cake_b200.run`` with prompts side by side: the tokens of ``PagedSessions.generate``, which are the first places of its steps' logits."""
+    import subprocess
+    import sys
+    from cake_b200.model import PagedSessions
+    from tests.test_cpp_host import _write_model
+    cfg = medium_config(num_hidden_layers=2, max_seq_len=128)
+    sd = checkpoint(cfg, "bf16", seed=17, peaked=True)
+    _write_model(tmp_path, cfg, sd)
+    m = model_for(cfg, "bf16", peaked=True)
+    rng = random.Random(2)
+    prompts = [[rng.randrange(cfg.vocab_size) for _ in range(n)] for n in (17, 1, 40)]
+    ses = PagedSessions(m, 12, 16, max_requests=3)
+    names = {str(i): p for i, p in enumerate(prompts)}
+    got = ses.generate(names, 9)
+    assert ses.cache.available == 12 and not ses.live
+    feed = dict(names)
+    for i in range(9):
+        logits = ses.step(feed)
+        m.ctx.sync()
+        feed = {}
+        for r in names:
+            if i < len(got[r]):
+                assert int(logits[r].float().argmax()) == got[r][i]
+                feed[r] = [got[r][i]]
+        if not feed:
+            break
+    assert max(map(len, got.values())) == 9
+    m.ctx.close()
+    run = subprocess.run([sys.executable, "-m", "cake_b200.run", str(tmp_path), "--prompt-ids", ";".join(",".join(map(str, p)) for p in prompts), "-n", "9"],
+                         capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    lines = run.stdout.splitlines()
+    assert [[int(t) for t in line.split(":")[1].split()] for line in lines[:3]] == [got[r] for r in names]
+    for bad in (["--prompt-ids", "1;;2"], ["--prompt-ids", "1;2", "--temperature", "0.5"], ["--prompt-ids", "1;2", "--cache-bits", "4"]):
+        assert subprocess.run([sys.executable, "-m", "cake_b200.run", str(tmp_path), *bad], capture_output=True, timeout=300).returncode == 2
+
+
+def test_a_wait_that_was_given_up_closes_the_cache_until_its_sequences_are_dropped():
+    import ctypes
+    from cake_b200.model import PagedSessions
+    from tests.test_gpu_waits import probe
+    cfg = medium_config(num_hidden_layers=1)
+    m = model_for(cfg, "bf16")
+    ses = PagedSessions(m, 20, 16, max_requests=2)
+    first = ses.step({"a": [1, 2, 3]})["a"].clone()
+    m.ctx.sync()
+    ok, kcycles = (ctypes.c_int * 2)(), (ctypes.c_int * 2)()
+    probe(m.ctx, 1, 8192, ok, kcycles)   # a probe kernel's wait for an arrival that nobody makes
+    with pytest.raises(CakeB200Error, match="gave up a wait"):
+        m.ctx.sync()
+    for _ in range(2):
+        with pytest.raises(CakeB200Error) as e:
+            ses.step({"a": [4]})
+        assert e.value.code == -4 and "gave up" in str(e.value)
+        with pytest.raises(CakeB200Error):
+            ses.step({"b": [4]})
+    assert ses.len("a") == 3 and set(ses.live) == {"a"}
+    ses.end("a")
+    again = ses.step({"b": [1, 2, 3]})["b"]
+    m.ctx.sync()
+    assert torch.equal(first, again)
+    m.ctx.close()
