@@ -2,10 +2,11 @@
 //
 // Bound by memory: every key and value is read once, 4 hd bytes a position and key head, for 4 operations an entry and query head.  The line of all
 // (sequence, key head, tile of 64 positions) is cut into equal shares, one a CTA (paged_plan.hpp, cut_few), so that sequences of any lengths fill the chip
-// evenly; the parts of a (sequence, key head) that is cut are joined by a kernel of its own (the CTA that comes last, behind a fence, a ticket and a loop over the
-// parts, took 4 to 9 us, others waiting for it).  In a CTA a warp copies tiles into a
-// ring of shared memory by bulk copies of whole pages (or halves of tiles), looking up the pages of up to 32 copies at once and ahead; four warps take 16
-// positions of a tile each and never wait for one another before the share's end.
+// evenly; the parts of a run (a sequence's key head) that is cut are joined by a kernel of its own (the CTA that comes last, behind a fence, a ticket and a loop over
+// the parts, took 4 to 9 us, others waiting for it).  Where the runs are few or alike, a cluster of CTAs has one and joins its parts itself (paged_cache.cu,
+// cluster_of).  In a CTA a warp copies tiles into a ring of shared memory by bulk copies of whole pages (or of 64 rows of one), looking up the pages of
+// up to 32 copies at once and ahead; four warps take 16 positions of a tile each and never wait for one another before the run's end.  One token at 131071
+// positions, 8 key heads of 128: 89 us, 6.0 TB/s; 32 tokens to 8191: 59 us, 5.7 TB/s, of 6.55.
 //
 // A warp's products are S^T [16 positions, 8 query rows] = K Q^T and O^T [hd, 8 query rows] += V^T P^T on mma.sync m16n8k16: the positions take the operand's
 // 16 rows, the query rows its 8 columns (twice 8 for more), so that a group of 4 or 8 heads wastes little, and the weights turn from S^T's layout to
@@ -21,7 +22,7 @@ namespace pg {
 
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int HD, int NT> struct FewCfg {
-  static constexpr int STAGES = HD == 64 ? 6 : NT == 1 ? 3 : 2;
+  static constexpr int STAGES = HD == 64 ? 6 : NT == 1 ? 3 : 2;   // (two CTAs an SM; the four warps' sums of 16 rows take the third one's room)
   static constexpr int ROWS_BYTES = TILE * HD * 2;          // keys, or values, of a tile
   static constexpr int COLS = 8 * NT;
   static constexpr int RED_BYTES = FEW_WARPS * COLS * HD * 4, ML_BYTES = FEW_WARPS * COLS * 8;

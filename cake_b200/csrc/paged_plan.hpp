@@ -126,9 +126,10 @@ struct Book {
   }
 
   // Few rows: all (sequence, key head)s' tiles in one line, cut into shares of the same cost: a tile 1, a piece of a run RUN_COST more (its sums have to be
-  // brought together).  A piece that would leave a single tile to the next share takes it.
+  // brought together).  A piece that would leave a single tile to the next share takes it.  RUN_COST 0.5, 1, 2, 4:  32 sequences to 8191 positions (8 key heads of 128)
+  // 60.6, 59.0, 60.1, 62.5 us, 9 of 3 to 5 rows to 5000 17.1, 18.3, 22.5, 26.4, 100 in a window of 1024 (2 of 64) 10.7, 11.3, 12.7, 16.3.
   void cut_few(const Window &win, int n_kv, int most, std::vector<Worker> *out, std::vector<Cut> *cuts) const {
-    constexpr double RUN_COST = 1;
+    constexpr double RUN_COST = 0.5;
     out->clear();
     cuts->clear();
     long long total = 0;

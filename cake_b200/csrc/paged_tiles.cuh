@@ -2,7 +2,11 @@
 //
 // The same division of work as attn_prefill_tc.cuh: 128 query rows (the G heads of a key head x 128 / G tokens) a CTA, softmax in warps 0-3 with a thread a
 // row, warp 4 copies, warp 5 multiplies; S in fp32 in TMEM, P as two operands of D (16 bits and more) over the S that it came from, O in TMEM, rescaled where a
-// maximum grew by more than tau.  Bound by the softmax's exponentials and conversions, then the products (6 hd operations a pair instead of 4: P V twice).
+// maximum grew by more than tau.  Bound by the softmax warps' chain beside the products (6 hd operations a pair instead of 4: P V twice) at the clock that the
+// chip's power leaves: two CTAs an SM take 1950 cycles for a tile of 64 keys each, of which the products are 1540 and the exponentials 1020 (MUFU), at 1.55 GHz;
+// 5 us a CTA go by before the first tile and behind the last.  A prompt of 4096, 32 / 8 heads of 128: 177 us (195 at the power cap),
+// 0.48 of measured bf16, 0.72 counting P V twice.  Tiles of 128 keys: with one S buffer 256 us for 206 (a CTA's S, softmax and P V follow one another, and two CTAs fall in step),
+// with two and one CTA an SM 263 (nothing beside a CTA's beginning and end).
 // What is different:
 //   - keys and values come page by page as they lie: a page's groups of eight rows are the operands' own layout, so that bulk copies without a tensor map fill
 //     a tile from pages of any size, and Q is laid out by the softmax warps (no map to encode, any stride)
@@ -176,6 +180,12 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_ptr)), "n"(C::TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the copying warp's first pages likewise
+  const int P = 1 << a.pool.page_log2, pr = min(P, TILE), ppt = TILE / pr, most = 32 / ppt, piece = lane % ppt;   // rows of a piece; pieces of a tile; tiles of a batch
+  const size_t head_bytes = rows_bytes(HD, 2 * P);
+  auto look = [&](int j, int n) -> int { return lane < n * ppt ? page_of(a.pool, it.s.slot, min((it.t0 + j + lane / ppt) * TILE + piece * pr, kv_end - 1)) : 0; };
+  int n = min(n_tiles, most), page = 0;
+  if (warp == 4) page = look(0, n);
   if (warp < 4) {
     if (!a.beside) pdl_wait();
     first = ask(0);
@@ -191,10 +201,6 @@ __global__ void __launch_bounds__(FT_THREADS, TileCfg<HD>::CTAS) tiles_kernel(co
 
   if (warp == 4) {
     // ---- copies.  A lane has one piece (a page, or 64 rows of one) of a batch of tiles
-    const int P = 1 << a.pool.page_log2, pr = min(P, TILE), ppt = TILE / pr, most = 32 / ppt, piece = lane % ppt;
-    const size_t head_bytes = rows_bytes(HD, 2 * P);
-    auto look = [&](int j, int n) -> int { return lane < n * ppt ? page_of(a.pool, it.s.slot, min((it.t0 + j + lane / ppt) * TILE + piece * pr, kv_end - 1)) : 0; };
-    int n = min(n_tiles, most), page = look(0, n);
     if (!a.beside) pdl_wait();
     for (int j0 = 0; j0 < n_tiles; j0 += most) {
       const uint32_t mark = lane < n * ppt ? __ldcg(a.pool.marks + (size_t)page * a.pool.n_kv + kvh) : 0u;
