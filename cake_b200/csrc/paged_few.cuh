@@ -6,7 +6,7 @@
 // the parts, took 4 to 9 us, others waiting for it).  Where the runs are few or alike, a cluster of CTAs has one and joins its parts itself (paged_cache.cu,
 // cluster_of).  In a CTA a warp copies tiles into a ring of shared memory by bulk copies of whole pages (or of 64 rows of one), looking up the pages of
 // up to 32 copies at once and ahead; four warps take 16 positions of a tile each and never wait for one another before the run's end.  One token at 131071
-// positions, 8 key heads of 128: 89 us, 6.0 TB/s; 32 tokens to 8191: 59 us, 5.7 TB/s, of 6.55.
+// positions, 8 key heads of 128: 89 us, 6.0 TB/s; 32 tokens to 8191: 60 us, 5.6 TB/s, of 6.55.
 //
 // A warp's products are S^T [16 positions, 8 query rows] = K Q^T and O^T [hd, 8 query rows] += V^T P^T on mma.sync m16n8k16: the positions take the operand's
 // 16 rows, the query rows its 8 columns (twice 8 for more), so that a group of 4 or 8 heads wastes little, and the weights turn from S^T's layout to

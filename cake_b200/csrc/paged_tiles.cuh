@@ -4,7 +4,7 @@
 // row, warp 4 copies, warp 5 multiplies; S in fp32 in TMEM, P as two operands of D (16 bits and more) over the S that it came from, O in TMEM, rescaled where a
 // maximum grew by more than tau.  Bound by the softmax warps' chain beside the products (6 hd operations a pair instead of 4: P V twice) at the clock that the
 // chip's power leaves: two CTAs an SM take 1950 cycles for a tile of 64 keys each, of which the products are 1540 and the exponentials 1020 (MUFU), at 1.55 GHz;
-// 5 us a CTA go by before the first tile and behind the last.  A prompt of 4096, 32 / 8 heads of 128: 177 us (195 at the power cap),
+// 5 us a CTA go by before the first tile and behind the last.  A prompt of 4096, 32 / 8 heads of 128: 177 us (195 to 204 at the power cap),
 // 0.48 of measured bf16, 0.72 counting P V twice.  Tiles of 128 keys: with one S buffer 256 us for 206 (a CTA's S, softmax and P V follow one another, and two CTAs fall in step),
 // with two and one CTA an SM 263 (nothing beside a CTA's beginning and end).
 // What is different:
