@@ -79,7 +79,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   if (!pg::head_dim_ok(f.head_dim)) return fail(CAKE_B200_EINVAL, "caches in pages hold heads of 64, 128 or 256 entries, not %d", f.head_dim);
   if (!pg::page_ok(page_size)) return fail(CAKE_B200_EINVAL, "a page holds 16, 32, .. 1024 positions (a power of two), not %d", page_size);
   if (n_pages < 1 || max_seqs < 1 || max_seq < 1) return fail(CAKE_B200_EINVAL, "pages, max_seqs and max_seq are 1 or more");
-  if ((long long)n_pages * page_size > (1ll << 30) || (long long)max_seqs * ((max_seq + page_size - 1) / page_size) > (1ll << 28))
+  if ((long long)n_pages * page_size > (1ll << 30) || max_seq > 1 << 30 || (long long)max_seqs * ((max_seq + page_size - 1) / page_size) > (1ll << 28))
     return fail(CAKE_B200_EINVAL, "%d pages of %d positions, %d sequences of %d: more than a cache in pages counts", n_pages, page_size, max_seqs, max_seq);
   const bool own = !cos_dev && !sin_dev;
   if (!own && (!cos_dev || !sin_dev)) return fail(CAKE_B200_EINVAL, "cos without sin");

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from cake_b200.capi import CakeB200Error
+from cake_b200.capi import CakeB200Error, byref, c_void_p, lib
 from cake_b200.config import Config
 from cake_b200.model import Context, PagedCache
 from cake_b200.synth import TORCH_DTYPES
@@ -735,6 +735,12 @@ def test_refusals():
         PagedCache(ctx, 4, 16, max_seq=40, rotation=(torch.zeros(40, 64),) * 2)
     with pytest.raises(ValueError):
         PagedCache(ctx, 4, 16, max_seq=40, rotation=(torch.zeros(40, 64, device="cuda", dtype=torch.float64),) * 2)
+    table = torch.zeros(40, 64, device="cuda")
+    for pages, page, seqs, n in ((4, 16, 1, 2147483647), (4, 16, 1 << 20, 1 << 20), (1 << 27, 16, 1, 40)):
+        rc = lib().cake_b200_pages_create(ctx.h, pages, page, seqs, n, table.data_ptr(), table.data_ptr(), 128, byref(c_void_p()))
+        assert rc == EINVAL
+    assert lib().cake_b200_pages_create(ctx.h, 4, 16, 1, 40, table.data_ptr(), None, 128, byref(c_void_p())) == EINVAL
+    assert lib().cake_b200_pages_create(ctx.h, 4, 16, 1, 40, table.data_ptr() + 4, table.data_ptr(), 128, byref(c_void_p())) == EINVAL
     for half in (4, 72):
         refused(EINVAL, PagedCache, ctx, 4, 16, max_seq=40, rotation=(torch.zeros(40, half, device="cuda"),) * 2)
     cache = PagedCache(ctx, 4, 16, max_seqs=2, max_seq=40)
@@ -793,6 +799,73 @@ def test_refusals():
     ctx.close()
     ctx = ctx_for(4, 2, 32, "bf16")
     refused(EINVAL, PagedCache, ctx, 4, 16)
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,page", [(8, 2, 64, 1024), (32, 8, 128, 512), (8, 4, 256, 1024)])
+def test_pages_that_are_many_tiles(heads, kv, hd, page):
+    ctx = ctx_for(heads, kv, hd, "f16")
+    talk = [(1000, 1), (1023, 2), (1024, 40), (0, 1100), (3000, 1), (511, 513), (2047, 130)]
+    cache = PagedCache(ctx, sum(-(-(h + r) // page) for h, r in talk), page, max_seqs=len(talk), max_seq=3001)
+    t = Talks(cache, kv, hd, "f16")
+    ids = [t.add() for _ in talk]
+    some = [i for i, (h, _) in enumerate(talk) if h]
+    t.step([ids[i] for i in some], [talk[i][0] for i in some], 1)
+    counts = [r for _, r in talk]
+    t.step(ids, counts, 2)
+    q = normal((sum(counts), heads, hd), "f16", 3)
+    t.check(q, ids, counts)
+    t.check(q, ids, counts, window=700)
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 64), (8, 8, 128), (8, 1, 256)])
+def test_hundreds_of_sequences(heads, kv, hd):
+    """More runs than CTAs, of every length up to a few tiles; then a few rows and portions of them mixed in any order."""
+    rng = random.Random(heads + hd)
+    ctx = ctx_for(heads, kv, hd, "bf16")
+    cache = PagedCache(ctx, 4000, 16, max_seqs=400, max_seq=400)
+    t = Talks(cache, kv, hd, "bf16")
+    ids = [t.add() for _ in range(400)]
+    t.step(ids, [rng.randint(1, 140) for _ in ids], 1)
+    who = rng.sample(ids, 333)
+    t.step(who, [1] * 333, 2)
+    q = normal((333, heads, hd), "bf16", 3)
+    out = cache.attend(0, q)
+    for i in rng.sample(range(333), 40):
+        check_rows(out[i:i + 1], q[i:i + 1], t.k[who[i]], t.v[who[i]], 0, 0.0, "bf16")
+    who = rng.sample(ids, 350)
+    counts = [rng.choice([1, 1, 2, 3, 17, 60]) for _ in who]
+    t.step(who, counts, 4)
+    q = normal((sum(counts), heads, hd), "bf16", 5)
+    for window in (0, 33):
+        out = cache.attend(0, q, window=window)
+        for i in rng.sample(range(350), 40):
+            a = sum(counts[:i])
+            check_rows(out[a:a + counts[i]], q[a:a + counts[i]], t.k[who[i]], t.v[who[i]], window, 0.0, "bf16")
+    ctx.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (8, 2, 64), (8, 4, 256)])
+def test_a_query_that_is_no_number_stays_alone(heads, kv, hd):
+    ctx = ctx_for(heads, kv, hd, "bf16")
+    cache = PagedCache(ctx, 80, 16, max_seqs=3, max_seq=400)
+    t = Talks(cache, kv, hd, "bf16")
+    ids, counts = [t.add() for _ in range(3)], [1, 2, 150]
+    t.step(ids, [200, 100, 77], 1)
+    t.step(ids, counts, 2)
+    q = normal((153, heads, hd), "bf16", 3)
+    want = cache.attend(0, q)
+    for row, head, bad in ((0, 0, float("nan")), (2, heads - 1, float("inf")), (3, 1, float("nan")), (90, 0, -float("inf")), (152, heads - 1, float("nan"))):
+        p = q.clone()
+        p[row, head, 5] = bad
+        got = cache.attend(0, p)
+        odd = torch.zeros(153, heads, dtype=torch.bool, device="cuda")
+        odd[row, head] = True
+        assert torch.equal(got[~odd], want[~odd]) and not torch.equal(got[odd], want[odd])
     ctx.close()
 
 
