@@ -32,21 +32,21 @@ template <typename T> struct Tag { typedef T type; };
 template <typename F> static int by_type(int dtype, F &&f) { return dtype == 1 ? f(Tag<__half>{}) : f(Tag<__nv_bfloat16>{}); }
 
 // ------------------------------------------------------------------------------------------ a step's sequences and rows
-__global__ void __launch_bounds__(256) spread_kernel(const StepHead *step, int max_seqs, int n_seqs, int *table, int2 *rows) {
+__global__ void __launch_bounds__(256) spread_kernel(const StepHead *step, int n_seqs, int *table, int2 *rows) {
   const SeqRow *seqs = reinterpret_cast<const SeqRow *>(step + 1);
   const int at = blockIdx.y * 256 + threadIdx.x, by = gridDim.y * 256;
   if ((int)blockIdx.x == n_seqs) {
-    const int2 *u = reinterpret_cast<const int2 *>(seqs + max_seqs);
+    const int2 *u = reinterpret_cast<const int2 *>(seqs + n_seqs);
     for (int i = at; i < step->n_updates; i += by) table[u[i].x] = u[i].y;
     return;
   }
   const SeqRow s = seqs[blockIdx.x];
   for (int i = at; i < s.count; i += by) rows[s.row0 + i] = make_int2(s.slot, s.pos0 + i);
 }
-int spread(cudaStream_t s, const StepHead *step, int max_seqs, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches) {
+int spread(cudaStream_t s, const StepHead *step, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches) {
   const int most = std::max(most_rows, n_updates);
   // (launched without the early start of the others: what runs behind it reads the table before it waits)
-  spread_kernel<<<dim3((unsigned)n_seqs + 1, (unsigned)std::min(64, (most + 255) / 256)), 256, 0, s>>>(step, max_seqs, n_seqs, table, rows);
+  spread_kernel<<<dim3((unsigned)n_seqs + 1, (unsigned)std::min(64, (most + 255) / 256)), 256, 0, s>>>(step, n_seqs, table, rows);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) ++*launches;
   return (int)e;

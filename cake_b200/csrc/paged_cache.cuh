@@ -30,9 +30,9 @@ inline bool page_ok(int page) { return page >= 16 && page <= 1024 && (page & (pa
 
 // dtype codes are those of include/cake_b200.h (0 bf16, 1 f16).  Every function returns a cudaError_t cast to int and adds its launches to *launches.
 
-struct StepHead { uint64_t shape; int n_seqs, n_rows, n_updates, pad[3]; };   // then SeqRow[max_seqs], then the updates of the table
+struct StepHead { uint64_t shape; int n_seqs, n_rows, n_updates, pad[3]; };   // then SeqRow[n_seqs], then the updates of the table
 // A step's sequences and rows for the kernels: the table's new entries and, for every row, its sequence's row of the table and its position
-int spread(cudaStream_t, const StepHead *step, int max_seqs, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches);
+int spread(cudaStream_t, const StepHead *step, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches);
 
 // what all calls on one block of a cache have in common
 struct Pool {

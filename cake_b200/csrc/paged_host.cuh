@@ -5,6 +5,7 @@ struct cake_b200_pages {
   cake_b200_ctx *ctx;
   int device = 0;
   pg::Book book;
+  std::vector<char> blob;            // a step on its way to the device
   // device memory, one piece of the ctx's pool: the step, the page table, the rows' places
   char *arena = nullptr;
   pg::StepHead *step = nullptr;
@@ -41,6 +42,14 @@ static int pages_call(const cake_b200_pages *g, const char *what) {
     return fail(CAKE_B200_ESTATE, "%s: a replayed graph's calls were made for steps of other counts than the present one and did nothing", what);
   }
   return CAKE_B200_OK;
+}
+// No exception leaves a C entry: what of them makes host memory runs in here (inside on_stream, which gives the ctx its stream back when the call returns)
+template <typename F> static int with_memory(F &&f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(CAKE_B200_ENOMEM, "out of host memory");
+  }
 }
 static bool is_capturing(cudaStream_t s) {
   cudaStreamCaptureStatus st;
@@ -79,7 +88,7 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
   if (!pg::head_dim_ok(f.head_dim)) return fail(CAKE_B200_EINVAL, "caches in pages hold heads of 64, 128 or 256 entries, not %d", f.head_dim);
   if (!pg::page_ok(page_size)) return fail(CAKE_B200_EINVAL, "a page holds 16, 32, .. 1024 positions (a power of two), not %d", page_size);
   if (n_pages < 1 || max_seqs < 1 || max_seq < 1) return fail(CAKE_B200_EINVAL, "pages, max_seqs and max_seq are 1 or more");
-  if ((long long)n_pages * page_size > (1ll << 30) || max_seq > 1 << 30 || (long long)max_seqs * ((max_seq + page_size - 1) / page_size) > (1ll << 28))
+  if ((long long)n_pages * page_size > (1ll << 30) || max_seq > 1 << 30 || max_seqs > 1 << 16 || (long long)max_seqs * ((max_seq + page_size - 1) / page_size) > (1ll << 28))
     return fail(CAKE_B200_EINVAL, "%d pages of %d positions, %d sequences of %d: more than a cache in pages counts", n_pages, page_size, max_seqs, max_seq);
   const bool own = !cos_dev && !sin_dev;
   if (!own && (!cos_dev || !sin_dev)) return fail(CAKE_B200_EINVAL, "cos without sin");
@@ -108,33 +117,36 @@ extern "C" int cake_b200_pages_create(cake_b200_ctx *c, int n_pages, int page_si
     c->pg_cos = both; c->pg_sin = both + n;
     c->pc_behind = true;
   }
-  auto *g = new cake_b200_pages{c, c->device};
-  struct Guard { cake_b200_pages *g; ~Guard() { if (g) cake_b200_pages_free(g); } } guard{g};
-  g->book.init(n_pages, page_size, max_seqs, max_seq);
-  g->pool.assign((size_t)f.n_layers, nullptr);
-  g->len.assign((size_t)f.n_layers, std::vector<int>((size_t)max_seqs, 0));
-  g->in_graph.assign((size_t)f.n_layers, 0);
-  g->rot = rot;
-  g->wait_failures = c->wait_failures;
-  if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
-  CU(cudaMallocHost(&g->bad, 4));
-  *g->bad = 0;
-  if (!c->pg_clusters.most[0][0]) CU((cudaError_t)pg::prepare(f.dtype, f.head_dim, &c->pg_clusters));
-  const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
-               s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
-  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  void *arena = nullptr;
-  CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_ws) + s_rows, c->pc_pool, c->stream));
-  g->arena = (char *)arena;
-  g->step = (pg::StepHead *)g->arena;
-  g->table = (int *)(g->arena + up(s_step));
-  g->few_ws = (float *)(g->arena + up(s_step) + up(s_table));
-  g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_ws));
-  CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table), c->stream));
-  c->pc_behind = true;
-  guard.g = nullptr;
-  *out = g;
-  return CAKE_B200_OK;
+  return with_memory([&]() -> int {
+    auto *g = new cake_b200_pages{c, c->device};
+    struct Guard { cake_b200_pages *g; ~Guard() { if (g) cake_b200_pages_free(g); } } guard{g};
+    g->book.init(n_pages, page_size, max_seqs, max_seq);
+    g->pool.assign((size_t)f.n_layers, nullptr);
+    g->len.assign((size_t)f.n_layers, std::vector<int>((size_t)max_seqs, 0));
+    g->in_graph.assign((size_t)f.n_layers, 0);
+    g->rot = rot;
+    g->wait_failures = c->wait_failures;
+    if (rot) { g->cos_t = own ? c->pg_cos : cos_dev; g->sin_t = own ? c->pg_sin : sin_dev; }
+    CU(cudaMallocHost(&g->bad, 4));
+    *g->bad = 0;
+    if (!c->pg_clusters.most[0][0]) CU((cudaError_t)pg::prepare(f.dtype, f.head_dim, &c->pg_clusters));
+    const size_t s_step = sizeof(pg::StepHead) + (size_t)max_seqs * sizeof(pg::SeqRow) + (size_t)n_pages * 8, s_table = (size_t)max_seqs * g->book.per_seq * 4,
+                 s_rows = (size_t)n_pages * page_size * 8, s_ws = pg::few_floats(f.head_dim, c->sm_count) * 4;
+    g->blob.reserve(s_step);
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    void *arena = nullptr;
+    CU(cudaMallocFromPoolAsync(&arena, up(s_step) + up(s_table) + up(s_ws) + s_rows, c->pc_pool, c->stream));
+    g->arena = (char *)arena;
+    g->step = (pg::StepHead *)g->arena;
+    g->table = (int *)(g->arena + up(s_step));
+    g->few_ws = (float *)(g->arena + up(s_step) + up(s_table));
+    g->rows = (int2 *)(g->arena + up(s_step) + up(s_table) + up(s_ws));
+    CU(cudaMemsetAsync(arena, 0, up(s_step) + up(s_table), c->stream));
+    c->pc_behind = true;
+    guard.g = nullptr;
+    *out = g;
+    return CAKE_B200_OK;
+  });
 }
 extern "C" void cake_b200_pages_free(cake_b200_pages *g) {
   if (!g) return;
@@ -260,7 +272,7 @@ static int pages_plan(cake_b200_pages *g, const pg::Window &win, bool capturing,
   p->used = ++g->calls;
   if (p->step != g->steps) {
     RC(no_capture(c->stream, "this step's plan of attention"));
-    RC(pages_plan_make(g, p));
+    RC(with_memory([&]() -> int { return pages_plan_make(g, p); }));
   }
   p->kept = p->kept || capturing;
   *out = p;
@@ -274,32 +286,35 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
   cake_b200_ctx *c = g->ctx;
   const OnDevice dev(g->device);
   if (is_capturing(stream ? (cudaStream_t)stream : c->stream)) return fail(CAKE_B200_ESTATE, "a step is planned outside captures; its calls may be captured");
-  pg::Book &k = g->book;
-  int i = 0;
-  switch (k.plan(seqs, counts, n, c->cfg.n_heads / c->cfg.n_kv_heads, &i)) {
-    case pg::Book::OK: break;
-    case pg::Book::NOT_LIVE: return fail(CAKE_B200_EINVAL, "there is no sequence %d", seqs[i]);
-    case pg::Book::TWICE: return fail(CAKE_B200_EINVAL, "sequence %d is twice in the step", seqs[i]);
-    case pg::Book::COUNT: return fail(CAKE_B200_EINVAL, "sequence %d brings %d rows", seqs[i], counts[i]);
-    case pg::Book::TOO_LONG: return fail(CAKE_B200_ESTATE, "sequence %d: %d + %d positions exceed max_seq %d", seqs[i], k.seqs[(size_t)seqs[i]].len, counts[i], k.max_seq);
-    case pg::Book::NO_PAGES: return fail(CAKE_B200_ENOMEM, "the step needs more pages than the %d that are free", (int)k.free_pages.size());
-  }
-  return on_stream(c, stream, [&]() -> int {
-    const size_t at = sizeof(pg::StepHead) + (size_t)k.max_seqs * sizeof(pg::SeqRow), bytes = at + k.updates.size() * 4;
-    std::vector<char> blob(bytes, 0);
-    pg::StepHead h{};
-    h.shape = k.shape; h.n_seqs = n; h.n_rows = k.n_rows; h.n_updates = (int)k.updates.size() / 2;
-    memcpy(blob.data(), &h, sizeof h);
-    memcpy(blob.data() + sizeof h, k.step.data(), k.step.size() * sizeof(pg::SeqRow));
-    if (!k.updates.empty()) memcpy(blob.data() + at, k.updates.data(), k.updates.size() * 4);
-    RC(pages_upload(c, g->step, blob.data(), bytes));
-    int most = 1;
-    for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
-    CU((cudaError_t)pg::spread(c->stream, g->step, k.max_seqs, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
-    g->steps++;
-    for (auto &p : g->plans)
-      if (p.kept) RC(pages_plan_make(g, &p));
-    return CAKE_B200_OK;
+  return with_memory([&]() -> int {
+    pg::Book &k = g->book;
+    int i = 0;
+    switch (k.plan(seqs, counts, n, c->cfg.n_heads / c->cfg.n_kv_heads, &i)) {
+      case pg::Book::OK: break;
+      case pg::Book::NOT_LIVE: return fail(CAKE_B200_EINVAL, "there is no sequence %d", seqs[i]);
+      case pg::Book::TWICE: return fail(CAKE_B200_EINVAL, "sequence %d is twice in the step", seqs[i]);
+      case pg::Book::COUNT: return fail(CAKE_B200_EINVAL, "sequence %d brings %d rows", seqs[i], counts[i]);
+      case pg::Book::TOO_LONG: return fail(CAKE_B200_ESTATE, "sequence %d: %d + %d positions exceed max_seq %d", seqs[i], k.seqs[(size_t)seqs[i]].len, counts[i], k.max_seq);
+      case pg::Book::NO_PAGES: return fail(CAKE_B200_ENOMEM, "the step needs more pages than the %d that are free", (int)k.free_pages.size());
+    }
+    return on_stream(c, stream, [&]() -> int {
+      const size_t at = sizeof(pg::StepHead) + (size_t)n * sizeof(pg::SeqRow), bytes = at + k.updates.size() * 4;
+      std::vector<char> &blob = g->blob;   // (has the room)
+      blob.assign(bytes, 0);
+      pg::StepHead h{};
+      h.shape = k.shape; h.n_seqs = n; h.n_rows = k.n_rows; h.n_updates = (int)k.updates.size() / 2;
+      memcpy(blob.data(), &h, sizeof h);
+      memcpy(blob.data() + sizeof h, k.step.data(), k.step.size() * sizeof(pg::SeqRow));
+      if (!k.updates.empty()) memcpy(blob.data() + at, k.updates.data(), k.updates.size() * 4);
+      RC(pages_upload(c, g->step, blob.data(), bytes));
+      int most = 1;
+      for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
+      CU((cudaError_t)pg::spread(c->stream, g->step, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
+      g->steps++;
+      for (auto &p : g->plans)
+        if (p.kept) RC(with_memory([&]() -> int { return pages_plan_make(g, &p); }));
+      return CAKE_B200_OK;
+    });
   });
 }
 

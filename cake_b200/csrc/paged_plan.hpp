@@ -98,13 +98,18 @@ struct Book {
       rows += counts[i];
     }
     if (need > (long long)free_pages.size()) return NO_PAGES;
+    std::vector<SeqRow> many;   // (all memory first: what can throw does so in front of any change)
+    std::vector<int> who(which, which + n);
+    many.reserve((size_t)n);
+    step.reserve((size_t)n);
+    updates.reserve(2 * (size_t)need);
+    for (int i = 0; i < n; i++) seqs[(size_t)which[i]].pages.reserve((size_t)((seqs[(size_t)which[i]].len + counts[i] + page - 1) / page));
     end_step();
-    ids.assign(which, which + n);
+    ids.swap(who);
     n_rows = (int)rows;
     shape = 1469598103934665603ull;
     for (int i = 0; i < n; i++) shape = (shape ^ (uint64_t)(uint32_t)counts[i]) * 1099511628211ull;
     shape = (shape ^ (uint64_t)n) * 1099511628211ull;
-    std::vector<SeqRow> many;
     int row0 = 0;
     for (int i = 0; i < n; i++) {
       Seq &q = seqs[(size_t)which[i]];

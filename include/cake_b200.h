@@ -421,7 +421,7 @@ int cake_b200_cache_attend(cake_b200_cache *, int block_idx, const void *q_dev, 
                            int first, float scale, void *stream);
 
 /* ---- caches in pages ----------------------------------------------------------------------------
- * K and V rows of many sequences of different lengths in pages of one pool: a page holds page_size consecutive positions (16, 32, .. 1024) of one sequence,
+ * K and V rows of many sequences (up to 65536) of different lengths in pages of one pool: a page holds page_size consecutive positions (16, 32, .. 1024) of one sequence,
  * for every block.  A sequence takes pages as it grows and gives them back when it is dropped or truncated.  Llama-family blocks with head_dim 64, 128 or
  * 256 and rotated parts of a multiple of 16 entries.  The pool of a block (n_pages pages) is made at its first append.
  * A STEP brings counts[i] new rows (1 or more) of each of some sequences, packed one sequence behind another in the order given: row r of a sequence that held
