@@ -257,7 +257,7 @@ int attend(cudaStream_t s, int dtype, const Pool &p, const Attend &a, const Scra
   if (a.n_few) {
     const Few f{p, a.plan, a.seqs, a.q, a.q_tok, a.out, w.few_ws, a.n_heads, G, a.win, scale_log2, a.err, a.n_items ? 1 : 0};
     const Cut *cuts = reinterpret_cast<const Cut *>(reinterpret_cast<const Worker *>(a.plan + 1) + few_ctas(p.hd, w.sms));
-    const int cluster = a.longest ? cluster_of(a.n_few * p.n_kv, a.longest, a.tiles, few_ctas(p.hd, w.sms), w.clusters->most[a.few_cols <= 8 ? 0 : 1]) : 0;
+    const int cluster = cluster_of(a.n_few * p.n_kv, a.longest, a.tiles, few_ctas(p.hd, w.sms), w.clusters->most[a.few_cols <= 8 ? 0 : 1]);
     const int e = by_kind(dtype, p.hd, [&](auto t, auto h) {
       typedef typename decltype(t)::type T;
       constexpr int HD = decltype(h)::value;

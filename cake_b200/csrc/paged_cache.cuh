@@ -86,7 +86,7 @@ struct Attend {
   Window win;
   const PlanHead *plan;
   int n_few, few_cols;           // sequences of few rows, query rows of a key head that they have at most
-  int longest, tiles;            // tiles of their longest run, of all; 0: a captured call, whose lengths may become any
+  int longest, tiles;            // tiles of their longest run, of all; of a captured call, whose lengths may become any: the most that a run can have, and 0
   int n_cuts, n_items;           // runs that are cut, items of the many-row kernel; of a captured call: as many as any plan of the step's shape can have
   int most_items;                // that many items: the list of cut tiles is behind them
   int n_cut_tiles;               // tiles that are cut (of a captured call: as many as may be)

@@ -365,10 +365,13 @@ static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_to
   const bool capturing = is_capturing(c->stream);
   RC(pages_plan(g, win, capturing, &plan));
   int cols = 0;
+  // a captured call's lengths may become any: up to what the cache and the window allow
+  const int most_seen = win.w > 0 && !win.by_call ? (int)std::min<long long>(g->book.max_seq, (long long)win.w + pg::TOKEN_COLS + pg::TILE) : g->book.max_seq;
+  const int longest = capturing ? (most_seen + pg::TILE - 1) / pg::TILE + 1 : plan->longest;
   const int most_cuts = std::min(g->book.n_few * c->cfg.n_kv_heads, pg::few_ctas(c->cfg.head_dim, c->sm_count));
   for (int i = 0; i < g->book.n_few; i++) cols = std::max(cols, g->book.step[(size_t)i].count * (c->cfg.n_heads / c->cfg.n_kv_heads));
   const pg::Attend a{q, (long long)q_tok, out, (const pg::SeqRow *)(g->step + 1), c->cfg.n_heads, scale, win, (const pg::PlanHead *)plan->dev, g->book.n_few, cols,
-                     capturing ? 0 : plan->longest, plan->tiles, capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, plan->most_items, capturing ? plan->most_cut_tiles : plan->n_cut_tiles, c->wait_err};
+                     longest, capturing ? 0 : plan->tiles, capturing ? most_cuts : plan->n_cuts, capturing ? plan->most_items : plan->n_items, plan->most_items, capturing ? plan->most_cut_tiles : plan->n_cut_tiles, c->wait_err};
   CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count, &c->pg_clusters}, launch_counter(c)));
   return CAKE_B200_OK;
 }

@@ -622,11 +622,12 @@ def test_pools_beyond_32_bits(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("max_seq", [2500, 65000])   # (what a run can have at most decides how a captured call is cut)
 @pytest.mark.parametrize("heads,kv,hd,counts", [(32, 8, 128, [1, 1, 1]), (8, 2, 64, [2, 1, 3]), (16, 8, 128, [1, 90, 1])])
-def test_captured_and_replayed(heads, kv, hd, counts):
+def test_captured_and_replayed(heads, kv, hd, counts, max_seq):
     """A step's calls captured once, replayed for steps of other sequences and lengths; a step of other counts is refused."""
     ctx = ctx_for(heads, kv, hd, "bf16")
-    cache = PagedCache(ctx, 400, 16, max_seqs=5, max_seq=2500)
+    cache = PagedCache(ctx, 400, 16, max_seqs=5, max_seq=max_seq)
     t = Talks(cache, kv, hd, "bf16")
     ids = [t.add() for _ in range(5)]
     t.step(ids, [40, 700, 3, 64, 1500], 1)
