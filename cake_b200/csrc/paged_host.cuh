@@ -57,9 +57,9 @@ static bool is_capturing(cudaStream_t s) {
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e != cudaSuccess || st != cudaStreamCaptureStatusNone;
 }
-// host data on its way to the device: pinned buffers in turn
-static int pages_upload(cake_b200_ctx *c, void *dst, const void *src, size_t bytes) {
-  cake_b200_ctx::Staging &t = c->pg_stage[c->pg_next++ % (sizeof c->pg_stage / sizeof c->pg_stage[0])];
+// host data on its way to the device: pinned buffers in turn.  pages_room: the next upload has the room for so much.
+static int pages_room(cake_b200_ctx *c, size_t bytes) {
+  cake_b200_ctx::Staging &t = c->pg_stage[c->pg_next % (sizeof c->pg_stage / sizeof c->pg_stage[0])];
   if (!t.done) CU(cudaEventCreateWithFlags(&t.done, cudaEventDisableTiming));
   if (t.busy) CU(cudaEventSynchronize(t.done));
   t.busy = false;
@@ -70,6 +70,11 @@ static int pages_upload(cake_b200_ctx *c, void *dst, const void *src, size_t byt
     CU(cudaMallocHost(&t.p, cap));
     t.cap = cap;
   }
+  return CAKE_B200_OK;
+}
+static int pages_upload(cake_b200_ctx *c, void *dst, const void *src, size_t bytes) {
+  RC(pages_room(c, bytes));
+  cake_b200_ctx::Staging &t = c->pg_stage[c->pg_next++ % (sizeof c->pg_stage / sizeof c->pg_stage[0])];
   memcpy(t.p, src, bytes);
   CU(cudaMemcpyAsync(dst, t.p, bytes, cudaMemcpyHostToDevice, c->stream));
   CU(cudaEventRecord(t.done, c->stream));
@@ -286,6 +291,9 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
   cake_b200_ctx *c = g->ctx;
   const OnDevice dev(g->device);
   if (is_capturing(stream ? (cudaStream_t)stream : c->stream)) return fail(CAKE_B200_ESTATE, "a step is planned outside captures; its calls may be captured");
+  long long pages = 0;   // that the step may take, at most
+  for (int i = 0; i < n; i++) pages += std::max(counts[i], 0) / g->book.page + 1;
+  RC(pages_room(c, sizeof(pg::StepHead) + (size_t)n * sizeof(pg::SeqRow) + (size_t)std::min<long long>(pages, (long long)g->book.free_pages.size()) * 8));
   return with_memory([&]() -> int {
     pg::Book &k = g->book;
     int i = 0;
@@ -311,8 +319,13 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
       for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
       CU((cudaError_t)pg::spread(c->stream, g->step, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
       g->steps++;
-      for (auto &p : g->plans)
-        if (p.kept) RC(with_memory([&]() -> int { return pages_plan_make(g, &p); }));
+      for (auto &p : g->plans) {
+        const int rc = !p.kept ? CAKE_B200_OK : with_memory([&]() -> int { return pages_plan_make(g, &p); });
+        if (rc == CAKE_B200_OK) continue;
+        k.step.clear();   // no step, and none for a replayed graph either: its calls would follow an older one's plan
+        (void)cudaMemsetAsync(g->step, 0, sizeof(pg::StepHead), c->stream);
+        return rc;
+      }
       return CAKE_B200_OK;
     });
   });
@@ -401,6 +414,10 @@ extern "C" int cake_b200_pages_attend(cake_b200_pages *g, int block_idx, const v
   const OnDevice dev(g->device);
   if (!q_dev || !out_dev) return fail(CAKE_B200_EINVAL, "null argument");
   if (unaligned(q_dev, q_tok) || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "pages_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
+  const cake_b200_config &f = g->ctx->cfg;
+  const size_t es = g->ctx->es, row = (size_t)f.n_heads * f.head_dim, rows = (size_t)g->book.n_rows;
+  if ((const char *)q_dev < (const char *)out_dev + rows * row * es && (const char *)out_dev < (const char *)q_dev + ((rows - 1) * q_tok + row) * es)
+    return fail(CAKE_B200_EINVAL, "pages_attend's out lies beside q, not on it");
   if (window < 0 || !(scale >= 0.f && scale <= 2e38f)) return fail(CAKE_B200_EINVAL, "window %d or scale %g out of range", window, (double)scale);
   if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);
   RC(pages_written(g, block_idx, true));

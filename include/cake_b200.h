@@ -456,7 +456,7 @@ int cake_b200_pages_append(cake_b200_pages *, int block_idx, const void *q_dev, 
                            void *q_out, int rotate, void *stream);
 /* out (rows, n_heads, head_dim): softmax(scale q . k_j) weighted sum of v_j over the positions j of a row's sequence up to its own position p, with window > 0
  * only p - window < j.  Scores, maxima and sums in fp32, weights as two operands of D (16 bits and more), one rounding to D; what a row does not see counts for
- * nothing, infinities and NaN included.  scale 0: head_dim^-1/2. */
+ * nothing, infinities and NaN included.  scale 0: head_dim^-1/2.  out does not overlap q. */
 int cake_b200_pages_attend(cake_b200_pages *, int block_idx, const void *q_dev, size_t q_tok, void *out_dev, int window, float scale, void *stream);
 /* Rows as the pages hold them -> k, v (rows, n_kv, head_dim), either may be NULL: the step's (seq < 0), or positions [first, first + n) of a sequence. */
 int cake_b200_pages_read(cake_b200_pages *, int block_idx, int seq, int first, int n, void *k_dev, void *v_dev, void *stream);

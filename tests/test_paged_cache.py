@@ -804,6 +804,32 @@ def test_refusals():
 
 
 @pytest.mark.gpu
+def test_a_result_on_its_queries_is_refused():
+    """Several CTAs read the same queries: a result that covers any of them is no call, one right beside them is."""
+    ctx = ctx_for(8, 2, 64, "bf16")
+    cache = PagedCache(ctx, 8, 16, max_seqs=2, max_seq=60)
+    s = cache.add()
+    cache.step([s], [2])
+    x = normal((2, 2, 64), "bf16", 1)
+    q = normal((4, 8, 64), "bf16", 2)
+    cache.append(0, None, x, x)
+    want = cache.attend(0, q[1:3])
+    at, row = q.data_ptr(), 8 * 64 * 2
+
+    def call(first, out, tok=8 * 64):
+        return lib().cake_b200_pages_attend(cache.h, 0, at + first * row, tok, at + out * row, 0, 0.0, cache._stream())
+    torch.cuda.synchronize()
+    for first, out, tok in ((1, 1, 512), (1, 0, 512), (1, 2, 512), (0, 1, 1024), (1, 0, 0)):
+        assert call(first, out, tok) == EINVAL
+    q[3] = q[1]
+    assert call(2, 0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q[0:2], cache.attend(0, q[2:4])) and torch.isfinite(want.float()).all()
+    cache.close()
+    ctx.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv,hd,page", [(8, 2, 64, 1024), (32, 8, 128, 512), (8, 4, 256, 1024)])
 def test_pages_that_are_many_tiles(heads, kv, hd, page):
     ctx = ctx_for(heads, kv, hd, "f16")
