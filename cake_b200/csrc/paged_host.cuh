@@ -433,6 +433,7 @@ extern "C" int cake_b200_pages_read(cake_b200_pages *g, int block_idx, int seq, 
   if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);
   pg::Read a{nullptr, seq, first, n, k_dev, v_dev};
   if (seq < 0) {
+    if (n != 0 && n != g->book.n_rows) return fail(CAKE_B200_EINVAL, "pages_read: room for %d rows, the step has %d", n, g->book.n_rows);
     RC(pages_written(g, block_idx, true));
     a = pg::Read{g->rows, 0, 0, g->book.n_rows, k_dev, v_dev};
   } else {

@@ -263,6 +263,8 @@ class PagedCache:
         of one sequence."""
         if seq is None:
             seq, n, like = -1, self._rows, self._kv_like
+        elif not 0 <= seq < self.max_seqs:   # (below 0 the library takes it for the step's rows)
+            raise capi.CakeB200Error(-1, f"there is no sequence {seq}")
         else:
             n = self.len(seq) - first if n is None else n
             like = self._one.expand(max(n, 0), self._kv, self._hd)

@@ -458,7 +458,8 @@ int cake_b200_pages_append(cake_b200_pages *, int block_idx, const void *q_dev, 
  * only p - window < j.  Scores, maxima and sums in fp32, weights as two operands of D (16 bits and more), one rounding to D; what a row does not see counts for
  * nothing, infinities and NaN included.  scale 0: head_dim^-1/2.  out does not overlap q. */
 int cake_b200_pages_attend(cake_b200_pages *, int block_idx, const void *q_dev, size_t q_tok, void *out_dev, int window, float scale, void *stream);
-/* Rows as the pages hold them -> k, v (rows, n_kv, head_dim), either may be NULL: the step's (seq < 0), or positions [first, first + n) of a sequence. */
+/* Rows as the pages hold them -> k, v (rows, n_kv, head_dim), either may be NULL: the step's (seq < 0; n: its rows, or 0), or positions [first, first + n)
+ * of a sequence. */
 int cake_b200_pages_read(cake_b200_pages *, int block_idx, int seq, int first, int n, void *k_dev, void *v_dev, void *stream);
 /* == cake_b200_forward_batch over the step: x_dev, y_dev (n_rows, hidden) in D.  A block's sliding window is that of forward_batch: all of a sequence's rows see
  * the last `window` positions that its last row does, and a first call everything. */
