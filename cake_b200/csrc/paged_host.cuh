@@ -388,6 +388,12 @@ static int pages_attend_on(cake_b200_pages *g, int l, const void *q, size_t q_to
   CU((cudaError_t)pg::attend(c->stream, c->cfg.dtype, pages_pool(g, l), a, pg::Scratch{g->few_ws, g->tiles_ws, c->sm_count, &c->pg_clusters}, launch_counter(c)));
   return CAKE_B200_OK;
 }
+// rows of `row` entries of `es` bytes, `tok` entries from one to the next: whether two sets of them, from their first byte to their last, share any
+struct RowsAt { const void *at; size_t rows, tok, row; };
+static bool on_another(const RowsAt &a, const RowsAt &b, size_t es) {
+  const char *pa = (const char *)a.at, *pb = (const char *)b.at;
+  return pa < pb + ((b.rows - 1) * b.tok + b.row) * es && pb < pa + ((a.rows - 1) * a.tok + a.row) * es;
+}
 extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev,
                                       size_t v_tok, void *q_out, int rotate, void *stream) {
   RC(pages_block(g, block_idx, "pages_append", true));
@@ -395,10 +401,18 @@ extern "C" int cake_b200_pages_append(cake_b200_pages *g, int block_idx, const v
   if (!k_dev || !v_dev || !q_dev != !q_out) return fail(CAKE_B200_EINVAL, "null argument");
   if (unaligned(k_dev, k_tok) || unaligned(v_dev, v_tok) || unaligned(q_dev, q_tok) || unaligned(q_out))
     return fail(CAKE_B200_EINVAL, "pages_append takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
-  RC(pages_written(g, block_idx, false));
   cake_b200_ctx *c = g->ctx;
-  if (!g->pool[(size_t)block_idx] && stream) RC(no_capture((cudaStream_t)stream, "a block's pages"));
   const cake_b200_config &f = c->cfg;
+  if (q_out) {   // a warp has one row: another row's may not have been read yet
+    const size_t rows = (size_t)g->book.n_rows, row = (size_t)f.n_heads * f.head_dim, kv = (size_t)f.n_kv_heads * f.head_dim;
+    const RowsAt out{q_out, rows, row, row};
+    const bool in_place = q_out == q_dev && (q_tok == row || rows == 1);
+    if ((!in_place && on_another(out, RowsAt{q_dev, rows, q_tok, row}, c->es)) || on_another(out, RowsAt{k_dev, rows, k_tok, kv}, c->es) ||
+        on_another(out, RowsAt{v_dev, rows, v_tok, kv}, c->es))
+      return fail(CAKE_B200_EINVAL, "pages_append's q_out lies beside q, k and v, or on a contiguous q");
+  }
+  RC(pages_written(g, block_idx, false));
+  if (!g->pool[(size_t)block_idx] && stream) RC(no_capture((cudaStream_t)stream, "a block's pages"));
   return on_stream(c, stream, [&]() -> int {
     RC(pages_ensure(g, block_idx));
     pg::Append a{};
@@ -415,8 +429,8 @@ extern "C" int cake_b200_pages_attend(cake_b200_pages *g, int block_idx, const v
   if (!q_dev || !out_dev) return fail(CAKE_B200_EINVAL, "null argument");
   if (unaligned(q_dev, q_tok) || unaligned(out_dev)) return fail(CAKE_B200_EINVAL, "pages_attend takes rows on 16-byte boundaries (strides of a multiple of 8 entries)");
   const cake_b200_config &f = g->ctx->cfg;
-  const size_t es = g->ctx->es, row = (size_t)f.n_heads * f.head_dim, rows = (size_t)g->book.n_rows;
-  if ((const char *)q_dev < (const char *)out_dev + rows * row * es && (const char *)out_dev < (const char *)q_dev + ((rows - 1) * q_tok + row) * es)
+  const size_t row = (size_t)f.n_heads * f.head_dim, rows = (size_t)g->book.n_rows;
+  if (on_another(RowsAt{out_dev, rows, row, row}, RowsAt{q_dev, rows, q_tok, row}, g->ctx->es))
     return fail(CAKE_B200_EINVAL, "pages_attend's out lies beside q, not on it");
   if (window < 0 || !(scale >= 0.f && scale <= 2e38f)) return fail(CAKE_B200_EINVAL, "window %d or scale %g out of range", window, (double)scale);
   if (!g->pool[(size_t)block_idx]) return fail(CAKE_B200_ESTATE, "block %d has no rows", block_idx);

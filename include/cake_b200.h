@@ -451,7 +451,8 @@ int cake_b200_pages_available(const cake_b200_pages *);            /* pages that
 int cake_b200_pages_step(cake_b200_pages *, const int *seqs, const int *counts, int n, void *stream);
 /* Rows k, v (rows, n_kv, head_dim) and q (rows, n_heads, head_dim) in D, *_tok entries (a multiple of 8) from row to row, heads side by side, pointers on 16
  * bytes.  k and v join the pages, k rotated by its position's row of the tables; q, rotated likewise, goes to q_out (rows, n_heads, head_dim) contiguous, which
- * may be q where that is contiguous.  q and q_out NULL: keys and values alone.  rotate 0: all as they are.  Products and sums in fp32, one rounding to D. */
+ * may be q where that is contiguous and else lies on none of q, k and v (CAKE_B200_EINVAL).  q and q_out NULL: keys and values alone.  rotate 0: all as they are.
+ * Products and sums in fp32, one rounding to D. */
 int cake_b200_pages_append(cake_b200_pages *, int block_idx, const void *q_dev, size_t q_tok, const void *k_dev, size_t k_tok, const void *v_dev, size_t v_tok,
                            void *q_out, int rotate, void *stream);
 /* out (rows, n_heads, head_dim): softmax(scale q . k_j) weighted sum of v_j over the positions j of a row's sequence up to its own position p, with window > 0

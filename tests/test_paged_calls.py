@@ -61,3 +61,56 @@ def test_room_for_other_rows_than_the_steps_is_refused():
     refused(EINVAL, cache.read, 0, -1, 0, 1)
     refused(EINVAL, cache.read, 0, -1)
     ctx.close()
+
+
+# ------------------------------------------------------------------------------------------------ results on their inputs
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3])
+def test_queries_rotated_onto_rows_that_are_still_read_are_refused(rows):
+    """A fused projection [rows, q | k | v]: results that would lie on rows of it are no call; a contiguous q in place, and room beside it, are."""
+    heads, kv, hd = 8, 2, 64
+    wide, row = (heads + 2 * kv) * hd, heads * hd
+    ctx = ctx_for(heads, kv, hd)
+    cache = PagedCache(ctx, 8, 16, max_seqs=2, max_seq=60)
+    s = cache.add()
+    cache.step([s], [4])
+    x = torch.randn(4, kv, hd, device="cuda").bfloat16()
+    cache.append(0, None, x, x)
+    cache.step([s], [rows])
+    buf = torch.randn(8 * wide, device="cuda").bfloat16()
+    fused = buf[wide:(1 + rows) * wide].view(rows, heads + 2 * kv, hd)
+    q, k, v = fused[:, :heads], fused[:, heads:heads + kv], fused[:, heads + kv:]
+    want, before = cache.append(0, q, k, v), buf.clone()
+    wk, wv = cache.read(0)
+    at = fused.data_ptr()
+
+    def call(out, q_at=at, tok=wide, k_at=at + 2 * row, v_at=at + 2 * (row + kv * hd), kv_tok=wide):
+        return lib().cake_b200_pages_append(cache.h, 0, q_at, tok, k_at, kv_tok, v_at, kv_tok, out, 1, cache._stream())
+    torch.cuda.synchronize()
+    inside = [at + 16, at + 2 * (row - 8), at - 16, at + 2 * row, at + 2 * (wide - 8)]
+    if rows > 1:
+        inside += [at, at + 2 * wide, at + 2 * ((rows - 1) * wide + 8)]
+    for out in inside:
+        assert call(out) == EINVAL, (out - at) / 2
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    free = buf.data_ptr() + 2 * (1 + rows) * wide   # right behind, and right in front
+    for out in (free, at - 2 * rows * row):
+        if out < buf.data_ptr():
+            continue
+        assert call(out) == 0
+        torch.cuda.synchronize()
+        first = (out - buf.data_ptr()) // 2
+        assert torch.equal(buf[first:first + rows * row].view(rows, heads, hd), want)
+        buf.copy_(before)
+    qc, kc, vc = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    for k_at, v_at in ((kc.data_ptr(), qc.data_ptr()), (qc.data_ptr(), vc.data_ptr())):   # its keys, or values, are its queries
+        assert call(qc.data_ptr(), qc.data_ptr(), row, k_at, v_at, kv * hd) == EINVAL
+    assert call(qc.data_ptr(), qc.data_ptr(), row, kc.data_ptr(), vc.data_ptr(), kv * hd) == 0
+    assert torch.equal(qc, want)
+    assert all(torch.equal(a, b) for a, b in zip(cache.read(0), (wk, wv)))
+    if rows == 1:   # one row is contiguous at any stride
+        assert call(at) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(fused[:, :heads], want)
+    ctx.close()
