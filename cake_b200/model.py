@@ -31,6 +31,8 @@ from .capi import byref, c_uint32, c_void_p, check, int_array, lib, ptr, ptr_arr
 from .config import CConfig, Config
 from .synth import TORCH_DTYPES
 
+MAX_LOGITS_ROWS = 64   # of one cake_b200_logits call
+
 
 class Cache:
     """KV cache of one session (cache.rs:9).  RoPE tables live in the ctx (computed once per model).
@@ -788,10 +790,14 @@ class TextModelBase:
             if n > len(counts):   # the last row of each
                 y = y.index_select(0, torch.from_numpy(np.cumsum(counts) - 1).to(y.device))
             logits = torch.empty(len(counts), ctx.config.vocab_size, dtype=ctx.logits_dtype, device=ctx.torch_device)
-            best = None if greedy is None else (c_uint32 * len(counts))()
-            check(L.cake_b200_logits(ctx.h, ptr(y), len(counts), 1, ptr(logits), best))
+            best = []
+            for at in range(0, len(counts), MAX_LOGITS_ROWS):
+                some, rows = logits[at:at + MAX_LOGITS_ROWS], y[at:at + MAX_LOGITS_ROWS]
+                top = None if greedy is None else (c_uint32 * len(some))()
+                check(L.cake_b200_logits(ctx.h, ptr(rows), len(some), 1, ptr(some), top))
+                best += top or ()
         if greedy is not None:
-            greedy[:] = [int(t) for t in best]
+            greedy[:] = best
         return logits
 
     def _local_run(self):

@@ -505,7 +505,7 @@ int cake_b200_head_load_tables(cake_b200_ctx *, const cake_b200_embed_tables *);
 int cake_b200_embed_at(cake_b200_ctx *, cake_b200_cache *, const uint32_t *ids_host, int batch, int seq, int index_pos, void *x_dev);
 /* ln_f on the last position of each batch row, lm_head, logits (batch, vocab) in D written to
  * logits_dev (nullable); if argmax_host != NULL also computes the greedy token per row
- * (first maximum wins), copies it to argmax_host and synchronises. */
+ * (first maximum wins), copies it to argmax_host and synchronises.  batch: up to 64. */
 int cake_b200_logits(cake_b200_ctx *, const void *x_dev, int batch, int seq, void *logits_dev, uint32_t *argmax_host);
 /* The same for ANY rows of x_dev ((n_rows_total, hidden), row = b * seq + t), in FP32: final norm -> lm_head -> logit
  * soft cap, logits_f32_dev[(i, vocab)] for i < n.  Layer-list models (fp32 residual stream) only.  Asynchronous. */
