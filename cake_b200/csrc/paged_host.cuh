@@ -305,7 +305,7 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
       case pg::Book::TOO_LONG: return fail(CAKE_B200_ESTATE, "sequence %d: %d + %d positions exceed max_seq %d", seqs[i], k.seqs[(size_t)seqs[i]].len, counts[i], k.max_seq);
       case pg::Book::NO_PAGES: return fail(CAKE_B200_ENOMEM, "the step needs more pages than the %d that are free", (int)k.free_pages.size());
     }
-    return on_stream(c, stream, [&]() -> int {
+    auto send = [&]() -> int {
       const size_t at = sizeof(pg::StepHead) + (size_t)n * sizeof(pg::SeqRow), bytes = at + k.updates.size() * 4;
       std::vector<char> &blob = g->blob;   // (has the room)
       blob.assign(bytes, 0);
@@ -319,15 +319,18 @@ extern "C" int cake_b200_pages_step(cake_b200_pages *g, const int *seqs, const i
       for (int j = 0; j < n; j++) most = std::max(most, counts[j]);
       CU((cudaError_t)pg::spread(c->stream, g->step, n, h.n_updates, most, g->table, g->rows, launch_counter(c)));
       g->steps++;
-      for (auto &p : g->plans) {
-        const int rc = !p.kept ? CAKE_B200_OK : with_memory([&]() -> int { return pages_plan_make(g, &p); });
-        if (rc == CAKE_B200_OK) continue;
-        k.step.clear();   // no step, and none for a replayed graph either: its calls would follow an older one's plan
-        (void)cudaMemsetAsync(g->step, 0, sizeof(pg::StepHead), c->stream);
-        return rc;
-      }
+      for (auto &p : g->plans)
+        if (p.kept) RC(with_memory([&]() -> int { return pages_plan_make(g, &p); }));
       return CAKE_B200_OK;
+    };
+    const int rc = on_stream(c, stream, [&]() -> int {
+      const int rc = send();
+      if (rc != CAKE_B200_OK) (void)cudaMemsetAsync(g->step, 0, sizeof(pg::StepHead), c->stream);   // none for a replayed graph either: its calls would follow an older one's plan
+      return rc;
     });
+    if (rc != CAKE_B200_OK)   // no step, and its sequences are as they were
+      for (int j = 0; j < n; j++) k.cut(seqs[j], k.seqs[(size_t)seqs[j]].len - counts[j]);
+    return rc;
   });
 }
 

@@ -447,7 +447,7 @@ int cake_b200_pages_truncate(cake_b200_pages *, int seq, int len); /* back to it
 int cake_b200_pages_len(const cake_b200_pages *, int seq);         /* positions, the step's included, or < 0 */
 int cake_b200_pages_available(const cake_b200_pages *);            /* pages that no sequence has */
 /* CAKE_B200_ENOMEM where the free pages do not suffice, CAKE_B200_ESTATE beyond max_seq, CAKE_B200_EINVAL for a sequence that is not there or is there
- * twice: nothing has changed then. */
+ * twice: nothing has changed then.  After any other error no step stands, and the sequences have the positions and pages that they had. */
 int cake_b200_pages_step(cake_b200_pages *, const int *seqs, const int *counts, int n, void *stream);
 /* Rows k, v (rows, n_kv, head_dim) and q (rows, n_heads, head_dim) in D, *_tok entries (a multiple of 8) from row to row, heads side by side, pointers on 16
  * bytes.  k and v join the pages, k rotated by its position's row of the tables; q, rotated likewise, goes to q_out (rows, n_heads, head_dim) contiguous, which
