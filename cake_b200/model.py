@@ -772,7 +772,8 @@ class TextModelBase:
 
     def forward_paged(self, pages: PagedCache, requests: Sequence[Tuple[int, Sequence[int]]], greedy: Optional[List[int]] = None) -> torch.Tensor:
         """One step of many sequences: requests [(sequence of ``pages``, its next token ids)] -> logits (len(requests), vocab) of their last tokens, a device
-        tensor in D.  ``greedy``: a list that receives each one's most likely next token (the call then waits for them).  All blocks are local ones."""
+        tensor in D.  ``greedy``: a list that receives each one's most likely next token (the call then waits for them).  All blocks are local ones.  Where the
+        call fails, the sequences are as they were."""
         ctx, L = self.ctx, lib()
         run = self._local_run()
         if run is None:
@@ -784,18 +785,23 @@ class TextModelBase:
             if n and (ids >= ctx.config.vocab_size).any():   # in front of the step, which takes its pages
                 raise ValueError(f"token id {ids.max()} out of range (vocab {ctx.config.vocab_size})")
             pages.step([s for s, _ in requests], counts)
-            x, y = (torch.empty(n, ctx.config.stream_width, dtype=ctx.stream_dtype, device=ctx.torch_device) for _ in range(2))
-            check(L.cake_b200_embed(ctx.h, ids.ctypes.data_as(ctypes.POINTER(c_uint32)), 1, n, ptr(x)))
-            check(L.cake_b200_forward_paged(ctx.h, run[0], run[1], run[2], pages.h, ptr(x), ptr(y), n))
-            if n > len(counts):   # the last row of each
-                y = y.index_select(0, torch.from_numpy(np.cumsum(counts) - 1).to(y.device))
-            logits = torch.empty(len(counts), ctx.config.vocab_size, dtype=ctx.logits_dtype, device=ctx.torch_device)
-            best = []
-            for at in range(0, len(counts), MAX_LOGITS_ROWS):
-                some, rows = logits[at:at + MAX_LOGITS_ROWS], y[at:at + MAX_LOGITS_ROWS]
-                top = None if greedy is None else (c_uint32 * len(some))()
-                check(L.cake_b200_logits(ctx.h, ptr(rows), len(some), 1, ptr(some), top))
-                best += top or ()
+            try:
+                x, y = (torch.empty(n, ctx.config.stream_width, dtype=ctx.stream_dtype, device=ctx.torch_device) for _ in range(2))
+                check(L.cake_b200_embed(ctx.h, ids.ctypes.data_as(ctypes.POINTER(c_uint32)), 1, n, ptr(x)))
+                check(L.cake_b200_forward_paged(ctx.h, run[0], run[1], run[2], pages.h, ptr(x), ptr(y), n))
+                if n > len(counts):   # the last row of each
+                    y = y.index_select(0, torch.from_numpy(np.cumsum(counts) - 1).to(y.device))
+                logits = torch.empty(len(counts), ctx.config.vocab_size, dtype=ctx.logits_dtype, device=ctx.torch_device)
+                best = []
+                for at in range(0, len(counts), MAX_LOGITS_ROWS):
+                    some, rows = logits[at:at + MAX_LOGITS_ROWS], y[at:at + MAX_LOGITS_ROWS]
+                    top = None if greedy is None else (c_uint32 * len(some))()
+                    check(L.cake_b200_logits(ctx.h, ptr(rows), len(some), 1, ptr(some), top))
+                    best += top or ()
+            except BaseException:
+                for (s, _), c in zip(requests, counts):
+                    pages.truncate(s, pages.len(s) - c)
+                raise
         if greedy is not None:
             greedy[:] = best
         return logits
@@ -959,7 +965,6 @@ class PagedSessions:
         fewer to go on."""
         best = None if greedy is None else []
         new = []
-        held = {rid: self.cache.len(self.live[rid]) for rid in tokens if rid in self.live}
         try:
             for rid in tokens:
                 if rid not in self.live:
@@ -967,8 +972,6 @@ class PagedSessions:
                     new.append(rid)
             logits = self.model.forward_paged(self.cache, [(self.live[rid], ids) for rid, ids in tokens.items()], best)
         except BaseException:
-            for rid, n in held.items():
-                self.cache.truncate(self.live[rid], n)
             for rid in new:
                 self.end(rid)
             raise

@@ -40,3 +40,33 @@ def test_more_requests_than_the_head_takes_at_once(requests):
             assert best[str(i)] == int(x.argmax())
         feed = [[int(w.argmax())] for w in want]
     m.ctx.close()
+
+
+@pytest.mark.gpu
+def test_a_step_that_the_blocks_refuse_is_none():
+    """More new rows than the window on a sequence that has some, a cache of another context: sequences as before, and they go on."""
+    from cake_b200.capi import CakeB200Error
+    from cake_b200.model import PagedCache
+    cfg = medium_config(sliding_window=5)
+    m, other = model_for(cfg), model_for(cfg)
+    pages = PagedCache(m.ctx, 12, 16, max_seqs=2)
+    a, b = pages.add(), pages.add()
+    m.forward_paged(pages, [(a, [3, 1, 4, 1])])
+    free = pages.available
+    with pytest.raises(CakeB200Error) as e:
+        m.forward_paged(pages, [(b, [7] * 20), (a, [1, 5, 9, 2, 6, 5])])
+    assert e.value.code == -1 and "window" in str(e.value)
+    assert (pages.len(a), pages.len(b), pages.available) == (4, 0, free)
+    with pytest.raises(CakeB200Error) as e:
+        other.forward_paged(pages, [(a, [1]), (b, [2])])
+    assert e.value.code == -1 and "context" in str(e.value)
+    assert (pages.len(a), pages.len(b), pages.available) == (4, 0, free)
+    got = m.forward_paged(pages, [(a, [1, 5]), (b, [2])])
+    fresh = PagedCache(m.ctx, 12, 16, max_seqs=2)
+    x, y = fresh.add(), fresh.add()
+    m.forward_paged(fresh, [(x, [3, 1, 4, 1])])
+    want = m.forward_paged(fresh, [(x, [1, 5]), (y, [2])])
+    m.ctx.sync()
+    assert torch.equal(got, want)
+    other.ctx.close()
+    m.ctx.close()
