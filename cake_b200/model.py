@@ -980,7 +980,11 @@ class PagedSessions:
         return dict(zip(tokens, logits))
 
     def generate(self, prompts: Dict[str, Sequence[int]], sample_len: int) -> Dict[str, List[int]]:
-        """Greedy generation of up to ``sample_len`` tokens for each of some new requests, all of them together; a request ends with its end of stream."""
+        """Greedy generation of up to ``sample_len`` tokens for each of some new requests, all of them together; a request ends with its end of stream, or with the
+        token behind its last position where it has reached the cache's ``max_seq``."""
+        taken = [rid for rid in prompts if rid in self.live]
+        if taken:
+            raise ValueError(f"requests {taken} are live: generate begins new ones")
         out: Dict[str, List[int]] = {rid: [] for rid in prompts}
         feed, best = dict(prompts), {}
         try:
@@ -993,9 +997,12 @@ class PagedSessions:
                 for rid, token in best.items():
                     if self.model.ctx.config.is_eos(token):
                         self.end(rid)
-                    else:
-                        out[rid].append(token)
+                        continue
+                    out[rid].append(token)
+                    if self.len(rid) < self.cache.max_seq:
                         feed[rid] = [token]
+                    else:   # there is no place for this one
+                        self.end(rid)
         finally:
             for rid in prompts:
                 self.end(rid)

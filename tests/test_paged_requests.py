@@ -70,3 +70,85 @@ def test_a_step_that_the_blocks_refuse_is_none():
     assert torch.equal(got, want)
     other.ctx.close()
     m.ctx.close()
+
+
+class Pages:
+    """Lengths of sequences, for PagedSessions without a GPU."""
+
+    def __init__(self, max_seq):
+        self.max_seq, self.lens = max_seq, {}
+
+    def add(self):
+        s = next(i for i in range(99) if i not in self.lens)
+        self.lens[s] = 0
+        return s
+
+    def drop(self, s):
+        del self.lens[s]
+
+    def len(self, s):
+        return self.lens[s]
+
+
+def sessions(max_seq, answer, eos=()):
+    """PagedSessions in front of a model that answers a request of length n with answer(n); a sequence beyond max_seq fails the whole step, as the library does."""
+    from types import SimpleNamespace
+    from cake_b200.capi import CakeB200Error
+    from cake_b200.model import PagedSessions
+    ses = PagedSessions.__new__(PagedSessions)
+
+    def forward(pages, requests, greedy):
+        if any(pages.lens[s] + len(t) > pages.max_seq for s, t in requests):
+            raise CakeB200Error(-4, "positions exceed max_seq")
+        for s, t in requests:
+            pages.lens[s] += len(t)
+        greedy[:] = [answer(pages.lens[s]) for s, _ in requests]
+        return [None] * len(requests)
+    ses.model = SimpleNamespace(forward_paged=forward, ctx=SimpleNamespace(config=SimpleNamespace(is_eos=lambda t: t in eos)))
+    ses.cache, ses.live = Pages(max_seq), {}
+    return ses
+
+
+def test_a_request_that_fills_its_sequence_ends_and_the_others_go_on():
+    ses = sessions(64, lambda n: n)
+    got = ses.generate({"long": [1] * 60, "short": [1] * 10, "full": [1] * 64}, 32)
+    assert got == {"long": [60, 61, 62, 63, 64], "short": list(range(10, 42)), "full": [64]}
+    assert not ses.live and not ses.cache.lens
+    ses = sessions(64, lambda n: n, eos=(62,))
+    assert ses.generate({"a": [1] * 60, "b": [1] * 63}, 9) == {"a": [60, 61], "b": [63, 64]}
+    assert ses.generate({"a": [1] * 60}, 3) == {"a": [60, 61]} and ses.generate({"a": [1] * 60}, 1) == {"a": [60]} and ses.generate({"a": [1]}, 0) == {"a": []}
+    assert not ses.live and not ses.cache.lens
+
+
+def test_generation_begins_no_request_that_is_live():
+    ses = sessions(64, lambda n: n)
+    ses.step({"a": [1, 2, 3]}, {})
+    with pytest.raises(ValueError):
+        ses.generate({"b": [1], "a": [4]}, 5)
+    assert list(ses.live) == ["a"] and ses.len("a") == 3
+    assert ses.generate({"b": [1]}, 2) == {"b": [1, 2]}
+    assert list(ses.live) == ["a"] and ses.len("a") == 3
+
+
+@pytest.mark.gpu
+def test_prompts_of_which_one_reaches_the_end_of_its_sequence():
+    from cake_b200.model import PagedSessions
+    cfg = medium_config()
+    m = model_for(cfg, max_seq=64)
+    g = np.random.default_rng(8)
+    prompts = {r: [int(t) for t in g.integers(0, cfg.vocab_size, n)] for r, n in (("long", 60), ("short", 10))}
+    got = PagedSessions(m, 8, 16, max_requests=2, max_seq=64).generate(prompts, 32)
+    wide = PagedSessions(m, 8, 16, max_requests=2, max_seq=64)
+    feed, best = dict(prompts), {}
+    for i in range(5):
+        wide.step(feed, best)
+        assert [best[r] for r in prompts] == [got[r][i] for r in prompts]
+        feed = {r: [best[r]] for r in prompts}
+    wide.end("long")
+    for i in range(5, 32):
+        best = {}
+        wide.step({"short": feed["short"]}, best)
+        assert best["short"] == got["short"][i]
+        feed = {"short": [best["short"]]}
+    assert len(got["long"]) == 5 and len(got["short"]) == 32
+    m.ctx.close()
