@@ -455,6 +455,8 @@ extern "C" int cake_b200_pages_read(cake_b200_pages *g, int block_idx, int seq, 
     a = pg::Read{g->rows, 0, 0, g->book.n_rows, k_dev, v_dev};
   } else {
     if (!g->book.has(seq)) return fail(CAKE_B200_EINVAL, "there is no sequence %d", seq);
+    if (is_capturing(stream ? (cudaStream_t)stream : g->ctx->stream))   // (when it is replayed, nothing says whose pages the table names in that row)
+      return fail(CAKE_B200_ESTATE, "positions of one sequence are read outside captures");
     const int have = g->in_graph[(size_t)block_idx] ? g->book.seqs[(size_t)seq].len : g->len[(size_t)block_idx][(size_t)seq];
     if (first < 0 || n < 1 || (long long)first + n > have)
       return fail(CAKE_B200_ESTATE, "block %d, sequence %d: positions %d .. + %d are not within %d", block_idx, seq, first, n, have);

@@ -429,11 +429,12 @@ int cake_b200_cache_attend(cake_b200_cache *, int block_idx, const void *q_dev, 
  * block, _append puts the step's k and v into the pages and _attend attends over them; both may be repeated while the step stands, and every block of a
  * sequence has to have the rows in front of a step's (CAKE_B200_ESTATE otherwise).  cake_b200_forward_paged does all of it for blocks.
  * stream, as for caches in four bits: the cudaStream_t that the call's tensors belong to (cudaStreamLegacy for the default stream; NULL: the ctx's own), behind
- * what the ctx's other calls have enqueued.  It may be capturing for _append, _attend and _read, once the same call has run outside a capture for a step of
- * the same counts and the present step (CAKE_B200_ESTATE otherwise).  A graph then does the captured calls for whatever step stands when it is replayed: steps of other sequences
+ * what the ctx's other calls have enqueued.  It may be capturing for _append, _attend and _read of the step's rows, once the same call has run outside a capture for a
+ * step of the same counts and the present step (CAKE_B200_ESTATE otherwise).  A graph then does the captured calls for whatever step stands when it is replayed: steps of other sequences
  * and lengths, but the same counts in the same order; the step is planned in front of the replay, outside the graph, on the stream of the replay or before it.
- * A replay for a step of other counts does nothing and makes the next call on the cache fail with CAKE_B200_ESTATE.  Whether a block that a graph appends
- * to has its rows is its user's to know.  Graphs that share a cache are replayed neither at the same time nor beside its calls, and not once it is closed; their
+ * A replay for a step of other counts does nothing, and once it has run it makes a call on the cache fail with CAKE_B200_ESTATE.  A step that _drop or _truncate has ended
+ * stands for graphs until the next one is planned: a replay goes on with the sequences that are left, and what it writes and reads of the others lies in pages, or
+ * behind positions, that nobody has; nothing reports it.  Whether a block that a graph appends to has its rows is its user's to know.  Graphs that share a cache are replayed neither at the same time nor beside its calls, and not once it is closed; their
  * calls may have used up to eight different windows.  (Captured calls suit any lengths; calls outside captures may cut their sums otherwise.)
  * After a wait that a kernel gave up (cake_b200_sync) a cache refuses further use until all its sequences have been dropped. */
 /* rot, cos_dev, sin_dev: rows [max_seq][rot / 2] fp32 in device memory, pairs (e, e + rot / 2), to rotate by instead of the ctx's tables; they stay the

@@ -114,3 +114,63 @@ def test_queries_rotated_onto_rows_that_are_still_read_are_refused(rows):
         torch.cuda.synchronize()
         assert torch.equal(fused[:, :heads], want)
     ctx.close()
+
+
+# ------------------------------------------------------------------------------------------------ replays
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["drop", "truncate"])
+def test_a_replay_behind_a_step_that_was_ended_touches_no_sequence(how):
+    """One of a step's sequences goes, the graph is replayed all the same: rows of all that are left stay, calls are refused, and what comes next is as if it had not run."""
+    heads, kv, hd = 8, 2, 64
+    ctx = ctx_for(heads, kv, hd)
+    cache = PagedCache(ctx, 24, 16, max_seqs=4, max_seq=100)
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def rows(n, x):
+        return torch.randn((n, x, hd), generator=g, device="cuda").bfloat16()
+    a, b, other = cache.add(), cache.add(), cache.add()
+    held = [37, 30, 45]
+    cache.step([a, b, other], held)
+    k, v = rows(sum(held), kv), rows(sum(held), kv)
+    cache.append(0, None, k, v, rotate=False)
+    cache.step([a, b], [1, 3])
+    q, nk, nv = rows(4, heads), rows(4, kv), rows(4, kv)
+
+    def calls():
+        cache.append(0, None, nk, nv, rotate=False)
+        return cache.attend(0, q)
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    graph.replay()
+    want = out.clone()
+    kept = {s: cache.read(0, s) for s in (a, other)}
+    if how == "drop":
+        cache.drop(b)
+        fresh = cache.add()   # in the same row of the table
+        assert fresh == b
+    else:
+        cache.truncate(b, 20)
+        kept[b] = cache.read(0, b)
+    nk.neg_(), nv.neg_()
+    nk[0].neg_(), nv[0].neg_()   # (the rows of the one that is left)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0])
+    refused(ESTATE, cache.attend, 0, q)
+    refused(ESTATE, cache.append, 0, None, nk, nv, False)
+    for s, (x, y) in kept.items():
+        assert all(torch.equal(p, r) for p, r in zip(cache.read(0, s), (x, y)))
+    grow = 33 if how == "drop" else 13   # b, or the one in its place, up to the same length: over pages that the replay wrote to
+    cache.step([b], [grow])
+    k2, v2 = rows(grow, kv), rows(grow, kv)
+    cache.append(0, None, k2, v2, rotate=False)
+    x, y = (k2, v2) if how == "drop" else (torch.cat(p) for p in zip(kept[b], (k2, v2)))
+    got = cache.read(0, b)
+    assert torch.equal(got[0], x) and torch.equal(got[1], y)
+    for s in (a, other):
+        assert all(torch.equal(p, r) for p, r in zip(cache.read(0, s), kept[s]))
+    del graph
+    ctx.close()

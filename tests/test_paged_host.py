@@ -221,3 +221,20 @@ def test_a_step_that_fails_takes_nothing(tmp_path, what):
     IS(live == 0);
   }
 '''.replace("WHAT", what))
+
+
+def test_positions_of_one_sequence_are_read_outside_captures(tmp_path):
+    """A graph would read whatever sequence, or none, has that row of the table by then."""
+    run(tmp_path, r'''
+  cake_b200_ctx *c = context(8, 2, 64);
+  cake_b200_pages *g = nullptr;
+  IS(cake_b200_pages_create(c, 40, 16, 4, 300, nullptr, nullptr, 0, &g) == 0);
+  int s, n = 20;
+  IS(cake_b200_pages_add(g, &s) == 0 && cake_b200_pages_step(g, &s, &n, 1, nullptr) == 0);
+  IS(cake_b200_pages_append(g, 0, nullptr, 0, mem, 128, mem, 128, nullptr, 0, nullptr) == 0);
+  IS(cake_b200_pages_read(g, 0, s, 3, 5, mem, mem + 65536, (void *)32) == 0 && pg::been_read == 1);
+  IS(cake_b200_pages_read(g, 0, s, 3, 5, mem, mem + 65536, CAPTURING) == CAKE_B200_ESTATE && pg::been_read == 1);
+  IS(cake_b200_pages_read(g, 0, -1, 0, 20, mem, mem + 65536, CAPTURING) == 0 && pg::been_read == 2);
+  cake_b200_pages_free(g);
+  gone(c);
+''')
