@@ -179,6 +179,7 @@ class PagedCache:
                     raise ValueError(f"a rotation table is {t.dtype} on {t.device}, expected {torch.float32} on cuda:{ctx.device}")
             cos, sin = cos.contiguous(), sin.contiguous()
             rot = 2 * cos.shape[1]
+            ctx.torch_stream.wait_stream(torch.cuda.current_stream(ctx.torch_device))   # calls on any stream come behind the tables' making
         self.rotation = (cos, sin)   # read by the library as long as the cache lives
         check(self._lib.cake_b200_pages_create(ctx.h, pages, page_size, max_seqs, self.max_seq, ptr(cos), ptr(sin), rot, byref(self.h)))
         ctx._children.append(weakref.ref(self))

@@ -174,3 +174,29 @@ def test_a_replay_behind_a_step_that_was_ended_touches_no_sequence(how):
         assert all(torch.equal(p, r) for p, r in zip(cache.read(0, s), kept[s]))
     del graph
     ctx.close()
+
+
+# ------------------------------------------------------------------------------------------------ streams
+@pytest.mark.gpu
+@pytest.mark.parametrize("copied", [False, True])
+def test_rotation_tables_that_are_still_on_their_way(copied):
+    """Tables made on one stream, where the cache is made too, and used on another one at once; copied: into the order that the library takes."""
+    ctx = ctx_for(8, 2, 64)
+    angles = torch.arange(60, device="cuda", dtype=torch.float64)[:, None] * 10.0 ** -torch.linspace(0, 4, 32, device="cuda", dtype=torch.float64)
+    cos, sin = angles.cos().float(), angles.sin().float()
+    q, k = (torch.randn(40, x, 64, device="cuda").bfloat16() for x in (8, 2))
+
+    def rows(cache):
+        cache.step([cache.add()], [40])
+        return cache.append(0, q, k, k)
+    want = rows(PagedCache(ctx, 4, 16, max_seqs=1, max_seq=60, rotation=(cos, sin)))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        late = [torch.zeros(32, 60, device="cuda").T if copied else torch.zeros(60, 32, device="cuda") for _ in range(2)]
+        torch.cuda._sleep(50_000_000)   # some 30 ms
+        late[0].copy_(cos), late[1].copy_(sin)
+        cache = PagedCache(ctx, 4, 16, max_seqs=1, max_seq=60, rotation=tuple(late))
+    got = rows(cache)
+    assert torch.equal(got, want)
+    ctx.close()
