@@ -773,8 +773,8 @@ class TextModelBase:
 
     def forward_paged(self, pages: PagedCache, requests: Sequence[Tuple[int, Sequence[int]]], greedy: Optional[List[int]] = None) -> torch.Tensor:
         """One step of many sequences: requests [(sequence of ``pages``, its next token ids)] -> logits (len(requests), vocab) of their last tokens, a device
-        tensor in D.  ``greedy``: a list that receives each one's most likely next token (the call then waits for them).  All blocks are local ones.  Where the
-        call fails, the sequences are as they were."""
+        tensor in D for the calling thread's current stream.  ``greedy``: a list that receives each one's most likely next token (the call then waits for them).
+        All blocks are local ones.  Where the call fails, the sequences are as they were."""
         ctx, L = self.ctx, lib()
         run = self._local_run()
         if run is None:
@@ -782,6 +782,7 @@ class TextModelBase:
         counts = [len(t) for _, t in requests]
         ids = np.ascontiguousarray([i for _, t in requests for i in t], dtype=np.uint32)
         n = len(ids)
+        mine = torch.cuda.current_stream(ctx.torch_device)
         with torch.cuda.stream(ctx.torch_stream):
             if n and (ids >= ctx.config.vocab_size).any():   # in front of the step, which takes its pages
                 raise ValueError(f"token id {ids.max()} out of range (vocab {ctx.config.vocab_size})")
@@ -803,6 +804,9 @@ class TextModelBase:
                 for (s, _), c in zip(requests, counts):
                     pages.truncate(s, pages.len(s) - c)
                 raise
+        if mine != ctx.torch_stream:   # the caller reads them on its own stream
+            mine.wait_stream(ctx.torch_stream)
+            logits.record_stream(mine)
         if greedy is not None:
             greedy[:] = best
         return logits

@@ -152,3 +152,34 @@ def test_prompts_of_which_one_reaches_the_end_of_its_sequence():
         feed = {"short": [best["short"]]}
     assert len(got["long"]) == 5 and len(got["short"]) == 32
     m.ctx.close()
+
+
+@pytest.mark.gpu
+def test_logits_are_read_on_the_callers_stream():
+    """Behind work that the library's stream still has in front of the step, and again after their memory has been given back and taken by the next step."""
+    from cake_b200.model import PagedSessions
+    cfg = medium_config()
+    m = model_for(cfg)
+    ses = [PagedSessions(m, 12, 16, max_requests=2) for _ in range(2)]
+    feeds = [{"a": [3, 1, 4], "b": [1, 5]}, {"a": [9]}, {"a": [2, 6], "b": [5]}]
+    want = []
+    for feed in feeds:
+        got = ses[0].step(feed)
+        m.ctx.sync()
+        want.append({r: x.clone() for r, x in got.items()})
+    for stream in (torch.cuda.default_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            kept = []
+            for feed in feeds:
+                with torch.cuda.stream(m.ctx.torch_stream):
+                    torch.cuda._sleep(30_000_000)   # some 15 ms
+                got = ses[1].step(feed)
+                torch.cuda._sleep(10_000_000)
+                kept.append({r: x + 0 for r, x in got.items()})
+                del got
+        stream.synchronize()
+        for w, k in zip(want, kept):
+            assert all(torch.equal(w[r], k[r]) for r in w)
+        for r in "ab":
+            ses[1].end(r)
+    m.ctx.close()
