@@ -963,6 +963,7 @@ class PagedSessions:
         self.model = model
         self.cache = PagedCache(model.ctx, pages, page_size, max_requests, max_seq)
         self.live: Dict[str, int] = {}
+        self.tok_s = 0.0   # of the last generate
 
     def step(self, tokens: Dict[str, Sequence[int]], greedy: Optional[Dict[str, int]] = None) -> Dict[str, torch.Tensor]:
         """{request: its next token ids} -> {request: logits (vocab) of the last of them}.  A request that is not live begins with these.  ``greedy``: receives each
@@ -986,18 +987,24 @@ class PagedSessions:
 
     def generate(self, prompts: Dict[str, Sequence[int]], sample_len: int) -> Dict[str, List[int]]:
         """Greedy generation of up to ``sample_len`` tokens for each of some new requests, all of them together; a request ends with its end of stream, or with the
-        token behind its last position where it has reached the cache's ``max_seq``."""
+        token behind its last position where it has reached the cache's ``max_seq``.  ``tok_s`` is then the rate of all of them together, as generate_text counts it: the
+        tokens behind the first step's (ends of stream are some), over the time since then."""
         taken = [rid for rid in prompts if rid in self.live]
         if taken:
             raise ValueError(f"requests {taken} are live: generate begins new ones")
         out: Dict[str, List[int]] = {rid: [] for rid in prompts}
         feed, best = dict(prompts), {}
+        generated, start, self.tok_s = 0, None, 0.0
         try:
             for _ in range(sample_len):
                 if not feed:
                     break
                 best.clear()
                 self.step(feed, best)
+                if start is None:
+                    start = time.perf_counter()
+                else:
+                    generated += len(best)
                 feed = {}
                 for rid, token in best.items():
                     if self.model.ctx.config.is_eos(token):
@@ -1008,6 +1015,8 @@ class PagedSessions:
                         feed[rid] = [token]
                     else:   # there is no place for this one
                         self.end(rid)
+            if generated:
+                self.tok_s = generated / (time.perf_counter() - start)
         finally:
             for rid in prompts:
                 self.end(rid)

@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import argparse
 import sys
-import time
 from typing import List, Optional
 
 
@@ -63,12 +62,10 @@ def main(argv: Optional[List[str]] = None) -> int:
         if len(prompts) > 1:
             page = 64
             requests = PagedSessions(model, sum((min(len(p) + a.n, max_seq) + page - 1) // page for p in prompts), page, len(prompts), max_seq)
-            began = time.perf_counter()
             out = requests.generate({str(i): p for i, p in enumerate(prompts)}, a.n)
-            took = time.perf_counter() - began
             for tokens in out.values():
                 print("tokens: " + " ".join(str(t) for t in tokens))
-            print(f"tok/s: {sum(map(len, out.values())) / took:.2f}")
+            print(f"tok/s: {requests.tok_s:.2f}")
             return 0
         out = Master(model).generate_text(prompt, a.n)
         print("tokens: " + " ".join(str(t) for t in out["tokens"]))

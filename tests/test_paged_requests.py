@@ -183,3 +183,38 @@ def test_logits_are_read_on_the_callers_stream():
         for r in "ab":
             ses[1].end(r)
     m.ctx.close()
+
+
+@pytest.mark.parametrize("prompts,n,eos,behind", [([3, 1], 5, (), 8), ([3, 1], 1, (), 0), ([3], 4, (5,), 2), ([3, 9], 6, (3, 9), 0), ([2], 0, (), 0), ([60, 1], 9, (), 12)])
+def test_the_rate_of_requests_together_leaves_the_prompts_out(monkeypatch, prompts, n, eos, behind):
+    """A clock on which a step takes 1 s and the prompts' step 100: tokens behind the first step's over the seconds since then."""
+    from cake_b200 import model
+    clock = [0.0]
+    monkeypatch.setattr(model.time, "perf_counter", lambda: clock[0])
+    ses = sessions(64, lambda n: n, eos)
+    step = ses.step
+
+    def timed(tokens, best):
+        clock[0] += 100.0 if not any(ses.len(r) for r in tokens) else 1.0
+        return step(tokens, best)
+    monkeypatch.setattr(ses, "step", timed)
+    ses.generate({str(i): [1] * x for i, x in enumerate(prompts)}, n)
+    steps = clock[0] - 100.0 if n else 0.0
+    assert ses.tok_s == (behind / steps if behind else 0.0)
+
+
+def test_both_rates_of_the_command_line_are_of_one_kind(monkeypatch, tmp_path, capsys):
+    """cake_b200.run prints what generate, or generate_text, counted, in the same line for one prompt and for several."""
+    from types import SimpleNamespace
+    from cake_b200 import build, loader, model, run
+    cfg = medium_config()
+    monkeypatch.setattr(loader, "open_model", lambda d: (cfg, {}))
+    monkeypatch.setattr(build, "build", lambda **kw: None)
+    monkeypatch.setattr(model, "Context", lambda *a, **kw: SimpleNamespace(close=lambda: None))
+    monkeypatch.setattr(model.TextModelBase, "load", classmethod(lambda cls, ctx, **kw: ctx))
+    monkeypatch.setattr(model, "Master", lambda m: SimpleNamespace(generate_text=lambda p, n: {"tokens": [4], "tok_s": 12.5}))
+    monkeypatch.setattr(model, "PagedSessions", lambda *a: SimpleNamespace(generate=lambda p, n: {r: [4] for r in p}, tok_s=37.25))
+    assert run.main([str(tmp_path), "--prompt-ids", "1,2"]) == 0
+    assert capsys.readouterr().out.splitlines() == ["tokens: 4", "tok/s: 12.50"]
+    assert run.main([str(tmp_path), "--prompt-ids", "1,2;3"]) == 0
+    assert capsys.readouterr().out.splitlines() == ["tokens: 4", "tokens: 4", "tok/s: 37.25"]
