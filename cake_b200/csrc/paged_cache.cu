@@ -178,9 +178,9 @@ __global__ void __launch_bounds__(256) read_kernel(const Pool p, const Read a) {
     if (a.v) reinterpret_cast<uint4 *>(a.v)[i] = *reinterpret_cast<const uint4 *>(rows_of(p, page, h, 1) + chunk_at(p.hd, r, c));
   }
 }
-int read(cudaStream_t s, int, const Pool &p, const Read &a, uint64_t *launches) {
+int read(cudaStream_t s, const Pool &p, const Read &a, int sms, uint64_t *launches) {
   const size_t n = (size_t)a.n * p.n_kv * (p.hd >> 3);
-  return launch(s, launches, read_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 148 * 32)), dim3(256), 0, 1, p, a);
+  return launch(s, launches, read_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, (size_t)sms * 32)), dim3(256), 0, 1, p, a);
 }
 
 // ------------------------------------------------------------------------------------------ attention

@@ -59,7 +59,7 @@ int append(cudaStream_t, int dtype, const Pool &, const Append &, int sms, uint6
 
 // rows of the present step (rows), or positions first .. of sequence slot (rows == nullptr) -> k, v [n][n_kv][hd]; either may be nullptr
 struct Read { const int2 *rows; int slot, first, n; void *k, *v; };
-int read(cudaStream_t, int dtype, const Pool &, const Read &, uint64_t *launches);
+int read(cudaStream_t, const Pool &, const Read &, int sms, uint64_t *launches);
 
 // A step's attention as it is cut for one window (paged_plan.hpp), on the device: this head, few_ctas workers and as many cuts of the few-row kernel, the items of
 // the many-row kernel.  What the calls on a cache share: sums of runs and tiles that are cut

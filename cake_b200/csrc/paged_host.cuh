@@ -462,7 +462,7 @@ extern "C" int cake_b200_pages_read(cake_b200_pages *g, int block_idx, int seq, 
       return fail(CAKE_B200_ESTATE, "block %d, sequence %d: positions %d .. + %d are not within %d", block_idx, seq, first, n, have);
   }
   return on_stream(g->ctx, stream, [&]() -> int {
-    CU((cudaError_t)pg::read(g->ctx->stream, g->ctx->cfg.dtype, pages_pool(g, block_idx), a, launch_counter(g->ctx)));
+    CU((cudaError_t)pg::read(g->ctx->stream, pages_pool(g, block_idx), a, g->ctx->sm_count, launch_counter(g->ctx)));
     return CAKE_B200_OK;
   });
 }

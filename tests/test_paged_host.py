@@ -131,7 +131,7 @@ int spread(cudaStream_t, const StepHead *h, int n_seqs, int, int, int *table, in
 }
 static int appended, attended, been_read;
 int append(cudaStream_t, int, const Pool &, const Append &, int, uint64_t *) { FAKE; appended++; return 0; }
-int read(cudaStream_t, int, const Pool &, const Read &, EXTRA_READ uint64_t *) { FAKE; been_read++; return 0; }
+int read(cudaStream_t, const Pool &, const Read &, int, uint64_t *) { FAKE; been_read++; return 0; }
 int attend(cudaStream_t, int, const Pool &, const Attend &, const Scratch &, uint64_t *) { FAKE; attended++; return 0; }
 } }
 #define IS(x) do { if (!(x)) { printf("line %d: %s   (%s)\n", __LINE__, #x, g_err); exit(1); } } while (0)
@@ -154,9 +154,8 @@ def run(tmp_path, main):
     text = open(os.path.join(CSRC, "paged_host.cuh")).read()
     text = re.sub(r"template <typename T> __global__ void widen_kernel.*?\n}\n", "", text, flags=re.S)   # (no rotation here: nothing to widen)
     text = re.sub(r"widen_kernel<T><<<.*?>>>\([^;]*\);", "(void)n;", text)
-    extra = "int, " if re.search(r"int read\([^;]*int sms", open(os.path.join(CSRC, "paged_cache.cuh")).read()) else ""
     src = tmp_path / "host.cpp"
-    src.write_text(FRONT.replace("EXTRA_READ ", extra) + text + "int main() {\n" + main + "\nreturn 0; }\n")
+    src.write_text(FRONT + text + "int main() {\n" + main + "\nreturn 0; }\n")
     exe = tmp_path / "host"
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=address,undefined", "-w", "-x", "c++", str(src), "-I", CSRC, "-I", os.path.join(ROOT, "include"),
                            "-I", "/usr/local/cuda/include", "-o", str(exe)])
