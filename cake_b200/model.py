@@ -805,7 +805,8 @@ class TextModelBase:
                     pages.truncate(s, pages.len(s) - c)
                 raise
         if mine != ctx.torch_stream:   # the caller reads them on its own stream
-            mine.wait_stream(ctx.torch_stream)
+            if greedy is None:   # (else they are there)
+                mine.wait_stream(ctx.torch_stream)
             logits.record_stream(mine)
         if greedy is not None:
             greedy[:] = best
