@@ -45,7 +45,9 @@ __global__ void __launch_bounds__(256) spread_kernel(const StepHead *step, int n
 }
 int spread(cudaStream_t s, const StepHead *step, int n_seqs, int n_updates, int most_rows, int *table, int2 *rows, uint64_t *launches) {
   const int most = std::max(most_rows, n_updates);
-  // (launched without the early start of the others: what runs behind it reads the table before it waits)
+  // Attention reads the step, its plan and the table in front of its wait for the launch before it.  Between this kernel and the first attention over a step with any
+  // window lies the copy of that window's plan (made by that call, or with the step where captured calls read it), and no launch behind a copy starts early: all
+  // that is in front of the copy is there for it and for what starts behind it.  Appends and reads look behind their wait.
   spread_kernel<<<dim3((unsigned)n_seqs + 1, (unsigned)std::min(64, (most + 255) / 256)), 256, 0, s>>>(step, n_seqs, table, rows);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) ++*launches;
@@ -241,7 +243,8 @@ int prepare(int dtype, int hd, Clusters *out) {
 // at once and no CTA has many more tiles than an equal share.  Clusters / shares in us (shares in a graph; alone their second launch costs 2 more of the
 // host's), sequences x positions:  8 key heads of 128, 1 x 500 7.1 (the host's) / 5.7, 1 x 4000 9.7 / 12.1, 4 x 1000 7.1 / 9.8, 9 x 500 7.4 / 8.8, 9 x 2000 (16 tiles a CTA,
 // an equal share 8) 15.0 / 13.9, 16 x 1000 10.7 / 11.7, 32 x 1000 23.5 / 27.3, 32 x 4000 81 / 84;  2 of 64, 1 x 4000 8.4 / 7.1, 32 x 1000 7.1 / 8.2, 64 x 4000 25 / 28;  4 of 256,
-// 2 x 2000 8.0 / 12.4, 4 x 4000 (16 tiles, 7) 15.9 / 14.8, 16 x 1000 11.1 / 12.6.
+// 2 x 2000 8.0 / 12.4, 4 x 4000 (16 tiles, 7) 15.9 / 14.8, 16 x 1000 11.1 / 12.6.  A captured call follows the same rule by the longest run that the cache allows: in a
+// graph 1 x 4000 of 2 x 64 takes 7.5 in clusters and 7.1 in shares, and 1 x 998 (8 of 128) 4.4 in a cache of up to some 4000 positions and 6.0, in shares, in larger ones.
 constexpr int CLUSTER_TILES = 8;
 static int cluster_of(int runs, int longest, int tiles, int ctas, const int (&most)[4]) {
   int best = 0;
