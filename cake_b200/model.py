@@ -1012,7 +1012,7 @@ class PagedSessions:
                         self.end(rid)
                         continue
                     out[rid].append(token)
-                    if self.len(rid) < self.cache.max_seq:
+                    if len(prompts[rid]) + len(out[rid]) <= self.cache.max_seq:
                         feed[rid] = [token]
                     else:   # there is no place for this one
                         self.end(rid)
